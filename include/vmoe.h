@@ -798,6 +798,88 @@ int vmoe_moe_f32_backward(const void* saved, const float* logits, int64_t num_to
                           float* grad_w1, int64_t ldgw1, float* grad_w2, int64_t ldgw2,
                           float* grad_logits, void* scratch, vmoe_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * The expert layer for a few tokens (a generation step), at most
+ * vmoe_few_max_tokens() tokens, 4096 token-expert pairs, top_k 64 and 2048
+ * experts; no counterpart in the reference, whose layer pads every expert's rows
+ * to a block (triton_moe/moe.py:148-250). Inference only. No rows are moved or
+ * padded, and the router's logits stay in fp32, so that its choice may differ
+ * from the training layer's where that layer's bf16 logits tie.
+ *
+ * vmoe_few_weights describes the experts (host memory, read during the call):
+ * w1 [hidden, columns] and w2 [rows, hidden] in bf16 or fp32 with row strides, or
+ * 4-bit blocks with scales. The tables hold four int32 a matrix: where it starts
+ * (a column of w1, a row of w2), its length along that axis, its first 4-bit
+ * block, 0. table1 has an entry for each expert (SwiGLU: two, gate and up),
+ * table2 one. Activations and outputs are bf16 (fp32 for fp32 weights). hidden,
+ * widths, starts and strides are multiples of 8 (fp32: 4), buffers 16-byte
+ * aligned. Every size is given once: lengths are at most max_width.
+ *
+ * vmoe_few_layer: logits = x router_weight^T in fp32; the top_k largest (ties:
+ * the lowest index; NaN above all), weights sigmoid(logit), over their sum +
+ * 1e-20 if normalize; out[t] = sum w act(x w1_e) w2_e. selected int32 and weights
+ * fp32 [T, top_k] are written if not NULL (the largest logit first).
+ * vmoe_few_experts: the same from given ids [T, top_k] (int32 or int64) and
+ * weights (fp32 or bf16), contiguous; an id outside 0..num_experts-1 is no expert
+ * (a token without any gets zeros), an id given twice counts twice.
+ * Workspace: vmoe_few_workspace_bytes, no initial value.
+ * ---------------------------------------------------------------------- */
+enum vmoe_few_format { VMOE_FEW_BF16 = 0, VMOE_FEW_F32 = 1, VMOE_FEW_Q4 = 2 };
+typedef struct vmoe_few_weights {
+  int32_t format, group, act, num_experts;
+  int64_t hidden, max_width;
+  const void* w1;
+  const uint16_t* scales1;
+  int64_t ldw1;
+  const int32_t* table1;
+  const void* w2;
+  const uint16_t* scales2;
+  int64_t ldw2;
+  const int32_t* table2;
+} vmoe_few_weights;
+int vmoe_few_max_tokens(void);
+size_t vmoe_few_workspace_bytes(int64_t num_tokens, int32_t num_experts, int32_t top_k,
+                                int64_t hidden, int64_t max_width, int32_t format);
+int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t ldx, int64_t num_tokens,
+                   const void* router_weight, int64_t ldwr, int32_t top_k, int32_t normalize,
+                   void* out, int64_t ldo, int32_t* selected, float* weights, void* workspace,
+                   size_t workspace_bytes, vmoe_stream_t stream);
+int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_t ldx, int64_t num_tokens,
+                     const void* ids, int32_t ids_are_i64, const void* weights,
+                     int32_t weights_are_bf16, int32_t top_k, void* out, int64_t ldo,
+                     void* workspace, size_t workspace_bytes, vmoe_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * 4-bit matrices with group scales (no counterpart in the reference). A value is
+ * an e2m1 float (+-0, 0.5, 1, 1.5, 2, 3, 4, 6) times the bf16 scale of its group:
+ * 32, 64 or 128 values of a column along the summed axis. Codes: blocks of 16
+ * columns x 128 rows, 1 KB, 16-byte aligned; scales bf16 [block][16][128/group]
+ * (layout: csrc/few_q4.h). A stack holds matrices side by side (by_rows = 0: all
+ * of `fixed` rows, a table entry's length its columns) or on top of each other
+ * (by_rows = 1: all of `fixed` columns).
+ *
+ * vmoe_q4_quantize: scale = bf16(max |w| / 6) of the group, values the nearest,
+ * ties to the even place; a group that holds a non-finite value gets the scale
+ * NaN. w bf16 or fp32, row-major. vmoe_q4_dequantize: the values in bf16 (rounded
+ * once) or fp32 (exact). max_len: the longest table entry.
+ * vmoe_q4_matvec: y[r, s] = x[r] M[ids[r, s]] in bf16, per_row ids for each of
+ * num_rows rows (limits as above), y [num_rows per_row, ldy]; ids NULL: one
+ * matrix and one id a row. Columns past a matrix's own, and rows whose id is no
+ * matrix, are zeros.
+ * ---------------------------------------------------------------------- */
+int vmoe_q4_quantize(const void* w, int32_t w_is_f32, int64_t ldw, const int32_t* table,
+                     int32_t num_matrices, int32_t by_rows, int64_t fixed, int64_t max_len,
+                     int32_t group, void* codes, uint16_t* scales, vmoe_stream_t stream);
+int vmoe_q4_dequantize(const void* codes, const uint16_t* scales, const int32_t* table,
+                       int32_t num_matrices, int32_t by_rows, int64_t fixed, int64_t max_len,
+                       int32_t group, void* out, int32_t out_is_f32, int64_t ldo,
+                       vmoe_stream_t stream);
+int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids,
+                   int32_t ids_are_i64, int32_t per_row, const void* codes,
+                   const uint16_t* scales, const int32_t* table, int32_t num_matrices,
+                   int64_t k_rows, int64_t max_cols, int32_t group, void* y, int64_t ldy,
+                   vmoe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

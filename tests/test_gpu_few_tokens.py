@@ -1,0 +1,562 @@
+"""The expert layer for a few tokens and the 4-bit matrices, against plain
+64-bit implementations.
+
+Tolerances are bounds, not fits. A bf16 rounding is off by at most 2^-8 of the
+value, an fp32 one by 2^-24; a sum of n fp32 terms in any order by at most
+n 2^-24 of the sum of the terms' magnitudes. The references carry these bounds
+along: magnitudes are propagated next to the values."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+from triton_moe import TritonMoEConfig, TritonMoEMLP
+from triton_moe import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+U32, U16 = 2.0 ** -24, 2.0 ** -8
+VALUES = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+D = torch.float64
+
+
+def normal(seed, *shape, std=1.0, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype)
+
+
+def plain_quantized(w, lengths, by_rows, group):
+    """(values float64 [K, N], scales per element) of a stack: by the distance
+    to every place, an equal distance to the even one."""
+    out, sc = torch.zeros(w.shape, dtype=D), torch.zeros(w.shape, dtype=D)
+    o = 0
+    for n in lengths:
+        part = w[o:o + n] if by_rows else w[:, o:o + n]
+        for r in range(0, part.shape[0], group):
+            v = part[r:r + group].to(D)
+            top = v.abs().amax(dim=0)
+            s = (top.float() / 6.0).to(torch.bfloat16).to(D)
+            s = torch.where(torch.isfinite(top), s, torch.nan)
+            best, near = torch.zeros_like(v), v.abs()
+            for j in range(1, 8):
+                dist = (v.abs() - VALUES[j] * s).abs()
+                take = (dist < near) if j % 2 else (dist <= near)
+                take &= s > 0
+                best = torch.where(take, VALUES[j].expand_as(best), best)
+                near = torch.where(take, dist, near)
+            q = torch.where(v < 0, -best, best) * s
+            end = r + v.shape[0]
+            where = (slice(o + r, o + end), slice(None)) if by_rows else \
+                (slice(r, end), slice(o, o + n))
+            out[where] = q
+            sc[where] = s.expand_as(v)
+        o += n
+    return out, sc
+
+
+def plain_experts(x, sel, wts, w1, w2, widths, act, half):
+    """(out, bound on |error|) of sum_s wts h w2, all float64. half: h is held
+    in two bf16 halves and the output rounded to bf16; else fp32."""
+    T, d = x.shape
+    E = len(widths)
+    out, err = torch.zeros(T, d, dtype=D), torch.zeros(T, d, dtype=D)
+    off = [0]
+    for w in widths:
+        off.append(off[-1] + w)
+    glu = 2 if act == "swiglu" else 1
+    for t in range(T):
+        for s in range(sel.shape[1]):
+            e = int(sel[t, s])
+            if not 0 <= e < E:
+                continue
+            w = widths[e]
+            a = w1[:, glu * off[e]:glu * off[e] + glu * w]
+            b = w2[off[e]:off[e] + w]
+            z, mag = x[t] @ a, x[t].abs() @ a.abs()
+            dz = (d + 8) * U32 * mag
+            if glu == 2:
+                g, u = z[:w], z[w:]
+                sg = torch.sigmoid(g)
+                h = g * sg * u
+                # |silu'| <= 1.1; exp, division and products: 16 roundings
+                dh = 1.1 * dz[:w] * (u.abs() + dz[w:]) + (g * sg).abs() * dz[w:] + \
+                    16 * U32 * h.abs() * (1 + g.abs())
+            else:
+                h = torch.relu(z).square()
+                dh = 2 * torch.relu(z) * dz + dz * dz + 2 * U32 * h
+            if half:
+                dh = dh + U16 * U16 * h.abs()
+            c = float(wts[t, s])
+            y, ymag = h @ b, h.abs() @ b.abs()
+            out[t] += c * y
+            err[t] += abs(c) * (dh @ b.abs() + (w + 8) * U32 * ymag + 32 * U32 * ymag)
+    err += out.abs() * (U16 if half else 8 * U32)
+    return out, err
+
+
+def hold(got, ref, err, what=""):
+    got = got.detach().cpu().to(D).reshape(ref.shape)
+    assert torch.isfinite(got).all(), what
+    bad = (got - ref).abs() > err + 1e-37
+    assert not bad.any(), (what, int(bad.sum()), float(((got - ref).abs() / (err + 1e-37)).max()))
+
+
+def expand(spec):
+    return [int(w) for n, w in (p.split("x") for p in spec.split(",")) for _ in range(int(n))]
+
+
+def layer_inputs(seed, d, widths, T, act="relu_squared", dtype=torch.bfloat16):
+    glu = 2 if act == "swiglu" else 1
+    x = normal(seed, T, d, dtype=dtype)
+    wr = normal(seed + 1, len(widths), d, std=0.05, dtype=dtype)
+    w1 = normal(seed + 2, d, glu * sum(widths), std=0.03, dtype=dtype)
+    w2 = normal(seed + 3, sum(widths), d, std=0.03, dtype=dtype)
+    return x, wr, w1, w2
+
+
+def plain_choice(x, wr, k, normalize):
+    """The choice in 64 bits, and whether every token's is clear: neighbours
+    among its k + 1 largest logits are further apart than two fp32 sums can be
+    off."""
+    logits = x.to(D) @ wr.to(D).t()
+    off = (x.shape[1] + 8) * U32 * (x.to(D).abs() @ wr.to(D).abs().t()).max()
+    top, sel = torch.sort(logits, dim=-1, descending=True, stable=True)
+    near = top[:, :k] - torch.cat([top, top[:, -1:] - 1], 1)[:, 1:k + 1]
+    p = torch.sigmoid(top[:, :k])
+    if normalize:
+        p = p / (p.sum(-1, keepdim=True) + 1e-20)
+    return sel[:, :k], p, bool((near > 2 * off).all())
+
+
+LAYERS = [
+    # d, experts, k, T, dtype, group, normalize
+    (64, "4x64", 2, 1, "bf16", 0, True),
+    (128, "8x64", 8, 1, "bf16", 0, True),          # every expert chosen
+    (200, "3x64,2x192,1x8", 2, 5, "bf16", 0, True),  # ragged widths, hidden not a multiple of 32
+    (1024, "64x256", 8, 1, "bf16", 0, True),
+    (1024, "64x256", 8, 16, "bf16", 0, False),
+    (768, "8x512", 2, 64, "bf16", 0, True),        # 16 rows an expert
+    (256, "2x128", 1, 100, "bf16", 0, True),       # 50 rows an expert: several row tiles
+    (72, "130x8", 3, 17, "bf16", 0, True),         # more experts than a wave is wide
+    (512, "2x1088", 2, 3, "bf16", 0, True),
+    (64, "4x64", 1, 256, "bf16", 0, True),         # the most tokens
+    (128, "4x256", 2, 1, "f32", 0, True),
+    (768, "4x512,8x256,4x128", 2, 13, "f32", 0, True),
+    (36, "5x12,3x20", 3, 40, "f32", 0, False),
+    (1024, "64x256", 8, 1, "q4", 32, True),
+    (1024, "16x256", 4, 33, "q4", 64, True),
+    (200, "3x64,2x192,1x8", 2, 5, "q4", 32, True),
+    (328, "3x136,2x72", 3, 21, "q4", 128, False),
+    (136, "2x1160", 2, 9, "q4", 64, True),
+]
+
+
+# the first seeds whose choice is clear (plain_choice), where 100 i is not
+SEEDS = {4: 930, 14: 1420}
+
+
+def layer_case(i):
+    d, spec, k, T, dt, group, norm = LAYERS[i]
+    widths = expand(spec)
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    inputs = layer_inputs(SEEDS.get(i, 100 * i), d, widths, T, dtype=dtype)
+    return d, widths, k, T, dt, group, norm, inputs
+
+
+@pytest.mark.parametrize("i", range(len(LAYERS)))
+def test_layer(device, i):
+    d, widths, k, T, dt, group, norm, (x, wr, w1, w2) = layer_case(i)
+    sel, wts, clear = plain_choice(x, wr, k, norm)
+    assert clear, "inputs with a near tie"
+    if dt == "q4":
+        e = K.quantize_experts(w1.to(device), w2.to(device), widths, group_size=group)
+        a, _ = plain_quantized(w1, widths, False, group)
+        b, _ = plain_quantized(w2, widths, True, group)
+    else:
+        e = K.few_token_experts(w1.to(device), w2.to(device), widths)
+        a, b = w1.to(D), w2.to(D)
+    out, gsel, gw = K.moe_few_tokens(x.to(device), wr.to(device), e, k, normalize=norm,
+                                     return_routing=True)
+    assert torch.equal(gsel.cpu().long(), sel)
+    # a logit is off by at most n 2^-24 of its magnitudes, its sigmoid by a
+    # quarter of that; exp, division and the sum over k add k + 8 roundings
+    dl = (d + 8) * U32 * (x.to(D).abs() @ wr.to(D).abs().t()).max()
+    assert ((gw.cpu().to(D) - wts).abs() <= wts * (2 * dl + (k + 8) * U32)).all()
+    ref, err = plain_experts(x.to(D), sel, wts, a, b, widths, "relu_squared", dt != "f32")
+    err = err + (2 * float(dl) + (k + 8) * U32) * plain_experts(
+        x.to(D).abs(), sel, wts, a.abs(), b.abs(), widths, "relu_squared", True)[0]
+    hold(out, ref, err, LAYERS[i])
+
+
+EXPERTS = [
+    # d, experts, k, T, dtype, group, act, ids
+    (128, "4x64", 2, 3, "bf16", 0, "swiglu", "plain"),
+    (1024, "16x512", 4, 23, "bf16", 0, "swiglu", "padded"),
+    (200, "3x72,2x200", 3, 37, "bf16", 0, "swiglu", "wild"),
+    (256, "4x128", 2, 40, "bf16", 0, "relu_squared", "one"),
+    (256, "4x128", 5, 9, "bf16", 0, "relu_squared", "wild"),
+    (64, "3x64", 2, 4, "bf16", 0, "relu_squared", "none"),
+    (64, "2x64", 16, 256, "bf16", 0, "relu_squared", "plain"),  # the most pairs
+    (132, "3x68,2x20", 3, 37, "f32", 0, "swiglu", "wild"),
+    (128, "4x64", 2, 70, "f32", 0, "relu_squared", "padded"),
+    (1024, "16x512", 4, 7, "q4", 128, "swiglu", "plain"),
+    (200, "3x72,2x200", 3, 37, "q4", 32, "swiglu", "wild"),
+    (320, "3x328", 2, 50, "q4", 64, "relu_squared", "one"),
+]
+
+
+def ids_of(kind, T, k, E, seed):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, E, (T, k), generator=g)
+    if kind == "padded":
+        ids[T - T // 3:] = -1
+    elif kind == "wild":  # no expert, far outside, the same twice
+        ids[0, 0], ids[T // 2, -1], ids[1, 0] = -1, E, 2 ** 30
+        ids[2, :] = ids[2, 0]
+        ids[T - 1] = -1
+    elif kind == "one":
+        ids[:] = E - 1
+    elif kind == "none":
+        ids[:] = -1
+    return ids
+
+
+@pytest.mark.parametrize("i", range(len(EXPERTS)))
+@pytest.mark.parametrize("types", ["i64_f32", "i32_bf16"])
+def test_experts(device, i, types):
+    d, spec, k, T, dt, group, act, kind = EXPERTS[i]
+    widths = expand(spec)
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    x, _, w1, w2 = layer_inputs(7000 + 100 * i, d, widths, T, act, dtype)
+    ids = ids_of(kind, T, k, len(widths), i).to(torch.int32 if "i32" in types else torch.int64)
+    wts = normal(7050 + i, T, k, dtype=torch.bfloat16 if "bf16" in types else torch.float32)
+    glu = 2 if act == "swiglu" else 1
+    if dt == "q4":
+        e = K.quantize_experts(w1.to(device), w2.to(device), widths, act, group)
+        a, _ = plain_quantized(w1, [w for w in widths for _ in range(glu)], False, group)
+        b, _ = plain_quantized(w2, widths, True, group)
+    else:
+        e = K.few_token_experts(w1.to(device), w2.to(device), widths, act)
+        a, b = w1.to(D), w2.to(D)
+    out = K.experts_few_tokens(x.to(device), ids.to(device), wts.to(device), e)
+    ref, err = plain_experts(x.to(D), ids, wts.to(D), a, b, widths, act, dt != "f32")
+    hold(out, ref, err, EXPERTS[i])
+    empty = ~((ids >= 0) & (ids < len(widths))).any(dim=1)
+    assert (out.cpu()[empty] == 0).all()
+
+
+QUANT = [
+    # K, lengths, stacked, group, dtype
+    (128, [16], "columns", 32, "bf16"),
+    (1024, [256] * 4, "columns", 64, "bf16"),
+    (72, [8, 200, 64], "columns", 32, "f32"),
+    (200, [40, 8], "columns", 128, "bf16"),
+    (88, [64, 136, 8, 1000], "rows", 64, "bf16"),
+    (256, [96, 32], "rows", 128, "f32"),
+]
+
+
+def awkward(w):
+    """Groups of zeros, of one value, of ties, tiny and large ones."""
+    w = w.clone()
+    w[:, 0] = 0
+    w[:, 1] = 6.0
+    w[:8, 2] = torch.tensor([6, 0.25, 0.75, 1.25, -1.75, -2.5, 3.5, -5]).to(w.dtype)
+    w[8:, 2] = 0
+    w[:, 3] *= 1e-38
+    w[:, 4] *= 1e30
+    w[:, 5] = 1e-40
+    return w
+
+
+@pytest.mark.parametrize("rows,lengths,stacked,group,dt", QUANT)
+def test_quantize(device, rows, lengths, stacked, group, dt):
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    shape = (rows, sum(lengths)) if stacked == "columns" else (sum(lengths), rows)
+    w = awkward(normal(5, *shape, dtype=dtype))
+    q = K.quantize_matrices(w.to(device), lengths, stacked, group)
+    ref, _ = plain_quantized(w, lengths, stacked == "rows", group)
+    assert torch.equal(q.dequantize(torch.float32).cpu().to(D), ref)
+    assert torch.equal(q.dequantize().cpu(), ref.float().to(torch.bfloat16))
+    # a view of a wider matrix (rows further apart)
+    wide = torch.zeros(shape[0], shape[1] + 24, dtype=dtype, device=device)
+    wide[:, :shape[1]] = w.to(device)
+    again = K.quantize_matrices(wide[:, :shape[1]], lengths, stacked, group)
+    assert torch.equal(again.codes, q.codes) and torch.equal(
+        again.scales.view(torch.int16), q.scales.view(torch.int16))
+
+
+def test_quantize_not_finite(device):
+    w = normal(6, 64, 32)
+    w[3, 5], w[40, 7], w[41, 7] = float("nan"), float("inf"), -1.0
+    v = K.quantize_matrices(w.to(device), group_size=32).dequantize(torch.float32).cpu()
+    bad = torch.zeros(64, 32, dtype=torch.bool)
+    bad[:32, 5] = True
+    bad[32:, 7] = True
+    assert torch.equal(torch.isnan(v), bad)
+
+
+MATVEC = [
+    # K, lengths, T, k (0: no ids), group, padded
+    (4096, [512], 1, 0, 128, 0),
+    (200, [72], 37, 0, 32, 0),
+    (8, [8], 1, 0, 32, 0),
+    (1024, [256] * 16, 61, 4, 32, 7),
+    (136, [8, 200, 64], 5, 3, 64, 1),
+    (264, [40] * 3, 256, 1, 128, 0),
+]
+
+
+@pytest.mark.parametrize("rows,lengths,T,k,group,padded", MATVEC)
+def test_matvec(device, rows, lengths, T, k, group, padded):
+    w = normal(11, rows, sum(lengths), std=0.05)
+    x = normal(12, T, rows)
+    q = K.quantize_matrices(w.to(device), lengths, "columns", group)
+    v, _ = plain_quantized(w, lengths, False, group)
+    N = max(lengths)
+    if not k:
+        y = K.matvec_q4(x.to(device), q)
+        ref, mag = x.to(D) @ v, x.to(D).abs() @ v.abs()
+    else:
+        ids = ids_of("plain", T, k, len(lengths), 13)
+        if padded:
+            ids[T - padded:] = -1
+        y = K.matvec_q4(x.to(device), q, ids.to(device))
+        ref, mag = torch.zeros(T, k, N, dtype=D), torch.zeros(T, k, N, dtype=D)
+        off = [sum(lengths[:i]) for i in range(len(lengths))]
+        for t in range(T):
+            for s in range(k):
+                m = int(ids[t, s])
+                if m >= 0:
+                    cols = slice(off[m], off[m] + lengths[m])
+                    ref[t, s, :lengths[m]] = x[t].to(D) @ v[:, cols]
+                    mag[t, s, :lengths[m]] = x[t].to(D).abs() @ v[:, cols].abs()
+        assert (y.cpu().to(D)[ref == 0] == 0).all()
+    assert y.shape == ref.shape
+    hold(y, ref, U16 * ref.abs() + (rows + 8) * U32 * mag)
+
+
+def test_matvec_shapes(device):
+    w, x = normal(21, 96, 64, std=0.1), normal(22, 2, 3, 96)
+    c = K.quantize_matrices(w.to(device))
+    with pytest.raises(NotImplementedError, match="side by side"):
+        K.matvec_q4(x.to(device), K.quantize_matrices(w.to(device), stacked="rows"))
+    ids = torch.zeros(2, 3, 1, dtype=torch.int32, device=device)
+    y = K.matvec_q4(x.to(device), c, ids)
+    assert y.shape == (2, 3, 1, 64)
+    assert torch.equal(y[..., 0, :], K.matvec_q4(x.to(device), c))
+
+
+def test_ties_go_to_the_lowest_index(device):
+    d, widths = 64, [64] * 70
+    x, wr, w1, w2 = layer_inputs(31, d, widths, 9)
+    wr[5::7] = wr[5]
+    wr[2] = 0
+    e = K.few_token_experts(w1.to(device), w2.to(device), widths)
+    logits = x.to(D) @ wr.to(D).t()
+    sel = torch.sort(logits, dim=-1, descending=True, stable=True)[1][:, :12]
+    _, got, _ = K.moe_few_tokens(x.to(device), wr.to(device), e, 12, return_routing=True)
+    assert torch.equal(got.cpu().long(), sel)
+    # all logits equal
+    _, got, wts = K.moe_few_tokens(x.to(device), torch.zeros_like(wr).to(device), e, 5,
+                                   return_routing=True)
+    assert torch.equal(got.cpu(), torch.arange(5, dtype=torch.int32).expand(9, 5))
+    assert torch.equal(wts.cpu(), torch.full((9, 5), 0.5).div(2.5))
+
+
+def test_not_finite_stays_where_it_is(device):
+    """NaN weights of experts no one chose, and a token of infinities, change
+    no other token's output."""
+    d, widths = 128, [64] * 8
+    x, wr, w1, w2 = layer_inputs(41, d, widths, 6)
+    e = K.few_token_experts(w1.to(device), w2.to(device), widths)
+    clean, sel, _ = K.moe_few_tokens(x.to(device), wr.to(device), e, 2, return_routing=True)
+    for left in set(range(8)) - set(sel.unique().tolist()):
+        w1[:, 64 * left:64 * left + 64] = float("nan")
+        w2[64 * left:64 * left + 64] = float("inf")
+    e = K.few_token_experts(w1.to(device), w2.to(device), widths)
+    assert torch.equal(K.moe_few_tokens(x.to(device), wr.to(device), e, 2), clean)
+    x[3, 7] = float("inf")
+    x[4, 0] = float("nan")
+    out = K.moe_few_tokens(x.to(device), wr.to(device), e, 2)
+    assert torch.isnan(out[4]).all()
+    keep = [0, 1, 2, 5]
+    assert torch.equal(out[keep], clean[keep])
+
+
+def test_large_activations(device):
+    """h = z^2 past fp32's range is an infinity, and an infinity times the zero
+    rows of w2 is NaN in any order of the sum; h between bf16's largest value
+    and fp32's stays finite in its two halves."""
+    d, widths = 64, [64]
+    x = torch.zeros(3, d, dtype=torch.bfloat16)
+    x[0, 0], x[1, 0], x[2, 0], x[2, 1] = 1.0, 2.0 ** 64, 2.0 ** 64, -2.0 ** 54
+    w1 = torch.zeros(d, 64, dtype=torch.bfloat16)
+    w1[:2] = 1.0
+    w2 = torch.zeros(64, d, dtype=torch.bfloat16)
+    w2[0] = 2.0 ** -60
+    e = K.few_token_experts(w1.to(device), w2.to(device), widths)
+    ids = torch.zeros(3, 1, dtype=torch.int64, device=device)
+    out = K.experts_few_tokens(x.to(device), ids, torch.ones(3, 1, device=device), e).cpu()
+    assert (out[0] == 2.0 ** -60).all()
+    assert torch.isnan(out[1]).all()
+    # (2^64 - 2^54)^2 2^-60 = 2^68 - 2^59 + 2^48, above the middle below 2^68
+    assert (out[2] == 2.0 ** 68).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32", "q4"])
+def test_layouts_and_shapes(device, dt):
+    """Strided and misaligned x, weights that are views, leading dimensions, one
+    token, no token: the same rows give the same bits."""
+    d, widths, k = 136, [64, 72, 8], 2
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    x, wr, w1, w2 = (t.to(device) for t in layer_inputs(51, d, widths, 12, dtype=dtype))
+
+    def handle(a, b):
+        return K.quantize_experts(a, b, widths) if dt == "q4" else \
+            K.few_token_experts(a, b, widths)
+
+    e = handle(w1, w2)
+    ref = K.moe_few_tokens(x, wr, e, k)
+    wide = torch.zeros(12, d + 8, dtype=dtype, device=device)
+    wide[:, :d] = x
+    assert torch.equal(K.moe_few_tokens(wide[:, :d], wr, e, k), ref)
+    odd = torch.zeros(12 * d + 1, dtype=dtype, device=device)[1:].view(12, d)
+    odd.copy_(x)
+    assert torch.equal(K.moe_few_tokens(odd, wr, e, k), ref)
+    assert torch.equal(K.moe_few_tokens(x.t().contiguous().t(), wr, e, k), ref)
+    assert torch.equal(K.moe_few_tokens(x[:1].expand(12, d), wr, e, k),
+                       K.moe_few_tokens(x[:1].repeat(12, 1), wr, e, k))
+    assert torch.equal(K.moe_few_tokens(x.view(3, 4, d), wr, e, k), ref.view(3, 4, d))
+    assert K.moe_few_tokens(x[0], wr, e, k).shape == (d,)
+    none = K.moe_few_tokens(x[:0].view(0, 5, d), wr, e, k, return_routing=True)
+    assert none[0].shape == (0, 5, d) and none[1].shape == (0, k)
+    assert torch.equal(K.moe_few_tokens(x, wr.t().contiguous().t(), e, k), ref)
+    wide1 = torch.zeros(d, w1.shape[1] + 16, dtype=dtype, device=device)
+    wide1[:, 8:-8] = w1
+    wide2 = torch.full((w2.shape[0], d + 8), float("nan"), dtype=dtype, device=device)
+    wide2[:, :d] = w2
+    assert torch.equal(K.moe_few_tokens(x, wr, handle(wide1[:, 8:-8], wide2[:, :d]), k), ref)
+    sel, wts = K.moe_few_tokens(x, wr, e, k, return_routing=True)[1:]
+    assert torch.equal(K.experts_few_tokens(x, sel, wts, e), ref)
+    assert torch.equal(K.experts_few_tokens(x, sel.t().contiguous().t(), wts, e), ref)
+    assert K.experts_few_tokens(x[:0], sel[:0], wts[:0], e).shape == (0, d)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "q4"])
+def test_graph_and_streams(device, dt):
+    """Captured and replayed with new inputs, between eager calls; two calls at
+    once on two streams."""
+    d, widths, k = 256, [128] * 8, 2
+    x, wr, w1, w2 = (t.to(device) for t in layer_inputs(61, d, widths, 20))
+    e = K.quantize_experts(w1, w2, widths) if dt == "q4" else K.few_token_experts(w1, w2, widths)
+    q = K.quantize_matrices(w1, widths)
+    inputs = [normal(62 + i, 20, d).to(device) for i in range(4)]
+    ref = [K.moe_few_tokens(i, wr, e, k, return_routing=True) for i in inputs]
+    prod = [K.matvec_q4(i, q, r[1]) for i, r in zip(inputs, ref)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.moe_few_tokens(x, wr, e, k)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, sel, wts = K.moe_few_tokens(x, wr, e, k, return_routing=True)
+        y = K.matvec_q4(x, q, sel)
+    for i, r, p in zip(inputs, ref, prod):
+        x.copy_(i)
+        g.replay()
+        eager = K.moe_few_tokens(i, wr, e, k)
+        torch.cuda.synchronize()
+        assert torch.equal(out, r[0]) and torch.equal(sel, r[1]) and torch.equal(wts, r[2])
+        assert torch.equal(y, p) and torch.equal(eager, r[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(K.moe_few_tokens(inputs[n], wr, e, k))
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert all(torch.equal(o, ref[n][0]) for o in got[n])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_module(device, dtype):
+    """TritonMoEMLP.few_tokens: the module's forward up to its roundings (where
+    both choose the same experts), its weights' updates, copies and moves."""
+    cfg = TritonMoEConfig(n_embd=256, expert_sizes=[(4, 128), (4, 64)], num_active_experts=2)
+    torch.manual_seed(3)
+    m = TritonMoEMLP(cfg).to(device).to(dtype)
+    with torch.no_grad():
+        m.router.weight.normal_(0, 0.1)
+    x = normal(71, 2, 9, 256, dtype=dtype).to(device)
+    out, sel, wts = m.few_tokens(x, return_routing=True)
+    assert out.shape == x.shape and not out.requires_grad
+    full = m.forward_with_intermediates(x)
+    same = (full["selected_experts"].view(18, 2) == sel).all(dim=1)
+    assert same.sum() >= 12
+    # forward rounds logits, weights, h and y to bf16 (fp32: sums alone differ):
+    # five roundings of terms that cancel, against the largest output
+    a, b = out.view(18, 256)[same].double(), full["output"].view(18, 256)[same].double()
+    limit = (5 * U16 if dtype == torch.bfloat16 else 1e-5) * 4
+    assert ((a - b).abs().max() <= limit * b.abs().max())
+    # updates in place, a replaced parameter, a moved storage
+    with torch.no_grad():
+        m.w2.mul_(2.0)
+        assert torch.equal(m.few_tokens(x), 2 * out)
+        m.w2 = torch.nn.Parameter(m.w2.detach() * 0.5)
+        assert torch.equal(m.few_tokens(x), out)
+        m.w1.data = m.w1.data.clone()
+        assert torch.equal(m.few_tokens(x), out)
+    # copies
+    twin = copy.deepcopy(m)
+    with torch.no_grad():
+        twin.w2.zero_()
+    assert (twin.few_tokens(x) == 0).all()
+    assert torch.equal(m.few_tokens(x), out)
+    pickle.loads(pickle.dumps(m.state_dict()))
+    pickle.dumps(m)
+
+
+def test_module_quantized_run(device):
+    """A layer's weights to 4 bits, generation with them, and a prompt through
+    forward() with the values they stand for: the same layer."""
+    cfg = TritonMoEConfig(n_embd=256, expert_sizes=[(4, 128), (4, 64)], num_active_experts=2)
+    torch.manual_seed(4)
+    m = TritonMoEMLP(cfg).to(device).to(torch.bfloat16)
+    with torch.no_grad():
+        m.router.weight.normal_(0, 0.1)
+    q = m.quantize_experts(group_size=64)
+    w1, w2 = q.dequantize()
+    x = normal(81, 1, 24, 256).to(device)
+    out, sel, _ = m.few_tokens(x, experts=q, return_routing=True)
+    assert not torch.equal(out, m.few_tokens(x))
+    f = copy.deepcopy(m)
+    with torch.no_grad():
+        f.w1.copy_(w1)
+        f.w2.copy_(w2)
+    near = f.few_tokens(x)
+    # bf16(value) is off by 2^-8 in each of two products, twice in relu^2
+    assert ((near.double() - out.double()).abs().max() <= 16 * U16 * out.double().abs().max())
+    # the first product alone: matvec_q4's bits are those of the plain product's bound
+    up = K.matvec_q4(x.view(24, 256), q.w1, sel)
+    v = q.w1.dequantize(torch.float32).cpu().to(D)
+    off = [sum(m.expert_widths[:i]) for i in range(8)]
+    for t in range(24):
+        for s in range(2):
+            e = int(sel[t, s])
+            cols = slice(off[e], off[e] + m.expert_widths[e])
+            xt = x.view(24, 256)[t].cpu().to(D)
+            ref, mag = xt @ v[:, cols], xt.abs() @ v[:, cols].abs()
+            hold(up[t, s, :m.expert_widths[e]], ref, U16 * ref.abs() + 264 * U32 * mag)
+    twin = copy.deepcopy(q)
+    assert torch.equal(m.few_tokens(x, experts=twin), out)
+    assert torch.equal(m.few_tokens(x, experts=pickle.loads(pickle.dumps(q))), out)
+    with pytest.raises(ValueError, match="widths"):
+        m.few_tokens(x, experts=K.quantize_experts(w1, w2, [96] * 8))

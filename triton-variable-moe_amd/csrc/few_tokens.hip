@@ -1,0 +1,872 @@
+// The expert layer for a few tokens (a generation step): router logits, choice
+// of experts, up and down projection and weighted sum, for bf16, fp32 and 4-bit
+// weights, and the products of rows with 4-bit matrices.
+//
+// With T tokens of k experts each, an expert gets T k / E rows: far fewer than
+// a matrix instruction's 16 or, at best, a few times that. Every weight of a
+// chosen expert is then used a handful of times, so what bounds the layer is
+// reading those weights once, and with one or two tokens the chain of dependent
+// launches. The kernels are built for that:
+//
+// - No token is moved and no row is padded: a workgroup takes one expert and a
+//   tile of its columns, finds the rows that chose the expert, and gathers them
+//   as the 16-row operand of the matrix instructions.
+// - Weights go from memory to registers, each exactly once, straight into
+//   operand form. A lane's operand is 8 values of one column that are 8 rows
+//   apart in memory; the lane loads 8 rows of CPL adjacent columns and forms
+//   CPL operands by byte permutes, no LDS between. The sum over k may run in any
+//   order as long as both operands agree, so lane group g takes rows 8 g..8 g + 7
+//   of each 32. 4-bit matrices are stored in operand order (few_q4.h).
+// - The waves of a workgroup split K; their partial sums meet in LDS in a fixed
+//   order, so results do not change from run to run.
+// - The router's choice needs no sort: expert e is chosen by a token if fewer
+//   than k experts precede it (larger logit, or an equal one of lower index), and
+//   that count is its place.
+//
+// Sums, logits, routing weights and the activation are fp32. The activations h
+// enter the second product as two bf16 halves, h = hi + lo to 2^-17: the matrix
+// instructions are far from their limit, and one bf16 rounding of h would add as
+// much error as the output's own.
+#include <algorithm>
+
+#include "few_q4.h"
+
+namespace vmoe {
+namespace {
+
+constexpr int kThreads = 512, kWaves = kThreads / kWave;
+constexpr int kMaxTokens = 256, kMaxRows = 4096, kMaxExperts = 2048, kMaxTopK = 64;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+struct Ids {
+  const void* p;  // nullptr: row r takes matrix 0
+  int is64;
+};
+
+__device__ __forceinline__ int load_id(const Ids& s, int i, int E) {
+  if (!s.p) return 0;
+  if (s.is64) {
+    const int64_t v = static_cast<const int64_t*>(s.p)[i];
+    return v >= 0 && v < E ? (int)v : -1;
+  }
+  const int32_t v = static_cast<const int32_t*>(s.p)[i];
+  return v >= 0 && v < E ? v : -1;
+}
+
+// Total order of the logits as unsigned integers: NaN above everything, as
+// torch.topk orders it; -0 and 0 equal.
+__device__ __forceinline__ uint32_t sort_key(float f) {
+  if (f != f) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(f == 0.0f ? 0.0f : f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ float sigmoid_f32(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// ---------------------------------------------------------------------------
+// Weight formats. A step is KS rows of K; a wave's tile is NC = 16 C columns.
+// load() brings one lane's part of a step, mma() multiplies it with 16 rows.
+// ---------------------------------------------------------------------------
+
+// bf16, row-major. CPL columns a lane: 16, 8 or 4 bytes of each row.
+template <int CPL>
+struct WBf16 {
+  static constexpr int KS = 32, C = CPL, NC = 16 * CPL;
+  using V = typename std::conditional<CPL == 8, u32x4,
+                                      typename std::conditional<CPL == 4, u32x2, uint32_t>::type>::type;
+  using Row = uint16_t;
+  struct A {
+    bf16x8_t v;
+  };
+  V r[8];
+
+  __device__ __forceinline__ static int col(int c, int lane) { return (lane & 15) * CPL + c; }
+
+  __device__ __forceinline__ void load(const Stack& w, int64_t row0, int64_t col0, int, int k0,
+                                       int K, int n0, int N, int lane) {
+    const int k = k0 + (lane >> 4) * 8, n = n0 + (lane & 15) * CPL;
+    if (k < K && n < N) {
+      const uint16_t* p = static_cast<const uint16_t*>(w.w) + (row0 + k) * w.ld + col0 + n;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const V*>(p + j * w.ld);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = V{};
+    }
+  }
+
+  __device__ __forceinline__ static void load_a(A& a, const Row* row, int k0, int K, int lane) {
+    const int k = k0 + (lane >> 4) * 8;
+    if (k < K)
+      a.v = *reinterpret_cast<const bf16x8_t*>(row + k);
+    else
+      a.v = bf16x8_t{};
+  }
+
+  // Operand of column c: the c-th value of each of the 8 rows.
+  __device__ __forceinline__ bf16x8_t operand(int c) const {
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(r);
+    constexpr int D = CPL / 2;  // dwords of a row
+    const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = __builtin_amdgcn_perm(q[(2 * i + 1) * D + c / 2], q[2 * i * D + c / 2], sel);
+    return __builtin_bit_cast(bf16x8_t, v);
+  }
+
+  template <int MT, int PL>
+  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles, f32x4_t (&acc)[MT][C]) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const bf16x8_t b = operand(c);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m > 0 && m >= tiles) break;
+#pragma unroll
+        for (int q = 0; q < PL; ++q)
+          acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m][q].v, b, acc[m][c], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// fp32, row-major: four columns a lane and 16 rows a step, lane group g taking
+// rows 4 g..4 g + 3.
+struct WF32 {
+  static constexpr int KS = 16, C = 4, NC = 64;
+  using Row = float;
+  struct A {
+    f32x4_t v;
+  };
+  f32x4_t r[4];
+
+  __device__ __forceinline__ static int col(int c, int lane) { return (lane & 15) * 4 + c; }
+
+  __device__ __forceinline__ void load(const Stack& w, int64_t row0, int64_t col0, int, int k0,
+                                       int K, int n0, int N, int lane) {
+    const int k = k0 + (lane >> 4) * 4, n = n0 + (lane & 15) * 4;
+    if (k < K && n < N) {
+      const float* p = static_cast<const float*>(w.w) + (row0 + k) * w.ld + col0 + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const f32x4_t*>(p + j * w.ld);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = f32x4_t{};
+    }
+  }
+
+  __device__ __forceinline__ static void load_a(A& a, const Row* row, int k0, int K, int lane) {
+    const int k = k0 + (lane >> 4) * 4;
+    if (k < K)
+      a.v = *reinterpret_cast<const f32x4_t*>(row + k);
+    else
+      a.v = f32x4_t{};
+  }
+
+  template <int MT, int PL>
+  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles, f32x4_t (&acc)[MT][C]) const {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m > 0 && m >= tiles) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[m][0].v[j], r[j][c], acc[m][c], 0, 0, 0);
+    }
+  }
+};
+
+// 4-bit, in operand order (few_q4.h): 16 bytes a lane are its column's values of
+// 128 rows, four operands. GJ: operands that share a scale (group = 32 GJ). The
+// values are exact in bf16; a group's fp32 sum is scaled once.
+template <int CB, int GJ>
+struct WQ4 {
+  static constexpr int KS = kQ4Rows, C = CB, NC = 16 * CB, S = 4 / GJ;
+  using Row = uint16_t;
+  struct A {
+    bf16x8_t v[4];
+  };
+  u32x4 r[CB];
+  uint16_t s[CB][S];
+
+  __device__ __forceinline__ static int col(int c, int lane) { return c * 16 + (lane & 15); }
+
+  __device__ __forceinline__ void load(const Stack& w, int64_t, int64_t, int base, int k0, int K,
+                                       int n0, int N, int lane) {
+    const int kb = k0 / KS, kbs = (K + KS - 1) / KS;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      const int nb = n0 / 16 + c;
+      if (nb * 16 < N && kb < kbs) {
+        const int64_t blk = base + (int64_t)nb * kbs + kb;
+        r[c] = static_cast<const u32x4*>(w.w)[blk * kWave + lane];
+        const uint16_t* p = w.scales + (blk * 16 + (lane & 15)) * S;
+        if constexpr (S == 4) {
+          const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+          s[c][0] = (uint16_t)v[0], s[c][1] = (uint16_t)(v[0] >> 16);
+          s[c][2] = (uint16_t)v[1], s[c][3] = (uint16_t)(v[1] >> 16);
+        } else if constexpr (S == 2) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+          s[c][0] = (uint16_t)v, s[c][1] = (uint16_t)(v >> 16);
+        } else {
+          s[c][0] = *p;
+        }
+      } else {
+        r[c] = u32x4{};
+#pragma unroll
+        for (int i = 0; i < S; ++i) s[c][i] = 0;
+      }
+    }
+  }
+
+  __device__ __forceinline__ static void load_a(A& a, const Row* row, int k0, int K, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + 32 * j + (lane >> 4) * 8;
+      if (k < K)
+        a.v[j] = *reinterpret_cast<const bf16x8_t*>(row + k);
+      else
+        a.v[j] = bf16x8_t{};
+    }
+  }
+
+  template <int MT, int PL>
+  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles, f32x4_t (&acc)[MT][C]) const {
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int g = 0; g < S; ++g) {
+        bf16x8_t b[GJ];
+#pragma unroll
+        for (int j = 0; j < GJ; ++j) b[j] = q4_values(r[c][g * GJ + j]);
+        const float scale = bf16_to_f32(s[c][g]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (m > 0 && m >= tiles) break;
+          f32x4_t part = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < GJ; ++j)
+#pragma unroll
+            for (int q = 0; q < PL; ++q)
+              part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m][q].v[g * GJ + j], b[j], part, 0,
+                                                             0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][c][i] = fmaf(scale, part[i], acc[m][c][i]);
+        }
+      }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// One expert's rows times its matrix
+// ---------------------------------------------------------------------------
+
+enum Mode { kUp, kDown, kPlain };
+
+struct FewArgs {
+  Stack w;
+  const MatEntry* tab;
+  const void* a;  // rows of x (kUp, kPlain) or h (kDown)
+  int64_t lda, lo;  // row stride; distance of the second half (kDown)
+  int T, k, E;
+  const float* logits;  // kUp: [T, E], or nullptr: ids
+  Ids ids;
+  int32_t* sel;  // kUp with logits: chosen experts and their sigmoids, [T, k]
+  float* prob;
+  int fixed;  // kUp, kPlain: K of every matrix; kDown: N
+  int cols;   // columns of the widest matrix
+  int tiles;  // its column tiles
+  int wk;     // waves that split K; kWaves / wk split the tile's columns
+  int act;
+  void* out;  // h, y (fp32) or the products
+  int64_t ldo;
+};
+
+// The assignments t k + s that take expert e, into LDS; their number. Their
+// order does not matter: each is a row of its own.
+__device__ __forceinline__ int find_rows(const FewArgs& p, int e, bool writer, uint16_t* rows,
+                                         int* count) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  if (p.logits) {
+    for (int t = wave; t < p.T; t += kWaves) {
+      const float* l = p.logits + (int64_t)t * p.E;
+      const float mine = l[e];
+      const uint32_t key = sort_key(mine);
+      int before = 0;
+      for (int f = lane; f < p.E; f += kWave) {
+        const uint32_t other = sort_key(l[f]);
+        before += other > key || (other == key && f < e);
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, kWave);
+      if (before < p.k && lane == 0) {
+        const int a = t * p.k + before;
+        rows[atomicAdd(count, 1)] = (uint16_t)a;
+        if (writer) {
+          p.sel[a] = e;
+          p.prob[a] = sigmoid_f32(mine);
+        }
+      }
+    }
+  } else {
+    for (int a = threadIdx.x; a < p.T * p.k; a += kThreads)
+      if (load_id(p.ids, a, p.E) == (e < p.E ? e : -1))
+        rows[atomicAdd(count, 1)] = (uint16_t)a;
+  }
+  __syncthreads();
+  return *count;
+}
+
+// Workgroup -> (expert, tile): an XCD (blockIdx % 8) takes a contiguous eighth,
+// so the tiles of an expert share its rows and lines in one L2.
+__device__ __forceinline__ int unit_of_block(int units) {
+  const int per = (units + 7) / 8;
+  const int j = blockIdx.x >> 3, u = (blockIdx.x & 7) * per + j;
+  return j < per && u < units ? u : -1;
+}
+
+template <class W, int MODE, int MT, int NS>
+__global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
+  constexpr int PL = (MODE == kDown && sizeof(typename W::Row) == 2) ? 2 : 1;
+  constexpr int NC = W::NC;
+  __shared__ float red[NS * 16 * kWaves * NC];  // [NS][wk][16][width]
+  __shared__ uint16_t rows[kMaxRows];
+  __shared__ int count;
+  // kPlain: one matrix more, for the rows that name none (their products are 0)
+  const int unit = unit_of_block((p.E + (MODE == kPlain ? 1 : 0)) * p.tiles);
+  if (unit < 0) return;
+  const int e = unit / p.tiles, tile = unit % p.tiles;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wn_count = kWaves / p.wk;
+  const int wk = wave / wn_count, wn = wave % wn_count;
+  const int width = wn_count * NC;  // columns of the workgroup, a power of two
+  const int shift = __builtin_ctz(width);
+  const MatEntry mat = MODE == kPlain && e == p.E ? MatEntry{} : p.tab[e * NS];
+  const int K = MODE == kDown ? mat.len : p.fixed;
+  const int N = MODE == kDown ? p.fixed : min(mat.len, p.cols);
+  const int nt = tile * width;  // the tile's first column
+  // (the first tile's workgroup also writes the router's choice)
+  if (MODE != kPlain && nt >= N && !(tile == 0 && p.logits)) return;
+  const int m = find_rows(p, e, tile == 0, rows, &count);
+  if (m == 0) return;
+  if constexpr (MODE == kPlain) {
+    // zeros in the columns of wider matrices than this one
+    const int z0 = max(nt, N), zw = min(nt + width, p.cols) - z0;
+    for (int x = threadIdx.x; x < m * zw; x += kThreads)
+      static_cast<uint16_t*>(p.out)[rows[x / zw] * p.ldo + z0 + x % zw] = 0;
+  }
+  if (nt >= N) return;
+  const int n0 = nt + wn * NC;
+
+  int64_t row0[NS], col0[NS];
+  int base[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const MatEntry t = p.tab[e * NS + s];
+    row0[s] = MODE == kDown ? t.off : 0;
+    col0[s] = MODE == kDown ? 0 : t.off;
+    base[s] = t.base;
+  }
+
+  for (int m0 = 0; m0 < m; m0 += 16 * MT) {
+    const int tiles = min(MT, (m - m0 + 15) / 16);
+    const typename W::Row* arow[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      // rows past the last repeat it; their results are not stored
+      const int r = rows[min(m0 + 16 * i + (lane & 15), m - 1)];
+      const int64_t src = MODE == kDown ? r : r / p.k;
+      arow[i] = static_cast<const typename W::Row*>(p.a) + src * p.lda;
+    }
+    f32x4_t acc[NS][MT][W::C];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int c = 0; c < W::C; ++c) acc[s][i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+    for (int k0 = wk * W::KS; k0 < K; k0 += p.wk * W::KS) {
+      W b[NS];
+      typename W::A a[MT][PL];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) b[s].load(p.w, row0[s], col0[s], base[s], k0, K, n0, N, lane);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (i > 0 && i >= tiles) break;
+        W::load_a(a[i][0], arow[i], k0, K, lane);
+        if constexpr (PL == 2) W::load_a(a[i][1], arow[i] + p.lo, k0, K, lane);
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) b[s].mma(a, tiles, acc[s]);
+    }
+
+    // join the waves' parts, one 16-row tile at a time
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (i > 0 && i >= tiles) break;
+      const int left = min(16, m - m0 - 16 * i);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int c = 0; c < W::C; ++c)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            red[((s * p.wk + wk) * 16 + (lane >> 4) * 4 + q) * width + wn * NC +
+                W::col(c, lane)] = acc[s][i][c][q];
+      __syncthreads();
+      for (int x = threadIdx.x; x < left * width; x += kThreads) {
+        const int r = x >> shift, n = nt + (x & (width - 1));
+        if (n >= N) continue;
+        float z[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          z[s] = 0.0f;
+          for (int v = 0; v < p.wk; ++v) z[s] += red[(s * p.wk + v) * 16 * width + x];
+        }
+        const int64_t at = (int64_t)rows[m0 + 16 * i + r] * p.ldo + n;
+        if constexpr (MODE == kUp) {
+          float h;
+          if constexpr (NS == 2) {
+            h = z[0] * sigmoid_f32(z[0]) * z[1];
+          } else {
+            h = z[0] > 0.0f || z[0] != z[0] ? z[0] * z[0] : 0.0f;
+          }
+          if constexpr (sizeof(typename W::Row) == 2) {
+            // a finite h past bf16's largest value keeps that as its first half
+            uint32_t hi = f32_to_bf16(h);
+            const bool finite = (__float_as_uint(h) & 0x7F800000u) != 0x7F800000u;
+            if (finite && (hi & 0x7FFFu) == 0x7F80u) --hi;
+            const uint32_t lo = finite ? f32_to_bf16(h - bf16_to_f32(hi)) : 0u;
+            static_cast<uint16_t*>(p.out)[at] = (uint16_t)hi;
+            static_cast<uint16_t*>(p.out)[at + p.lo] = (uint16_t)lo;
+          } else {
+            static_cast<float*>(p.out)[at] = h;
+          }
+        } else if constexpr (MODE == kDown) {
+          static_cast<float*>(p.out)[at] = z[0];
+        } else {
+          static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16(z[0]);
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+
+// ---------------------------------------------------------------------------
+// Router logits: 16 tokens x 16 experts a workgroup, its waves split the hidden
+// axis. fp32 sums of exact products, not rounded.
+// ---------------------------------------------------------------------------
+
+template <bool F32>
+__global__ __launch_bounds__(kThreads) void few_logits_kernel(const void* x, int64_t ldx, int T,
+                                                              const void* wr, int64_t ldwr, int E,
+                                                              int d, float* logits) {
+  __shared__ float red[kWaves][16][16];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int t0 = blockIdx.y * 16, e0 = blockIdx.x * 16;
+  const int64_t ra = (int64_t)min(t0 + (lane & 15), T - 1) * ldx;
+  const int64_t rb = (int64_t)min(e0 + (lane & 15), E - 1) * ldwr;
+  constexpr int KS = F32 ? 16 : 32, PER = F32 ? 4 : 8;
+  f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int k0 = wave * KS; k0 < d; k0 += kWaves * KS) {
+    const int k = k0 + (lane >> 4) * PER;
+    if constexpr (F32) {
+      f32x4_t a = {}, b = {};
+      if (k < d) {
+        a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(x) + ra + k);
+        b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(wr) + rb + k);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+    } else {
+      bf16x8_t a = {}, b = {};
+      if (k < d) {
+        a = *reinterpret_cast<const bf16x8_t*>(static_cast<const uint16_t*>(x) + ra + k);
+        b = *reinterpret_cast<const bf16x8_t*>(static_cast<const uint16_t*>(wr) + rb + k);
+      }
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) red[wave][(lane >> 4) * 4 + q][lane & 15] = acc[q];
+  __syncthreads();
+  if (threadIdx.x < 256) {
+    const int t = t0 + threadIdx.x / 16, e = e0 + threadIdx.x % 16;
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) s += red[v][threadIdx.x / 16][threadIdx.x % 16];
+    if (t < T && e < E) logits[(int64_t)t * E + e] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// out[t] = sum_s weight[t, s] y[t k + s] over the slots that name an expert.
+// Weights: the layer's sigmoids (normalised over the token's slots if asked) or
+// the caller's.
+// ---------------------------------------------------------------------------
+
+struct CombineArgs {
+  const float* y;
+  int T, k, E, d;
+  Ids ids;
+  const void* weights;
+  int wbf16, normalize;
+  void* out;
+  int64_t ldo;
+  int out_f32;
+  int32_t* sel_out;  // nullptr, or where the layer's choice goes
+  float* wts_out;
+};
+
+constexpr int kCombineThreads = 128;
+
+__global__ __launch_bounds__(kCombineThreads) void few_combine_kernel(CombineArgs p) {
+  __shared__ float w[kMaxTopK];
+  __shared__ int id[kMaxTopK];
+  const int t = blockIdx.y;
+  if (threadIdx.x < kMaxTopK) {
+    const int s = threadIdx.x;
+    float v = 0.0f;
+    int e = -1;
+    if (s < p.k) {
+      const int a = t * p.k + s;
+      e = load_id(p.ids, a, p.E);
+      v = p.wbf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.weights)[a])
+                  : static_cast<const float*>(p.weights)[a];
+    }
+    id[s] = e;
+    w[s] = v;
+    if (p.normalize) {
+      float sum = v;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+      w[s] = v / (sum + 1e-20f);
+    }
+    if (blockIdx.x == 0 && s < p.k) {
+      if (p.sel_out) p.sel_out[t * p.k + s] = e;
+      if (p.wts_out) p.wts_out[t * p.k + s] = w[s];
+    }
+  }
+  __syncthreads();
+  const int n = (blockIdx.x * kCombineThreads + threadIdx.x) * 4;
+  if (n >= p.d) return;
+  f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* y = p.y + (int64_t)t * p.k * p.d + n;
+#pragma unroll 4
+  for (int s = 0; s < p.k; ++s) {
+    if (id[s] < 0) continue;
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(y + (int64_t)s * p.d);
+    const float f = w[s];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+  }
+  if (p.out_f32) {
+    *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + t * p.ldo + n) = acc;
+  } else {
+    u32x2 v = {pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + t * p.ldo + n) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <class W, int MODE, int MT, int NS>
+int launch(FewArgs p, hipStream_t stream) {
+  const int width = kWaves / p.wk * W::NC;
+  p.tiles = div_up(p.cols, width);
+  const int64_t units = (int64_t)(p.E + (MODE == kPlain ? 1 : 0)) * p.tiles;
+  if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
+  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS>), dim3(div_up(units, 8) * 8), dim3(kThreads), 0, stream,
+              p);
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+
+// Waves that split K, `steps` steps long for the longest matrix.
+int split_waves(int64_t steps) {
+  int wk = 1;
+  while (wk < kWaves && wk < steps) wk *= 2;
+  return wk;
+}
+
+// Experts that get rows, at most.
+int64_t live_experts(const FewArgs& p) { return std::min<int64_t>(p.E, (int64_t)p.T * p.k); }
+
+template <int MODE, int NS>
+int launch_bf16(FewArgs p, hipStream_t stream) {
+  p.wk = kWaves;
+  const int64_t live = live_experts(p);
+  if constexpr (NS == 1)
+    if (live * div_up(p.cols, 128) >= 256) return launch<WBf16<8>, MODE, 2, NS>(p, stream);
+  if (live * div_up(p.cols, 64) >= 256) return launch<WBf16<4>, MODE, 2, NS>(p, stream);
+  return launch<WBf16<2>, MODE, 2, NS>(p, stream);
+}
+
+template <int MODE, int NS>
+int launch_q4(FewArgs p, int group, int64_t max_k, hipStream_t stream) {
+  p.wk = split_waves(div_up(max_k, kQ4Rows));
+  switch (group) {
+    case 32: return launch<WQ4<2, 1>, MODE, 2, NS>(p, stream);
+    case 64: return launch<WQ4<2, 2>, MODE, 2, NS>(p, stream);
+    default: return launch<WQ4<2, 4>, MODE, 2, NS>(p, stream);
+  }
+}
+
+template <int MODE, int NS>
+int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t stream) {
+  if (format == VMOE_FEW_Q4) return launch_q4<MODE, NS>(p, group, max_k, stream);
+  if constexpr (MODE != kPlain) {
+    if (format == VMOE_FEW_BF16) return launch_bf16<MODE, NS>(p, stream);
+    p.wk = kWaves;
+    return launch<WF32, MODE, 2, NS>(p, stream);
+  }
+  return VMOE_ERR_UNSUPPORTED;
+}
+
+struct FewLayout {
+  int64_t logits, prob, sel, h, y, bytes, ldh;
+};
+
+bool few_layout(int64_t T, int64_t E, int64_t k, int64_t d, int64_t w, int format, FewLayout& L) {
+  if (T < 0 || E <= 0 || k <= 0 || d <= 0 || w <= 0 || format < 0 || format > VMOE_FEW_Q4)
+    return false;
+  const int64_t A = T * k;
+  int64_t off = 0;
+  auto slot = [&](int64_t bytes) {
+    const int64_t o = off;
+    off += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  L.ldh = (w + 7) / 8 * 8;
+  L.logits = slot(4 * T * E);
+  L.prob = slot(4 * A);
+  L.sel = slot(4 * A);
+  L.h = slot(4 * A * L.ldh);  // fp32, or two bf16 halves
+  L.y = slot(4 * A * d);
+  L.bytes = std::max<int64_t>(off, 256);
+  return true;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_sizes(int64_t T, int64_t E, int64_t k) {
+  if (T < 0 || E <= 0 || k <= 0) return VMOE_ERR_INVALID_ARG;
+  if (T > kMaxTokens || T * k > kMaxRows || E > kMaxExperts || k > kMaxTopK)
+    return VMOE_ERR_UNSUPPORTED;
+  return VMOE_OK;
+}
+
+int check_weights(const vmoe_few_weights* w) {
+  if (!w || w->num_experts <= 0 || w->hidden <= 0 || w->max_width <= 0 || w->format < 0 ||
+      w->format > VMOE_FEW_Q4)
+    return VMOE_ERR_INVALID_ARG;
+  if (w->act != VMOE_ACT_RELU_SQUARED && w->act != VMOE_ACT_SWIGLU) return VMOE_ERR_INVALID_ARG;
+  if (!w->w1 || !w->w2 || !w->table1 || !w->table2) return VMOE_ERR_INVALID_ARG;
+  const int64_t per = w->format == VMOE_FEW_F32 ? 4 : 8;
+  if (w->hidden % per || w->max_width % per || w->hidden > (1 << 28) || w->max_width > (1 << 28))
+    return VMOE_ERR_UNSUPPORTED;
+  if (!aligned16(w->w1) || !aligned16(w->w2) || !aligned16(w->table1) || !aligned16(w->table2))
+    return VMOE_ERR_UNSUPPORTED;
+  if (w->format == VMOE_FEW_Q4) {
+    if (!w->scales1 || !w->scales2) return VMOE_ERR_INVALID_ARG;
+    if (w->group != 32 && w->group != 64 && w->group != 128) return VMOE_ERR_INVALID_ARG;
+    if (!aligned16(w->scales1) || !aligned16(w->scales2)) return VMOE_ERR_UNSUPPORTED;
+  } else {
+    if (w->ldw1 <= 0 || w->ldw2 < w->hidden) return VMOE_ERR_INVALID_ARG;
+    if (w->ldw1 % per || w->ldw2 % per) return VMOE_ERR_UNSUPPORTED;
+  }
+  return VMOE_OK;
+}
+
+int check_rows(const void* x, int64_t ldx, int64_t cols, const void* out, int64_t ldo,
+               int64_t ocols, int64_t per) {
+  if (!x || !out || ldx < cols || ldo < ocols) return VMOE_ERR_INVALID_ARG;
+  if (ldx % per || ldo % per || !aligned16(x) || !aligned16(out)) return VMOE_ERR_UNSUPPORTED;
+  return VMOE_OK;
+}
+
+// Up, down and sum, the choice of experts being either logits or ids.
+int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, int T, int k,
+                const float* logits, Ids ids, const void* weights, int wbf16, int normalize,
+                int32_t* sel, float* prob, void* h, float* y, int64_t ldh, void* out, int64_t ldo,
+                int32_t* sel_out, float* wts_out, hipStream_t stream) {
+  FewArgs p = {};
+  p.w = {w.w1, w.scales1, w.ldw1};
+  p.tab = reinterpret_cast<const MatEntry*>(w.table1);
+  p.a = x;
+  p.lda = ldx;
+  p.T = T;
+  p.k = k;
+  p.E = w.num_experts;
+  p.logits = logits;
+  p.ids = ids;
+  p.sel = sel;
+  p.prob = prob;
+  p.fixed = (int)w.hidden;
+  p.cols = (int)w.max_width;
+  p.act = w.act;
+  p.out = h;
+  p.ldo = w.format == VMOE_FEW_F32 ? ldh : 2 * ldh;
+  p.lo = ldh;
+  int st = w.act == VMOE_ACT_SWIGLU
+               ? launch_format<kUp, 2>(p, w.format, w.group, w.hidden, stream)
+               : launch_format<kUp, 1>(p, w.format, w.group, w.hidden, stream);
+  if (st != VMOE_OK) return st;
+
+  p.w = {w.w2, w.scales2, w.ldw2};
+  p.tab = reinterpret_cast<const MatEntry*>(w.table2);
+  p.a = h;
+  p.lda = p.ldo;
+  p.logits = nullptr;
+  p.ids = ids;
+  p.cols = p.fixed = (int)w.hidden;
+  p.out = y;
+  p.ldo = w.hidden;
+  st = launch_format<kDown, 1>(p, w.format, w.group, w.max_width, stream);
+  if (st != VMOE_OK) return st;
+
+  CombineArgs c = {};
+  c.y = y;
+  c.T = T;
+  c.k = k;
+  c.E = w.num_experts;
+  c.d = (int)w.hidden;
+  c.ids = ids;
+  c.weights = weights;
+  c.wbf16 = wbf16;
+  c.normalize = normalize;
+  c.out = out;
+  c.ldo = ldo;
+  c.out_f32 = w.format == VMOE_FEW_F32;
+  c.sel_out = sel_out;
+  c.wts_out = wts_out;
+  VMOE_LAUNCH(few_combine_kernel, dim3(div_up(w.hidden, 4 * kCombineThreads), T),
+              dim3(kCombineThreads), 0, stream, c);
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+
+}  // namespace
+}  // namespace vmoe
+
+using namespace vmoe;
+
+extern "C" int vmoe_few_max_tokens(void) { return kMaxTokens; }
+
+extern "C" size_t vmoe_few_workspace_bytes(int64_t T, int32_t E, int32_t k, int64_t hidden,
+                                           int64_t max_width, int32_t format) {
+  FewLayout L;
+  return few_layout(T, E, k, hidden, max_width, format, L) ? (size_t)L.bytes : 0;
+}
+
+extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t ldx,
+                              int64_t num_tokens, const void* router_weight, int64_t ldwr,
+                              int32_t top_k, int32_t normalize, void* out, int64_t ldo,
+                              int32_t* selected, float* weights, void* workspace,
+                              size_t workspace_bytes, vmoe_stream_t stream) {
+  int st = check_weights(w);
+  if (st != VMOE_OK) return st;
+  st = check_sizes(num_tokens, w->num_experts, top_k);
+  if (st != VMOE_OK) return st;
+  if (top_k > w->num_experts) return VMOE_ERR_INVALID_ARG;
+  if (num_tokens == 0) return VMOE_OK;
+  const bool f32 = w->format == VMOE_FEW_F32;
+  st = check_rows(x, ldx, w->hidden, out, ldo, w->hidden, f32 ? 4 : 8);
+  if (st != VMOE_OK) return st;
+  if (!router_weight || ldwr < w->hidden || !workspace) return VMOE_ERR_INVALID_ARG;
+  if (ldwr % (f32 ? 4 : 8) || !aligned16(router_weight) || !aligned16(workspace))
+    return VMOE_ERR_UNSUPPORTED;
+  FewLayout L;
+  if (!few_layout(num_tokens, w->num_experts, top_k, w->hidden, w->max_width, w->format, L))
+    return VMOE_ERR_INVALID_ARG;
+  if (workspace_bytes < (size_t)L.bytes) return VMOE_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  float* logits = reinterpret_cast<float*>(ws + L.logits);
+  const int T = (int)num_tokens, E = w->num_experts;
+  const dim3 grid(div_up(E, 16), div_up(T, 16));
+  if (f32)
+    VMOE_LAUNCH((few_logits_kernel<true>), grid, dim3(kThreads), 0, stream, x, ldx, T,
+                router_weight, ldwr, E, (int)w->hidden, logits);
+  else
+    VMOE_LAUNCH((few_logits_kernel<false>), grid, dim3(kThreads), 0, stream, x, ldx, T,
+                router_weight, ldwr, E, (int)w->hidden, logits);
+  VMOE_CHECK_LAUNCH();
+  int32_t* sel = reinterpret_cast<int32_t*>(ws + L.sel);
+  float* prob = reinterpret_cast<float*>(ws + L.prob);
+  return few_experts(*w, x, ldx, T, top_k, logits, Ids{sel, 0}, prob, 0, normalize != 0, sel,
+                     prob, ws + L.h, reinterpret_cast<float*>(ws + L.y), L.ldh, out, ldo,
+                     selected, weights, stream);
+}
+
+extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_t ldx,
+                                int64_t num_tokens, const void* ids, int32_t ids_are_i64,
+                                const void* weights, int32_t weights_are_bf16, int32_t top_k,
+                                void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                                vmoe_stream_t stream) {
+  int st = check_weights(w);
+  if (st != VMOE_OK) return st;
+  st = check_sizes(num_tokens, w->num_experts, top_k);
+  if (st != VMOE_OK) return st;
+  if (num_tokens == 0) return VMOE_OK;
+  st = check_rows(x, ldx, w->hidden, out, ldo, w->hidden, w->format == VMOE_FEW_F32 ? 4 : 8);
+  if (st != VMOE_OK) return st;
+  if (!ids || !weights || !workspace) return VMOE_ERR_INVALID_ARG;
+  if (!aligned16(workspace)) return VMOE_ERR_UNSUPPORTED;
+  FewLayout L;
+  if (!few_layout(num_tokens, w->num_experts, top_k, w->hidden, w->max_width, w->format, L))
+    return VMOE_ERR_INVALID_ARG;
+  if (workspace_bytes < (size_t)L.bytes) return VMOE_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  return few_experts(*w, x, ldx, (int)num_tokens, top_k, nullptr, Ids{ids, ids_are_i64}, weights,
+                     weights_are_bf16, 0, nullptr, nullptr, ws + L.h,
+                     reinterpret_cast<float*>(ws + L.y), L.ldh, out, ldo, nullptr, nullptr,
+                     stream);
+}
+
+extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids,
+                              int32_t ids_are_i64, int32_t per_row, const void* codes,
+                              const uint16_t* scales, const int32_t* table, int32_t num_matrices,
+                              int64_t k_rows, int64_t max_cols, int32_t group, void* y,
+                              int64_t ldy, vmoe_stream_t stream) {
+  int st = check_sizes(num_rows, num_matrices, per_row);
+  if (st != VMOE_OK) return st;
+  if (k_rows <= 0 || max_cols <= 0 || !codes || !scales || !table) return VMOE_ERR_INVALID_ARG;
+  if (group != 32 && group != 64 && group != 128) return VMOE_ERR_INVALID_ARG;
+  if (!ids && (num_matrices != 1 || per_row != 1)) return VMOE_ERR_INVALID_ARG;
+  if (num_rows == 0) return VMOE_OK;
+  if (k_rows % 8 || max_cols % 8 || k_rows > (1 << 28) || max_cols > (1 << 28) ||
+      !aligned16(codes) || !aligned16(scales) || !aligned16(table))
+    return VMOE_ERR_UNSUPPORTED;
+  st = check_rows(x, ldx, k_rows, y, ldy, max_cols, 8);
+  if (st != VMOE_OK) return st;
+  FewArgs p = {};
+  p.w = {codes, scales, 0};
+  p.tab = reinterpret_cast<const MatEntry*>(table);
+  p.a = x;
+  p.lda = ldx;
+  p.T = (int)num_rows;
+  p.k = per_row;
+  p.E = num_matrices;
+  p.ids = {ids, ids_are_i64};
+  p.fixed = (int)k_rows;
+  p.cols = (int)max_cols;
+  p.out = y;
+  p.ldo = ldy;
+  return launch_q4<kPlain, 1>(p, group, k_rows, stream);
+}

@@ -132,6 +132,16 @@ _SIGNATURES = {
                             _vp],
     "vmoe_router_weight_bwd": [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _i64,
                                _vp],
+    "vmoe_few_max_tokens": [],
+    "vmoe_few_workspace_bytes": [_i64, _i32, _i32, _i64, _i64, _i32],
+    "vmoe_few_layer": [_vp, _vp, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp, _vp, _vp,
+                       ctypes.c_size_t, _vp],
+    "vmoe_few_experts": [_vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _vp, _i64, _vp,
+                         ctypes.c_size_t, _vp],
+    "vmoe_q4_quantize": [_vp, _i32, _i64, _vp, _i32, _i32, _i64, _i64, _i32, _vp, _vp, _vp],
+    "vmoe_q4_dequantize": [_vp, _vp, _vp, _i32, _i32, _i64, _i64, _i32, _vp, _i32, _i64, _vp],
+    "vmoe_q4_matvec": [_vp, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _i64, _i32,
+                       _vp, _i64, _vp],
 }
 _RESTYPES = {
     "vmoe_status_string": ctypes.c_char_p,
@@ -141,12 +151,14 @@ _RESTYPES = {
     "vmoe_gemm_dw_workspace_zero_bytes": ctypes.c_size_t,
     "vmoe_router_partial_floats": ctypes.c_size_t,
     "vmoe_router_linear_bwd_workspace_bytes": ctypes.c_size_t,
+    "vmoe_few_workspace_bytes": ctypes.c_size_t,
 }
 
 # Status codes (include/vmoe.h).
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_WORKSPACE = 0, 1, 2, 3, 4
 ROUNDING = {"up": 0, "down": 1, "nearest": 2}
 ACT_NONE, ACT_RELU_SQUARED, ACT_SWIGLU = 0, 1, 2
+FEW_BF16, FEW_F32, FEW_Q4 = 0, 1, 2  # enum vmoe_few_format
 INFO_ROWS, INFO_KEPT, INFO_ERRORS, INFO_LEN = 0, 1, 2, 4
 # Slots of vmoe_expert_layout's saved buffer (enum vmoe_expert_slot).
 (X_BIN_IDS, X_INDICES, X_TPE, X_BINS, X_PADDED_BINS, X_ROW_SRC, X_GATHER_MAP, X_ASSIGNMENT_ROW,

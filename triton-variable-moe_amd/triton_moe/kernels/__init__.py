@@ -1,5 +1,6 @@
-"""gfx950 HIP kernel implementations of the MoE operations (same export
-surface as triton_moe/kernels/__init__.py:18-40 of the reference)."""
+"""gfx950 HIP kernel implementations of the MoE operations (the
+export surface of triton_moe/kernels/__init__.py:18-40 of the reference, and the
+operators for a few tokens, which it lacks)."""
 
 from .gather import padded_gather, padded_gather_autograd
 from .scatter import padded_scatter, padded_scatter_autograd
@@ -15,6 +16,18 @@ from .grouped_gemm import (
     GroupedGemmDown,
 )
 from .fused_cumsum import fused_route
+from .few_tokens import (
+    FewTokenExperts,
+    QuantizedExperts,
+    QuantizedMatrices,
+    experts_few_tokens,
+    few_token_experts,
+    few_tokens_max,
+    matvec_q4,
+    moe_few_tokens,
+    quantize_experts,
+    quantize_matrices,
+)
 
 __all__ = [
     # Gather/Scatter
@@ -38,4 +51,15 @@ __all__ = [
     "GroupedGemmDown",
     # Routing
     "fused_route",
+    # Few tokens (generation): bf16, fp32 and 4-bit expert weights
+    "few_token_experts",
+    "quantize_experts",
+    "quantize_matrices",
+    "moe_few_tokens",
+    "experts_few_tokens",
+    "matvec_q4",
+    "few_tokens_max",
+    "FewTokenExperts",
+    "QuantizedExperts",
+    "QuantizedMatrices",
 ]

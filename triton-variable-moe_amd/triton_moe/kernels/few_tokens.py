@@ -1,0 +1,445 @@
+"""The expert layer for a few tokens (a generation step), in bf16, fp32 or with
+4-bit expert weights, and products of rows with 4-bit matrices
+(csrc/few_tokens.hip, csrc/few_q4.hip). Inference only: nothing here records
+gradients. The reference has no counterpart; its layer pads each expert's rows
+to a block (triton_moe/moe.py:148-250).
+
+A program keeps a handle of its weights, made once:
+
+    experts = few_token_experts(w1, w2, widths)             # the weights themselves
+    experts = quantize_experts(w1, w2, widths)              # a 4-bit copy
+    out = moe_few_tokens(x, router_weight, experts, top_k)  # the whole layer
+    out = experts_few_tokens(x, selected, weights, experts)  # with a router of one's own
+
+and, for a single matrix or a stack of them,
+
+    q = quantize_matrices(w)
+    y = matvec_q4(x, q)                                     # x @ w, w in 4 bits
+
+Calls take 1 to few_tokens_max() tokens, run on the current stream of x's
+device without a host sync, allocate their output and workspace from torch's
+allocator, and can be captured into a graph.
+
+A 4-bit value is 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign, times a bf16 scale
+that a group of 32, 64 or 128 values of a column shares along the summed axis.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+
+_ACT = {"relu_squared": _lib.ACT_RELU_SQUARED, "swiglu": _lib.ACT_SWIGLU}
+_GROUPS = (32, 64, 128)
+_MAX_PAIRS, _MAX_TOP_K, _MAX_EXPERTS = 4096, 64, 2048
+_Q4_ROWS, _Q4_COLS, _Q4_BLOCK = 128, 16, 1024
+
+
+def few_tokens_max() -> int:
+    """The most tokens (rows of x) a call takes."""
+    return int(_lib.lib().vmoe_few_max_tokens())
+
+
+def _widths_of(widths) -> list[int]:
+    if isinstance(widths, torch.Tensor):
+        widths = widths.tolist()
+    widths = [int(w) for w in widths]
+    if not widths or min(widths) <= 0:
+        raise ValueError("expert_widths must hold at least one width, all positive")
+    return widths
+
+
+def _weight(w: torch.Tensor, what: str, dtypes, mult: int) -> torch.Tensor:
+    """A weight matrix as the kernels read it: on the GPU, rows contiguous,
+    aligned and a multiple of 16 bytes apart. Not copied: a handle's weights are
+    the caller's."""
+    _lib.require_gpu(w, what)
+    if w.dim() != 2:
+        raise ValueError(f"{what} must have two dimensions (got {w.dim()})")
+    if w.dtype not in dtypes:
+        raise NotImplementedError(f"{what} must be one of {dtypes} (got {w.dtype})")
+    if w.stride(1) != 1 or w.stride(0) % mult or w.data_ptr() % 16:
+        raise NotImplementedError(f"{what} must have contiguous 16-byte aligned rows")
+    return w
+
+
+def _entries(lengths: list[int], blocks: list[int], device) -> torch.Tensor:
+    """int32 [matrices, 4]: start, length, first 4-bit block, 0."""
+    rows, off, base = [], 0, 0
+    for n, b in zip(lengths, blocks):
+        rows.append([off, n, base, 0])
+        off, base = off + n, base + b
+    if off >= 2 ** 31 or base >= 2 ** 31:
+        raise NotImplementedError("the matrices are too many or too long")
+    return torch.tensor(rows, dtype=torch.int32, device=device)
+
+
+class _FewWeights(ctypes.Structure):
+    """struct vmoe_few_weights."""
+
+    _fields_ = [("format", ctypes.c_int32), ("group", ctypes.c_int32), ("act", ctypes.c_int32),
+                ("num_experts", ctypes.c_int32), ("hidden", ctypes.c_int64),
+                ("max_width", ctypes.c_int64), ("w1", ctypes.c_void_p),
+                ("scales1", ctypes.c_void_p), ("ldw1", ctypes.c_int64),
+                ("table1", ctypes.c_void_p), ("w2", ctypes.c_void_p),
+                ("scales2", ctypes.c_void_p), ("ldw2", ctypes.c_int64),
+                ("table2", ctypes.c_void_p)]
+
+
+class _Experts:
+    """What the two kinds of expert handles share."""
+
+    def _init_common(self, fmt, group, activation, widths, hidden, dtype, device):
+        self.expert_widths = widths
+        self.num_experts = len(widths)
+        self.hidden = hidden
+        self.activation = activation
+        self.dtype = dtype  # of x and out
+        self.device = device
+        self._max_width = max(widths)
+        self._format = fmt
+        self._group = group
+        self._desc = None  # made by the first call, and again after a copy
+        self._bytes: dict = {}  # (tokens, top_k) -> workspace bytes
+
+    def __getstate__(self):
+        return {**self.__dict__, "_desc": None, "_desc_ptr": None}
+
+    def _new_desc(self) -> _FewWeights:
+        self._desc = _FewWeights(self._format, self._group, _ACT[self.activation],
+                                 self.num_experts, self.hidden, self._max_width)
+        self._desc_ptr = ctypes.addressof(self._desc)
+        return self._desc
+
+    def _workspace_bytes(self, T: int, k: int) -> int:
+        n = self._bytes.get((T, k))
+        if n is None:
+            n = self._bytes[(T, k)] = int(_lib.lib().vmoe_few_workspace_bytes(
+                T, self.num_experts, k, self.hidden, self._max_width, self._format))
+        return n
+
+
+def _check_layer(w1, w2, widths, activation):
+    if activation not in _ACT:
+        raise ValueError(f"Unknown activation: {activation} "
+                         f"(expected one of {sorted(_ACT)})")
+    glu = 2 if activation == "swiglu" else 1
+    d, W = w1.shape[0], sum(widths)
+    if w1.shape[1] != glu * W:
+        raise ValueError(f"w1 must have {glu * W} columns for these widths (got {w1.shape[1]})")
+    if w2.shape != (W, d):
+        raise ValueError(f"w2 must be [{W}, {d}] (got {tuple(w2.shape)})")
+    if w1.device != w2.device:
+        raise ValueError("w1 and w2 must be on one device")
+    if w1.dtype != w2.dtype:
+        raise ValueError(f"w1 and w2 must have one type (got {w1.dtype} and {w2.dtype})")
+    return glu, d
+
+
+class FewTokenExperts(_Experts):
+    """Handle of bf16 or fp32 expert weights: few_token_experts."""
+
+    def __init__(self, w1, w2, expert_widths, activation="relu_squared"):
+        f32 = w1.dtype == torch.float32
+        mult = 4 if f32 else 8
+        types = (torch.bfloat16, torch.float32)
+        self.w1, self.w2 = (_weight(w, n, types, mult) for w, n in ((w1, "w1"), (w2, "w2")))
+        widths = _widths_of(expert_widths)
+        glu, d = _check_layer(w1, w2, widths, activation)
+        if d % mult or any(w % mult for w in widths):
+            raise NotImplementedError(f"hidden size and widths must be multiples of {mult} "
+                                      f"for {w1.dtype} weights")
+        self._init_common(_lib.FEW_F32 if f32 else _lib.FEW_BF16, 0, activation, widths, d,
+                          w1.dtype, w1.device)
+        each = [w for w in widths for _ in range(glu)]
+        self._t1 = _entries(each, [0] * len(each), w1.device)
+        self._t2 = _entries(widths, [0] * len(widths), w1.device)
+        self._at = None
+
+    def _weights(self) -> int:
+        """Address of the description; where the weights' storage has moved
+        since the last call (module.to, .data assigned), it is read anew."""
+        a, b = self.w1, self.w2
+        at = (a.data_ptr(), b.data_ptr())
+        if self._desc is None or at != self._at:
+            mult = 4 if self._format == _lib.FEW_F32 else 8
+            for w, n in ((a, "w1"), (b, "w2")):
+                _weight(w, n, (self.dtype,), mult)
+                if w.device != self.device:
+                    raise ValueError(f"{n} has moved to {w.device}: make a new handle")
+            if a.shape[0] != self.hidden or b.shape[1] != self.hidden:
+                raise ValueError("w1 or w2 has another shape now: make a new handle")
+            q = self._new_desc()
+            q.w1, q.w2, q.ldw1, q.ldw2 = at[0], at[1], a.stride(0), b.stride(0)
+            q.table1, q.table2 = self._t1.data_ptr(), self._t2.data_ptr()
+            self._at = at
+        return self._desc_ptr
+
+
+def few_token_experts(w1, w2, expert_widths, activation="relu_squared") -> FewTokenExperts:
+    """Handle of expert weights for moe_few_tokens and experts_few_tokens.
+
+    w1 [hidden, sum(widths)] holds the experts side by side ("swiglu":
+    [hidden, 2 sum(widths)], gate and up of an expert next to each other), w2
+    [sum(widths), hidden] on top of each other; bf16 or fp32, widths and hidden
+    size multiples of 8 (fp32: 4). expert_widths: a list of ints or a tensor
+    (read back once). The handle refers to w1 and w2 and sees their updates."""
+    return FewTokenExperts(w1, w2, expert_widths, activation)
+
+
+class QuantizedMatrices:
+    """A stack of 4-bit matrices in the kernels' order: quantize_matrices."""
+
+    def __init__(self, w, lengths, stacked: str, group_size: int):
+        if stacked not in ("columns", "rows"):
+            raise ValueError(f"stacked must be 'columns' or 'rows' (got {stacked!r})")
+        if group_size not in _GROUPS:
+            raise ValueError(f"group_size must be one of {_GROUPS} (got {group_size})")
+        _weight(w, "w", (torch.bfloat16, torch.float32), 1)
+        by_rows = stacked == "rows"
+        fixed, total = (w.shape[1], w.shape[0]) if by_rows else (w.shape[0], w.shape[1])
+        lengths = [total] if lengths is None else _widths_of(lengths)
+        if sum(lengths) != total:
+            raise ValueError(f"lengths must add up to the matrix's {total} {stacked}")
+        if fixed % 8 or any(n % 8 for n in lengths):
+            raise NotImplementedError("matrix sizes must be multiples of 8")
+        if len(lengths) > 65535:
+            raise NotImplementedError("at most 65535 matrices")
+        self.lengths, self.stacked, self.group_size = lengths, stacked, group_size
+        self.fixed, self.total, self.max_len = fixed, total, max(lengths)
+        self.device = w.device
+
+        def blocks(n):
+            k, c = (n, fixed) if by_rows else (fixed, n)
+            return -(-k // _Q4_ROWS) * -(-c // _Q4_COLS)
+
+        per = [blocks(n) for n in lengths]
+        self._table = _entries(lengths, per, w.device)
+        count = sum(per)
+        with torch.cuda.device(w.device):
+            self.codes = torch.empty(count * _Q4_BLOCK, dtype=torch.uint8, device=w.device)
+            self.scales = torch.empty(count, _Q4_COLS, _Q4_ROWS // group_size,
+                                      dtype=torch.bfloat16, device=w.device)
+            _lib.call("vmoe_q4_quantize", w.data_ptr(), int(w.dtype == torch.float32),
+                      w.stride(0), self._table.data_ptr(), len(lengths), int(by_rows), fixed,
+                      self.max_len, group_size, self.codes.data_ptr(), self.scales.data_ptr(),
+                      _lib.stream(w.device))
+
+    def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
+        """The values, row-major: float32 exactly, bfloat16 rounded once."""
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise NotImplementedError(f"dequantize to bfloat16 or float32 (got {dtype})")
+        by_rows = self.stacked == "rows"
+        shape = (self.total, self.fixed) if by_rows else (self.fixed, self.total)
+        with torch.cuda.device(self.device):
+            out = torch.empty(shape, dtype=dtype, device=self.device)
+            _lib.call("vmoe_q4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(),
+                      self._table.data_ptr(), len(self.lengths), int(by_rows), self.fixed,
+                      self.max_len, self.group_size, out.data_ptr(), int(dtype == torch.float32),
+                      out.stride(0), _lib.stream(self.device))
+        return out
+
+
+def quantize_matrices(w, lengths=None, stacked="columns", group_size=32) -> QuantizedMatrices:
+    """A 4-bit copy of w [rows, columns] (bf16 or fp32): one matrix, or several
+    of `lengths` columns side by side (stacked="columns") or `lengths` rows on
+    top of each other ("rows"), grouped along the rows of each. Sizes are
+    multiples of 8; a matrix's last group may be short. The scale is
+    bf16(max |w| / 6), values the nearest, ties to the even place; a group that
+    holds an infinity or NaN stands for NaN."""
+    return QuantizedMatrices(w, lengths, stacked, group_size)
+
+
+class QuantizedExperts(_Experts):
+    """Handle of 4-bit expert weights: quantize_experts."""
+
+    def __init__(self, w1, w2, expert_widths, activation="relu_squared", group_size=32):
+        widths = _widths_of(expert_widths)
+        for w, n in ((w1, "w1"), (w2, "w2")):
+            _weight(w, n, (torch.bfloat16, torch.float32), 1)
+        glu, d = _check_layer(w1, w2, widths, activation)
+        self.w1 = quantize_matrices(w1, [w for w in widths for _ in range(glu)], "columns",
+                                    group_size)
+        self.w2 = quantize_matrices(w2, widths, "rows", group_size)
+        self.group_size = group_size
+        self._init_common(_lib.FEW_Q4, group_size, activation, widths, d, torch.bfloat16,
+                          w1.device)
+
+    def _weights(self) -> int:
+        if self._desc is None:
+            q = self._new_desc()
+            q.w1, q.scales1 = self.w1.codes.data_ptr(), self.w1.scales.data_ptr()
+            q.w2, q.scales2 = self.w2.codes.data_ptr(), self.w2.scales.data_ptr()
+            q.table1, q.table2 = self.w1._table.data_ptr(), self.w2._table.data_ptr()
+        return self._desc_ptr
+
+    def dequantize(self, dtype=torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """(w1, w2) that the 4-bit values stand for, as quantize_experts took them."""
+        return self.w1.dequantize(dtype), self.w2.dequantize(dtype)
+
+
+def quantize_experts(w1, w2, expert_widths, activation="relu_squared",
+                     group_size=32) -> QuantizedExperts:
+    """A 4-bit copy of expert weights (layout as few_token_experts; bf16 or
+    fp32) for moe_few_tokens and experts_few_tokens on bf16 activations. The
+    copy does not follow later updates of w1 and w2."""
+    return QuantizedExperts(w1, w2, expert_widths, activation, group_size)
+
+
+def _rows(x: torch.Tensor, width: int, dtype, device, what: str) -> torch.Tensor:
+    """x as rows of `width` values that the kernels can read (copied if they
+    are not contiguous or not 16-byte aligned)."""
+    _lib.require_gpu(x, what)
+    if x.dim() < 1 or x.shape[-1] != width:
+        raise ValueError(f"{what} must have {width} values in its last dimension "
+                         f"(got {tuple(x.shape)})")
+    if x.dtype != dtype:
+        raise NotImplementedError(f"{what} must be {dtype} with these weights (got {x.dtype})")
+    if x.device != device:
+        raise ValueError(f"{what} is on {x.device}, the weights on {device}")
+    if x.dim() != 2:
+        x = x.reshape(-1, width)
+    mult = 4 if dtype == torch.float32 else 8
+    if (x.stride(1) != 1 or x.stride(0) % mult or x.data_ptr() % 16 or
+            (x.shape[0] > 1 and x.stride(0) < width)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _check_count(T: int, k: int, what: str) -> None:
+    if k > _MAX_TOP_K:
+        raise NotImplementedError(f"{what} takes at most {_MAX_TOP_K} experts a token (got {k})")
+    if T > few_tokens_max() or T * k > _MAX_PAIRS:
+        raise NotImplementedError(
+            f"{what} takes at most {few_tokens_max()} tokens and {_MAX_PAIRS} token-expert pairs "
+            f"(got {T} x {k}); larger batches are the layer's own forward's")
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    # (the stride of a single row is arbitrary)
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True,
+                   return_routing: bool = False):
+    """The whole layer for a few tokens: router, top_k experts of each token,
+    their weighted sum.
+
+    x [..., hidden] in the handle's type, router_weight [num_experts, hidden] in
+    the same type. Logits are fp32 and not rounded; the top_k largest are taken
+    (equal ones: the lowest index; NaN above all), with weights sigmoid(logit),
+    divided by their sum + 1e-20 if normalize. Returns out like x, and with
+    return_routing also the chosen experts int32 [tokens, top_k] (largest logit
+    first) and their fp32 weights. (TritonMoEMLP.forward rounds its logits to
+    bf16, so that near ties may fall differently there.)"""
+    d = experts.hidden
+    rows = _rows(x, d, experts.dtype, experts.device, "x")
+    T = rows.shape[0]
+    k = int(top_k)
+    E = experts.num_experts
+    if not 1 <= k <= E:
+        raise ValueError(f"top_k must be between 1 and {E} (got {top_k})")
+    _check_count(T, k, "moe_few_tokens")
+    if router_weight.shape != (E, d):
+        raise ValueError(f"router_weight must be [{E}, {d}] (got {tuple(router_weight.shape)})")
+    wr = _rows(router_weight, d, experts.dtype, experts.device, "router_weight")
+    dev = x.device
+    n = experts._workspace_bytes(T, k)
+    with torch.cuda.device(dev):
+        out = torch.empty((T, d), dtype=experts.dtype, device=dev)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        sel = wts = None
+        if return_routing:
+            sel = torch.empty((T, k), dtype=torch.int32, device=dev)
+            wts = torch.empty((T, k), dtype=torch.float32, device=dev)
+        _lib.call("vmoe_few_layer", experts._weights(), rows.data_ptr(), _row_stride(rows), T,
+                  wr.data_ptr(), _row_stride(wr), k, int(bool(normalize)), out.data_ptr(), d,
+                  _lib.ptr(sel), _lib.ptr(wts), ws.data_ptr(), n, _lib.stream(dev))
+    out = out.view(x.shape)
+    return (out, sel, wts) if return_routing else out
+
+
+def experts_few_tokens(x, selected, weights, experts):
+    """The experts' part of the layer for given choices: out[t] = sum_s
+    weights[t, s] expert_{selected[t, s]}(x[t]).
+
+    x [..., hidden] in the handle's type; selected [..., k] int32 or int64 and
+    weights [..., k] bf16 or fp32, a row for each of x. An id outside
+    0..num_experts-1 (say -1, for the padding of a batch) is no expert: a token
+    without any gets zeros. An expert named twice counts twice."""
+    d = experts.hidden
+    rows = _rows(x, d, experts.dtype, experts.device, "x")
+    T = rows.shape[0]
+    ids, k = _ids(selected, T, experts.device, "selected")
+    if weights.shape != selected.shape:
+        raise ValueError(f"weights must have the shape of selected, {tuple(selected.shape)} "
+                         f"(got {tuple(weights.shape)})")
+    if weights.dtype not in (torch.bfloat16, torch.float32):
+        raise NotImplementedError(f"weights must be bfloat16 or float32 (got {weights.dtype})")
+    if weights.device != experts.device:
+        raise ValueError(f"weights are on {weights.device}, the experts on {experts.device}")
+    _check_count(T, k, "experts_few_tokens")
+    wts = weights if weights.is_contiguous() else weights.contiguous()
+    dev = x.device
+    n = experts._workspace_bytes(T, k)
+    with torch.cuda.device(dev):
+        out = torch.empty((T, d), dtype=experts.dtype, device=dev)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _lib.call("vmoe_few_experts", experts._weights(), rows.data_ptr(), _row_stride(rows), T,
+                  ids.data_ptr(), int(ids.dtype == torch.int64), wts.data_ptr(),
+                  int(wts.dtype == torch.bfloat16), k, out.data_ptr(), d, ws.data_ptr(), n,
+                  _lib.stream(dev))
+    return out.view(x.shape)
+
+
+def _ids(ids, T: int, device, what: str):
+    """(contiguous ids, ids a row)."""
+    _lib.require_gpu(ids, what)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} must be int32 or int64 (got {ids.dtype})")
+    if ids.dim() < 1 or ids.shape[-1] < 1 or ids.numel() != T * ids.shape[-1]:
+        raise ValueError(f"{what} must have a row of at least one id for each of {T} rows of x "
+                         f"(got {tuple(ids.shape)})")
+    if ids.device != device:
+        raise ValueError(f"{what} is on {ids.device}, the weights on {device}")
+    return (ids if ids.is_contiguous() else ids.contiguous()), ids.shape[-1]
+
+
+def matvec_q4(x, q: QuantizedMatrices, ids=None):
+    """Products of a few rows with 4-bit matrices.
+
+    Without ids, q is one matrix [K, N] and y = x @ q, [..., N] for x [..., K].
+    With ids [..., k] (int32 or int64, a row for each of x), q's matrices are
+    side by side (stacked="columns") and y[..., s, :] = x @ q_{ids[..., s]},
+    [..., k, max N]; columns past a matrix's own and rows whose id names no
+    matrix are zeros. bf16, fp32 sums rounded once."""
+    if q.stacked != "columns":
+        raise NotImplementedError("matvec_q4 takes matrices that are side by side "
+                                  "(stacked='columns')")
+    K, N = q.fixed, q.max_len
+    rows = _rows(x, K, torch.bfloat16, q.device, "x")
+    T = rows.shape[0]
+    if ids is None:
+        if len(q.lengths) != 1:
+            raise ValueError(f"q holds {len(q.lengths)} matrices: ids must say which")
+        k, shape = 1, (*x.shape[:-1], N)
+    else:
+        if ids.shape[:-1] != x.shape[:-1]:
+            raise ValueError(f"ids must have a row for each of x: {tuple(x.shape[:-1])} "
+                             f"(got {tuple(ids.shape)})")
+        ids, k = _ids(ids, T, q.device, "ids")
+        shape = (*x.shape[:-1], k, N)
+    if len(q.lengths) > _MAX_EXPERTS:
+        raise NotImplementedError(f"matvec_q4 takes at most {_MAX_EXPERTS} matrices")
+    _check_count(T, k, "matvec_q4")
+    dev = x.device
+    with torch.cuda.device(dev):
+        y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        _lib.call("vmoe_q4_matvec", rows.data_ptr(), _row_stride(rows), T, _lib.ptr(ids),
+                  int(ids is not None and ids.dtype == torch.int64), k, q.codes.data_ptr(),
+                  q.scales.data_ptr(), q._table.data_ptr(), len(q.lengths), K, N, q.group_size,
+                  y.data_ptr(), N, _lib.stream(dev))
+    return y

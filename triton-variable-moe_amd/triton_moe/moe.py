@@ -18,6 +18,7 @@ device.
 
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass, field
 from typing import Any
 
@@ -36,6 +37,7 @@ from .kernels import (
 from . import _lib
 from .kernels.fused_cumsum import route_device
 from .kernels.gather import combine_rows
+from .kernels import few_tokens as ft
 from .kernels import grouped_gemm as gg
 from .kernels.grouped_gemm import (CompactRoutedMoEOp, ExpertPathOp, GemmMeta, MoELayerOp,
                                    MoELayerOpF32, MoERouterLayerOp, NoTokensOp,
@@ -48,6 +50,10 @@ from .kernels.router import (RouterAuxOp, RouterLinear, RouterWeightOp, router_b
 # Whether hooks on every module's call are registered (not public API: without
 # it the router keeps its own call).
 _has_global_hook = getattr(nn.modules.module, "_has_any_global_hook", lambda: True)
+
+# Each module's handle for few_tokens(), apart from the module: copying or
+# pickling a module does not meet it.
+_FEW_HANDLES = weakref.WeakKeyDictionary()
 
 
 @dataclass
@@ -367,6 +373,36 @@ class TritonMoEMLP(nn.Module):
         output = output_flat.view(batch_size, seq_len, n_embd)
         aux_loss, f_i = self._aux(router_logits, state, tokens_per_expert, x.dtype)
         return output, aux_loss, f_i
+
+    # ------------------------------------------------------------------
+    # a generation step (not in the reference)
+    # ------------------------------------------------------------------
+
+    @torch.no_grad()
+    def few_tokens(self, x: torch.Tensor, experts=None, return_routing: bool = False):
+        """The layer's output for a few tokens, for inference: x [..., n_embd],
+        at most few_tokens_max() tokens, without auxiliary losses or gradients
+        (kernels.moe_few_tokens on this module's weights). experts: a handle
+        from quantize_experts() for 4-bit expert weights. The router's logits
+        are not rounded to bf16 as forward()'s are, so near ties between experts
+        may fall differently; the router's weight is used as it is, without the
+        router module's hooks."""
+        if experts is None:
+            experts = _FEW_HANDLES.get(self)
+            if experts is None or experts.w1 is not self.w1 or experts.w2 is not self.w2 or \
+                    experts.device != self.w1.device or experts.dtype != self.w1.dtype:
+                experts = ft.few_token_experts(self.w1, self.w2, self.expert_widths)
+                _FEW_HANDLES[self] = experts
+        elif experts.expert_widths != self.expert_widths:
+            raise ValueError("experts is a handle of other expert widths than this layer's")
+        return ft.moe_few_tokens(x, self.router.weight, experts, self.num_active_experts,
+                                 self.norm_topk_prob, return_routing)
+
+    @torch.no_grad()
+    def quantize_experts(self, group_size: int = 32):
+        """A 4-bit copy of the expert weights, for few_tokens(x, experts=...):
+        kernels.quantize_experts. It does not follow later updates."""
+        return ft.quantize_experts(self.w1, self.w2, self.expert_widths, group_size=group_size)
 
     def forward_with_intermediates(self, x: torch.Tensor) -> dict[str, Any]:
         """Forward returning every intermediate (reference moe.py:305-409), exact shapes."""
