@@ -813,7 +813,8 @@ int vmoe_moe_f32_backward(const void* saved, const float* logits, int64_t num_to
  * block, 0. table1 has an entry for each expert (SwiGLU: two, gate and up),
  * table2 one. Activations and outputs are bf16 (fp32 for fp32 weights). hidden,
  * widths, starts and strides are multiples of 8 (fp32: 4), buffers 16-byte
- * aligned. Every size is given once: lengths are at most max_width.
+ * aligned; lengths are at most max_width, hidden, max_width and strides of the
+ * weights at most 2^24, x and the activations span less than 4 GiB.
  *
  * vmoe_few_layer: logits = x router_weight^T in fp32; the top_k largest (ties:
  * the lowest index; NaN above all), weights sigmoid(logit), over their sum +

@@ -65,17 +65,23 @@ __device__ __forceinline__ uint32_t sort_key(float f) {
 
 __device__ __forceinline__ float sigmoid_f32(float x) { return 1.0f / (1.0f + expf(-x)); }
 
+// *(base + off bytes): a base that is one for the wave and a 32-bit offset of the
+// lane, so that an address costs no vector registers.
+template <class V>
+__device__ __forceinline__ V at(const void* base, uint32_t off) {
+  return *reinterpret_cast<const V*>(static_cast<const char*>(base) + off);
+}
+
 // ---------------------------------------------------------------------------
 // Weight formats. A step is KS rows of K; a wave's tile is NC = 16 C columns.
 // load() brings one lane's part of a step, mma() multiplies it with 16 rows.
 // ---------------------------------------------------------------------------
 
-// bf16, row-major. CPL columns a lane: 16, 8 or 4 bytes of each row.
+// bf16, row-major. CPL columns a lane: 8 or 4 bytes of each row.
 template <int CPL>
 struct WBf16 {
   static constexpr int KS = 32, C = CPL, NC = 16 * CPL;
-  using V = typename std::conditional<CPL == 8, u32x4,
-                                      typename std::conditional<CPL == 4, u32x2, uint32_t>::type>::type;
+  using V = typename std::conditional<CPL == 4, u32x2, uint32_t>::type;
   using Row = uint16_t;
   struct A {
     bf16x8_t v;
@@ -84,25 +90,34 @@ struct WBf16 {
 
   __device__ __forceinline__ static int col(int c, int lane) { return (lane & 15) * CPL + c; }
 
-  __device__ __forceinline__ void load(const Stack& w, int64_t row0, int64_t col0, int, int k0,
-                                       int K, int n0, int N, int lane) {
-    const int k = k0 + (lane >> 4) * 8, n = n0 + (lane & 15) * CPL;
-    if (k < K && n < N) {
-      const uint16_t* p = static_cast<const uint16_t*>(w.w) + (row0 + k) * w.ld + col0 + n;
+  // A lane's offset in bytes from the step's first row and the matrix's first
+  // column. Columns past N read the last ones (not stored).
+  __device__ __forceinline__ static uint32_t lane_offset(const Stack& w, int n0, int N, int lane) {
+    const int n = min(n0 + (lane & 15) * CPL, N - CPL);
+    return ((uint32_t)(lane >> 4) * 8 * (uint32_t)w.ld + n) * 2;
+  }
+
+  // Rows past K are zero.
+  __device__ __forceinline__ void load(const Stack& w, const MatEntry& m, bool by_rows, int k0,
+                                       int K, int, int, uint32_t off, int lane) {
+    const uint16_t* p = static_cast<const uint16_t*>(w.w) +
+                        ((by_rows ? (int64_t)m.off : 0) + k0) * w.ld + (by_rows ? 0 : m.off);
+    if (k0 + KS <= K) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const V*>(p + j * w.ld);
+      for (int j = 0; j < 8; ++j) r[j] = at<V>(p + j * w.ld, off);
     } else {
+      const bool in = k0 + (lane >> 4) * 8 < K;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = V{};
+      for (int j = 0; j < 8; ++j) r[j] = in ? at<V>(p + j * w.ld, off) : V{};
     }
   }
 
-  __device__ __forceinline__ static void load_a(A& a, const Row* row, int k0, int K, int lane) {
-    const int k = k0 + (lane >> 4) * 8;
-    if (k < K)
-      a.v = *reinterpret_cast<const bf16x8_t*>(row + k);
+  __device__ __forceinline__ static void load_a(A& a, const Row* base, uint32_t off, int k0, int K,
+                                                int lane) {
+    if (k0 + KS <= K)
+      a.v = at<bf16x8_t>(base + k0, off);
     else
-      a.v = bf16x8_t{};
+      a.v = k0 + (lane >> 4) * 8 < K ? at<bf16x8_t>(base + k0, off) : bf16x8_t{};
   }
 
   // Operand of column c: the c-th value of each of the 8 rows.
@@ -145,25 +160,31 @@ struct WF32 {
 
   __device__ __forceinline__ static int col(int c, int lane) { return (lane & 15) * 4 + c; }
 
-  __device__ __forceinline__ void load(const Stack& w, int64_t row0, int64_t col0, int, int k0,
-                                       int K, int n0, int N, int lane) {
-    const int k = k0 + (lane >> 4) * 4, n = n0 + (lane & 15) * 4;
-    if (k < K && n < N) {
-      const float* p = static_cast<const float*>(w.w) + (row0 + k) * w.ld + col0 + n;
+  __device__ __forceinline__ static uint32_t lane_offset(const Stack& w, int n0, int N, int lane) {
+    const int n = min(n0 + (lane & 15) * 4, N - 4);
+    return ((uint32_t)(lane >> 4) * 4 * (uint32_t)w.ld + n) * 4;
+  }
+
+  __device__ __forceinline__ void load(const Stack& w, const MatEntry& m, bool by_rows, int k0,
+                                       int K, int, int, uint32_t off, int lane) {
+    const float* p = static_cast<const float*>(w.w) +
+                     ((by_rows ? (int64_t)m.off : 0) + k0) * w.ld + (by_rows ? 0 : m.off);
+    if (k0 + KS <= K) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const f32x4_t*>(p + j * w.ld);
+      for (int j = 0; j < 4; ++j) r[j] = at<f32x4_t>(p + j * w.ld, off);
     } else {
+      const bool in = k0 + (lane >> 4) * 4 < K;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = f32x4_t{};
+      for (int j = 0; j < 4; ++j) r[j] = in ? at<f32x4_t>(p + j * w.ld, off) : f32x4_t{};
     }
   }
 
-  __device__ __forceinline__ static void load_a(A& a, const Row* row, int k0, int K, int lane) {
-    const int k = k0 + (lane >> 4) * 4;
-    if (k < K)
-      a.v = *reinterpret_cast<const f32x4_t*>(row + k);
+  __device__ __forceinline__ static void load_a(A& a, const Row* base, uint32_t off, int k0, int K,
+                                                int lane) {
+    if (k0 + KS <= K)
+      a.v = at<f32x4_t>(base + k0, off);
     else
-      a.v = f32x4_t{};
+      a.v = k0 + (lane >> 4) * 4 < K ? at<f32x4_t>(base + k0, off) : f32x4_t{};
   }
 
   template <int MT, int PL>
@@ -191,46 +212,49 @@ struct WQ4 {
     bf16x8_t v[4];
   };
   u32x4 r[CB];
-  uint16_t s[CB][S];
+  using Scales = typename std::conditional<
+      S == 4, u32x2, typename std::conditional<S == 2, uint32_t, uint16_t>::type>::type;
+  Scales s[CB];
 
   __device__ __forceinline__ static int col(int c, int lane) { return c * 16 + (lane & 15); }
 
-  __device__ __forceinline__ void load(const Stack& w, int64_t, int64_t, int base, int k0, int K,
-                                       int n0, int N, int lane) {
+  __device__ __forceinline__ static uint32_t lane_offset(const Stack&, int, int, int lane) {
+    return lane * 16;
+  }
+
+  __device__ __forceinline__ void load(const Stack& w, const MatEntry& m, bool, int k0, int K,
+                                       int n0, int N, uint32_t off, int lane) {
     const int kb = k0 / KS, kbs = (K + KS - 1) / KS;
 #pragma unroll
     for (int c = 0; c < CB; ++c) {
-      const int nb = n0 / 16 + c;
-      if (nb * 16 < N && kb < kbs) {
-        const int64_t blk = base + (int64_t)nb * kbs + kb;
-        r[c] = static_cast<const u32x4*>(w.w)[blk * kWave + lane];
-        const uint16_t* p = w.scales + (blk * 16 + (lane & 15)) * S;
-        if constexpr (S == 4) {
-          const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-          s[c][0] = (uint16_t)v[0], s[c][1] = (uint16_t)(v[0] >> 16);
-          s[c][2] = (uint16_t)v[1], s[c][3] = (uint16_t)(v[1] >> 16);
-        } else if constexpr (S == 2) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
-          s[c][0] = (uint16_t)v, s[c][1] = (uint16_t)(v >> 16);
-        } else {
-          s[c][0] = *p;
-        }
-      } else {
-        r[c] = u32x4{};
-#pragma unroll
-        for (int i = 0; i < S; ++i) s[c][i] = 0;
-      }
+      // (blocks past the last column read that one; not stored)
+      const int nb = min(n0 / 16 + c, (N - 1) / 16);
+      const int64_t blk = m.base + (int64_t)nb * kbs + kb;
+      r[c] = at<u32x4>(static_cast<const char*>(w.w) + blk * kQ4BlockBytes, off);
+      s[c] = at<Scales>(w.scales + blk * 16 * S, (lane & 15) * S * 2);
     }
   }
 
-  __device__ __forceinline__ static void load_a(A& a, const Row* row, int k0, int K, int lane) {
+  // Scale of group g: the g-th 16 bits, as fp32.
+  __device__ __forceinline__ float scale(int c, int g) const {
+    if constexpr (S == 4) {
+      return (g & 1) ? hi_f32(s[c][g / 2]) : lo_f32(s[c][g / 2]);
+    } else if constexpr (S == 2) {
+      return g ? hi_f32(s[c]) : lo_f32(s[c]);
+    } else {
+      return bf16_to_f32(s[c]);
+    }
+  }
+
+  __device__ __forceinline__ static void load_a(A& a, const Row* base, uint32_t off, int k0, int K,
+                                                int lane) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int k = k0 + 32 * j + (lane >> 4) * 8;
-      if (k < K)
-        a.v[j] = *reinterpret_cast<const bf16x8_t*>(row + k);
+      const Row* p = base + k0 + 32 * j;
+      if (k0 + KS <= K)
+        a.v[j] = at<bf16x8_t>(p, off);
       else
-        a.v[j] = bf16x8_t{};
+        a.v[j] = k0 + 32 * j + (lane >> 4) * 8 < K ? at<bf16x8_t>(p, off) : bf16x8_t{};
     }
   }
 
@@ -243,7 +267,7 @@ struct WQ4 {
         bf16x8_t b[GJ];
 #pragma unroll
         for (int j = 0; j < GJ; ++j) b[j] = q4_values(r[c][g * GJ + j]);
-        const float scale = bf16_to_f32(s[c][g]);
+        const float f = scale(c, g);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           if (m > 0 && m >= tiles) break;
@@ -255,7 +279,7 @@ struct WQ4 {
               part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m][q].v[g * GJ + j], b[j], part, 0,
                                                              0, 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][c][i] = fmaf(scale, part[i], acc[m][c][i]);
+          for (int i = 0; i < 4; ++i) acc[m][c][i] = fmaf(f, part[i], acc[m][c][i]);
         }
       }
   }
@@ -273,7 +297,9 @@ struct FewArgs {
   const void* a;  // rows of x (kUp, kPlain) or h (kDown)
   int64_t lda, lo;  // row stride; distance of the second half (kDown)
   int T, k, E;
-  const float* logits;  // kUp: [T, E], or nullptr: ids
+  const float* logits;  // kUp: [T, ldl], or nullptr: ids
+  int ldl;
+  int early;  // load weights before the rows are known
   Ids ids;
   int32_t* sel;  // kUp with logits: chosen experts and their sigmoids, [T, k]
   float* prob;
@@ -286,26 +312,46 @@ struct FewArgs {
   int64_t ldo;
 };
 
+// Orders LDS accesses of the workgroup; global loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// How many experts of a token come before expert e, whose logit is `mine`:
+// eight lanes share the row (padded to kLogitPad with -inf), each gets the count.
+constexpr int kLogitPad = 32;
+__device__ __forceinline__ int place_of(const float* l, int ldl, int e, float mine, int part) {
+  const uint32_t key = sort_key(mine);
+  int before = 0;
+#pragma unroll 4
+  for (int f = part * 4; f < ldl; f += kLogitPad) {
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(l + f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t other = sort_key(v[i]);
+      before += other > key || (other == key && f + i < e);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) before += __shfl_xor(before, o, kWave);
+  return before;
+}
+
 // The assignments t k + s that take expert e, into LDS; their number. Their
 // order does not matter: each is a row of its own.
 __device__ __forceinline__ int find_rows(const FewArgs& p, int e, bool writer, uint16_t* rows,
                                          int* count) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   if (threadIdx.x == 0) *count = 0;
-  __syncthreads();
+  lds_barrier();
   if (p.logits) {
-    for (int t = wave; t < p.T; t += kWaves) {
-      const float* l = p.logits + (int64_t)t * p.E;
+    const int part = threadIdx.x & 7;
+    for (int t = threadIdx.x / 8; t < p.T; t += kThreads / 8) {
+      const float* l = p.logits + (int64_t)t * p.ldl;
       const float mine = l[e];
-      const uint32_t key = sort_key(mine);
-      int before = 0;
-      for (int f = lane; f < p.E; f += kWave) {
-        const uint32_t other = sort_key(l[f]);
-        before += other > key || (other == key && f < e);
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, kWave);
-      if (before < p.k && lane == 0) {
+      const int before = place_of(l, p.ldl, e, mine, part);
+      if (before < p.k && part == 0) {
         const int a = t * p.k + before;
         rows[atomicAdd(count, 1)] = (uint16_t)a;
         if (writer) {
@@ -319,8 +365,28 @@ __device__ __forceinline__ int find_rows(const FewArgs& p, int e, bool writer, u
       if (load_id(p.ids, a, p.E) == (e < p.E ? e : -1))
         rows[atomicAdd(count, 1)] = (uint16_t)a;
   }
-  __syncthreads();
+  lds_barrier();
   return *count;
+}
+
+// The expert of assignment a, or -1.
+__device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer, int* found) {
+  if (!p.logits) return __builtin_amdgcn_readfirstlane(load_id(p.ids, a, p.E));
+  const int part = threadIdx.x & 7, t = a / p.k, s = a % p.k;
+  const float* l = p.logits + (int64_t)t * p.ldl;
+  for (int e = threadIdx.x / 8; e < p.E; e += kThreads / 8) {
+    const float mine = l[e];
+    const int before = place_of(l, p.ldl, e, mine, part);
+    if (before == s && part == 0) {
+      *found = e;
+      if (writer) {
+        p.sel[a] = e;
+        p.prob[a] = sigmoid_f32(mine);
+      }
+    }
+  }
+  lds_barrier();
+  return *found;
 }
 
 // Workgroup -> (expert, tile): an XCD (blockIdx % 8) takes a contiguous eighth,
@@ -331,59 +397,85 @@ __device__ __forceinline__ int unit_of_block(int units) {
   return j < per && u < units ? u : -1;
 }
 
-template <class W, int MODE, int MT, int NS>
+// SLOT: a unit is an assignment and a tile (one row), else an expert and a tile.
+// DEPTH steps of a wave are in flight.
+template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
 __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
   constexpr int PL = (MODE == kDown && sizeof(typename W::Row) == 2) ? 2 : 1;
   constexpr int NC = W::NC;
-  __shared__ float red[NS * 16 * kWaves * NC];  // [NS][wk][16][width]
-  __shared__ uint16_t rows[kMaxRows];
+  constexpr int kPerLane = 16 / sizeof(typename W::Row);  // values of a 16-byte load
+  __shared__ float red[NS * 16 * kWaves * NC];            // [NS][wk][16][width]
+  __shared__ uint16_t rows[SLOT ? 8 : kMaxRows];
   __shared__ int count;
   // kPlain: one matrix more, for the rows that name none (their products are 0)
-  const int unit = unit_of_block((p.E + (MODE == kPlain ? 1 : 0)) * p.tiles);
+  const int owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
+  const int unit = unit_of_block(owners * p.tiles);
   if (unit < 0) return;
-  const int e = unit / p.tiles, tile = unit % p.tiles;
+  const int owner = unit / p.tiles, tile = unit % p.tiles;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wn_count = kWaves / p.wk;
   const int wk = wave / wn_count, wn = wave % wn_count;
   const int width = wn_count * NC;  // columns of the workgroup, a power of two
   const int shift = __builtin_ctz(width);
-  const MatEntry mat = MODE == kPlain && e == p.E ? MatEntry{} : p.tab[e * NS];
-  const int K = MODE == kDown ? mat.len : p.fixed;
-  const int N = MODE == kDown ? p.fixed : min(mat.len, p.cols);
   const int nt = tile * width;  // the tile's first column
-  // (the first tile's workgroup also writes the router's choice)
-  if (MODE != kPlain && nt >= N && !(tile == 0 && p.logits)) return;
-  const int m = find_rows(p, e, tile == 0, rows, &count);
-  if (m == 0) return;
-  if constexpr (MODE == kPlain) {
-    // zeros in the columns of wider matrices than this one
-    const int z0 = max(nt, N), zw = min(nt + width, p.cols) - z0;
-    for (int x = threadIdx.x; x < m * zw; x += kThreads)
-      static_cast<uint16_t*>(p.out)[rows[x / zw] * p.ldo + z0 + x % zw] = 0;
-  }
-  if (nt >= N) return;
   const int n0 = nt + wn * NC;
 
-  int64_t row0[NS], col0[NS];
-  int base[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const MatEntry t = p.tab[e * NS + s];
-    row0[s] = MODE == kDown ? t.off : 0;
-    col0[s] = MODE == kDown ? 0 : t.off;
-    base[s] = t.base;
+  int e = owner, m = 1;
+  if constexpr (SLOT) {
+    e = find_expert(p, owner, tile == 0, &count);
+    if (e < 0) return;
   }
+  MatEntry mats[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    mats[s] = MODE == kPlain && e == p.E ? MatEntry{} : p.tab[e * NS + s];
+  const int K = MODE == kDown ? mats[0].len : p.fixed;
+  const int N = MODE == kDown ? p.fixed : min(mats[0].len, p.cols);
+  // (the first tile's workgroup also writes the router's choice)
+  if (MODE != kPlain && nt >= N && (SLOT || tile > 0 || !p.logits)) return;
+
+  const uint32_t boff = W::lane_offset(p.w, n0, N, lane);
+  const int stride = p.wk * W::KS, first = wk * W::KS;
+  W b[DEPTH][NS];
+  auto load_b = [&](int d, int k0) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      b[d][s].load(p.w, mats[s], MODE == kDown, k0, K, n0, N, boff, lane);
+  };
+  // Where most experts have rows, the first weights are on their way before it
+  // is known which rows.
+  const bool early = !SLOT && p.early && nt < N;
+  if (early) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+      if (first + d * stride < K) load_b(d, first + d * stride);
+  }
+  if constexpr (SLOT) {
+    if (threadIdx.x == 0) rows[0] = (uint16_t)owner;
+    lds_barrier();
+  } else {
+    m = find_rows(p, e, tile == 0, rows, &count);
+    if (m == 0) return;
+    if constexpr (MODE == kPlain) {
+      // zeros in the columns of wider matrices than this one
+      const int z0 = max(nt, N), zw = min(nt + width, p.cols) - z0;
+      for (int x = threadIdx.x; x < m * zw; x += kThreads)
+        static_cast<uint16_t*>(p.out)[rows[x / zw] * p.ldo + z0 + x % zw] = 0;
+    }
+    if (nt >= N) return;
+  }
+  const typename W::Row* abase = static_cast<const typename W::Row*>(p.a);
 
   for (int m0 = 0; m0 < m; m0 += 16 * MT) {
     const int tiles = min(MT, (m - m0 + 15) / 16);
-    const typename W::Row* arow[MT];
+    uint32_t aoff[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       // rows past the last repeat it; their results are not stored
       const int r = rows[min(m0 + 16 * i + (lane & 15), m - 1)];
-      const int64_t src = MODE == kDown ? r : r / p.k;
-      arow[i] = static_cast<const typename W::Row*>(p.a) + src * p.lda;
+      const uint32_t src = MODE == kDown ? r : r / p.k;
+      aoff[i] = (src * (uint32_t)p.lda + (lane >> 4) * kPerLane) * sizeof(typename W::Row);
     }
     f32x4_t acc[NS][MT][W::C];
 #pragma unroll
@@ -393,19 +485,30 @@ __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
 #pragma unroll
         for (int c = 0; c < W::C; ++c) acc[s][i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (int k0 = wk * W::KS; k0 < K; k0 += p.wk * W::KS) {
-      W b[NS];
-      typename W::A a[MT][PL];
-#pragma unroll
-      for (int s = 0; s < NS; ++s) b[s].load(p.w, row0[s], col0[s], base[s], k0, K, n0, N, lane);
+    typename W::A a[DEPTH][MT][PL];
+    auto load_a = [&](int d, int k0) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         if (i > 0 && i >= tiles) break;
-        W::load_a(a[i][0], arow[i], k0, K, lane);
-        if constexpr (PL == 2) W::load_a(a[i][1], arow[i] + p.lo, k0, K, lane);
+        W::load_a(a[d][i][0], abase, aoff[i], k0, K, lane);
+        if constexpr (PL == 2) W::load_a(a[d][i][1], abase + p.lo, aoff[i], k0, K, lane);
       }
+    };
+    bool have = early && m0 == 0;
+    for (int k0 = first; k0 < K; k0 += DEPTH * stride) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s) b[s].mma(a, tiles, acc[s]);
+      for (int d = 0; d < DEPTH; ++d) {
+        if (k0 + d * stride >= K) break;
+        if (!have) load_b(d, k0 + d * stride);
+        load_a(d, k0 + d * stride);
+      }
+      have = false;
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        if (k0 + d * stride >= K) break;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) b[d][s].mma(a[d], tiles, acc[s]);
+      }
     }
 
     // join the waves' parts, one 16-row tile at a time
@@ -421,7 +524,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
           for (int q = 0; q < 4; ++q)
             red[((s * p.wk + wk) * 16 + (lane >> 4) * 4 + q) * width + wn * NC +
                 W::col(c, lane)] = acc[s][i][c][q];
-      __syncthreads();
+      lds_barrier();
       for (int x = threadIdx.x; x < left * width; x += kThreads) {
         const int r = x >> shift, n = nt + (x & (width - 1));
         if (n >= N) continue;
@@ -456,11 +559,183 @@ __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
           static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16(z[0]);
         }
       }
-      __syncthreads();
+      lds_barrier();
     }
   }
 }
 
+// ---------------------------------------------------------------------------
+// Weights of a token's slots: the layer's sigmoids (normalised over the slots if
+// asked) or the caller's.
+// ---------------------------------------------------------------------------
+
+struct SumArgs {
+  int T, k, E, d;
+  Ids ids;
+  const void* weights;
+  int wbf16, normalize;
+  void* out;
+  int64_t ldo;
+  int out_f32;
+  int32_t* sel_out;  // nullptr, or where the layer's choice goes
+  float* wts_out;
+};
+
+// By the first wave of a workgroup, into LDS.
+__device__ __forceinline__ void slot_weights(const SumArgs& p, int t, bool writer, int* id,
+                                             float* w) {
+  static_assert(kMaxTopK == kWave, "a slot per lane");
+  const int s = threadIdx.x;
+  float v = 0.0f;
+  int e = -1;
+  if (s < p.k) {
+    const int a = t * p.k + s;
+    e = load_id(p.ids, a, p.E);
+    v = p.wbf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.weights)[a])
+                : static_cast<const float*>(p.weights)[a];
+  }
+  if (p.normalize) {
+    float sum = v;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+    v = v / (sum + 1e-20f);
+  }
+  id[s] = e;
+  w[s] = v;
+  if (writer && s < p.k) {
+    if (p.sel_out) p.sel_out[t * p.k + s] = e;
+    if (p.wts_out) p.wts_out[t * p.k + s] = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// out[t] = sum_s weight[t, s] y[t k + s] over the slots that name an expert.
+// ---------------------------------------------------------------------------
+
+constexpr int kCombineThreads = 128;
+
+__global__ __launch_bounds__(kCombineThreads) void few_combine_kernel(SumArgs p, const float* y0) {
+  __shared__ float w[kMaxTopK];
+  __shared__ int id[kMaxTopK];
+  const int t = blockIdx.y;
+  if (threadIdx.x < kWave) slot_weights(p, t, blockIdx.x == 0, id, w);
+  lds_barrier();
+  const int n = (blockIdx.x * kCombineThreads + threadIdx.x) * 4;
+  if (n >= p.d) return;
+  f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* y = y0 + (int64_t)t * p.k * p.d + n;
+#pragma unroll 4
+  for (int s = 0; s < p.k; ++s) {
+    if (id[s] < 0) continue;
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(y + (int64_t)s * p.d);
+    const float f = w[s];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+  }
+  if (p.out_f32) {
+    *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + t * p.ldo + n) = acc;
+  } else {
+    u32x2 v = {pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + t * p.ldo + n) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Down projection and sum of one token: the experts of its slots one after the
+// other as a single long K, so that no partial result leaves the workgroup. For
+// calls with so few tokens that they share no weights.
+// ---------------------------------------------------------------------------
+
+constexpr int kTokenWaves = 16;
+
+template <class W, int DEPTH>
+__global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p, Stack w,
+                                                                      const MatEntry* tab,
+                                                                      const void* h, int64_t ldh,
+                                                                      int64_t lo, int tiles) {
+  using Row = typename W::Row;
+  constexpr int PL = sizeof(Row) == 2 ? 2 : 1;
+  __shared__ float red[kTokenWaves][W::NC];
+  __shared__ float wts[kMaxTopK];
+  __shared__ int id[kMaxTopK];
+  const int unit = unit_of_block(p.T * tiles);
+  if (unit < 0) return;
+  const int t = unit / tiles, tile = unit % tiles;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (wave == 0) slot_weights(p, t, tile == 0, id, wts);
+  lds_barrier();
+  const int n0 = tile * W::NC;
+  const uint32_t boff = W::lane_offset(w, n0, p.d, lane);
+  const uint32_t aoff = (lane >> 4) * 16;
+
+  // The wave's next step: slot s, step j of its expert's n.
+  int s = -1, j = wave, n = 0;
+  MatEntry mat = {};
+  auto settle = [&]() {
+    while (s < p.k && j >= n) {
+      j -= n;
+      ++s;
+      n = 0;
+      if (s < p.k) {
+        const int e = __builtin_amdgcn_readfirstlane(id[s]);
+        if (e >= 0) {
+          mat = tab[e];
+          n = (mat.len + W::KS - 1) / W::KS;
+        }
+      }
+    }
+  };
+  settle();
+  float total[W::C];
+#pragma unroll
+  for (int c = 0; c < W::C; ++c) total[c] = 0.0f;
+  while (s < p.k) {
+    W b[DEPTH];
+    typename W::A a[DEPTH][1][PL];
+    int slot[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      slot[d] = s;
+      if (s >= p.k) continue;
+      const int k0 = j * W::KS;
+      b[d].load(w, mat, true, k0, mat.len, n0, p.d, boff, lane);
+      const Row* row = static_cast<const Row*>(h) + (int64_t)(t * p.k + s) * ldh;
+      W::load_a(a[d][0][0], row, aoff, k0, mat.len, lane);
+      if constexpr (PL == 2) W::load_a(a[d][0][1], row + lo, aoff, k0, mat.len, lane);
+      j += kTokenWaves;
+      settle();
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (slot[d] >= p.k) continue;
+      f32x4_t acc[1][W::C];
+#pragma unroll
+      for (int c = 0; c < W::C; ++c) acc[0][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      b[d].mma(a[d], 1, acc);
+      const float f = wts[slot[d]];
+#pragma unroll
+      for (int c = 0; c < W::C; ++c) total[c] = fmaf(f, acc[0][c][0], total[c]);
+    }
+  }
+  // every row of the tile is the token's; the first lanes hold row 0
+  if (lane < 16) {
+#pragma unroll
+    for (int c = 0; c < W::C; ++c) red[wave][W::col(c, lane)] = total[c];
+  }
+  lds_barrier();
+  const int x = threadIdx.x;
+  if (x < W::NC && n0 + x < p.d) {
+    float z = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kTokenWaves; ++v) z += red[v][x];
+    const int64_t at = t * p.ldo + n0 + x;
+    if (p.out_f32)
+      static_cast<float*>(p.out)[at] = z;
+    else
+      static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16(z);
+  }
+}
 
 // ---------------------------------------------------------------------------
 // Router logits: 16 tokens x 16 experts a workgroup, its waves split the hidden
@@ -470,7 +745,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
 template <bool F32>
 __global__ __launch_bounds__(kThreads) void few_logits_kernel(const void* x, int64_t ldx, int T,
                                                               const void* wr, int64_t ldwr, int E,
-                                                              int d, float* logits) {
+                                                              int d, float* logits, int ldl) {
   __shared__ float red[kWaves][16][16];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int t0 = blockIdx.y * 16, e0 = blockIdx.x * 16;
@@ -507,76 +782,7 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const void* x, int
     float s = 0.0f;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) s += red[v][threadIdx.x / 16][threadIdx.x % 16];
-    if (t < T && e < E) logits[(int64_t)t * E + e] = s;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// out[t] = sum_s weight[t, s] y[t k + s] over the slots that name an expert.
-// Weights: the layer's sigmoids (normalised over the token's slots if asked) or
-// the caller's.
-// ---------------------------------------------------------------------------
-
-struct CombineArgs {
-  const float* y;
-  int T, k, E, d;
-  Ids ids;
-  const void* weights;
-  int wbf16, normalize;
-  void* out;
-  int64_t ldo;
-  int out_f32;
-  int32_t* sel_out;  // nullptr, or where the layer's choice goes
-  float* wts_out;
-};
-
-constexpr int kCombineThreads = 128;
-
-__global__ __launch_bounds__(kCombineThreads) void few_combine_kernel(CombineArgs p) {
-  __shared__ float w[kMaxTopK];
-  __shared__ int id[kMaxTopK];
-  const int t = blockIdx.y;
-  if (threadIdx.x < kMaxTopK) {
-    const int s = threadIdx.x;
-    float v = 0.0f;
-    int e = -1;
-    if (s < p.k) {
-      const int a = t * p.k + s;
-      e = load_id(p.ids, a, p.E);
-      v = p.wbf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.weights)[a])
-                  : static_cast<const float*>(p.weights)[a];
-    }
-    id[s] = e;
-    w[s] = v;
-    if (p.normalize) {
-      float sum = v;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-      w[s] = v / (sum + 1e-20f);
-    }
-    if (blockIdx.x == 0 && s < p.k) {
-      if (p.sel_out) p.sel_out[t * p.k + s] = e;
-      if (p.wts_out) p.wts_out[t * p.k + s] = w[s];
-    }
-  }
-  __syncthreads();
-  const int n = (blockIdx.x * kCombineThreads + threadIdx.x) * 4;
-  if (n >= p.d) return;
-  f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  const float* y = p.y + (int64_t)t * p.k * p.d + n;
-#pragma unroll 4
-  for (int s = 0; s < p.k; ++s) {
-    if (id[s] < 0) continue;
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(y + (int64_t)s * p.d);
-    const float f = w[s];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
-  }
-  if (p.out_f32) {
-    *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + t * p.ldo + n) = acc;
-  } else {
-    u32x2 v = {pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + t * p.ldo + n) = v;
+    if (t < T) logits[(int64_t)t * ldl + e] = e < E ? s : -INFINITY;
   }
 }
 
@@ -586,16 +792,25 @@ __global__ __launch_bounds__(kCombineThreads) void few_combine_kernel(CombineArg
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <class W, int MODE, int MT, int NS>
-int launch(FewArgs p, hipStream_t stream) {
+template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
+int launch_tiles(FewArgs p, hipStream_t stream) {
   const int width = kWaves / p.wk * W::NC;
   p.tiles = div_up(p.cols, width);
-  const int64_t units = (int64_t)(p.E + (MODE == kPlain ? 1 : 0)) * p.tiles;
+  const int64_t owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
+  const int64_t units = owners * p.tiles;
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
-  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS>), dim3(div_up(units, 8) * 8), dim3(kThreads), 0, stream,
-              p);
+  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS, SLOT, DEPTH>), dim3(div_up(units, 8) * 8),
+              dim3(kThreads), 0, stream, p);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
+}
+
+template <class W, int MODE, int NS>
+int launch(const FewArgs& p, hipStream_t stream) {
+  // row tiles in one pass over the weights: the mean number of rows, doubled
+  const int64_t rows = p.ids.p || p.logits ? 2 * (int64_t)p.T * p.k / p.E : p.T;
+  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, 1>(p, stream)
+                    : launch_tiles<W, MODE, 2, NS, false, 1>(p, stream);
 }
 
 // Waves that split K, `steps` steps long for the longest matrix.
@@ -605,42 +820,52 @@ int split_waves(int64_t steps) {
   return wk;
 }
 
-// Experts that get rows, at most.
-int64_t live_experts(const FewArgs& p) { return std::min<int64_t>(p.E, (int64_t)p.T * p.k); }
+// Whether the call's assignments share few experts: a workgroup then takes one
+// assignment, and one token's down projections at once.
+bool few_pairs(int64_t T, int64_t k, int64_t E) { return T * k * 2 <= E && E <= 256; }
 
 template <int MODE, int NS>
-int launch_bf16(FewArgs p, hipStream_t stream) {
-  p.wk = kWaves;
-  const int64_t live = live_experts(p);
-  if constexpr (NS == 1)
-    if (live * div_up(p.cols, 128) >= 256) return launch<WBf16<8>, MODE, 2, NS>(p, stream);
-  if (live * div_up(p.cols, 64) >= 256) return launch<WBf16<4>, MODE, 2, NS>(p, stream);
-  return launch<WBf16<2>, MODE, 2, NS>(p, stream);
-}
-
-template <int MODE, int NS>
-int launch_q4(FewArgs p, int group, int64_t max_k, hipStream_t stream) {
-  p.wk = split_waves(div_up(max_k, kQ4Rows));
+int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
   switch (group) {
-    case 32: return launch<WQ4<2, 1>, MODE, 2, NS>(p, stream);
-    case 64: return launch<WQ4<2, 2>, MODE, 2, NS>(p, stream);
-    default: return launch<WQ4<2, 4>, MODE, 2, NS>(p, stream);
+    case 32: return launch<WQ4<2, 1>, MODE, NS>(p, stream);
+    case 64: return launch<WQ4<2, 2>, MODE, NS>(p, stream);
+    default: return launch<WQ4<2, 4>, MODE, NS>(p, stream);
   }
 }
 
+// max_k: rows of the longest matrix.
 template <int MODE, int NS>
 int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t stream) {
-  if (format == VMOE_FEW_Q4) return launch_q4<MODE, NS>(p, group, max_k, stream);
-  if constexpr (MODE != kPlain) {
-    if (format == VMOE_FEW_BF16) return launch_bf16<MODE, NS>(p, stream);
-    p.wk = kWaves;
-    return launch<WF32, MODE, 2, NS>(p, stream);
+  p.early = (int64_t)p.T * p.k >= p.E;
+  p.wk = split_waves(div_up(max_k, format == VMOE_FEW_Q4 ? kQ4Rows : format ? 16 : 32));
+  if (MODE == kUp && few_pairs(p.T, p.k, p.E)) {
+    if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, MODE, 1, NS, true, 4>(p, stream);
+    if (format == VMOE_FEW_F32) return launch_tiles<WF32, MODE, 1, NS, true, 2>(p, stream);
+    switch (group) {
+      case 32: return launch_tiles<WQ4<1, 1>, MODE, 1, NS, true, 2>(p, stream);
+      case 64: return launch_tiles<WQ4<1, 2>, MODE, 1, NS, true, 2>(p, stream);
+      default: return launch_tiles<WQ4<1, 4>, MODE, 1, NS, true, 2>(p, stream);
+    }
   }
-  return VMOE_ERR_UNSUPPORTED;
+  if (format == VMOE_FEW_Q4) return launch_q4<MODE, NS>(p, group, stream);
+  if (format == VMOE_FEW_BF16) return launch<WBf16<4>, MODE, NS>(p, stream);
+  return launch<WF32, MODE, NS>(p, stream);
+}
+
+template <class W, int DEPTH>
+int launch_token(const SumArgs& p, const Stack& w, const MatEntry* tab, const void* h, int64_t ldh,
+                 int64_t lo, hipStream_t stream) {
+  const int tiles = div_up(p.d, W::NC);
+  const int64_t units = (int64_t)p.T * tiles;
+  if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
+  VMOE_LAUNCH((few_token_kernel<W, DEPTH>), dim3(div_up(units, 8) * 8), dim3(kTokenWaves * kWave),
+              0, stream, p, w, tab, h, ldh, lo, tiles);
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
 }
 
 struct FewLayout {
-  int64_t logits, prob, sel, h, y, bytes, ldh;
+  int64_t logits, prob, sel, h, y, bytes, ldh, ldl;
 };
 
 bool few_layout(int64_t T, int64_t E, int64_t k, int64_t d, int64_t w, int format, FewLayout& L) {
@@ -654,7 +879,8 @@ bool few_layout(int64_t T, int64_t E, int64_t k, int64_t d, int64_t w, int forma
     return o;
   };
   L.ldh = (w + 7) / 8 * 8;
-  L.logits = slot(4 * T * E);
+  L.ldl = (E + kLogitPad - 1) / kLogitPad * kLogitPad;
+  L.logits = slot(4 * T * L.ldl);
   L.prob = slot(4 * A);
   L.sel = slot(4 * A);
   L.h = slot(4 * A * L.ldh);  // fp32, or two bf16 halves
@@ -679,7 +905,7 @@ int check_weights(const vmoe_few_weights* w) {
   if (w->act != VMOE_ACT_RELU_SQUARED && w->act != VMOE_ACT_SWIGLU) return VMOE_ERR_INVALID_ARG;
   if (!w->w1 || !w->w2 || !w->table1 || !w->table2) return VMOE_ERR_INVALID_ARG;
   const int64_t per = w->format == VMOE_FEW_F32 ? 4 : 8;
-  if (w->hidden % per || w->max_width % per || w->hidden > (1 << 28) || w->max_width > (1 << 28))
+  if (w->hidden % per || w->max_width % per || w->hidden > (1 << 24) || w->max_width > (1 << 24))
     return VMOE_ERR_UNSUPPORTED;
   if (!aligned16(w->w1) || !aligned16(w->w2) || !aligned16(w->table1) || !aligned16(w->table2))
     return VMOE_ERR_UNSUPPORTED;
@@ -689,41 +915,46 @@ int check_weights(const vmoe_few_weights* w) {
     if (!aligned16(w->scales1) || !aligned16(w->scales2)) return VMOE_ERR_UNSUPPORTED;
   } else {
     if (w->ldw1 <= 0 || w->ldw2 < w->hidden) return VMOE_ERR_INVALID_ARG;
-    if (w->ldw1 % per || w->ldw2 % per) return VMOE_ERR_UNSUPPORTED;
+    // (a lane's offset, up to 25 rows, has 32 bits)
+    if (w->ldw1 % per || w->ldw2 % per || w->ldw1 > (1 << 24) || w->ldw2 > (1 << 24))
+      return VMOE_ERR_UNSUPPORTED;
   }
   return VMOE_OK;
 }
 
-int check_rows(const void* x, int64_t ldx, int64_t cols, const void* out, int64_t ldo,
+// (rows are addressed by 32-bit offsets)
+bool spans(int64_t rows, int64_t ld, int64_t size) { return rows * ld * size >= (1ll << 32); }
+
+int check_rows(int64_t T, const void* x, int64_t ldx, int64_t cols, const void* out, int64_t ldo,
                int64_t ocols, int64_t per) {
   if (!x || !out || ldx < cols || ldo < ocols) return VMOE_ERR_INVALID_ARG;
+  if (ldx > (1ll << 31) || spans(T, ldx, 16 / per)) return VMOE_ERR_UNSUPPORTED;
   if (ldx % per || ldo % per || !aligned16(x) || !aligned16(out)) return VMOE_ERR_UNSUPPORTED;
   return VMOE_OK;
 }
 
-// Up, down and sum, the choice of experts being either logits or ids.
-int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, int T, int k,
-                const float* logits, Ids ids, const void* weights, int wbf16, int normalize,
-                int32_t* sel, float* prob, void* h, float* y, int64_t ldh, void* out, int64_t ldo,
-                int32_t* sel_out, float* wts_out, hipStream_t stream) {
+// Up, down and sum; the choice of experts is the logits' or the caller's ids'.
+int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const float* logits,
+                int32_t* sel, float* prob, const SumArgs& c, const FewLayout& L, char* ws,
+                hipStream_t stream) {
   FewArgs p = {};
   p.w = {w.w1, w.scales1, w.ldw1};
   p.tab = reinterpret_cast<const MatEntry*>(w.table1);
   p.a = x;
   p.lda = ldx;
-  p.T = T;
-  p.k = k;
-  p.E = w.num_experts;
+  p.T = c.T;
+  p.k = c.k;
+  p.E = c.E;
   p.logits = logits;
-  p.ids = ids;
+  p.ldl = (int)L.ldl;
+  p.ids = c.ids;
   p.sel = sel;
   p.prob = prob;
   p.fixed = (int)w.hidden;
   p.cols = (int)w.max_width;
-  p.act = w.act;
-  p.out = h;
-  p.ldo = w.format == VMOE_FEW_F32 ? ldh : 2 * ldh;
-  p.lo = ldh;
+  p.out = ws + L.h;
+  p.ldo = w.format == VMOE_FEW_F32 ? L.ldh : 2 * L.ldh;
+  p.lo = L.ldh;
   int st = w.act == VMOE_ACT_SWIGLU
                ? launch_format<kUp, 2>(p, w.format, w.group, w.hidden, stream)
                : launch_format<kUp, 1>(p, w.format, w.group, w.hidden, stream);
@@ -731,33 +962,29 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, int T, in
 
   p.w = {w.w2, w.scales2, w.ldw2};
   p.tab = reinterpret_cast<const MatEntry*>(w.table2);
-  p.a = h;
+  if (few_pairs(c.T, c.k, c.E)) {
+    const void* h = ws + L.h;
+    if (w.format == VMOE_FEW_BF16)
+      return launch_token<WBf16<2>, 4>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+    if (w.format == VMOE_FEW_F32)
+      return launch_token<WF32, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+    switch (w.group) {
+      case 32: return launch_token<WQ4<1, 1>, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+      case 64: return launch_token<WQ4<1, 2>, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+      default: return launch_token<WQ4<1, 4>, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+    }
+  }
+  p.a = ws + L.h;
   p.lda = p.ldo;
   p.logits = nullptr;
-  p.ids = ids;
   p.cols = p.fixed = (int)w.hidden;
+  float* y = reinterpret_cast<float*>(ws + L.y);
   p.out = y;
   p.ldo = w.hidden;
   st = launch_format<kDown, 1>(p, w.format, w.group, w.max_width, stream);
   if (st != VMOE_OK) return st;
-
-  CombineArgs c = {};
-  c.y = y;
-  c.T = T;
-  c.k = k;
-  c.E = w.num_experts;
-  c.d = (int)w.hidden;
-  c.ids = ids;
-  c.weights = weights;
-  c.wbf16 = wbf16;
-  c.normalize = normalize;
-  c.out = out;
-  c.ldo = ldo;
-  c.out_f32 = w.format == VMOE_FEW_F32;
-  c.sel_out = sel_out;
-  c.wts_out = wts_out;
-  VMOE_LAUNCH(few_combine_kernel, dim3(div_up(w.hidden, 4 * kCombineThreads), T),
-              dim3(kCombineThreads), 0, stream, c);
+  VMOE_LAUNCH(few_combine_kernel, dim3(div_up(w.hidden, 4 * kCombineThreads), c.T),
+              dim3(kCombineThreads), 0, stream, c, y);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
 }
@@ -787,7 +1014,7 @@ extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t 
   if (top_k > w->num_experts) return VMOE_ERR_INVALID_ARG;
   if (num_tokens == 0) return VMOE_OK;
   const bool f32 = w->format == VMOE_FEW_F32;
-  st = check_rows(x, ldx, w->hidden, out, ldo, w->hidden, f32 ? 4 : 8);
+  st = check_rows(num_tokens, x, ldx, w->hidden, out, ldo, w->hidden, f32 ? 4 : 8);
   if (st != VMOE_OK) return st;
   if (!router_weight || ldwr < w->hidden || !workspace) return VMOE_ERR_INVALID_ARG;
   if (ldwr % (f32 ? 4 : 8) || !aligned16(router_weight) || !aligned16(workspace))
@@ -796,22 +1023,23 @@ extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t 
   if (!few_layout(num_tokens, w->num_experts, top_k, w->hidden, w->max_width, w->format, L))
     return VMOE_ERR_INVALID_ARG;
   if (workspace_bytes < (size_t)L.bytes) return VMOE_ERR_WORKSPACE;
+  if (spans(num_tokens * top_k, L.ldh, 4)) return VMOE_ERR_UNSUPPORTED;
   char* ws = static_cast<char*>(workspace);
   float* logits = reinterpret_cast<float*>(ws + L.logits);
   const int T = (int)num_tokens, E = w->num_experts;
-  const dim3 grid(div_up(E, 16), div_up(T, 16));
+  const dim3 grid(div_up(L.ldl, 16), div_up(T, 16));
   if (f32)
     VMOE_LAUNCH((few_logits_kernel<true>), grid, dim3(kThreads), 0, stream, x, ldx, T,
-                router_weight, ldwr, E, (int)w->hidden, logits);
+                router_weight, ldwr, E, (int)w->hidden, logits, (int)L.ldl);
   else
     VMOE_LAUNCH((few_logits_kernel<false>), grid, dim3(kThreads), 0, stream, x, ldx, T,
-                router_weight, ldwr, E, (int)w->hidden, logits);
+                router_weight, ldwr, E, (int)w->hidden, logits, (int)L.ldl);
   VMOE_CHECK_LAUNCH();
   int32_t* sel = reinterpret_cast<int32_t*>(ws + L.sel);
   float* prob = reinterpret_cast<float*>(ws + L.prob);
-  return few_experts(*w, x, ldx, T, top_k, logits, Ids{sel, 0}, prob, 0, normalize != 0, sel,
-                     prob, ws + L.h, reinterpret_cast<float*>(ws + L.y), L.ldh, out, ldo,
-                     selected, weights, stream);
+  const SumArgs c = {T, top_k, E, (int)w->hidden, {sel, 0}, prob, 0, normalize != 0, out, ldo, f32,
+                     selected, weights};
+  return few_experts(*w, x, ldx, logits, sel, prob, c, L, ws, stream);
 }
 
 extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_t ldx,
@@ -824,7 +1052,7 @@ extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_
   st = check_sizes(num_tokens, w->num_experts, top_k);
   if (st != VMOE_OK) return st;
   if (num_tokens == 0) return VMOE_OK;
-  st = check_rows(x, ldx, w->hidden, out, ldo, w->hidden, w->format == VMOE_FEW_F32 ? 4 : 8);
+  st = check_rows(num_tokens, x, ldx, w->hidden, out, ldo, w->hidden, w->format == VMOE_FEW_F32 ? 4 : 8);
   if (st != VMOE_OK) return st;
   if (!ids || !weights || !workspace) return VMOE_ERR_INVALID_ARG;
   if (!aligned16(workspace)) return VMOE_ERR_UNSUPPORTED;
@@ -832,11 +1060,12 @@ extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_
   if (!few_layout(num_tokens, w->num_experts, top_k, w->hidden, w->max_width, w->format, L))
     return VMOE_ERR_INVALID_ARG;
   if (workspace_bytes < (size_t)L.bytes) return VMOE_ERR_WORKSPACE;
+  if (spans(num_tokens * top_k, L.ldh, 4)) return VMOE_ERR_UNSUPPORTED;
   char* ws = static_cast<char*>(workspace);
-  return few_experts(*w, x, ldx, (int)num_tokens, top_k, nullptr, Ids{ids, ids_are_i64}, weights,
-                     weights_are_bf16, 0, nullptr, nullptr, ws + L.h,
-                     reinterpret_cast<float*>(ws + L.y), L.ldh, out, ldo, nullptr, nullptr,
-                     stream);
+  const SumArgs c = {(int)num_tokens, top_k, w->num_experts, (int)w->hidden, {ids, ids_are_i64},
+                     weights, weights_are_bf16, 0, out, ldo, w->format == VMOE_FEW_F32, nullptr,
+                     nullptr};
+  return few_experts(*w, x, ldx, nullptr, nullptr, nullptr, c, L, ws, stream);
 }
 
 extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids,
@@ -850,10 +1079,10 @@ extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, cons
   if (group != 32 && group != 64 && group != 128) return VMOE_ERR_INVALID_ARG;
   if (!ids && (num_matrices != 1 || per_row != 1)) return VMOE_ERR_INVALID_ARG;
   if (num_rows == 0) return VMOE_OK;
-  if (k_rows % 8 || max_cols % 8 || k_rows > (1 << 28) || max_cols > (1 << 28) ||
+  if (k_rows % 8 || max_cols % 8 || k_rows > (1 << 24) || max_cols > (1 << 24) ||
       !aligned16(codes) || !aligned16(scales) || !aligned16(table))
     return VMOE_ERR_UNSUPPORTED;
-  st = check_rows(x, ldx, k_rows, y, ldy, max_cols, 8);
+  st = check_rows(num_rows, x, ldx, k_rows, y, ldy, max_cols, 8);
   if (st != VMOE_OK) return st;
   FewArgs p = {};
   p.w = {codes, scales, 0};
@@ -868,5 +1097,7 @@ extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, cons
   p.cols = (int)max_cols;
   p.out = y;
   p.ldo = ldy;
-  return launch_q4<kPlain, 1>(p, group, k_rows, stream);
+  p.early = (int64_t)num_rows * per_row >= num_matrices;
+  p.wk = split_waves(div_up(k_rows, kQ4Rows));
+  return launch_q4<kPlain, 1>(p, group, stream);
 }
