@@ -810,8 +810,9 @@ int vmoe_moe_f32_backward(const void* saved, const float* logits, int64_t num_to
  * w1 [hidden, columns] and w2 [rows, hidden] in bf16 or fp32 with row strides, or
  * 4-bit blocks with scales. The tables hold four int32 a matrix: where it starts
  * (a column of w1, a row of w2), its length along that axis, its first 4-bit
- * block, 0. table1 has an entry for each expert (SwiGLU: two, gate and up),
- * table2 one. Activations and outputs are bf16 (fp32 for fp32 weights). hidden,
+ * block, and (table1) its expert's first tile. table1 has an entry for each expert
+ * (SwiGLU: two, gate and up), table2 one. tiles1 names the expert of each 64
+ * columns: every expert has ceil(width / 64) tiles, in order. Activations and outputs are bf16 (fp32 for fp32 weights). hidden,
  * widths, starts and strides are multiples of 8 (fp32: 4), buffers 16-byte
  * aligned; lengths are at most max_width, hidden, max_width and strides of the
  * weights at most 2^24, x and the activations span less than 4 GiB.
@@ -837,6 +838,8 @@ typedef struct vmoe_few_weights {
   const uint16_t* scales2;
   int64_t ldw2;
   const int32_t* table2;
+  const int32_t* tiles1;
+  int32_t num_tiles1;
 } vmoe_few_weights;
 int vmoe_few_max_tokens(void);
 size_t vmoe_few_workspace_bytes(int64_t num_tokens, int32_t num_experts, int32_t top_k,

@@ -34,9 +34,10 @@ struct Stack {
 };
 
 // A matrix of a stack: where it starts along the axis the matrices share
-// (column of W1, row of W2), its length along it, its first block (4-bit).
+// (column of W1, row of W2), its length along it, its first block (4-bit), its
+// first tile of 64 along that axis.
 struct MatEntry {
-  int32_t off, len, base, pad;
+  int32_t off, len, base, first_tile;
 };
 
 // Eight values of a dword as bf16, the lowest bits first (exact).
@@ -48,6 +49,13 @@ __device__ __forceinline__ bf16x8_t q4_values(uint32_t codes) {
   v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.0f, 2));
   v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.0f, 3));
   return __builtin_bit_cast(bf16x8_t, v);
+}
+
+// Orders LDS accesses of the workgroup; global loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 }  // namespace vmoe

@@ -1,13 +1,19 @@
 // Laying out matrices in 4 bits with group scales, and reading them back
 // (layout: few_q4.h).
 //
-// Both move each byte once. A workgroup takes 128 rows x 64 columns, four blocks:
-// it reads or writes the row-major side in runs of 64 columns (128 bytes a row
-// in bf16) and the blocks in whole kilobytes, and LDS turns one order into the
-// other. The nearest value is found by comparing |w| with the middles between
-// values times the scale: a bf16 scale times a middle of at most three bits is
-// exact in fp32, so no choice depends on a rounding, and a tie goes to the even
-// place. Only the scale itself, max / 6, rounds.
+// Both move each byte once and need no LDS. A wave takes 128 rows x 64 columns,
+// four blocks: lane l has four adjacent columns, 4 (l % 16).., of rows
+// 8 (l / 16) + 0..7 of each 32, which is what the block order wants of a column in
+// one lane; the four columns are 64 contiguous bytes of a block. Row-major
+// accesses are runs of 64 columns (128 bytes in bf16). The maximum of a group is
+// the maximum of four lanes.
+//
+// The nearest value: |w| against the middles between values times the scale. Those
+// products are exact in fp32 (a scale of 8 bits, a middle of 3), so no choice
+// depends on a rounding, and a tie goes to the even place; only the scale itself,
+// max / 6, rounds. For bf16 w the conversion instruction compares instead: it gets
+// the quotient w / s, whose two-step reciprocal form is exact where w is a middle
+// times s, and elsewhere w / s is at least 2^-12 of itself away from a middle.
 #include <math.h>
 
 #include "few_q4.h"
@@ -15,7 +21,7 @@
 namespace vmoe {
 namespace {
 
-constexpr int kThreads = 256, kTileCols = 64;
+constexpr int kThreads = 256, kWaves = kThreads / kWave, kTileCols = 64;
 
 struct Q4Args {
   const void* w;
@@ -24,7 +30,8 @@ struct Q4Args {
   const MatEntry* tab;
   void* codes;
   uint16_t* scales;
-  int by_rows, fixed, tiles_n, tiles_k;
+  int by_rows, fixed, tiles_n, tiles_k, units;
+  int wide;  // four columns of w or out can be one access
 };
 
 struct TilePos {
@@ -33,13 +40,20 @@ struct TilePos {
   bool ok;
 };
 
+// Wave -> tile, the columns fastest; an XCD (blockIdx % 8) takes a contiguous
+// eighth, so that it uses every channel of its L2 whatever the row stride.
 __device__ __forceinline__ TilePos tile_pos(const Q4Args& p) {
-  const MatEntry m = p.tab[blockIdx.y];
-  TilePos t;
+  TilePos t = {};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int per = (p.units + 7) / 8, j = (blockIdx.x >> 3) * kWaves + wave;
+  const int u = (blockIdx.x & 7) * per + j;
+  if (j >= per || u >= p.units) return t;
+  const int nt = u % p.tiles_n, mk = u / p.tiles_n;
+  const MatEntry m = p.tab[mk / p.tiles_k];
   t.K = p.by_rows ? m.len : p.fixed;
   t.N = p.by_rows ? p.fixed : m.len;
-  t.k0 = (int)(blockIdx.x / p.tiles_n) * kQ4Rows;
-  t.n0 = (int)(blockIdx.x % p.tiles_n) * kTileCols;
+  t.k0 = mk % p.tiles_k * kQ4Rows;
+  t.n0 = nt * kTileCols;
   t.base = m.base;
   t.row0 = p.by_rows ? m.off : 0;
   t.col0 = p.by_rows ? 0 : m.off;
@@ -55,61 +69,106 @@ __device__ __forceinline__ uint32_t code_of(float w, float s) {
   return c ? c | (w < 0.0f ? 8u : 0u) : 0u;
 }
 
+// w / s for bf16 values, r = 1 / s to a unit in the last place.
+__device__ __forceinline__ float quotient(float w, float s, float r) {
+  const float q = w * r;
+  return fmaf(fmaf(-q, s, w), r, q);
+}
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+constexpr int kLaneCols = 4;
+
+// Four columns of a row as fp32 bits; zeros past the matrix.
+template <bool F32>
+struct Quad {
+  typename std::conditional<F32, u32x4_t, u32x2_t>::type v;
+  __device__ __forceinline__ uint32_t bits(int c) const {
+    if constexpr (F32) {
+      return v[c];
+    } else {
+      return (c & 1) ? v[c / 2] & 0xFFFF0000u : v[c / 2] << 16;
+    }
+  }
+};
+
 template <bool F32, int G>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(Q4Args p) {
-  constexpr int S = kQ4Rows / G;  // groups of a tile's column
+  constexpr int S = kQ4Rows / G;  // groups of a column
+  constexpr int J = G / 32;       // 32-row quarters of a group
   const TilePos t = tile_pos(p);
   if (!t.ok) return;
-  __shared__ float tile[kQ4Rows][kTileCols + 1];
-  __shared__ float scale[S][kTileCols];
-  const int c = threadIdx.x % kTileCols;
-  for (int r = threadIdx.x / kTileCols; r < kQ4Rows; r += kThreads / kTileCols) {
-    float v = 0.0f;
-    if (t.k0 + r < t.K && t.n0 + c < t.N) {
-      const int64_t at = (t.row0 + t.k0 + r) * p.ld + t.col0 + t.n0 + c;
-      v = F32 ? static_cast<const float*>(p.w)[at]
-              : bf16_to_f32(static_cast<const uint16_t*>(p.w)[at]);
-    }
-    tile[r][c] = v;
-  }
-  __syncthreads();
-  const int kbs = (t.K + kQ4Rows - 1) / kQ4Rows, kb = t.k0 / kQ4Rows;
-  for (int i = threadIdx.x; i < S * kTileCols; i += kThreads) {
-    const int g = i / kTileCols, n = i % kTileCols;
-    float top = 0.0f;
-    bool finite = true;
-    for (int r = 0; r < G; ++r) {
-      const float a = fabsf(tile[g * G + r][n]);
-      finite = finite && a <= 3.4028234e38f;
-      top = fmaxf(top, a);
-    }
-    const uint32_t bits = finite ? f32_to_bf16(top / 6.0f) : 0x7FC0u;
-    scale[g][n] = bf16_to_f32(bits);
-    const int nb = (t.n0 + n) / kQ4Cols;
-    if (nb * kQ4Cols < t.N) {
-      const int64_t blk = t.base + (int64_t)nb * kbs + kb;
-      p.scales[(blk * kQ4Cols + n % kQ4Cols) * S + g] = (uint16_t)bits;
-    }
-  }
-  __syncthreads();
-  // a thread writes the 16 bytes of one lane of a block
-  const int b = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int nb = t.n0 / kQ4Cols + b, n = b * kQ4Cols + (lane & 15);
-  if (nb * kQ4Cols >= t.N) return;
-  uint32_t word[4];
+  const int lane = threadIdx.x % kWave, g = lane >> 4;
+  const int c0 = t.n0 + (lane & 15) * kLaneCols;
+  if (c0 >= (t.N + kQ4Cols - 1) / kQ4Cols * kQ4Cols) return;  // (whole quads of lanes)
+  const bool in = c0 < t.N;
+  Quad<F32> w[4][8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = 32 * j + (lane >> 4) * 8;
-    const float s = scale[r / G][n];
-    uint32_t v = 0;
-    if (s > 0.0f) {
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v |= code_of(tile[r + i][n], s) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      const int r = t.k0 + 32 * j + 8 * g + i;
+      w[j][i] = {};
+      if (!in || r >= t.K) continue;
+      const int64_t at = (t.row0 + r) * p.ld + t.col0 + c0;
+      if (p.wide) {
+        w[j][i].v = *reinterpret_cast<const decltype(w[j][i].v)*>(
+            static_cast<const char*>(p.w) + at * (F32 ? 4 : 2));
+      } else if constexpr (F32) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[j][i].v[c] = static_cast<const uint32_t*>(p.w)[at + c];
+      } else {
+        const uint16_t* q = static_cast<const uint16_t*>(p.w) + at;
+        w[j][i].v[0] = q[0] | (uint32_t)q[1] << 16;
+        w[j][i].v[1] = q[2] | (uint32_t)q[3] << 16;
+      }
     }
-    word[j] = v;
+  const int kbs = (t.K + kQ4Rows - 1) / kQ4Rows;
+  const int64_t blk = t.base + (int64_t)(c0 / kQ4Cols) * kbs + t.k0 / kQ4Rows;
+#pragma unroll
+  for (int c = 0; c < kLaneCols; ++c) {
+    const int col = c0 % kQ4Cols + c;  // of the block
+    u32x4_t word;
+#pragma unroll
+    for (int q = 0; q < S; ++q) {
+      // magnitudes order as their bits, infinities and NaN above all numbers
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, w[q * J + j][i].bits(c) & 0x7FFFFFFFu);
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, kWave));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, kWave));
+      const uint32_t sb = top < 0x7F800000u ? f32_to_bf16(__uint_as_float(top) / 6.0f) : 0x7FC0u;
+      const float s = bf16_to_f32(sb);
+      if (g == 0) p.scales[(blk * kQ4Cols + col) * S + q] = (uint16_t)sb;
+      // (the reciprocal of smaller scales would leave fp32's range)
+      const bool fast = !F32 && s >= 0x1p-100f;
+      const float r = fast ? __builtin_amdgcn_rcpf(s) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const Quad<F32>* v = w[q * J + j];
+        uint32_t codes = 0;
+        if (fast) {
+          auto two = [&](int i) {
+            return f32x2_t{quotient(__uint_as_float(v[i].bits(c)), s, r),
+                           quotient(__uint_as_float(v[i + 1].bits(c)), s, r)};
+          };
+          const f32x2_t q0 = two(0), q1 = two(2), q2 = two(4), q3 = two(6);
+          codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, q0.x, q0.y, 1.0f, 0);
+          codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, q1.x, q1.y, 1.0f, 1);
+          codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, q2.x, q2.y, 1.0f, 2);
+          codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, q3.x, q3.y, 1.0f, 3);
+        } else if (s > 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            codes |= code_of(__uint_as_float(v[i].bits(c)), s) << (4 * i);
+        }
+        word[q * J + j] = codes;
+      }
+    }
+    reinterpret_cast<u32x4_t*>(p.codes)[blk * kWave + g * 16 + col] = word;
   }
-  const int64_t blk = t.base + (int64_t)nb * kbs + kb;
-  reinterpret_cast<uint4*>(p.codes)[blk * kWave + lane] = {word[0], word[1], word[2], word[3]};
 }
 
 template <bool F32, int G>
@@ -117,32 +176,52 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(Q4Args p) {
   constexpr int S = kQ4Rows / G;
   const TilePos t = tile_pos(p);
   if (!t.ok) return;
-  __shared__ float tile[kQ4Rows][kTileCols + 1];
-  const int b = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int nb = t.n0 / kQ4Cols + b, n = b * kQ4Cols + (lane & 15);
-  if (nb * kQ4Cols < t.N) {
-    const int kbs = (t.K + kQ4Rows - 1) / kQ4Rows;
-    const int64_t blk = t.base + (int64_t)nb * kbs + t.k0 / kQ4Rows;
-    const uint4 word = reinterpret_cast<const uint4*>(p.codes)[blk * kWave + lane];
-    const uint32_t words[4] = {word.x, word.y, word.z, word.w};
+  const int lane = threadIdx.x % kWave, g = lane >> 4;
+  const int c0 = t.n0 + (lane & 15) * kLaneCols;
+  if (c0 >= t.N) return;
+  const int kbs = (t.K + kQ4Rows - 1) / kQ4Rows;
+  const int64_t blk = t.base + (int64_t)(c0 / kQ4Cols) * kbs + t.k0 / kQ4Rows;
+  u32x4_t word[kLaneCols];
+  float s[kLaneCols][S];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = 32 * j + (lane >> 4) * 8;
-      const float s = bf16_to_f32(p.scales[(blk * kQ4Cols + (lane & 15)) * S + r / G]);
-      const bf16x8_t v = q4_values(words[j]);
+  for (int c = 0; c < kLaneCols; ++c) {
+    const int64_t col = blk * kQ4Cols + c0 % kQ4Cols + c;
+    word[c] = reinterpret_cast<const u32x4_t*>(p.codes)[blk * kWave + g * 16 + c0 % kQ4Cols + c];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) tile[r + i][n] = s * (float)v[i];
-    }
+    for (int q = 0; q < S; ++q) s[c][q] = bf16_to_f32(p.scales[col * S + q]);
   }
-  __syncthreads();
-  const int c = threadIdx.x % kTileCols;
-  for (int r = threadIdx.x / kTileCols; r < kQ4Rows; r += kThreads / kTileCols) {
-    if (t.k0 + r >= t.K || t.n0 + c >= t.N) continue;
-    const int64_t at = (t.row0 + t.k0 + r) * p.ld + t.col0 + t.n0 + c;
-    if (F32)
-      static_cast<float*>(p.out)[at] = tile[r][c];
-    else
-      static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16(tile[r][c]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    bf16x8_t v[kLaneCols];
+#pragma unroll
+    for (int c = 0; c < kLaneCols; ++c) v[c] = q4_values(word[c][j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = t.k0 + 32 * j + 8 * g + i;
+      if (r >= t.K) break;
+      const int64_t at = (t.row0 + r) * p.ld + t.col0 + c0;
+      float f[kLaneCols];
+#pragma unroll
+      for (int c = 0; c < kLaneCols; ++c) f[c] = s[c][32 * j / G] * (float)v[c][i];
+      if constexpr (F32) {
+        float* out = static_cast<float*>(p.out) + at;
+        if (p.wide) {
+          *reinterpret_cast<f32x4_t*>(out) = f32x4_t{f[0], f[1], f[2], f[3]};
+        } else {
+#pragma unroll
+          for (int c = 0; c < kLaneCols; ++c) out[c] = f[c];
+        }
+      } else {
+        uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+        const u32x2_t two = {pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])};
+        if (p.wide) {
+          *reinterpret_cast<u32x2_t*>(out) = two;
+        } else {
+#pragma unroll
+          for (int c = 0; c < kLaneCols; ++c) out[c] = (uint16_t)(two[c / 2] >> (c % 2 * 16));
+        }
+      }
+    }
   }
 }
 
@@ -159,13 +238,17 @@ int check(const void* w, int64_t ld, const int32_t* table, int32_t M, int32_t by
   return VMOE_OK;
 }
 
-bool grid_of(Q4Args& p, int M, int64_t max_len, dim3& grid) {
+bool grid_of(Q4Args& p, int M, int64_t max_len, bool f32, dim3& grid) {
+  // (starts and lengths along the columns are multiples of 8)
+  const uintptr_t base = reinterpret_cast<uintptr_t>(p.w ? p.w : p.out);
+  p.wide = base % 16 == 0 && p.ld % 4 == 0;
   const int64_t k = p.by_rows ? max_len : p.fixed, n = p.by_rows ? p.fixed : max_len;
   p.tiles_k = (int)((k + kQ4Rows - 1) / kQ4Rows);
   p.tiles_n = (int)((n + kTileCols - 1) / kTileCols);
-  const int64_t tiles = (int64_t)p.tiles_k * p.tiles_n;
-  grid = dim3((unsigned)tiles, M);
-  return tiles <= (1 << 30);
+  const int64_t units = (int64_t)p.tiles_k * p.tiles_n * M;
+  p.units = (int)units;
+  grid = dim3((unsigned)(((units + 7) / 8 + kWaves - 1) / kWaves * 8));
+  return units <= (1 << 30);
 }
 
 }  // namespace
@@ -193,7 +276,7 @@ extern "C" int vmoe_q4_quantize(const void* w, int32_t w_is_f32, int64_t ldw, co
   Q4Args p = {w, nullptr, ldw, reinterpret_cast<const MatEntry*>(table), codes, scales, by_rows,
               (int)fixed};
   dim3 grid;
-  if (!grid_of(p, num_matrices, max_len, grid)) return VMOE_ERR_UNSUPPORTED;
+  if (!grid_of(p, num_matrices, max_len, w_is_f32, grid)) return VMOE_ERR_UNSUPPORTED;
   if (w_is_f32)
     VMOE_Q4_LAUNCH(quantize_kernel, true, group);
   else
@@ -212,7 +295,7 @@ extern "C" int vmoe_q4_dequantize(const void* codes, const uint16_t* scales, con
   Q4Args p = {nullptr, out, ldo, reinterpret_cast<const MatEntry*>(table),
               const_cast<void*>(codes), const_cast<uint16_t*>(scales), by_rows, (int)fixed};
   dim3 grid;
-  if (!grid_of(p, num_matrices, max_len, grid)) return VMOE_ERR_UNSUPPORTED;
+  if (!grid_of(p, num_matrices, max_len, out_is_f32, grid)) return VMOE_ERR_UNSUPPORTED;
   if (out_is_f32)
     VMOE_Q4_LAUNCH(dequantize_kernel, true, group);
   else

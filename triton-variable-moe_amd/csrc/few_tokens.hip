@@ -35,6 +35,7 @@ namespace vmoe {
 namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / kWave;
+constexpr int kTileCols = 64;  // of an up projection's workgroup
 constexpr int kMaxTokens = 256, kMaxRows = 4096, kMaxExperts = 2048, kMaxTopK = 64;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -306,18 +307,13 @@ struct FewArgs {
   int fixed;  // kUp, kPlain: K of every matrix; kDown: N
   int cols;   // columns of the widest matrix
   int tiles;  // its column tiles
+  const int32_t* tile_of;  // kUp: the expert of each kTileCols columns
+  int num_tiles;
   int wk;     // waves that split K; kWaves / wk split the tile's columns
   int act;
   void* out;  // h, y (fp32) or the products
   int64_t ldo;
 };
-
-// Orders LDS accesses of the workgroup; global loads stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 
 // How many experts of a token come before expert e, whose logit is `mine`:
 // eight lanes share the row (padded to kLogitPad with -inf), each gets the count.
@@ -389,18 +385,36 @@ __device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer,
   return *found;
 }
 
-// Workgroup -> (expert, tile): an XCD (blockIdx % 8) takes a contiguous eighth,
-// so the tiles of an expert share its rows and lines in one L2.
-__device__ __forceinline__ int unit_of_block(int units) {
-  const int per = (units + 7) / 8;
-  const int j = blockIdx.x >> 3, u = (blockIdx.x & 7) * per + j;
-  return j < per && u < units ? u : -1;
+// Workgroup -> unit. An XCD (blockIdx % 8) has an L2 of its own, whose 16 channels
+// take 256 bytes each in turn, and the rows of a weight matrix are a multiple of
+// 4 KB apart: an XCD that reads every eighth 256 bytes of a row uses an eighth of
+// its L2 (up projection of 128 experts 2048 x 576: 87 us so, 60 us with a
+// contiguous run of columns).
+//   kRuns: an XCD takes a contiguous eighth of the units.
+//   kDeal: the owners (experts) are dealt over the XCDs, all tiles of one to the
+//   same; owners of unequal length spread evenly.
+//   kPairs: pairs of units are dealt; for calls too small to fill the card, where
+//   two narrow tiles share a line.
+// The grid is a multiple of 16.
+enum Order { kRuns, kDeal, kPairs };
+__device__ __forceinline__ int unit_of_block(Order order, int units, int tiles) {
+  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+  if (order == kRuns) {
+    const int per = (units + 7) / 8, u = xcd * per + j;
+    return j < per && u < units ? u : -1;
+  }
+  const int u = order == kDeal ? (j / tiles * 8 + xcd) * tiles + j % tiles
+                               : (j >> 1) * 16 + xcd * 2 + (j & 1);
+  return u < units ? u : -1;
 }
 
 // SLOT: a unit is an assignment and a tile (one row), else an expert and a tile.
 // DEPTH steps of a wave are in flight.
+#ifndef FEW_B
+#define FEW_B 1
+#endif
 template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
-__global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
+__global__ __launch_bounds__(kThreads, FEW_B) void few_kernel(FewArgs p) {
   constexpr int PL = (MODE == kDown && sizeof(typename W::Row) == 2) ? 2 : 1;
   constexpr int NC = W::NC;
   constexpr int kPerLane = 16 / sizeof(typename W::Row);  // values of a 16-byte load
@@ -409,9 +423,18 @@ __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
   __shared__ int count;
   // kPlain: one matrix more, for the rows that name none (their products are 0)
   const int owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
-  const int unit = unit_of_block(owners * p.tiles);
-  if (unit < 0) return;
-  const int owner = unit / p.tiles, tile = unit % p.tiles;
+  int owner, tile;
+  if constexpr (MODE == kUp && !SLOT) {
+    const int unit = unit_of_block(kRuns, p.num_tiles, 1);
+    if (unit < 0) return;
+    owner = p.tile_of[unit];
+    tile = unit - p.tab[owner * NS].first_tile;
+  } else {
+    const int unit = unit_of_block(SLOT ? kPairs : MODE == kDown ? kDeal : kRuns,
+                                   owners * p.tiles, p.tiles);
+    if (unit < 0) return;
+    owner = unit / p.tiles, tile = unit % p.tiles;
+  }
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wn_count = kWaves / p.wk;
@@ -432,8 +455,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(FewArgs p) {
     mats[s] = MODE == kPlain && e == p.E ? MatEntry{} : p.tab[e * NS + s];
   const int K = MODE == kDown ? mats[0].len : p.fixed;
   const int N = MODE == kDown ? p.fixed : min(mats[0].len, p.cols);
-  // (the first tile's workgroup also writes the router's choice)
-  if (MODE != kPlain && nt >= N && (SLOT || tile > 0 || !p.logits)) return;
+  if (MODE != kPlain && nt >= N) return;
 
   const uint32_t boff = W::lane_offset(p.w, n0, N, lane);
   const int stride = p.wk * W::KS, first = wk * W::KS;
@@ -583,7 +605,8 @@ struct SumArgs {
 
 // By the first wave of a workgroup, into LDS.
 __device__ __forceinline__ void slot_weights(const SumArgs& p, int t, bool writer, int* id,
-                                             float* w) {
+                                             float* w, const MatEntry* tab = nullptr,
+                                             MatEntry* entries = nullptr) {
   static_assert(kMaxTopK == kWave, "a slot per lane");
   const int s = threadIdx.x;
   float v = 0.0f;
@@ -594,6 +617,7 @@ __device__ __forceinline__ void slot_weights(const SumArgs& p, int t, bool write
     v = p.wbf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.weights)[a])
                 : static_cast<const float*>(p.weights)[a];
   }
+  if (entries) entries[s] = e >= 0 ? tab[e] : MatEntry{};
   if (p.normalize) {
     float sum = v;
 #pragma unroll
@@ -658,12 +682,13 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
   __shared__ float red[kTokenWaves][W::NC];
   __shared__ float wts[kMaxTopK];
   __shared__ int id[kMaxTopK];
-  const int unit = unit_of_block(p.T * tiles);
+  __shared__ MatEntry mats[kMaxTopK];  // length 0 where a slot names no expert
+  const int unit = unit_of_block(kPairs, p.T * tiles, tiles);
   if (unit < 0) return;
   const int t = unit / tiles, tile = unit % tiles;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (wave == 0) slot_weights(p, t, tile == 0, id, wts);
+  if (wave == 0) slot_weights(p, t, tile == 0, id, wts, tab, mats);
   lds_barrier();
   const int n0 = tile * W::NC;
   const uint32_t boff = W::lane_offset(w, n0, p.d, lane);
@@ -678,11 +703,10 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
       ++s;
       n = 0;
       if (s < p.k) {
-        const int e = __builtin_amdgcn_readfirstlane(id[s]);
-        if (e >= 0) {
-          mat = tab[e];
-          n = (mat.len + W::KS - 1) / W::KS;
-        }
+        mat.off = __builtin_amdgcn_readfirstlane(mats[s].off);
+        mat.len = __builtin_amdgcn_readfirstlane(mats[s].len);
+        mat.base = __builtin_amdgcn_readfirstlane(mats[s].base);
+        n = (mat.len + W::KS - 1) / W::KS;
       }
     }
   };
@@ -797,9 +821,14 @@ int launch_tiles(FewArgs p, hipStream_t stream) {
   const int width = kWaves / p.wk * W::NC;
   p.tiles = div_up(p.cols, width);
   const int64_t owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
-  const int64_t units = owners * p.tiles;
+  // (dealt owners: eight at a time)
+  int64_t units = (MODE == kDown ? div_up(owners, 8) * 8 : owners) * (int64_t)p.tiles;
+  if (MODE == kUp && !SLOT) {
+    if (width != kTileCols) return VMOE_ERR_UNSUPPORTED;
+    units = p.num_tiles;
+  }
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
-  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS, SLOT, DEPTH>), dim3(div_up(units, 8) * 8),
+  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS, SLOT, DEPTH>), dim3(div_up(units, 16) * 16),
               dim3(kThreads), 0, stream, p);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
@@ -807,10 +836,17 @@ int launch_tiles(FewArgs p, hipStream_t stream) {
 
 template <class W, int MODE, int NS>
 int launch(const FewArgs& p, hipStream_t stream) {
+#ifndef FEW_W
+#define FEW_W 1
+#endif
+#ifndef FEW_D
+#define FEW_D 1
+#endif
+  constexpr int D = FEW_D;
   // row tiles in one pass over the weights: the mean number of rows, doubled
   const int64_t rows = p.ids.p || p.logits ? 2 * (int64_t)p.T * p.k / p.E : p.T;
-  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, 1>(p, stream)
-                    : launch_tiles<W, MODE, 2, NS, false, 1>(p, stream);
+  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, D>(p, stream)
+                    : launch_tiles<W, MODE, 2, NS, false, D >= 2 ? D / 2 : 1>(p, stream);
 }
 
 // Waves that split K, `steps` steps long for the longest matrix.
@@ -824,12 +860,12 @@ int split_waves(int64_t steps) {
 // assignment, and one token's down projections at once.
 bool few_pairs(int64_t T, int64_t k, int64_t E) { return T * k * 2 <= E && E <= 256; }
 
-template <int MODE, int NS>
+template <int CB, int MODE, int NS>
 int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
   switch (group) {
-    case 32: return launch<WQ4<2, 1>, MODE, NS>(p, stream);
-    case 64: return launch<WQ4<2, 2>, MODE, NS>(p, stream);
-    default: return launch<WQ4<2, 4>, MODE, NS>(p, stream);
+    case 32: return launch<WQ4<CB, 1>, MODE, NS>(p, stream);
+    case 64: return launch<WQ4<CB, 2>, MODE, NS>(p, stream);
+    default: return launch<WQ4<CB, 4>, MODE, NS>(p, stream);
   }
 }
 
@@ -837,7 +873,10 @@ int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
 template <int MODE, int NS>
 int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t stream) {
   p.early = (int64_t)p.T * p.k >= p.E;
-  p.wk = split_waves(div_up(max_k, format == VMOE_FEW_Q4 ? kQ4Rows : format ? 16 : 32));
+  // the columns of an up projection's tile are fixed (kTileCols)
+  const int steps = div_up(max_k, format == VMOE_FEW_Q4 ? kQ4Rows : format ? 16 : 32);
+  p.wk = kWaves;
+  if (MODE == kDown) p.wk = split_waves(format != VMOE_FEW_Q4 ? div_up(steps, FEW_W) : steps);
   if (MODE == kUp && few_pairs(p.T, p.k, p.E)) {
     if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, MODE, 1, NS, true, 4>(p, stream);
     if (format == VMOE_FEW_F32) return launch_tiles<WF32, MODE, 1, NS, true, 2>(p, stream);
@@ -847,7 +886,11 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
       default: return launch_tiles<WQ4<1, 4>, MODE, 1, NS, true, 2>(p, stream);
     }
   }
-  if (format == VMOE_FEW_Q4) return launch_q4<MODE, NS>(p, group, stream);
+  if (format == VMOE_FEW_Q4) {
+    if (MODE == kUp && steps > 4) return launch_q4<4, MODE, NS>(p, group, stream);
+    if (MODE == kUp) p.wk = 4;
+    return launch_q4<2, MODE, NS>(p, group, stream);
+  }
   if (format == VMOE_FEW_BF16) return launch<WBf16<4>, MODE, NS>(p, stream);
   return launch<WF32, MODE, NS>(p, stream);
 }
@@ -858,7 +901,7 @@ int launch_token(const SumArgs& p, const Stack& w, const MatEntry* tab, const vo
   const int tiles = div_up(p.d, W::NC);
   const int64_t units = (int64_t)p.T * tiles;
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
-  VMOE_LAUNCH((few_token_kernel<W, DEPTH>), dim3(div_up(units, 8) * 8), dim3(kTokenWaves * kWave),
+  VMOE_LAUNCH((few_token_kernel<W, DEPTH>), dim3(div_up(units, 16) * 16), dim3(kTokenWaves * kWave),
               0, stream, p, w, tab, h, ldh, lo, tiles);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
@@ -903,7 +946,8 @@ int check_weights(const vmoe_few_weights* w) {
       w->format > VMOE_FEW_Q4)
     return VMOE_ERR_INVALID_ARG;
   if (w->act != VMOE_ACT_RELU_SQUARED && w->act != VMOE_ACT_SWIGLU) return VMOE_ERR_INVALID_ARG;
-  if (!w->w1 || !w->w2 || !w->table1 || !w->table2) return VMOE_ERR_INVALID_ARG;
+  if (!w->w1 || !w->w2 || !w->table1 || !w->table2 || !w->tiles1 || w->num_tiles1 <= 0)
+    return VMOE_ERR_INVALID_ARG;
   const int64_t per = w->format == VMOE_FEW_F32 ? 4 : 8;
   if (w->hidden % per || w->max_width % per || w->hidden > (1 << 24) || w->max_width > (1 << 24))
     return VMOE_ERR_UNSUPPORTED;
@@ -952,6 +996,8 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const flo
   p.prob = prob;
   p.fixed = (int)w.hidden;
   p.cols = (int)w.max_width;
+  p.tile_of = w.tiles1;
+  p.num_tiles = w.num_tiles1;
   p.out = ws + L.h;
   p.ldo = w.format == VMOE_FEW_F32 ? L.ldh : 2 * L.ldh;
   p.lo = L.ldh;
@@ -1099,5 +1145,5 @@ extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, cons
   p.ldo = ldy;
   p.early = (int64_t)num_rows * per_row >= num_matrices;
   p.wk = split_waves(div_up(k_rows, kQ4Rows));
-  return launch_q4<kPlain, 1>(p, group, stream);
+  return launch_q4<2, kPlain, 1>(p, group, stream);
 }

@@ -36,6 +36,7 @@ _ACT = {"relu_squared": _lib.ACT_RELU_SQUARED, "swiglu": _lib.ACT_SWIGLU}
 _GROUPS = (32, 64, 128)
 _MAX_PAIRS, _MAX_TOP_K, _MAX_EXPERTS = 4096, 64, 2048
 _Q4_ROWS, _Q4_COLS, _Q4_BLOCK = 128, 16, 1024
+_TILE = 64  # columns of an up projection's workgroup
 
 
 def few_tokens_max() -> int:
@@ -66,15 +67,24 @@ def _weight(w: torch.Tensor, what: str, dtypes, mult: int) -> torch.Tensor:
     return w
 
 
-def _entries(lengths: list[int], blocks: list[int], device) -> torch.Tensor:
-    """int32 [matrices, 4]: start, length, first 4-bit block, 0."""
-    rows, off, base = [], 0, 0
-    for n, b in zip(lengths, blocks):
-        rows.append([off, n, base, 0])
+def _entries(lengths: list[int], blocks: list[int], device, each: int = 1) -> torch.Tensor:
+    """int32 [matrices, 4]: start, length, first 4-bit block, first tile (of
+    _TILE along that axis; the `each` matrices of an expert count once)."""
+    rows, off, base, tile = [], 0, 0, 0
+    for i, (n, b) in enumerate(zip(lengths, blocks)):
+        rows.append([off, n, base, tile])
         off, base = off + n, base + b
+        if i % each == each - 1:
+            tile += -(-n // _TILE)
     if off >= 2 ** 31 or base >= 2 ** 31:
         raise NotImplementedError("the matrices are too many or too long")
     return torch.tensor(rows, dtype=torch.int32, device=device)
+
+
+def _tiles(widths: list[int], device) -> torch.Tensor:
+    """int32: the expert of each tile."""
+    return torch.tensor([e for e, w in enumerate(widths) for _ in range(-(-w // _TILE))],
+                        dtype=torch.int32, device=device)
 
 
 class _FewWeights(ctypes.Structure):
@@ -86,7 +96,8 @@ class _FewWeights(ctypes.Structure):
                 ("scales1", ctypes.c_void_p), ("ldw1", ctypes.c_int64),
                 ("table1", ctypes.c_void_p), ("w2", ctypes.c_void_p),
                 ("scales2", ctypes.c_void_p), ("ldw2", ctypes.c_int64),
-                ("table2", ctypes.c_void_p)]
+                ("table2", ctypes.c_void_p), ("tiles1", ctypes.c_void_p),
+                ("num_tiles1", ctypes.c_int32)]
 
 
 class _Experts:
@@ -102,6 +113,7 @@ class _Experts:
         self._max_width = max(widths)
         self._format = fmt
         self._group = group
+        self._tiles = _tiles(widths, device)
         self._desc = None  # made by the first call, and again after a copy
         self._bytes: dict = {}  # (tokens, top_k) -> workspace bytes
 
@@ -111,6 +123,7 @@ class _Experts:
     def _new_desc(self) -> _FewWeights:
         self._desc = _FewWeights(self._format, self._group, _ACT[self.activation],
                                  self.num_experts, self.hidden, self._max_width)
+        self._desc.tiles1, self._desc.num_tiles1 = self._tiles.data_ptr(), self._tiles.numel()
         self._desc_ptr = ctypes.addressof(self._desc)
         return self._desc
 
@@ -155,7 +168,7 @@ class FewTokenExperts(_Experts):
         self._init_common(_lib.FEW_F32 if f32 else _lib.FEW_BF16, 0, activation, widths, d,
                           w1.dtype, w1.device)
         each = [w for w in widths for _ in range(glu)]
-        self._t1 = _entries(each, [0] * len(each), w1.device)
+        self._t1 = _entries(each, [0] * len(each), w1.device, glu)
         self._t2 = _entries(widths, [0] * len(widths), w1.device)
         self._at = None
 
@@ -193,7 +206,7 @@ def few_token_experts(w1, w2, expert_widths, activation="relu_squared") -> FewTo
 class QuantizedMatrices:
     """A stack of 4-bit matrices in the kernels' order: quantize_matrices."""
 
-    def __init__(self, w, lengths, stacked: str, group_size: int):
+    def __init__(self, w, lengths, stacked: str, group_size: int, each: int = 1):
         if stacked not in ("columns", "rows"):
             raise ValueError(f"stacked must be 'columns' or 'rows' (got {stacked!r})")
         if group_size not in _GROUPS:
@@ -217,7 +230,7 @@ class QuantizedMatrices:
             return -(-k // _Q4_ROWS) * -(-c // _Q4_COLS)
 
         per = [blocks(n) for n in lengths]
-        self._table = _entries(lengths, per, w.device)
+        self._table = _entries(lengths, per, w.device, each)
         count = sum(per)
         with torch.cuda.device(w.device):
             self.codes = torch.empty(count * _Q4_BLOCK, dtype=torch.uint8, device=w.device)
@@ -261,8 +274,8 @@ class QuantizedExperts(_Experts):
         for w, n in ((w1, "w1"), (w2, "w2")):
             _weight(w, n, (torch.bfloat16, torch.float32), 1)
         glu, d = _check_layer(w1, w2, widths, activation)
-        self.w1 = quantize_matrices(w1, [w for w in widths for _ in range(glu)], "columns",
-                                    group_size)
+        self.w1 = QuantizedMatrices(w1, [w for w in widths for _ in range(glu)], "columns",
+                                    group_size, glu)
         self.w2 = quantize_matrices(w2, widths, "rows", group_size)
         self.group_size = group_size
         self._init_common(_lib.FEW_Q4, group_size, activation, widths, d, torch.bfloat16,
