@@ -26,7 +26,9 @@ that a group of 32, 64 or 128 values of a column shares along the summed axis.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -39,6 +41,7 @@ _Q4_ROWS, _Q4_COLS, _Q4_BLOCK = 128, 16, 1024
 _TILE = 64  # columns of an up projection's workgroup
 
 
+@functools.lru_cache(maxsize=None)
 def few_tokens_max() -> int:
     """The most tokens (rows of x) a call takes."""
     return int(_lib.lib().vmoe_few_max_tokens())
@@ -47,7 +50,7 @@ def few_tokens_max() -> int:
 def _widths_of(widths) -> list[int]:
     if isinstance(widths, torch.Tensor):
         widths = widths.tolist()
-    widths = [int(w) for w in widths]
+    widths = list(map(int, widths))
     if not widths or min(widths) <= 0:
         raise ValueError("expert_widths must hold at least one width, all positive")
     return widths
@@ -67,24 +70,36 @@ def _weight(w: torch.Tensor, what: str, dtypes, mult: int) -> torch.Tensor:
     return w
 
 
-def _entries(lengths: list[int], blocks: list[int], device, each: int = 1) -> torch.Tensor:
-    """int32 [matrices, 4]: start, length, first 4-bit block, first tile (of
-    _TILE along that axis; the `each` matrices of an expert count once)."""
+@functools.lru_cache(maxsize=256)
+def _entries(lengths: tuple, fixed: int, by_rows: bool, each: int, device) -> tuple:
+    """(int32 [matrices, 4] on the device: start, length, first 4-bit block, first
+    tile (of _TILE along that axis; the `each` matrices of an expert count
+    once); number of 4-bit blocks). A layout's tables, shared by its handles."""
     rows, off, base, tile = [], 0, 0, 0
-    for i, (n, b) in enumerate(zip(lengths, blocks)):
-        rows.append([off, n, base, tile])
-        off, base = off + n, base + b
+    for i, n in enumerate(lengths):
+        rows.append((off, n, base, tile))
+        k, c = (n, fixed) if by_rows else (fixed, n)
+        off, base = off + n, base + -(-k // _Q4_ROWS) * -(-c // _Q4_COLS)
         if i % each == each - 1:
             tile += -(-n // _TILE)
     if off >= 2 ** 31 or base >= 2 ** 31:
         raise NotImplementedError("the matrices are too many or too long")
-    return torch.tensor(rows, dtype=torch.int32, device=device)
+    return torch.tensor(rows, dtype=torch.int32, device=device), base
 
 
-def _tiles(widths: list[int], device) -> torch.Tensor:
-    """int32: the expert of each tile."""
+@functools.lru_cache(maxsize=256)
+def _tiles(widths: tuple, device) -> torch.Tensor:
+    """int32 on the device: the expert of each tile of _TILE columns."""
     return torch.tensor([e for e, w in enumerate(widths) for _ in range(-(-w // _TILE))],
                         dtype=torch.int32, device=device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The device as the current one (kernels and allocations go to it)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 class _FewWeights(ctypes.Structure):
@@ -113,7 +128,7 @@ class _Experts:
         self._max_width = max(widths)
         self._format = fmt
         self._group = group
-        self._tiles = _tiles(widths, device)
+        self._tiles = _tiles(tuple(widths), device)
         self._desc = None  # made by the first call, and again after a copy
         self._bytes: dict = {}  # (tokens, top_k) -> workspace bytes
 
@@ -168,8 +183,8 @@ class FewTokenExperts(_Experts):
         self._init_common(_lib.FEW_F32 if f32 else _lib.FEW_BF16, 0, activation, widths, d,
                           w1.dtype, w1.device)
         each = [w for w in widths for _ in range(glu)]
-        self._t1 = _entries(each, [0] * len(each), w1.device, glu)
-        self._t2 = _entries(widths, [0] * len(widths), w1.device)
+        self._t1, _ = _entries(tuple(each), d, False, glu, w1.device)
+        self._t2, _ = _entries(tuple(widths), d, True, 1, w1.device)
         self._at = None
 
     def _weights(self) -> int:
@@ -217,7 +232,7 @@ class QuantizedMatrices:
         lengths = [total] if lengths is None else _widths_of(lengths)
         if sum(lengths) != total:
             raise ValueError(f"lengths must add up to the matrix's {total} {stacked}")
-        if fixed % 8 or any(n % 8 for n in lengths):
+        if fixed % 8 or any([n % 8 for n in lengths]):
             raise NotImplementedError("matrix sizes must be multiples of 8")
         if len(lengths) > 65535:
             raise NotImplementedError("at most 65535 matrices")
@@ -225,14 +240,8 @@ class QuantizedMatrices:
         self.fixed, self.total, self.max_len = fixed, total, max(lengths)
         self.device = w.device
 
-        def blocks(n):
-            k, c = (n, fixed) if by_rows else (fixed, n)
-            return -(-k // _Q4_ROWS) * -(-c // _Q4_COLS)
-
-        per = [blocks(n) for n in lengths]
-        self._table = _entries(lengths, per, w.device, each)
-        count = sum(per)
-        with torch.cuda.device(w.device):
+        self._table, count = _entries(tuple(lengths), fixed, by_rows, each, w.device)
+        with _on(w.device):
             self.codes = torch.empty(count * _Q4_BLOCK, dtype=torch.uint8, device=w.device)
             self.scales = torch.empty(count, _Q4_COLS, _Q4_ROWS // group_size,
                                       dtype=torch.bfloat16, device=w.device)
@@ -247,7 +256,7 @@ class QuantizedMatrices:
             raise NotImplementedError(f"dequantize to bfloat16 or float32 (got {dtype})")
         by_rows = self.stacked == "rows"
         shape = (self.total, self.fixed) if by_rows else (self.fixed, self.total)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             out = torch.empty(shape, dtype=dtype, device=self.device)
             _lib.call("vmoe_q4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(),
                       self._table.data_ptr(), len(self.lengths), int(by_rows), self.fixed,
@@ -361,7 +370,7 @@ def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True
     wr = _rows(router_weight, d, experts.dtype, experts.device, "router_weight")
     dev = x.device
     n = experts._workspace_bytes(T, k)
-    with torch.cuda.device(dev):
+    with _on(dev):
         out = torch.empty((T, d), dtype=experts.dtype, device=dev)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         sel = wts = None
@@ -398,7 +407,7 @@ def experts_few_tokens(x, selected, weights, experts):
     wts = weights if weights.is_contiguous() else weights.contiguous()
     dev = x.device
     n = experts._workspace_bytes(T, k)
-    with torch.cuda.device(dev):
+    with _on(dev):
         out = torch.empty((T, d), dtype=experts.dtype, device=dev)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         _lib.call("vmoe_few_experts", experts._weights(), rows.data_ptr(), _row_stride(rows), T,
@@ -449,7 +458,7 @@ def matvec_q4(x, q: QuantizedMatrices, ids=None):
         raise NotImplementedError(f"matvec_q4 takes at most {_MAX_EXPERTS} matrices")
     _check_count(T, k, "matvec_q4")
     dev = x.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
         _lib.call("vmoe_q4_matvec", rows.data_ptr(), _row_stride(rows), T, _lib.ptr(ids),
                   int(ids is not None and ids.dtype == torch.int64), k, q.codes.data_ptr(),
