@@ -36,9 +36,20 @@ struct Stack {
 // A matrix of a stack: where it starts along the axis the matrices share
 // (column of W1, row of W2), its length along it, its first block (4-bit), its
 // first tile of 64 along that axis.
-struct MatEntry {
+struct alignas(16) MatEntry {
   int32_t off, len, base, first_tile;
 };
+
+// (One 16-byte load; a struct copied under a condition would go through memory.)
+__device__ __forceinline__ MatEntry load_entry(const MatEntry* p) {
+  typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+  const i32x4 v = *reinterpret_cast<const i32x4*>(p);
+  return {v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ void store_entry(MatEntry* p, const MatEntry& m) {
+  typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<i32x4*>(p) = i32x4{m.off, m.len, m.base, m.first_tile};
+}
 
 // Eight values of a dword as bf16, the lowest bits first (exact).
 __device__ __forceinline__ bf16x8_t q4_values(uint32_t codes) {

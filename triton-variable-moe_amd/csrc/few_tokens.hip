@@ -302,8 +302,12 @@ struct FewArgs {
   int ldl;
   int early;  // load weights before the rows are known
   Ids ids;
+  const void* wr;  // slots: the router's weights, where its logits are formed here
+  int64_t ldwr;
   int32_t* sel;  // kUp with logits: chosen experts and their sigmoids, [T, k]
   float* prob;
+  const MatEntry* tab2;  // slots: the down projections' entries, and where the
+  MatEntry* entry;       // assignments' go, [T, k]
   int fixed;  // kUp, kPlain: K of every matrix; kDown: N
   int cols;   // columns of the widest matrix
   int tiles;  // its column tiles
@@ -365,24 +369,110 @@ __device__ __forceinline__ int find_rows(const FewArgs& p, int e, bool writer, u
   return *count;
 }
 
+constexpr int kSlotExperts = 256;  // at most, where a workgroup takes one assignment
+constexpr int kFusedExperts = 128;  // ... and forms its token's logits itself,
+constexpr int64_t kFusedBytes = 256 << 10;  // from router weights of so many bytes
+
+// The logits of token t, padded as place_of wants them, into LDS: the waves split
+// the hidden axis; 16 experts are the rows of an operand and the token every
+// column of the other.
+template <class Row, int ET>
+__device__ __forceinline__ void slot_logits(const FewArgs& p, int t, float* lg, float* part) {
+  constexpr int PER = 16 / sizeof(Row), KS = 4 * PER;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int d = p.fixed;
+  const Row* x = static_cast<const Row*>(p.a) + (int64_t)t * p.lda;
+  const Row* wr = static_cast<const Row*>(p.wr);
+  f32x4_t acc[ET];
+#pragma unroll
+  for (int i = 0; i < ET; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  using V = typename std::conditional<PER == 8, bf16x8_t, f32x4_t>::type;
+  // A wave's columns are adjacent: the rows are a power of two apart in memory, and
+  // it is the columns that spread the waves' reads over the L2's channels. The
+  // loads of U steps go out together.
+  constexpr int U = 16 / ET;
+  const int per = (d + kWaves * KS - 1) / (kWaves * KS) * KS, end = min(d, wave * per + per);
+  for (int k0 = wave * per; k0 < end; k0 += U * KS) {
+    V a[U][ET], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * KS + (lane >> 4) * PER, kc = k < end ? k : 0;
+      b[u] = *reinterpret_cast<const V*>(x + kc);
+#pragma unroll
+      for (int i = 0; i < ET; ++i)
+        a[u][i] = *reinterpret_cast<const V*>(
+            wr + min(i * 16 + (lane & 15), p.E - 1) * p.ldwr + kc);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = k0 + u * KS + (lane >> 4) * PER < end;
+      b[u] = in ? b[u] : V{};
+#pragma unroll
+      for (int i = 0; i < ET; ++i) {
+        const V w = in ? a[u][i] : V{};
+        if constexpr (PER == 8) {
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, b[u], acc[i], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], b[u][j], acc[i], 0, 0, 0);
+        }
+      }
+    }
+  }
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < ET; ++i)
+      *reinterpret_cast<f32x4_t*>(&part[wave * kFusedExperts + i * 16 + (lane >> 4) * 4]) = acc[i];
+  }
+  lds_barrier();
+  if (threadIdx.x < kFusedExperts) {
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) s += part[v * kFusedExperts + threadIdx.x];
+    lg[threadIdx.x] = (int)threadIdx.x < p.E ? s : -INFINITY;
+  }
+  lds_barrier();
+}
+
 // The expert of assignment a, or -1.
-__device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer, int* found) {
-  if (!p.logits) return __builtin_amdgcn_readfirstlane(load_id(p.ids, a, p.E));
-  const int part = threadIdx.x & 7, t = a / p.k, s = a % p.k;
+template <class Row>
+__device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer, float* lg,
+                                           float* part, int* found) {
+  if (!p.logits && !p.wr) {
+    const int e = __builtin_amdgcn_readfirstlane(load_id(p.ids, a, p.E));
+    if (writer && threadIdx.x == 0) {
+      MatEntry m = load_entry(p.tab2 + max(e, 0));
+      if (e < 0) m.len = 0;
+      store_entry(p.entry + a, m);
+    }
+    return e;
+  }
+  const int lane8 = threadIdx.x & 7, t = a / p.k, s = a % p.k;
+  const bool fused = p.wr != nullptr;
+  if (fused) {
+    if (p.E <= 64)
+      slot_logits<Row, 4>(p, t, lg, part);
+    else
+      slot_logits<Row, 8>(p, t, lg, part);
+  }
   const float* l = p.logits + (int64_t)t * p.ldl;
   for (int e = threadIdx.x / 8; e < p.E; e += kThreads / 8) {
-    const float mine = l[e];
-    const int before = place_of(l, p.ldl, e, mine, part);
-    if (before == s && part == 0) {
+    const float mine = fused ? lg[e] : l[e];
+    const int before =
+        fused ? place_of(lg, p.ldl, e, mine, lane8) : place_of(l, p.ldl, e, mine, lane8);
+    if (before == s && lane8 == 0) {
       *found = e;
       if (writer) {
         p.sel[a] = e;
         p.prob[a] = sigmoid_f32(mine);
+        store_entry(p.entry + a, load_entry(p.tab2 + e));
       }
     }
   }
   lds_barrier();
-  return *found;
+  return __builtin_amdgcn_readfirstlane(*found);
 }
 
 // Workgroup -> unit. An XCD (blockIdx % 8) has an L2 of its own, whose 16 channels
@@ -410,17 +500,22 @@ __device__ __forceinline__ int unit_of_block(Order order, int units, int tiles) 
 
 // SLOT: a unit is an assignment and a tile (one row), else an expert and a tile.
 // DEPTH steps of a wave are in flight.
-#ifndef FEW_B
-#define FEW_B 1
-#endif
+// Waves a SIMD holds at least: the long K of a down projection's many small tiles is
+// covered by other workgroups (128 experts 576 x 2048: 65 us with two on a CU, 58
+// with three).
+template <class W, int MODE>
+constexpr int kMinWaves = MODE == kDown && sizeof(typename W::Row) == 2 && W::KS == 32 ? 6 : 1;
+
 template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
-__global__ __launch_bounds__(kThreads, FEW_B) void few_kernel(FewArgs p) {
+__global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE>)) void few_kernel(FewArgs p) {
   constexpr int PL = (MODE == kDown && sizeof(typename W::Row) == 2) ? 2 : 1;
   constexpr int NC = W::NC;
   constexpr int kPerLane = 16 / sizeof(typename W::Row);  // values of a 16-byte load
   __shared__ float red[NS * 16 * kWaves * NC];            // [NS][wk][16][width]
   __shared__ uint16_t rows[SLOT ? 8 : kMaxRows];
   __shared__ int count;
+  __shared__ MatEntry found[2];
+  static_assert(!SLOT || kSlotExperts * NS <= kThreads, "an entry a thread");
   // kPlain: one matrix more, for the rows that name none (their products are 0)
   const int owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
   int owner, tile;
@@ -446,13 +541,28 @@ __global__ __launch_bounds__(kThreads, FEW_B) void few_kernel(FewArgs p) {
 
   int e = owner, m = 1;
   if constexpr (SLOT) {
-    e = find_expert(p, owner, tile == 0, &count);
+    // (red is free until the products are joined)
+    static_assert(NS * 16 * kWaves * NC >= (kWaves + 1) * kFusedExperts, "room for the logits");
+    // the entries of all experts come in meanwhile
+    const MatEntry early_entry = load_entry(p.tab + min((int)threadIdx.x, p.E * NS - 1));
+    e = find_expert<typename W::Row>(p, owner, tile == 0, red, red + kFusedExperts, &count);
     if (e < 0) return;
+    if ((int)threadIdx.x / NS == e) store_entry(&found[threadIdx.x % NS], early_entry);
+    if (threadIdx.x == 0) rows[0] = (uint16_t)owner;
+    lds_barrier();  // (also: the logits in red have been read)
   }
   MatEntry mats[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s)
-    mats[s] = MODE == kPlain && e == p.E ? MatEntry{} : p.tab[e * NS + s];
+  for (int s = 0; s < NS; ++s) {
+    if constexpr (SLOT) {
+      mats[s].off = __builtin_amdgcn_readfirstlane(found[s].off);
+      mats[s].len = __builtin_amdgcn_readfirstlane(found[s].len);
+      mats[s].base = __builtin_amdgcn_readfirstlane(found[s].base);
+    } else {
+      mats[s] = load_entry(p.tab + min(e, p.E - 1) * NS + s);
+    }
+  }
+  if (MODE == kPlain && e == p.E) mats[0].len = 0;
   const int K = MODE == kDown ? mats[0].len : p.fixed;
   const int N = MODE == kDown ? p.fixed : min(mats[0].len, p.cols);
   if (MODE != kPlain && nt >= N) return;
@@ -473,10 +583,7 @@ __global__ __launch_bounds__(kThreads, FEW_B) void few_kernel(FewArgs p) {
     for (int d = 0; d < DEPTH; ++d)
       if (first + d * stride < K) load_b(d, first + d * stride);
   }
-  if constexpr (SLOT) {
-    if (threadIdx.x == 0) rows[0] = (uint16_t)owner;
-    lds_barrier();
-  } else {
+  if constexpr (!SLOT) {
     m = find_rows(p, e, tile == 0, rows, &count);
     if (m == 0) return;
     if constexpr (MODE == kPlain) {
@@ -603,33 +710,35 @@ struct SumArgs {
   float* wts_out;
 };
 
-// By the first wave of a workgroup, into LDS.
-__device__ __forceinline__ void slot_weights(const SumArgs& p, int t, bool writer, int* id,
-                                             float* w, const MatEntry* tab = nullptr,
-                                             MatEntry* entries = nullptr) {
+// A slot a lane: its expert (-1: none) and its weight as stored.
+struct SlotWeight {
+  int id;
+  float raw;
+};
+__device__ __forceinline__ SlotWeight load_slot(const SumArgs& p, int t) {
   static_assert(kMaxTopK == kWave, "a slot per lane");
-  const int s = threadIdx.x;
-  float v = 0.0f;
-  int e = -1;
-  if (s < p.k) {
-    const int a = t * p.k + s;
-    e = load_id(p.ids, a, p.E);
-    v = p.wbf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.weights)[a])
-                : static_cast<const float*>(p.weights)[a];
-  }
-  if (entries) entries[s] = e >= 0 ? tab[e] : MatEntry{};
+  const int s = threadIdx.x & (kWave - 1), a = t * p.k + min(s, p.k - 1);
+  SlotWeight v = {load_id(p.ids, a, p.E),
+                  p.wbf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.weights)[a])
+                          : static_cast<const float*>(p.weights)[a]};
+  if (s >= p.k) v = {-1, 0.0f};
+  return v;
+}
+__device__ __forceinline__ float slot_weight(const SumArgs& p, int t, const SlotWeight& v,
+                                             bool writer) {
+  const int s = threadIdx.x & (kWave - 1);
+  float w = v.raw;
   if (p.normalize) {
-    float sum = v;
+    float sum = w;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-    v = v / (sum + 1e-20f);
+    w = w / (sum + 1e-20f);
   }
-  id[s] = e;
-  w[s] = v;
   if (writer && s < p.k) {
-    if (p.sel_out) p.sel_out[t * p.k + s] = e;
-    if (p.wts_out) p.wts_out[t * p.k + s] = v;
+    if (p.sel_out) p.sel_out[t * p.k + s] = v.id;
+    if (p.wts_out) p.wts_out[t * p.k + s] = w;
   }
+  return w;
 }
 
 // ---------------------------------------------------------------------------
@@ -639,23 +748,30 @@ __device__ __forceinline__ void slot_weights(const SumArgs& p, int t, bool write
 constexpr int kCombineThreads = 128;
 
 __global__ __launch_bounds__(kCombineThreads) void few_combine_kernel(SumArgs p, const float* y0) {
-  __shared__ float w[kMaxTopK];
-  __shared__ int id[kMaxTopK];
   const int t = blockIdx.y;
-  if (threadIdx.x < kWave) slot_weights(p, t, blockIdx.x == 0, id, w);
-  lds_barrier();
+  const SlotWeight sw = load_slot(p, t);  // (in every wave: no barrier)
   const int n = (blockIdx.x * kCombineThreads + threadIdx.x) * 4;
-  if (n >= p.d) return;
+  const float* y = y0 + (int64_t)t * p.k * p.d + min(n, p.d - 4);
   f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  const float* y = y0 + (int64_t)t * p.k * p.d + n;
-#pragma unroll 4
-  for (int s = 0; s < p.k; ++s) {
-    if (id[s] < 0) continue;
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(y + (int64_t)s * p.d);
-    const float f = w[s];
+  float weight = 0.0f;
+  constexpr int S = 8;  // rows on their way together, before it is known which count
+  for (int s0 = 0; s0 < p.k; s0 += S) {
+    f32x4_t v[S];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+    for (int s = 0; s < S; ++s)
+      v[s] = *reinterpret_cast<const f32x4_t*>(y + (int64_t)min(s0 + s, p.k - 1) * p.d);
+    if (s0 == 0) weight = slot_weight(p, t, sw, blockIdx.x == 0 && threadIdx.x < kWave);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      // (a slot's row is written only where it names an expert)
+      const int lane = min(s0 + s, kWave - 1);
+      if (s0 + s >= p.k || __builtin_amdgcn_readlane(sw.id, lane) < 0) continue;
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), lane));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[s][i], acc[i]);
+    }
   }
+  if (n >= p.d) return;
   if (p.out_f32) {
     *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + t * p.ldo + n) = acc;
   } else {
@@ -674,22 +790,21 @@ constexpr int kTokenWaves = 16;
 
 template <class W, int DEPTH>
 __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p, Stack w,
-                                                                      const MatEntry* tab,
+                                                                      const MatEntry* entry,
                                                                       const void* h, int64_t ldh,
                                                                       int64_t lo, int tiles) {
   using Row = typename W::Row;
   constexpr int PL = sizeof(Row) == 2 ? 2 : 1;
   __shared__ float red[kTokenWaves][W::NC];
-  __shared__ float wts[kMaxTopK];
-  __shared__ int id[kMaxTopK];
-  __shared__ MatEntry mats[kMaxTopK];  // length 0 where a slot names no expert
   const int unit = unit_of_block(kPairs, p.T * tiles, tiles);
   if (unit < 0) return;
   const int t = unit / tiles, tile = unit % tiles;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (wave == 0) slot_weights(p, t, tile == 0, id, wts, tab, mats);
-  lds_barrier();
+  // A slot a lane, in every wave: no barrier before the weights are on their way.
+  // An entry of length 0 is a slot without an expert.
+  const MatEntry mine = load_entry(entry + t * p.k + min(lane, p.k - 1));
+  const SlotWeight sw = load_slot(p, t);
   const int n0 = tile * W::NC;
   const uint32_t boff = W::lane_offset(w, n0, p.d, lane);
   const uint32_t aoff = (lane >> 4) * 16;
@@ -703,14 +818,16 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
       ++s;
       n = 0;
       if (s < p.k) {
-        mat.off = __builtin_amdgcn_readfirstlane(mats[s].off);
-        mat.len = __builtin_amdgcn_readfirstlane(mats[s].len);
-        mat.base = __builtin_amdgcn_readfirstlane(mats[s].base);
+        mat.off = __builtin_amdgcn_readlane(mine.off, s);
+        mat.len = __builtin_amdgcn_readlane(mine.len, s);
+        mat.base = __builtin_amdgcn_readlane(mine.base, s);
         n = (mat.len + W::KS - 1) / W::KS;
       }
     }
   };
   settle();
+  float weight = 0.0f;
+  bool weighed = false;
   float total[W::C];
 #pragma unroll
   for (int c = 0; c < W::C; ++c) total[c] = 0.0f;
@@ -730,6 +847,10 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
       j += kTokenWaves;
       settle();
     }
+    if (!weighed) {
+      weighed = true;
+      weight = slot_weight(p, t, sw, wave == 0 && tile == 0);
+    }
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (slot[d] >= p.k) continue;
@@ -737,11 +858,13 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
 #pragma unroll
       for (int c = 0; c < W::C; ++c) acc[0][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
       b[d].mma(a[d], 1, acc);
-      const float f = wts[slot[d]];
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), slot[d]));
 #pragma unroll
       for (int c = 0; c < W::C; ++c) total[c] = fmaf(f, acc[0][c][0], total[c]);
     }
   }
+  // (a wave without steps may still be the one that writes the choice)
+  if (!weighed) slot_weight(p, t, sw, wave == 0 && tile == 0);
   // every row of the tile is the token's; the first lanes hold row 0
   if (lane < 16) {
 #pragma unroll
@@ -771,31 +894,38 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const void* x, int
                                                               const void* wr, int64_t ldwr, int E,
                                                               int d, float* logits, int ldl) {
   __shared__ float red[kWaves][16][16];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int t0 = blockIdx.y * 16, e0 = blockIdx.x * 16;
   const int64_t ra = (int64_t)min(t0 + (lane & 15), T - 1) * ldx;
   const int64_t rb = (int64_t)min(e0 + (lane & 15), E - 1) * ldwr;
   constexpr int KS = F32 ? 16 : 32, PER = F32 ? 4 : 8;
   f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int k0 = wave * KS; k0 < d; k0 += kWaves * KS) {
-    const int k = k0 + (lane >> 4) * PER;
-    if constexpr (F32) {
-      f32x4_t a = {}, b = {};
-      if (k < d) {
-        a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(x) + ra + k);
-        b = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(wr) + rb + k);
-      }
+  // (as slot_logits)
+  constexpr int U = 4;
+  using V = typename std::conditional<F32, f32x4_t, bf16x8_t>::type;
+  using Row = typename std::conditional<F32, float, uint16_t>::type;
+  const int per = (d + kWaves * KS - 1) / (kWaves * KS) * KS, end = min(d, wave * per + per);
+  for (int k0 = wave * per; k0 < end; k0 += U * KS) {
+    V a[U], b[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
-    } else {
-      bf16x8_t a = {}, b = {};
-      if (k < d) {
-        a = *reinterpret_cast<const bf16x8_t*>(static_cast<const uint16_t*>(x) + ra + k);
-        b = *reinterpret_cast<const bf16x8_t*>(static_cast<const uint16_t*>(wr) + rb + k);
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * KS + (lane >> 4) * PER, kc = k < end ? k : 0;
+      a[u] = *reinterpret_cast<const V*>(static_cast<const Row*>(x) + ra + kc);
+      b[u] = *reinterpret_cast<const V*>(static_cast<const Row*>(wr) + rb + kc);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = k0 + u * KS + (lane >> 4) * PER < end;
+      a[u] = in ? a[u] : V{};
+      b[u] = in ? b[u] : V{};
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][j], b[u][j], acc, 0, 0, 0);
+      } else {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[u], b[u], acc, 0, 0, 0);
       }
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
     }
   }
 #pragma unroll
@@ -836,17 +966,10 @@ int launch_tiles(FewArgs p, hipStream_t stream) {
 
 template <class W, int MODE, int NS>
 int launch(const FewArgs& p, hipStream_t stream) {
-#ifndef FEW_W
-#define FEW_W 1
-#endif
-#ifndef FEW_D
-#define FEW_D 1
-#endif
-  constexpr int D = FEW_D;
   // row tiles in one pass over the weights: the mean number of rows, doubled
   const int64_t rows = p.ids.p || p.logits ? 2 * (int64_t)p.T * p.k / p.E : p.T;
-  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, D>(p, stream)
-                    : launch_tiles<W, MODE, 2, NS, false, D >= 2 ? D / 2 : 1>(p, stream);
+  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, 1>(p, stream)
+                    : launch_tiles<W, MODE, 2, NS, false, 1>(p, stream);
 }
 
 // Waves that split K, `steps` steps long for the longest matrix.
@@ -858,7 +981,7 @@ int split_waves(int64_t steps) {
 
 // Whether the call's assignments share few experts: a workgroup then takes one
 // assignment, and one token's down projections at once.
-bool few_pairs(int64_t T, int64_t k, int64_t E) { return T * k * 2 <= E && E <= 256; }
+bool few_pairs(int64_t T, int64_t k, int64_t E) { return T * k * 2 <= E && E <= kSlotExperts; }
 
 template <int CB, int MODE, int NS>
 int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
@@ -876,7 +999,7 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
   // the columns of an up projection's tile are fixed (kTileCols)
   const int steps = div_up(max_k, format == VMOE_FEW_Q4 ? kQ4Rows : format ? 16 : 32);
   p.wk = kWaves;
-  if (MODE == kDown) p.wk = split_waves(format != VMOE_FEW_Q4 ? div_up(steps, FEW_W) : steps);
+  if (MODE == kDown) p.wk = split_waves(steps);
   if (MODE == kUp && few_pairs(p.T, p.k, p.E)) {
     if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, MODE, 1, NS, true, 4>(p, stream);
     if (format == VMOE_FEW_F32) return launch_tiles<WF32, MODE, 1, NS, true, 2>(p, stream);
@@ -896,19 +1019,19 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
 }
 
 template <class W, int DEPTH>
-int launch_token(const SumArgs& p, const Stack& w, const MatEntry* tab, const void* h, int64_t ldh,
+int launch_token(const SumArgs& p, const Stack& w, const MatEntry* entry, const void* h, int64_t ldh,
                  int64_t lo, hipStream_t stream) {
   const int tiles = div_up(p.d, W::NC);
   const int64_t units = (int64_t)p.T * tiles;
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
   VMOE_LAUNCH((few_token_kernel<W, DEPTH>), dim3(div_up(units, 16) * 16), dim3(kTokenWaves * kWave),
-              0, stream, p, w, tab, h, ldh, lo, tiles);
+              0, stream, p, w, entry, h, ldh, lo, tiles);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
 }
 
 struct FewLayout {
-  int64_t logits, prob, sel, h, y, bytes, ldh, ldl;
+  int64_t logits, prob, sel, entry, h, y, bytes, ldh, ldl;
 };
 
 bool few_layout(int64_t T, int64_t E, int64_t k, int64_t d, int64_t w, int format, FewLayout& L) {
@@ -926,6 +1049,7 @@ bool few_layout(int64_t T, int64_t E, int64_t k, int64_t d, int64_t w, int forma
   L.logits = slot(4 * T * L.ldl);
   L.prob = slot(4 * A);
   L.sel = slot(4 * A);
+  L.entry = slot(sizeof(MatEntry) * A);
   L.h = slot(4 * A * L.ldh);  // fp32, or two bf16 halves
   L.y = slot(4 * A * d);
   L.bytes = std::max<int64_t>(off, 256);
@@ -979,8 +1103,8 @@ int check_rows(int64_t T, const void* x, int64_t ldx, int64_t cols, const void* 
 
 // Up, down and sum; the choice of experts is the logits' or the caller's ids'.
 int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const float* logits,
-                int32_t* sel, float* prob, const SumArgs& c, const FewLayout& L, char* ws,
-                hipStream_t stream) {
+                const void* wr, int64_t ldwr, int32_t* sel, float* prob, const SumArgs& c,
+                const FewLayout& L, char* ws, hipStream_t stream) {
   FewArgs p = {};
   p.w = {w.w1, w.scales1, w.ldw1};
   p.tab = reinterpret_cast<const MatEntry*>(w.table1);
@@ -992,6 +1116,10 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const flo
   p.logits = logits;
   p.ldl = (int)L.ldl;
   p.ids = c.ids;
+  p.wr = wr;
+  p.ldwr = ldwr;
+  p.tab2 = reinterpret_cast<const MatEntry*>(w.table2);
+  p.entry = reinterpret_cast<MatEntry*>(ws + L.entry);
   p.sel = sel;
   p.prob = prob;
   p.fixed = (int)w.hidden;
@@ -1011,13 +1139,13 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const flo
   if (few_pairs(c.T, c.k, c.E)) {
     const void* h = ws + L.h;
     if (w.format == VMOE_FEW_BF16)
-      return launch_token<WBf16<2>, 4>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+      return launch_token<WBf16<2>, 4>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
     if (w.format == VMOE_FEW_F32)
-      return launch_token<WF32, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+      return launch_token<WF32, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
     switch (w.group) {
-      case 32: return launch_token<WQ4<1, 1>, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
-      case 64: return launch_token<WQ4<1, 2>, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
-      default: return launch_token<WQ4<1, 4>, 2>(c, p.w, p.tab, h, p.ldo, p.lo, stream);
+      case 32: return launch_token<WQ4<1, 1>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
+      case 64: return launch_token<WQ4<1, 2>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
+      default: return launch_token<WQ4<1, 4>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
     }
   }
   p.a = ws + L.h;
@@ -1073,6 +1201,12 @@ extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t 
   char* ws = static_cast<char*>(workspace);
   float* logits = reinterpret_cast<float*>(ws + L.logits);
   const int T = (int)num_tokens, E = w->num_experts;
+  int32_t* sel = reinterpret_cast<int32_t*>(ws + L.sel);
+  float* prob = reinterpret_cast<float*>(ws + L.prob);
+  const SumArgs c = {T, top_k, E, (int)w->hidden, {sel, 0}, prob, 0, normalize != 0, out, ldo, f32,
+                     selected, weights};
+  if (few_pairs(T, top_k, E) && E <= kFusedExperts && w->hidden * E * (f32 ? 4 : 2) <= kFusedBytes)
+    return few_experts(*w, x, ldx, nullptr, router_weight, ldwr, sel, prob, c, L, ws, stream);
   const dim3 grid(div_up(L.ldl, 16), div_up(T, 16));
   if (f32)
     VMOE_LAUNCH((few_logits_kernel<true>), grid, dim3(kThreads), 0, stream, x, ldx, T,
@@ -1081,11 +1215,7 @@ extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t 
     VMOE_LAUNCH((few_logits_kernel<false>), grid, dim3(kThreads), 0, stream, x, ldx, T,
                 router_weight, ldwr, E, (int)w->hidden, logits, (int)L.ldl);
   VMOE_CHECK_LAUNCH();
-  int32_t* sel = reinterpret_cast<int32_t*>(ws + L.sel);
-  float* prob = reinterpret_cast<float*>(ws + L.prob);
-  const SumArgs c = {T, top_k, E, (int)w->hidden, {sel, 0}, prob, 0, normalize != 0, out, ldo, f32,
-                     selected, weights};
-  return few_experts(*w, x, ldx, logits, sel, prob, c, L, ws, stream);
+  return few_experts(*w, x, ldx, logits, nullptr, 0, sel, prob, c, L, ws, stream);
 }
 
 extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_t ldx,
@@ -1111,7 +1241,7 @@ extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_
   const SumArgs c = {(int)num_tokens, top_k, w->num_experts, (int)w->hidden, {ids, ids_are_i64},
                      weights, weights_are_bf16, 0, out, ldo, w->format == VMOE_FEW_F32, nullptr,
                      nullptr};
-  return few_experts(*w, x, ldx, nullptr, nullptr, nullptr, c, L, ws, stream);
+  return few_experts(*w, x, ldx, nullptr, nullptr, 0, nullptr, nullptr, c, L, ws, stream);
 }
 
 extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids,

@@ -142,11 +142,11 @@ class _Experts:
         self._desc_ptr = ctypes.addressof(self._desc)
         return self._desc
 
-    def _workspace_bytes(self, T: int, k: int) -> int:
-        n = self._bytes.get((T, k))
-        if n is None:
-            n = self._bytes[(T, k)] = int(_lib.lib().vmoe_few_workspace_bytes(
-                T, self.num_experts, k, self.hidden, self._max_width, self._format))
+    def _workspace_bytes(self, T: int, k: int, what: str) -> int:
+        """Of a call of this size (refused if it is too large); kept in _bytes."""
+        _check_count(T, k, what)
+        n = self._bytes[(T, k)] = int(_lib.lib().vmoe_few_workspace_bytes(
+            T, self.num_experts, k, self.hidden, self._max_width, self._format))
         return n
 
 
@@ -239,6 +239,7 @@ class QuantizedMatrices:
         self.lengths, self.stacked, self.group_size = lengths, stacked, group_size
         self.fixed, self.total, self.max_len = fixed, total, max(lengths)
         self.device = w.device
+        self._sizes: set = set()  # (rows, ids a row) of calls that were checked
 
         self._table, count = _entries(tuple(lengths), fixed, by_rows, each, w.device)
         with _on(w.device):
@@ -311,9 +312,14 @@ def quantize_experts(w1, w2, expert_widths, activation="relu_squared",
     return QuantizedExperts(w1, w2, expert_widths, activation, group_size)
 
 
-def _rows(x: torch.Tensor, width: int, dtype, device, what: str) -> torch.Tensor:
-    """x as rows of `width` values that the kernels can read (copied if they
-    are not contiguous or not 16-byte aligned)."""
+def _rows(x: torch.Tensor, width: int, dtype, device, what: str):
+    """(x, address, row stride, rows): x as rows of `width` values that the
+    kernels can read, copied if they are not contiguous or not 16-byte aligned."""
+    if (x.dtype is dtype and x.device == device and x.dim() and x.shape[-1] == width and
+            x.is_contiguous()):
+        at = x.data_ptr()
+        if not at % 16:
+            return x, at, width, x.numel() // width
     _lib.require_gpu(x, what)
     if x.dim() < 1 or x.shape[-1] != width:
         raise ValueError(f"{what} must have {width} values in its last dimension "
@@ -325,10 +331,11 @@ def _rows(x: torch.Tensor, width: int, dtype, device, what: str) -> torch.Tensor
     if x.dim() != 2:
         x = x.reshape(-1, width)
     mult = 4 if dtype == torch.float32 else 8
-    if (x.stride(1) != 1 or x.stride(0) % mult or x.data_ptr() % 16 or
-            (x.shape[0] > 1 and x.stride(0) < width)):
+    one = x.shape[0] <= 1  # (the stride of a single row is arbitrary)
+    if (x.stride(1) != 1 or x.data_ptr() % 16 or
+            (not one and (x.stride(0) % mult or x.stride(0) < width))):
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    return x, x.data_ptr(), width if one else x.stride(0), x.shape[0]
 
 
 def _check_count(T: int, k: int, what: str) -> None:
@@ -338,11 +345,6 @@ def _check_count(T: int, k: int, what: str) -> None:
         raise NotImplementedError(
             f"{what} takes at most {few_tokens_max()} tokens and {_MAX_PAIRS} token-expert pairs "
             f"(got {T} x {k}); larger batches are the layer's own forward's")
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    # (the stride of a single row is arbitrary)
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True,
@@ -357,30 +359,25 @@ def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True
     return_routing also the chosen experts int32 [tokens, top_k] (largest logit
     first) and their fp32 weights. (TritonMoEMLP.forward rounds its logits to
     bf16, so that near ties may fall differently there.)"""
-    d = experts.hidden
-    rows = _rows(x, d, experts.dtype, experts.device, "x")
-    T = rows.shape[0]
+    d, E, dev, dtype = experts.hidden, experts.num_experts, experts.device, experts.dtype
     k = int(top_k)
-    E = experts.num_experts
     if not 1 <= k <= E:
         raise ValueError(f"top_k must be between 1 and {E} (got {top_k})")
-    _check_count(T, k, "moe_few_tokens")
-    if router_weight.shape != (E, d):
+    if router_weight.dim() != 2 or router_weight.shape[0] != E:
         raise ValueError(f"router_weight must be [{E}, {d}] (got {tuple(router_weight.shape)})")
-    wr = _rows(router_weight, d, experts.dtype, experts.device, "router_weight")
-    dev = x.device
-    n = experts._workspace_bytes(T, k)
+    rows, at, ldx, T = _rows(x, d, dtype, dev, "x")
+    wr, wr_at, ldwr, _ = _rows(router_weight, d, dtype, dev, "router_weight")
+    n = experts._bytes.get((T, k)) or experts._workspace_bytes(T, k, "moe_few_tokens")
     with _on(dev):
-        out = torch.empty((T, d), dtype=experts.dtype, device=dev)
+        out = torch.empty(x.shape, dtype=dtype, device=dev)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         sel = wts = None
         if return_routing:
             sel = torch.empty((T, k), dtype=torch.int32, device=dev)
             wts = torch.empty((T, k), dtype=torch.float32, device=dev)
-        _lib.call("vmoe_few_layer", experts._weights(), rows.data_ptr(), _row_stride(rows), T,
-                  wr.data_ptr(), _row_stride(wr), k, int(bool(normalize)), out.data_ptr(), d,
-                  _lib.ptr(sel), _lib.ptr(wts), ws.data_ptr(), n, _lib.stream(dev))
-    out = out.view(x.shape)
+        _lib.call("vmoe_few_layer", experts._weights(), at, ldx, T, wr_at, ldwr, k,
+                  1 if normalize else 0, out.data_ptr(), d, _lib.ptr(sel), _lib.ptr(wts),
+                  ws.data_ptr(), n, _lib.stream(dev))
     return (out, sel, wts) if return_routing else out
 
 
@@ -392,34 +389,32 @@ def experts_few_tokens(x, selected, weights, experts):
     weights [..., k] bf16 or fp32, a row for each of x. An id outside
     0..num_experts-1 (say -1, for the padding of a batch) is no expert: a token
     without any gets zeros. An expert named twice counts twice."""
-    d = experts.hidden
-    rows = _rows(x, d, experts.dtype, experts.device, "x")
-    T = rows.shape[0]
-    ids, k = _ids(selected, T, experts.device, "selected")
+    d, dev, dtype = experts.hidden, experts.device, experts.dtype
+    rows, at, ldx, T = _rows(x, d, dtype, dev, "x")
+    ids, k = _ids(selected, T, dev, "selected")
     if weights.shape != selected.shape:
         raise ValueError(f"weights must have the shape of selected, {tuple(selected.shape)} "
                          f"(got {tuple(weights.shape)})")
     if weights.dtype not in (torch.bfloat16, torch.float32):
         raise NotImplementedError(f"weights must be bfloat16 or float32 (got {weights.dtype})")
-    if weights.device != experts.device:
-        raise ValueError(f"weights are on {weights.device}, the experts on {experts.device}")
-    _check_count(T, k, "experts_few_tokens")
+    if weights.device != dev:
+        raise ValueError(f"weights are on {weights.device}, the experts on {dev}")
+    n = experts._bytes.get((T, k)) or experts._workspace_bytes(T, k, "experts_few_tokens")
     wts = weights if weights.is_contiguous() else weights.contiguous()
-    dev = x.device
-    n = experts._workspace_bytes(T, k)
     with _on(dev):
-        out = torch.empty((T, d), dtype=experts.dtype, device=dev)
+        out = torch.empty(x.shape, dtype=dtype, device=dev)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.call("vmoe_few_experts", experts._weights(), rows.data_ptr(), _row_stride(rows), T,
-                  ids.data_ptr(), int(ids.dtype == torch.int64), wts.data_ptr(),
+        _lib.call("vmoe_few_experts", experts._weights(), at, ldx, T, ids.data_ptr(),
+                  int(ids.dtype == torch.int64), wts.data_ptr(),
                   int(wts.dtype == torch.bfloat16), k, out.data_ptr(), d, ws.data_ptr(), n,
                   _lib.stream(dev))
-    return out.view(x.shape)
+    return out
 
 
 def _ids(ids, T: int, device, what: str):
     """(contiguous ids, ids a row)."""
-    _lib.require_gpu(ids, what)
+    if not ids.is_cuda:
+        _lib.require_gpu(ids, what)
     if ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what} must be int32 or int64 (got {ids.dtype})")
     if ids.dim() < 1 or ids.shape[-1] < 1 or ids.numel() != T * ids.shape[-1]:
@@ -441,9 +436,8 @@ def matvec_q4(x, q: QuantizedMatrices, ids=None):
     if q.stacked != "columns":
         raise NotImplementedError("matvec_q4 takes matrices that are side by side "
                                   "(stacked='columns')")
-    K, N = q.fixed, q.max_len
-    rows = _rows(x, K, torch.bfloat16, q.device, "x")
-    T = rows.shape[0]
+    K, N, dev = q.fixed, q.max_len, q.device
+    rows, at, ldx, T = _rows(x, K, torch.bfloat16, dev, "x")
     if ids is None:
         if len(q.lengths) != 1:
             raise ValueError(f"q holds {len(q.lengths)} matrices: ids must say which")
@@ -452,15 +446,16 @@ def matvec_q4(x, q: QuantizedMatrices, ids=None):
         if ids.shape[:-1] != x.shape[:-1]:
             raise ValueError(f"ids must have a row for each of x: {tuple(x.shape[:-1])} "
                              f"(got {tuple(ids.shape)})")
-        ids, k = _ids(ids, T, q.device, "ids")
+        ids, k = _ids(ids, T, dev, "ids")
         shape = (*x.shape[:-1], k, N)
     if len(q.lengths) > _MAX_EXPERTS:
         raise NotImplementedError(f"matvec_q4 takes at most {_MAX_EXPERTS} matrices")
-    _check_count(T, k, "matvec_q4")
-    dev = x.device
+    if (T, k) not in q._sizes:
+        _check_count(T, k, "matvec_q4")
+        q._sizes.add((T, k))
     with _on(dev):
         y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        _lib.call("vmoe_q4_matvec", rows.data_ptr(), _row_stride(rows), T, _lib.ptr(ids),
+        _lib.call("vmoe_q4_matvec", at, ldx, T, _lib.ptr(ids),
                   int(ids is not None and ids.dtype == torch.int64), k, q.codes.data_ptr(),
                   q.scales.data_ptr(), q._table.data_ptr(), len(q.lengths), K, N, q.group_size,
                   y.data_ptr(), N, _lib.stream(dev))
