@@ -98,27 +98,32 @@ struct WBf16 {
     return ((uint32_t)(lane >> 4) * 8 * (uint32_t)w.ld + n) * 2;
   }
 
-  // Rows past K are zero.
+  // Every lane loads, so that the number of loads in flight is known where their
+  // results are awaited: rows past K are those of the first lanes, and finish()
+  // takes them as zeros.
   __device__ __forceinline__ void load(const Stack& w, const MatEntry& m, bool by_rows, int k0,
                                        int K, int, int, uint32_t off, int lane) {
     const uint16_t* p = static_cast<const uint16_t*>(w.w) +
                         ((by_rows ? (int64_t)m.off : 0) + k0) * w.ld + (by_rows ? 0 : m.off);
-    if (k0 + KS <= K) {
+    const uint32_t down = (lane >> 4) * 8;
+    if (k0 + (int)down >= K) off -= down * (uint32_t)w.ld * 2;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = at<V>(p + j * w.ld, off);
-    } else {
-      const bool in = k0 + (lane >> 4) * 8 < K;
+    for (int j = 0; j < 8; ++j) r[j] = at<V>(p + j * w.ld, off);
+  }
+  __device__ __forceinline__ void finish(int k0, int K, int lane) {
+    if (k0 + KS <= K) return;
+    const bool in = k0 + (lane >> 4) * 8 < K;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = in ? at<V>(p + j * w.ld, off) : V{};
-    }
+    for (int j = 0; j < 8; ++j) r[j] = in ? r[j] : V{};
   }
 
   __device__ __forceinline__ static void load_a(A& a, const Row* base, uint32_t off, int k0, int K,
                                                 int lane) {
-    if (k0 + KS <= K)
-      a.v = at<bf16x8_t>(base + k0, off);
-    else
-      a.v = k0 + (lane >> 4) * 8 < K ? at<bf16x8_t>(base + k0, off) : bf16x8_t{};
+    const uint32_t right = (lane >> 4) * 8;
+    a.v = at<bf16x8_t>(base + k0, k0 + (int)right < K ? off : off - right * 2);
+  }
+  __device__ __forceinline__ static void finish_a(A& a, int k0, int K, int lane) {
+    if (k0 + KS > K) a.v = k0 + (lane >> 4) * 8 < K ? a.v : bf16x8_t{};
   }
 
   // Operand of column c: the c-th value of each of the 8 rows.
@@ -149,20 +154,22 @@ struct WBf16 {
   }
 };
 
-// fp32, row-major: four columns a lane and 16 rows a step, lane group g taking
-// rows 4 g..4 g + 3.
+// fp32, row-major: CPL (four or two) columns a lane and 16 rows a step, lane group
+// g taking rows 4 g..4 g + 3.
+template <int CPL>
 struct WF32 {
-  static constexpr int KS = 16, C = 4, NC = 64;
+  static constexpr int KS = 16, C = CPL, NC = 16 * CPL;
+  using V = typename std::conditional<CPL == 4, f32x4_t, f32x2_t>::type;
   using Row = float;
   struct A {
     f32x4_t v;
   };
-  f32x4_t r[4];
+  V r[4];
 
-  __device__ __forceinline__ static int col(int c, int lane) { return (lane & 15) * 4 + c; }
+  __device__ __forceinline__ static int col(int c, int lane) { return (lane & 15) * CPL + c; }
 
   __device__ __forceinline__ static uint32_t lane_offset(const Stack& w, int n0, int N, int lane) {
-    const int n = min(n0 + (lane & 15) * 4, N - 4);
+    const int n = min(n0 + (lane & 15) * CPL, N - CPL);
     return ((uint32_t)(lane >> 4) * 4 * (uint32_t)w.ld + n) * 4;
   }
 
@@ -170,22 +177,25 @@ struct WF32 {
                                        int K, int, int, uint32_t off, int lane) {
     const float* p = static_cast<const float*>(w.w) +
                      ((by_rows ? (int64_t)m.off : 0) + k0) * w.ld + (by_rows ? 0 : m.off);
-    if (k0 + KS <= K) {
+    const uint32_t down = (lane >> 4) * 4;
+    if (k0 + (int)down >= K) off -= down * (uint32_t)w.ld * 4;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = at<f32x4_t>(p + j * w.ld, off);
-    } else {
-      const bool in = k0 + (lane >> 4) * 4 < K;
+    for (int j = 0; j < 4; ++j) r[j] = at<V>(p + j * w.ld, off);
+  }
+  __device__ __forceinline__ void finish(int k0, int K, int lane) {
+    if (k0 + KS <= K) return;
+    const bool in = k0 + (lane >> 4) * 4 < K;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = in ? at<f32x4_t>(p + j * w.ld, off) : f32x4_t{};
-    }
+    for (int j = 0; j < 4; ++j) r[j] = in ? r[j] : V{};
   }
 
   __device__ __forceinline__ static void load_a(A& a, const Row* base, uint32_t off, int k0, int K,
                                                 int lane) {
-    if (k0 + KS <= K)
-      a.v = at<f32x4_t>(base + k0, off);
-    else
-      a.v = k0 + (lane >> 4) * 4 < K ? at<f32x4_t>(base + k0, off) : f32x4_t{};
+    const uint32_t right = (lane >> 4) * 4;
+    a.v = at<f32x4_t>(base + k0, k0 + (int)right < K ? off : off - right * 4);
+  }
+  __device__ __forceinline__ static void finish_a(A& a, int k0, int K, int lane) {
+    if (k0 + KS > K) a.v = k0 + (lane >> 4) * 4 < K ? a.v : f32x4_t{};
   }
 
   template <int MT, int PL>
@@ -247,16 +257,22 @@ struct WQ4 {
     }
   }
 
+  __device__ __forceinline__ void finish(int, int, int) {}  // (blocks are whole)
+
   __device__ __forceinline__ static void load_a(A& a, const Row* base, uint32_t off, int k0, int K,
                                                 int lane) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const Row* p = base + k0 + 32 * j;
-      if (k0 + KS <= K)
-        a.v[j] = at<bf16x8_t>(p, off);
-      else
-        a.v[j] = k0 + 32 * j + (lane >> 4) * 8 < K ? at<bf16x8_t>(p, off) : bf16x8_t{};
+      const uint32_t right = (lane >> 4) * 8;
+      a.v[j] = at<bf16x8_t>(base + k0, k0 + 32 * j + (int)right < K ? off + 64 * j
+                                                                   : off - right * 2);
     }
+  }
+  __device__ __forceinline__ static void finish_a(A& a, int k0, int K, int lane) {
+    if (k0 + KS <= K) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      a.v[j] = k0 + 32 * j + (lane >> 4) * 8 < K ? a.v[j] : bf16x8_t{};
   }
 
   template <int MT, int PL>
@@ -300,7 +316,6 @@ struct FewArgs {
   int T, k, E;
   const float* logits;  // kUp: [T, ldl], or nullptr: ids
   int ldl;
-  int early;  // load weights before the rows are known
   Ids ids;
   const void* wr;  // slots: the router's weights, where its logits are formed here
   int64_t ldwr;
@@ -321,48 +336,84 @@ struct FewArgs {
 
 // How many experts of a token come before expert e, whose logit is `mine`:
 // eight lanes share the row (padded to kLogitPad with -inf), each gets the count.
+// HAVE: the row's first values are in registers already.
 constexpr int kLogitPad = 32;
-__device__ __forceinline__ int place_of(const float* l, int ldl, int e, float mine, int part) {
+template <bool HAVE = false>
+__device__ __forceinline__ int place_of(const float* l, int ldl, int e, float mine, int part,
+                                        const f32x4_t* have = nullptr) {
   const uint32_t key = sort_key(mine);
   int before = 0;
-#pragma unroll 4
-  for (int f = part * 4; f < ldl; f += kLogitPad) {
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(l + f);
+  auto count = [&](const f32x4_t& v, int f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t other = sort_key(v[i]);
       before += other > key || (other == key && f + i < e);
     }
-  }
+  };
+  constexpr int N = HAVE ? 4 : 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i * kLogitPad < ldl) count(have[i], part * 4 + i * kLogitPad);
+#pragma unroll 4
+  for (int f = part * 4 + N * kLogitPad; f < ldl; f += kLogitPad)
+    count(*reinterpret_cast<const f32x4_t*>(l + f), f);
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) before += __shfl_xor(before, o, kWave);
   return before;
 }
 
-// The assignments t k + s that take expert e, into LDS; their number. Their
-// order does not matter: each is a row of its own.
-__device__ __forceinline__ int find_rows(const FewArgs& p, int e, bool writer, uint16_t* rows,
-                                         int* count) {
+// The assignments t k + s that take expert e, into LDS, and their number, in two
+// steps: a thread's first loads, then the rest. Loads return in the order of their
+// issue, so what is issued between the two comes after them. The rows' order does
+// not matter: each is on its own.
+struct RowProbe {
+  static constexpr int N = 4;
+  float mine;    // logits: of expert e and of others, for the thread's first token
+  f32x4_t v[N];
+  int id;        // ids: the thread's first one
+};
+__device__ __forceinline__ RowProbe probe_rows(const FewArgs& p, int e) {
+  RowProbe r;
+  if (p.logits) {
+    const float* l = p.logits + (int64_t)min((int)threadIdx.x / 8, p.T - 1) * p.ldl;
+    r.mine = l[e];
+#pragma unroll
+    for (int i = 0; i < RowProbe::N; ++i)
+      r.v[i] = *reinterpret_cast<const f32x4_t*>(
+          l + min((int)(threadIdx.x & 7) * 4 + i * kLogitPad, p.ldl - 4));
+  } else {
+    r.id = load_id(p.ids, min((int)threadIdx.x, p.T * p.k - 1), p.E);
+  }
+  return r;
+}
+__device__ __forceinline__ int find_rows(const FewArgs& p, int e, const RowProbe& first,
+                                         bool writer, uint16_t* rows, int* count) {
   if (threadIdx.x == 0) *count = 0;
   lds_barrier();
   if (p.logits) {
     const int part = threadIdx.x & 7;
-    for (int t = threadIdx.x / 8; t < p.T; t += kThreads / 8) {
-      const float* l = p.logits + (int64_t)t * p.ldl;
-      const float mine = l[e];
-      const int before = place_of(l, p.ldl, e, mine, part);
-      if (before < p.k && part == 0) {
-        const int a = t * p.k + before;
-        rows[atomicAdd(count, 1)] = (uint16_t)a;
-        if (writer) {
-          p.sel[a] = e;
-          p.prob[a] = sigmoid_f32(mine);
-        }
+    auto take = [&](int t, float mine, int before) {
+      if (before >= p.k || part != 0) return;
+      const int a = t * p.k + before;
+      rows[atomicAdd(count, 1)] = (uint16_t)a;
+      if (writer) {
+        p.sel[a] = e;
+        p.prob[a] = sigmoid_f32(mine);
       }
+    };
+    int t = threadIdx.x / 8;
+    const float* l = p.logits + (int64_t)min(t, p.T - 1) * p.ldl;
+    const int before = place_of<true>(l, p.ldl, e, first.mine, part, first.v);
+    if (t < p.T) take(t, first.mine, before);
+    for (t += kThreads / 8; t < p.T; t += kThreads / 8) {
+      l = p.logits + (int64_t)t * p.ldl;
+      const float mine = l[e];
+      take(t, mine, place_of(l, p.ldl, e, mine, part));
     }
   } else {
+    const int want = e < p.E ? e : -1;
     for (int a = threadIdx.x; a < p.T * p.k; a += kThreads)
-      if (load_id(p.ids, a, p.E) == (e < p.E ? e : -1))
+      if ((a < kThreads ? first.id : load_id(p.ids, a, p.E)) == want)
         rows[atomicAdd(count, 1)] = (uint16_t)a;
   }
   lds_barrier();
@@ -450,18 +501,17 @@ __device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer,
     return e;
   }
   const int lane8 = threadIdx.x & 7, t = a / p.k, s = a % p.k;
-  const bool fused = p.wr != nullptr;
-  if (fused) {
-    if (p.E <= 64)
-      slot_logits<Row, 4>(p, t, lg, part);
-    else
-      slot_logits<Row, 8>(p, t, lg, part);
+  if (!p.wr) {
+    if ((int)threadIdx.x < p.ldl) lg[threadIdx.x] = p.logits[(int64_t)t * p.ldl + threadIdx.x];
+    lds_barrier();
+  } else if (p.E <= 64) {
+    slot_logits<Row, 4>(p, t, lg, part);
+  } else {
+    slot_logits<Row, 8>(p, t, lg, part);
   }
-  const float* l = p.logits + (int64_t)t * p.ldl;
   for (int e = threadIdx.x / 8; e < p.E; e += kThreads / 8) {
-    const float mine = fused ? lg[e] : l[e];
-    const int before =
-        fused ? place_of(lg, p.ldl, e, mine, lane8) : place_of(l, p.ldl, e, mine, lane8);
+    const float mine = lg[e];
+    const int before = place_of(lg, p.ldl, e, mine, lane8);
     if (before == s && lane8 == 0) {
       *found = e;
       if (writer) {
@@ -503,19 +553,18 @@ __device__ __forceinline__ int unit_of_block(Order order, int units, int tiles) 
 // Waves a SIMD holds at least: the long K of a down projection's many small tiles is
 // covered by other workgroups (128 experts 576 x 2048: 65 us with two on a CU, 58
 // with three).
-template <class W, int MODE>
-constexpr int kMinWaves = MODE == kDown && sizeof(typename W::Row) == 2 && W::KS == 32 ? 6 : 1;
+template <class W, int MODE, int MT, int DEPTH>
+constexpr int kMinWaves =
+    MODE == kDown && MT == 1 && DEPTH == 1 && sizeof(typename W::Row) == 2 && W::KS == 32 ? 6 : 1;
 
-template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
-__global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE>)) void few_kernel(FewArgs p) {
+template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH, bool EARLY>
+__global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE, MT, DEPTH>)) void few_kernel(FewArgs p) {
   constexpr int PL = (MODE == kDown && sizeof(typename W::Row) == 2) ? 2 : 1;
   constexpr int NC = W::NC;
   constexpr int kPerLane = 16 / sizeof(typename W::Row);  // values of a 16-byte load
   __shared__ float red[NS * 16 * kWaves * NC];            // [NS][wk][16][width]
   __shared__ uint16_t rows[SLOT ? 8 : kMaxRows];
   __shared__ int count;
-  __shared__ MatEntry found[2];
-  static_assert(!SLOT || kSlotExperts * NS <= kThreads, "an entry a thread");
   // kPlain: one matrix more, for the rows that name none (their products are 0)
   const int owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
   int owner, tile;
@@ -542,26 +591,17 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE>)) void few_kernel(Few
   int e = owner, m = 1;
   if constexpr (SLOT) {
     // (red is free until the products are joined)
-    static_assert(NS * 16 * kWaves * NC >= (kWaves + 1) * kFusedExperts, "room for the logits");
-    // the entries of all experts come in meanwhile
-    const MatEntry early_entry = load_entry(p.tab + min((int)threadIdx.x, p.E * NS - 1));
+    static_assert(NS * 16 * kWaves * NC >= (kWaves + 1) * kFusedExperts &&
+                      NS * 16 * kWaves * NC >= kSlotExperts,
+                  "room for the logits");
     e = find_expert<typename W::Row>(p, owner, tile == 0, red, red + kFusedExperts, &count);
     if (e < 0) return;
-    if ((int)threadIdx.x / NS == e) store_entry(&found[threadIdx.x % NS], early_entry);
     if (threadIdx.x == 0) rows[0] = (uint16_t)owner;
     lds_barrier();  // (also: the logits in red have been read)
   }
   MatEntry mats[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    if constexpr (SLOT) {
-      mats[s].off = __builtin_amdgcn_readfirstlane(found[s].off);
-      mats[s].len = __builtin_amdgcn_readfirstlane(found[s].len);
-      mats[s].base = __builtin_amdgcn_readfirstlane(found[s].base);
-    } else {
-      mats[s] = load_entry(p.tab + min(e, p.E - 1) * NS + s);
-    }
-  }
+  for (int s = 0; s < NS; ++s) mats[s] = load_entry(p.tab + min(e, p.E - 1) * NS + s);
   if (MODE == kPlain && e == p.E) mats[0].len = 0;
   const int K = MODE == kDown ? mats[0].len : p.fixed;
   const int N = MODE == kDown ? p.fixed : min(mats[0].len, p.cols);
@@ -575,24 +615,25 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE>)) void few_kernel(Few
     for (int s = 0; s < NS; ++s)
       b[d][s].load(p.w, mats[s], MODE == kDown, k0, K, n0, N, boff, lane);
   };
-  // Where most experts have rows, the first weights are on their way before it
-  // is known which rows.
-  const bool early = !SLOT && p.early && nt < N;
-  if (early) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-      if (first + d * stride < K) load_b(d, first + d * stride);
-  }
   if constexpr (!SLOT) {
-    m = find_rows(p, e, tile == 0, rows, &count);
-    if (m == 0) return;
-    if constexpr (MODE == kPlain) {
+    const RowProbe probe = probe_rows(p, min(e, p.E - 1));
+    if (MODE == kPlain && nt + width > N) {
       // zeros in the columns of wider matrices than this one
+      m = find_rows(p, e, probe, false, rows, &count);
       const int z0 = max(nt, N), zw = min(nt + width, p.cols) - z0;
       for (int x = threadIdx.x; x < m * zw; x += kThreads)
         static_cast<uint16_t*>(p.out)[rows[x / zw] * p.ldo + z0 + x % zw] = 0;
+      if (nt >= N) return;
+      lds_barrier();
     }
-    if (nt >= N) return;
+    // EARLY: where most experts have rows, the first weights are on their way before
+    // it is known which rows (a wave without steps loads some all the same)
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) load_b(d, first + d * stride < K ? first + d * stride : 0);
+    }
+    m = find_rows(p, e, probe, tile == 0, rows, &count);
+    if (m == 0) return;
   }
   const typename W::Row* abase = static_cast<const typename W::Row*>(p.a);
 
@@ -623,7 +664,7 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE>)) void few_kernel(Few
         if constexpr (PL == 2) W::load_a(a[d][i][1], abase + p.lo, aoff[i], k0, K, lane);
       }
     };
-    bool have = early && m0 == 0;
+    bool have = EARLY && m0 == 0;
     for (int k0 = first; k0 < K; k0 += DEPTH * stride) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
@@ -634,9 +675,17 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE>)) void few_kernel(Few
       have = false;
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
-        if (k0 + d * stride >= K) break;
+        const int kd = k0 + d * stride;
+        if (kd >= K) break;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) b[d][s].mma(a[d], tiles, acc[s]);
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int q = 0; q < PL; ++q) W::finish_a(a[d][i][q], kd, K, lane);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          b[d][s].finish(kd, K, lane);
+          b[d][s].mma(a[d], tiles, acc[s]);
+        }
       }
     }
 
@@ -834,12 +883,14 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
   while (s < p.k) {
     W b[DEPTH];
     typename W::A a[DEPTH][1][PL];
-    int slot[DEPTH];
+    int slot[DEPTH], at_k[DEPTH], len[DEPTH];
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       slot[d] = s;
       if (s >= p.k) continue;
       const int k0 = j * W::KS;
+      at_k[d] = k0;
+      len[d] = mat.len;
       b[d].load(w, mat, true, k0, mat.len, n0, p.d, boff, lane);
       const Row* row = static_cast<const Row*>(h) + (int64_t)(t * p.k + s) * ldh;
       W::load_a(a[d][0][0], row, aoff, k0, mat.len, lane);
@@ -857,6 +908,9 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
       f32x4_t acc[1][W::C];
 #pragma unroll
       for (int c = 0; c < W::C; ++c) acc[0][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      b[d].finish(at_k[d], len[d], lane);
+#pragma unroll
+      for (int q = 0; q < PL; ++q) W::finish_a(a[d][0][q], at_k[d], len[d], lane);
       b[d].mma(a[d], 1, acc);
       const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), slot[d]));
 #pragma unroll
@@ -946,8 +1000,8 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const void* x, int
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
-int launch_tiles(FewArgs p, hipStream_t stream) {
+template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH, bool EARLY>
+int launch_early(FewArgs p, hipStream_t stream) {
   const int width = kWaves / p.wk * W::NC;
   p.tiles = div_up(p.cols, width);
   const int64_t owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
@@ -958,17 +1012,24 @@ int launch_tiles(FewArgs p, hipStream_t stream) {
     units = p.num_tiles;
   }
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
-  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS, SLOT, DEPTH>), dim3(div_up(units, 16) * 16),
+  VMOE_LAUNCH((few_kernel<W, MODE, MT, NS, SLOT, DEPTH, EARLY>), dim3(div_up(units, 16) * 16),
               dim3(kThreads), 0, stream, p);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
 }
 
-template <class W, int MODE, int NS>
+template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
+int launch_tiles(const FewArgs& p, hipStream_t stream) {
+  if (!SLOT && (int64_t)p.T * p.k >= p.E)
+    return launch_early<W, MODE, MT, NS, SLOT, DEPTH, !SLOT>(p, stream);
+  return launch_early<W, MODE, MT, NS, SLOT, DEPTH, false>(p, stream);
+}
+
+template <class W, int MODE, int NS, int DEPTH = 1>
 int launch(const FewArgs& p, hipStream_t stream) {
   // row tiles in one pass over the weights: the mean number of rows, doubled
   const int64_t rows = p.ids.p || p.logits ? 2 * (int64_t)p.T * p.k / p.E : p.T;
-  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, 1>(p, stream)
+  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, DEPTH>(p, stream)
                     : launch_tiles<W, MODE, 2, NS, false, 1>(p, stream);
 }
 
@@ -995,27 +1056,35 @@ int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
 // max_k: rows of the longest matrix.
 template <int MODE, int NS>
 int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t stream) {
-  p.early = (int64_t)p.T * p.k >= p.E;
   // the columns of an up projection's tile are fixed (kTileCols)
   const int steps = div_up(max_k, format == VMOE_FEW_Q4 ? kQ4Rows : format ? 16 : 32);
   p.wk = kWaves;
   if (MODE == kDown) p.wk = split_waves(steps);
-  if (MODE == kUp && few_pairs(p.T, p.k, p.E)) {
-    if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, MODE, 1, NS, true, 4>(p, stream);
-    if (format == VMOE_FEW_F32) return launch_tiles<WF32, MODE, 1, NS, true, 2>(p, stream);
-    switch (group) {
-      case 32: return launch_tiles<WQ4<1, 1>, MODE, 1, NS, true, 2>(p, stream);
-      case 64: return launch_tiles<WQ4<1, 2>, MODE, 1, NS, true, 2>(p, stream);
-      default: return launch_tiles<WQ4<1, 4>, MODE, 1, NS, true, 2>(p, stream);
+  if constexpr (MODE == kUp) {
+    if (few_pairs(p.T, p.k, p.E)) {
+      if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, MODE, 1, NS, true, 4>(p, stream);
+      if (format == VMOE_FEW_F32) return launch_tiles<WF32<2>, MODE, 1, NS, true, 2>(p, stream);
+      switch (group) {
+        case 32: return launch_tiles<WQ4<1, 1>, MODE, 1, NS, true, 2>(p, stream);
+        case 64: return launch_tiles<WQ4<1, 2>, MODE, 1, NS, true, 2>(p, stream);
+        default: return launch_tiles<WQ4<1, 4>, MODE, 1, NS, true, 2>(p, stream);
+      }
+    }
+    // (kTileCols columns a workgroup)
+    if (format == VMOE_FEW_Q4) {
+      if constexpr (NS == 1)
+        if (steps > 4) return launch_q4<4, MODE, NS>(p, group, stream);
+      p.wk = 4;
     }
   }
-  if (format == VMOE_FEW_Q4) {
-    if (MODE == kUp && steps > 4) return launch_q4<4, MODE, NS>(p, group, stream);
-    if (MODE == kUp) p.wk = 4;
-    return launch_q4<2, MODE, NS>(p, group, stream);
-  }
-  if (format == VMOE_FEW_BF16) return launch<WBf16<4>, MODE, NS>(p, stream);
-  return launch<WF32, MODE, NS>(p, stream);
+  if (format == VMOE_FEW_Q4) return launch_q4<2, MODE, NS>(p, group, stream);
+  if (format == VMOE_FEW_F32) return launch<WF32<4>, MODE, NS>(p, stream);
+  if constexpr (MODE == kDown)
+    if (steps <= 8) {
+      p.wk = split_waves(div_up(steps, 2));
+      return launch<WBf16<4>, MODE, NS, 2>(p, stream);
+    }
+  return launch<WBf16<4>, MODE, NS>(p, stream);
 }
 
 template <class W, int DEPTH>
@@ -1141,7 +1210,7 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const flo
     if (w.format == VMOE_FEW_BF16)
       return launch_token<WBf16<2>, 4>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
     if (w.format == VMOE_FEW_F32)
-      return launch_token<WF32, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
+      return launch_token<WF32<2>, 4>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
     switch (w.group) {
       case 32: return launch_token<WQ4<1, 1>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
       case 64: return launch_token<WQ4<1, 2>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
@@ -1273,7 +1342,6 @@ extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, cons
   p.cols = (int)max_cols;
   p.out = y;
   p.ldo = ldy;
-  p.early = (int64_t)num_rows * per_row >= num_matrices;
   p.wk = split_waves(div_up(k_rows, kQ4Rows));
   return launch_q4<2, kPlain, 1>(p, group, stream);
 }
