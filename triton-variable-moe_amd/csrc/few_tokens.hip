@@ -317,8 +317,6 @@ struct FewArgs {
   const float* logits;  // kUp: [T, ldl], or nullptr: ids
   int ldl;
   Ids ids;
-  const void* wr;  // slots: the router's weights, where its logits are formed here
-  int64_t ldwr;
   int32_t* sel;  // kUp with logits: chosen experts and their sigmoids, [T, k]
   float* prob;
   const MatEntry* tab2;  // slots: the down projections' entries, and where the
@@ -421,77 +419,10 @@ __device__ __forceinline__ int find_rows(const FewArgs& p, int e, const RowProbe
 }
 
 constexpr int kSlotExperts = 256;  // at most, where a workgroup takes one assignment
-constexpr int kFusedExperts = 128;  // ... and forms its token's logits itself,
-constexpr int64_t kFusedBytes = 256 << 10;  // from router weights of so many bytes
-
-// The logits of token t, padded as place_of wants them, into LDS: the waves split
-// the hidden axis; 16 experts are the rows of an operand and the token every
-// column of the other.
-template <class Row, int ET>
-__device__ __forceinline__ void slot_logits(const FewArgs& p, int t, float* lg, float* part) {
-  constexpr int PER = 16 / sizeof(Row), KS = 4 * PER;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int d = p.fixed;
-  const Row* x = static_cast<const Row*>(p.a) + (int64_t)t * p.lda;
-  const Row* wr = static_cast<const Row*>(p.wr);
-  f32x4_t acc[ET];
-#pragma unroll
-  for (int i = 0; i < ET; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  using V = typename std::conditional<PER == 8, bf16x8_t, f32x4_t>::type;
-  // A wave's columns are adjacent: the rows are a power of two apart in memory, and
-  // it is the columns that spread the waves' reads over the L2's channels. The
-  // loads of U steps go out together.
-  constexpr int U = 16 / ET;
-  const int per = (d + kWaves * KS - 1) / (kWaves * KS) * KS, end = min(d, wave * per + per);
-  for (int k0 = wave * per; k0 < end; k0 += U * KS) {
-    V a[U][ET], b[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * KS + (lane >> 4) * PER, kc = k < end ? k : 0;
-      b[u] = *reinterpret_cast<const V*>(x + kc);
-#pragma unroll
-      for (int i = 0; i < ET; ++i)
-        a[u][i] = *reinterpret_cast<const V*>(
-            wr + min(i * 16 + (lane & 15), p.E - 1) * p.ldwr + kc);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = k0 + u * KS + (lane >> 4) * PER < end;
-      b[u] = in ? b[u] : V{};
-#pragma unroll
-      for (int i = 0; i < ET; ++i) {
-        const V w = in ? a[u][i] : V{};
-        if constexpr (PER == 8) {
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, b[u], acc[i], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], b[u][j], acc[i], 0, 0, 0);
-        }
-      }
-    }
-  }
-  if ((lane & 15) == 0) {
-#pragma unroll
-    for (int i = 0; i < ET; ++i)
-      *reinterpret_cast<f32x4_t*>(&part[wave * kFusedExperts + i * 16 + (lane >> 4) * 4]) = acc[i];
-  }
-  lds_barrier();
-  if (threadIdx.x < kFusedExperts) {
-    float s = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) s += part[v * kFusedExperts + threadIdx.x];
-    lg[threadIdx.x] = (int)threadIdx.x < p.E ? s : -INFINITY;
-  }
-  lds_barrier();
-}
-
 // The expert of assignment a, or -1.
-template <class Row>
 __device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer, float* lg,
-                                           float* part, int* found) {
-  if (!p.logits && !p.wr) {
+                                           int* found) {
+  if (!p.logits) {
     const int e = __builtin_amdgcn_readfirstlane(load_id(p.ids, a, p.E));
     if (writer && threadIdx.x == 0) {
       MatEntry m = load_entry(p.tab2 + max(e, 0));
@@ -501,14 +432,8 @@ __device__ __forceinline__ int find_expert(const FewArgs& p, int a, bool writer,
     return e;
   }
   const int lane8 = threadIdx.x & 7, t = a / p.k, s = a % p.k;
-  if (!p.wr) {
-    if ((int)threadIdx.x < p.ldl) lg[threadIdx.x] = p.logits[(int64_t)t * p.ldl + threadIdx.x];
-    lds_barrier();
-  } else if (p.E <= 64) {
-    slot_logits<Row, 4>(p, t, lg, part);
-  } else {
-    slot_logits<Row, 8>(p, t, lg, part);
-  }
+  if ((int)threadIdx.x < p.ldl) lg[threadIdx.x] = p.logits[(int64_t)t * p.ldl + threadIdx.x];
+  lds_barrier();
   for (int e = threadIdx.x / 8; e < p.E; e += kThreads / 8) {
     const float mine = lg[e];
     const int before = place_of(lg, p.ldl, e, mine, lane8);
@@ -569,10 +494,11 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE, MT, DEPTH>)) void few
   const int owners = SLOT ? p.T * p.k : p.E + (MODE == kPlain ? 1 : 0);
   int owner, tile;
   if constexpr (MODE == kUp && !SLOT) {
-    const int unit = unit_of_block(kRuns, p.num_tiles, 1);
+    const int parts = kTileCols / (kWaves / p.wk * NC);  // a workgroup may take a part
+    const int unit = unit_of_block(kRuns, p.num_tiles * parts, 1);
     if (unit < 0) return;
-    owner = p.tile_of[unit];
-    tile = unit - p.tab[owner * NS].first_tile;
+    owner = p.tile_of[unit / parts];
+    tile = unit - p.tab[owner * NS].first_tile * parts;
   } else {
     const int unit = unit_of_block(SLOT ? kPairs : MODE == kDown ? kDeal : kRuns,
                                    owners * p.tiles, p.tiles);
@@ -591,10 +517,8 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE, MT, DEPTH>)) void few
   int e = owner, m = 1;
   if constexpr (SLOT) {
     // (red is free until the products are joined)
-    static_assert(NS * 16 * kWaves * NC >= (kWaves + 1) * kFusedExperts &&
-                      NS * 16 * kWaves * NC >= kSlotExperts,
-                  "room for the logits");
-    e = find_expert<typename W::Row>(p, owner, tile == 0, red, red + kFusedExperts, &count);
+    static_assert(NS * 16 * kWaves * NC >= kSlotExperts, "room for the logits");
+    e = find_expert(p, owner, tile == 0, red, &count);
     if (e < 0) return;
     if (threadIdx.x == 0) rows[0] = (uint16_t)owner;
     lds_barrier();  // (also: the logits in red have been read)
@@ -955,7 +879,9 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const void* x, int
   const int64_t rb = (int64_t)min(e0 + (lane & 15), E - 1) * ldwr;
   constexpr int KS = F32 ? 16 : 32, PER = F32 ? 4 : 8;
   f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  // (as slot_logits)
+  // A wave's columns are adjacent: the rows are a power of two apart in memory, and it
+  // is the columns that spread the waves' reads over the L2's channels. The loads of
+  // U steps go out together.
   constexpr int U = 4;
   using V = typename std::conditional<F32, f32x4_t, bf16x8_t>::type;
   using Row = typename std::conditional<F32, float, uint16_t>::type;
@@ -1008,8 +934,8 @@ int launch_early(FewArgs p, hipStream_t stream) {
   // (dealt owners: eight at a time)
   int64_t units = (MODE == kDown ? div_up(owners, 8) * 8 : owners) * (int64_t)p.tiles;
   if (MODE == kUp && !SLOT) {
-    if (width != kTileCols) return VMOE_ERR_UNSUPPORTED;
-    units = p.num_tiles;
+    if (kTileCols % width) return VMOE_ERR_UNSUPPORTED;
+    units = (int64_t)p.num_tiles * (kTileCols / width);
   }
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
   VMOE_LAUNCH((few_kernel<W, MODE, MT, NS, SLOT, DEPTH, EARLY>), dim3(div_up(units, 16) * 16),
@@ -1053,6 +979,17 @@ int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
   }
 }
 
+template <int NS>
+int launch_slots(const FewArgs& p, int format, int group, hipStream_t stream) {
+  if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, kUp, 1, NS, true, 4>(p, stream);
+  if (format == VMOE_FEW_F32) return launch_tiles<WF32<2>, kUp, 1, NS, true, 2>(p, stream);
+  switch (group) {
+    case 32: return launch_tiles<WQ4<1, 1>, kUp, 1, NS, true, 2>(p, stream);
+    case 64: return launch_tiles<WQ4<1, 2>, kUp, 1, NS, true, 2>(p, stream);
+    default: return launch_tiles<WQ4<1, 4>, kUp, 1, NS, true, 2>(p, stream);
+  }
+}
+
 // max_k: rows of the longest matrix.
 template <int MODE, int NS>
 int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t stream) {
@@ -1061,23 +998,27 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
   p.wk = kWaves;
   if (MODE == kDown) p.wk = split_waves(steps);
   if constexpr (MODE == kUp) {
-    if (few_pairs(p.T, p.k, p.E)) {
-      if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, MODE, 1, NS, true, 4>(p, stream);
-      if (format == VMOE_FEW_F32) return launch_tiles<WF32<2>, MODE, 1, NS, true, 2>(p, stream);
-      switch (group) {
-        case 32: return launch_tiles<WQ4<1, 1>, MODE, 1, NS, true, 2>(p, stream);
-        case 64: return launch_tiles<WQ4<1, 2>, MODE, 1, NS, true, 2>(p, stream);
-        default: return launch_tiles<WQ4<1, 4>, MODE, 1, NS, true, 2>(p, stream);
-      }
-    }
-    // (kTileCols columns a workgroup)
+    if (few_pairs(p.T, p.k, p.E))
+      return launch_slots<NS>(p, format, group, stream);
+    // A workgroup takes kTileCols columns, or half of them where the tiles are fewer
+    // than CUs.
     if (format == VMOE_FEW_Q4) {
+      if (steps > 4 && p.num_tiles < 256) return launch_q4<2, MODE, NS>(p, group, stream);
       if constexpr (NS == 1)
         if (steps > 4) return launch_q4<4, MODE, NS>(p, group, stream);
       p.wk = 4;
+      return launch_q4<2, MODE, NS>(p, group, stream);
     }
+    if (p.num_tiles < 256)
+      return format == VMOE_FEW_F32 ? launch<WF32<2>, MODE, NS>(p, stream)
+                                    : launch<WBf16<2>, MODE, NS>(p, stream);
+  } else if (format == VMOE_FEW_Q4) {
+    // Four blocks a wave reuse its rows' operands twice as often (64 experts 256 x
+    // 1024, 512 rows: 9.0 us with two, 7.9 with four), where enough workgroups are left.
+    if ((int64_t)p.E * div_up(p.cols, kWaves / p.wk * 64) >= 256)
+      return launch_q4<4, MODE, NS>(p, group, stream);
+    return launch_q4<2, MODE, NS>(p, group, stream);
   }
-  if (format == VMOE_FEW_Q4) return launch_q4<2, MODE, NS>(p, group, stream);
   if (format == VMOE_FEW_F32) return launch<WF32<4>, MODE, NS>(p, stream);
   if constexpr (MODE == kDown)
     if (steps <= 8) {
@@ -1172,7 +1113,7 @@ int check_rows(int64_t T, const void* x, int64_t ldx, int64_t cols, const void* 
 
 // Up, down and sum; the choice of experts is the logits' or the caller's ids'.
 int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const float* logits,
-                const void* wr, int64_t ldwr, int32_t* sel, float* prob, const SumArgs& c,
+                int32_t* sel, float* prob, const SumArgs& c,
                 const FewLayout& L, char* ws, hipStream_t stream) {
   FewArgs p = {};
   p.w = {w.w1, w.scales1, w.ldw1};
@@ -1185,8 +1126,6 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const flo
   p.logits = logits;
   p.ldl = (int)L.ldl;
   p.ids = c.ids;
-  p.wr = wr;
-  p.ldwr = ldwr;
   p.tab2 = reinterpret_cast<const MatEntry*>(w.table2);
   p.entry = reinterpret_cast<MatEntry*>(ws + L.entry);
   p.sel = sel;
@@ -1274,8 +1213,6 @@ extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t 
   float* prob = reinterpret_cast<float*>(ws + L.prob);
   const SumArgs c = {T, top_k, E, (int)w->hidden, {sel, 0}, prob, 0, normalize != 0, out, ldo, f32,
                      selected, weights};
-  if (few_pairs(T, top_k, E) && E <= kFusedExperts && w->hidden * E * (f32 ? 4 : 2) <= kFusedBytes)
-    return few_experts(*w, x, ldx, nullptr, router_weight, ldwr, sel, prob, c, L, ws, stream);
   const dim3 grid(div_up(L.ldl, 16), div_up(T, 16));
   if (f32)
     VMOE_LAUNCH((few_logits_kernel<true>), grid, dim3(kThreads), 0, stream, x, ldx, T,
@@ -1284,7 +1221,7 @@ extern "C" int vmoe_few_layer(const vmoe_few_weights* w, const void* x, int64_t 
     VMOE_LAUNCH((few_logits_kernel<false>), grid, dim3(kThreads), 0, stream, x, ldx, T,
                 router_weight, ldwr, E, (int)w->hidden, logits, (int)L.ldl);
   VMOE_CHECK_LAUNCH();
-  return few_experts(*w, x, ldx, logits, nullptr, 0, sel, prob, c, L, ws, stream);
+  return few_experts(*w, x, ldx, logits, sel, prob, c, L, ws, stream);
 }
 
 extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_t ldx,
@@ -1310,7 +1247,7 @@ extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_
   const SumArgs c = {(int)num_tokens, top_k, w->num_experts, (int)w->hidden, {ids, ids_are_i64},
                      weights, weights_are_bf16, 0, out, ldo, w->format == VMOE_FEW_F32, nullptr,
                      nullptr};
-  return few_experts(*w, x, ldx, nullptr, nullptr, 0, nullptr, nullptr, c, L, ws, stream);
+  return few_experts(*w, x, ldx, nullptr, nullptr, nullptr, c, L, ws, stream);
 }
 
 extern "C" int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids,
