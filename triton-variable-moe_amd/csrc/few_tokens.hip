@@ -326,6 +326,7 @@ struct FewArgs {
   int tiles;  // its column tiles
   const int32_t* tile_of;  // kUp: the expert of each kTileCols columns
   int num_tiles;
+  bool slots;  // a workgroup takes an assignment
   int wk;     // waves that split K; kWaves / wk split the tile's columns
   int act;
   void* out;  // h, y (fp32) or the products
@@ -756,12 +757,13 @@ __global__ __launch_bounds__(kCombineThreads) void few_combine_kernel(SumArgs p,
 // ---------------------------------------------------------------------------
 // Down projection and sum of one token: the experts of its slots one after the
 // other as a single long K, so that no partial result leaves the workgroup. For
-// calls with so few tokens that they share no weights.
+// calls with so few tokens that reading an expert's weights once for each costs less
+// than another launch. BY_ID: `entry` is the experts' table, not the slots' entries.
 // ---------------------------------------------------------------------------
 
 constexpr int kTokenWaves = 16;
 
-template <class W, int DEPTH>
+template <class W, int DEPTH, bool BY_ID>
 __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p, Stack w,
                                                                       const MatEntry* entry,
                                                                       const void* h, int64_t ldh,
@@ -776,8 +778,9 @@ __global__ __launch_bounds__(kTokenWaves* kWave) void few_token_kernel(SumArgs p
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   // A slot a lane, in every wave: no barrier before the weights are on their way.
   // An entry of length 0 is a slot without an expert.
-  const MatEntry mine = load_entry(entry + t * p.k + min(lane, p.k - 1));
   const SlotWeight sw = load_slot(p, t);
+  MatEntry mine = load_entry(BY_ID ? entry + max(sw.id, 0) : entry + t * p.k + min(lane, p.k - 1));
+  if (BY_ID && sw.id < 0) mine.len = 0;
   const int n0 = tile * W::NC;
   const uint32_t boff = W::lane_offset(w, n0, p.d, lane);
   const uint32_t aoff = (lane >> 4) * 16;
@@ -946,8 +949,15 @@ int launch_early(FewArgs p, hipStream_t stream) {
 
 template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH>
 int launch_tiles(const FewArgs& p, hipStream_t stream) {
-  if (!SLOT && (int64_t)p.T * p.k >= p.E)
-    return launch_early<W, MODE, MT, NS, SLOT, DEPTH, !SLOT>(p, stream);
+  // Early weights where most experts have rows. They cost registers, in 4 bits so many
+  // that fewer workgroups share a CU; where those come in several rounds, they cover
+  // for one another without (128 experts 2048 x 512, 128 rows: 24 us with, 16 without).
+  if constexpr (!SLOT) {
+    const int64_t units = MODE == kUp ? (int64_t)p.num_tiles * kTileCols / (kWaves / p.wk * W::NC)
+                                      : (int64_t)p.E * div_up(p.cols, kWaves / p.wk * W::NC);
+    if ((int64_t)p.T * p.k >= p.E && (W::KS != kQ4Rows || units <= 512))
+      return launch_early<W, MODE, MT, NS, SLOT, DEPTH, true>(p, stream);
+  }
   return launch_early<W, MODE, MT, NS, SLOT, DEPTH, false>(p, stream);
 }
 
@@ -966,9 +976,18 @@ int split_waves(int64_t steps) {
   return wk;
 }
 
-// Whether the call's assignments share few experts: a workgroup then takes one
-// assignment, and one token's down projections at once.
-bool few_pairs(int64_t T, int64_t k, int64_t E) { return T * k * 2 <= E && E <= kSlotExperts; }
+// Whether a token's down projections run in one workgroup: while the call's pairs
+// read at most 2^24 weights of one matrix (2^23 in fp32). Measured over 1 to 48
+// tokens of seven layers: up to 20 % faster than the experts' products and their sum
+// at half of that, even at it, 5-8 % slower half above it (4 bits: 20 %).
+bool small_call(const vmoe_few_weights& w, int64_t pairs) {
+  const double width = (double)w.num_tiles1 * kTileCols / w.num_experts;  // in the mean
+  return pairs * width * w.hidden <= (w.format == VMOE_FEW_F32 ? 1 << 23 : 1 << 24);
+}
+
+// Whether, in such a call, the pairs share few experts: an up projection's workgroup
+// then takes a pair.
+bool few_pairs(int64_t pairs, int64_t E) { return pairs * 2 <= E && E <= kSlotExperts; }
 
 template <int CB, int MODE, int NS>
 int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
@@ -998,8 +1017,7 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
   p.wk = kWaves;
   if (MODE == kDown) p.wk = split_waves(steps);
   if constexpr (MODE == kUp) {
-    if (few_pairs(p.T, p.k, p.E))
-      return launch_slots<NS>(p, format, group, stream);
+    if (p.slots) return launch_slots<NS>(p, format, group, stream);
     // A workgroup takes kTileCols columns, or half of them where the tiles are fewer
     // than CUs.
     if (format == VMOE_FEW_Q4) {
@@ -1013,8 +1031,9 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
       return format == VMOE_FEW_F32 ? launch<WF32<2>, MODE, NS>(p, stream)
                                     : launch<WBf16<2>, MODE, NS>(p, stream);
   } else if (format == VMOE_FEW_Q4) {
-    // Four blocks a wave reuse its rows' operands twice as often (64 experts 256 x
-    // 1024, 512 rows: 9.0 us with two, 7.9 with four), where enough workgroups are left.
+    // Four blocks a wave reuse its rows' operands twice as often as two (64 experts
+    // 256 x 1024, 512 rows: 9.0 us with two, 7.9 with four; 128 experts 512 x 2048, 128
+    // rows: 26 and 18), where enough workgroups are left.
     if ((int64_t)p.E * div_up(p.cols, kWaves / p.wk * 64) >= 256)
       return launch_q4<4, MODE, NS>(p, group, stream);
     return launch_q4<2, MODE, NS>(p, group, stream);
@@ -1028,16 +1047,31 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
   return launch<WBf16<4>, MODE, NS>(p, stream);
 }
 
-template <class W, int DEPTH>
+template <class W, int DEPTH, bool BY_ID>
 int launch_token(const SumArgs& p, const Stack& w, const MatEntry* entry, const void* h, int64_t ldh,
                  int64_t lo, hipStream_t stream) {
   const int tiles = div_up(p.d, W::NC);
   const int64_t units = (int64_t)p.T * tiles;
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
-  VMOE_LAUNCH((few_token_kernel<W, DEPTH>), dim3(div_up(units, 16) * 16), dim3(kTokenWaves * kWave),
-              0, stream, p, w, entry, h, ldh, lo, tiles);
+  VMOE_LAUNCH((few_token_kernel<W, DEPTH, BY_ID>), dim3(div_up(units, 16) * 16),
+              dim3(kTokenWaves * kWave), 0, stream, p, w, entry, h, ldh, lo, tiles);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
+}
+
+template <bool BY_ID>
+int launch_tokens(const SumArgs& p, const vmoe_few_weights& w, const MatEntry* entry,
+                  const void* h, int64_t ldh, int64_t lo, hipStream_t stream) {
+  const Stack s = {w.w2, w.scales2, w.ldw2};
+  if (w.format == VMOE_FEW_BF16)
+    return launch_token<WBf16<2>, 4, BY_ID>(p, s, entry, h, ldh, lo, stream);
+  if (w.format == VMOE_FEW_F32)
+    return launch_token<WF32<2>, 4, BY_ID>(p, s, entry, h, ldh, lo, stream);
+  switch (w.group) {
+    case 32: return launch_token<WQ4<1, 1>, 2, BY_ID>(p, s, entry, h, ldh, lo, stream);
+    case 64: return launch_token<WQ4<1, 2>, 2, BY_ID>(p, s, entry, h, ldh, lo, stream);
+    default: return launch_token<WQ4<1, 4>, 2, BY_ID>(p, s, entry, h, ldh, lo, stream);
+  }
 }
 
 struct FewLayout {
@@ -1137,26 +1171,19 @@ int few_experts(const vmoe_few_weights& w, const void* x, int64_t ldx, const flo
   p.out = ws + L.h;
   p.ldo = w.format == VMOE_FEW_F32 ? L.ldh : 2 * L.ldh;
   p.lo = L.ldh;
+  const bool small = small_call(w, (int64_t)c.T * c.k);
+  p.slots = small && few_pairs((int64_t)c.T * c.k, c.E);
   int st = w.act == VMOE_ACT_SWIGLU
                ? launch_format<kUp, 2>(p, w.format, w.group, w.hidden, stream)
                : launch_format<kUp, 1>(p, w.format, w.group, w.hidden, stream);
   if (st != VMOE_OK) return st;
 
+  const void* h = ws + L.h;
+  if (p.slots) return launch_tokens<false>(c, w, p.entry, h, p.ldo, p.lo, stream);
+  if (small) return launch_tokens<true>(c, w, p.tab2, h, p.ldo, p.lo, stream);
   p.w = {w.w2, w.scales2, w.ldw2};
-  p.tab = reinterpret_cast<const MatEntry*>(w.table2);
-  if (few_pairs(c.T, c.k, c.E)) {
-    const void* h = ws + L.h;
-    if (w.format == VMOE_FEW_BF16)
-      return launch_token<WBf16<2>, 4>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
-    if (w.format == VMOE_FEW_F32)
-      return launch_token<WF32<2>, 4>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
-    switch (w.group) {
-      case 32: return launch_token<WQ4<1, 1>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
-      case 64: return launch_token<WQ4<1, 2>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
-      default: return launch_token<WQ4<1, 4>, 2>(c, p.w, p.entry, h, p.ldo, p.lo, stream);
-    }
-  }
-  p.a = ws + L.h;
+  p.tab = p.tab2;
+  p.a = h;
   p.lda = p.ldo;
   p.logits = nullptr;
   p.cols = p.fixed = (int)w.hidden;
