@@ -152,11 +152,17 @@ LAYERS = [
     (200, "3x64,2x192,1x8", 2, 5, "q4", 32, True),
     (328, "3x136,2x72", 3, 21, "q4", 128, False),
     (136, "2x1160", 2, 9, "q4", 64, True),
+    (64, "300x8", 2, 7, "bf16", 0, True),            # more experts than a slot's workgroup takes
+    (128, "32x512", 8, 64, "bf16", 0, True),         # 64-column tiles, 16 rows an expert
+    (768, "4x512,8x256,4x128", 2, 48, "f32", 0, True),  # past one-token down projections
+    (256, "64x256", 4, 20, "f32", 0, True),
+    (1024, "64x256", 8, 33, "q4", 32, True),
+    (640, "130x256", 4, 33, "q4", 128, True),        # 4-bit weights not early
 ]
 
 
 # the first seeds whose choice is clear (plain_choice), where 100 i is not
-SEEDS = {4: 930, 14: 1420}
+SEEDS = {4: 930, 14: 1420, 22: 19370}
 
 
 def layer_case(i):
@@ -206,6 +212,10 @@ EXPERTS = [
     (1024, "16x512", 4, 7, "q4", 128, "swiglu", "plain"),
     (200, "3x72,2x200", 3, 37, "q4", 32, "swiglu", "wild"),
     (320, "3x328", 2, 50, "q4", 64, "relu_squared", "one"),
+    (128, "64x256", 4, 40, "bf16", 0, "swiglu", "wild"),
+    (640, "64x256", 2, 20, "q4", 32, "swiglu", "wild"),
+    (1024, "16x520", 3, 60, "f32", 0, "relu_squared", "wild"),
+    (1024, "16x520", 3, 60, "bf16", 0, "relu_squared", "wild"),
 ]
 
 
@@ -560,3 +570,82 @@ def test_module_quantized_run(device):
     assert torch.equal(m.few_tokens(x, experts=pickle.loads(pickle.dumps(q))), out)
     with pytest.raises(ValueError, match="widths"):
         m.few_tokens(x, experts=K.quantize_experts(w1, w2, [96] * 8))
+
+
+def test_refusals(device):
+    """Arguments that are refused before anything is launched."""
+    d, widths = 64, [64, 32]
+    x, wr, w1, w2 = (t.to(device) for t in layer_inputs(91, d, widths, 3))
+    e = K.few_token_experts(w1, w2, widths)
+    q4 = K.quantize_experts(w1, w2, widths)
+    ids = torch.zeros(3, 2, dtype=torch.int64, device=device)
+    wts = torch.ones(3, 2, device=device)
+    for args, error in (
+            ((w1, w2, [64, 64]), ValueError), ((w1, w2, [96, 0]), ValueError),
+            ((w1, w2.float(), widths), ValueError), ((w1, w2, widths, "gelu"), ValueError),
+            ((w1, w2, widths, "swiglu"), ValueError), ((w1[:, :96], w2[:90], [48, 42]), ValueError),
+            ((w1.half(), w2.half(), widths), NotImplementedError),
+            ((w1.t().contiguous().t(), w2, widths), NotImplementedError),
+            ((w1, w2, [92, 4]), NotImplementedError), ((w1[0], w2, widths), ValueError),
+            ((w1[:60], w2[:, :60].contiguous(), widths), NotImplementedError)):
+        with pytest.raises(error):
+            K.few_token_experts(*args)
+    with pytest.raises(NotImplementedError, match="multiples of 8"):
+        K.quantize_experts(w1.float(), w2.float(), [92, 4])
+    for h in (e, q4):
+        for args, error in (
+                ((x, wr, h, 0), ValueError), ((x, wr, h, 3), ValueError),
+                ((x[:, :56], wr, h, 1), ValueError), ((x.float(), wr, h, 1), NotImplementedError),
+                ((x, wr[:1], h, 1), ValueError), ((x, wr.float(), h, 1), NotImplementedError),
+                ((x, wr[:, :56], h, 1), ValueError), ((x.cpu(), wr, h, 1), AssertionError),
+                ((x[:1].expand(257, d), wr, h, 1), NotImplementedError)):
+            with pytest.raises(error):
+                K.moe_few_tokens(*args)
+        for args, error in (
+                ((x, ids[:2], wts[:2], h), ValueError), ((x, ids, wts[:, :1], h), ValueError),
+                ((x, ids.float(), wts, h), ValueError),
+                ((x, ids[:, :0], wts[:, :0], h), ValueError),
+                ((x, ids, wts.double(), h), NotImplementedError),
+                ((x, ids, wts.cpu(), h), ValueError), ((x, ids.cpu(), wts, h), AssertionError),
+                ((x, torch.zeros(3, 65, dtype=torch.int64, device=device),
+                  torch.zeros(3, 65, device=device), h), NotImplementedError)):
+            with pytest.raises(error):
+                K.experts_few_tokens(*args)
+    m = q4.w1
+    for args, error in (((x, m), ValueError), ((x, q4.w2), NotImplementedError),
+                        ((x, m, ids[:2]), ValueError), ((x.float(), m, ids), NotImplementedError),
+                        ((x[:, :56], m, ids), ValueError), ((x, m, ids.short()), ValueError)):
+        with pytest.raises(error):
+            K.matvec_q4(*args)
+    with pytest.raises(NotImplementedError):
+        q4.dequantize(torch.float16)
+    with pytest.raises(ValueError, match="add up"):
+        K.quantize_matrices(w1, [64, 64])
+    with pytest.raises(NotImplementedError):
+        K.quantize_matrices(w1[:, :92])
+
+
+def test_threads_share_a_handle(device):
+    """Two threads' first calls on one new handle, each on its own stream."""
+    import threading
+
+    d, widths, k = 128, [64] * 8, 2
+    x, wr, w1, w2 = (t.to(device) for t in layer_inputs(95, d, widths, 9))
+    ref = K.moe_few_tokens(x, wr, K.few_token_experts(w1, w2, widths), k)
+    torch.cuda.synchronize()
+    for make in (K.few_token_experts, lambda a, b, w: copy.copy(K.few_token_experts(a, b, w))):
+        e = make(w1, w2, widths)
+        torch.cuda.synchronize()
+        got = {}
+
+        def work(n):
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[n] = [K.moe_few_tokens(x, wr, e, k) for _ in range(20)]
+                torch.cuda.current_stream().synchronize()
+
+        threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert all(torch.equal(o, ref) for n in range(2) for o in got[n])

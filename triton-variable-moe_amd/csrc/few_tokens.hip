@@ -139,7 +139,8 @@ struct WBf16 {
   }
 
   template <int MT, int PL>
-  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles, f32x4_t (&acc)[MT][C]) const {
+  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles,
+                                      f32x4_t (&acc)[MT][C]) const {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const bf16x8_t b = operand(c);
@@ -199,7 +200,8 @@ struct WF32 {
   }
 
   template <int MT, int PL>
-  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles, f32x4_t (&acc)[MT][C]) const {
+  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles,
+                                      f32x4_t (&acc)[MT][C]) const {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (m > 0 && m >= tiles) break;
@@ -207,7 +209,8 @@ struct WF32 {
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int c = 0; c < C; ++c)
-          acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[m][0].v[j], r[j][c], acc[m][c], 0, 0, 0);
+          acc[m][c] =
+              __builtin_amdgcn_mfma_f32_16x16x4f32(a[m][0].v[j], r[j][c], acc[m][c], 0, 0, 0);
     }
   }
 };
@@ -276,7 +279,8 @@ struct WQ4 {
   }
 
   template <int MT, int PL>
-  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles, f32x4_t (&acc)[MT][C]) const {
+  __device__ __forceinline__ void mma(const A (&a)[MT][PL], int tiles,
+                                      f32x4_t (&acc)[MT][C]) const {
 #pragma unroll
     for (int c = 0; c < CB; ++c)
 #pragma unroll
@@ -328,7 +332,6 @@ struct FewArgs {
   int num_tiles;
   bool slots;  // a workgroup takes an assignment
   int wk;     // waves that split K; kWaves / wk split the tile's columns
-  int act;
   void* out;  // h, y (fp32) or the products
   int64_t ldo;
 };
@@ -474,8 +477,6 @@ __device__ __forceinline__ int unit_of_block(Order order, int units, int tiles) 
   return u < units ? u : -1;
 }
 
-// SLOT: a unit is an assignment and a tile (one row), else an expert and a tile.
-// DEPTH steps of a wave are in flight.
 // Waves a SIMD holds at least: the long K of a down projection's many small tiles is
 // covered by other workgroups (128 experts 576 x 2048: 65 us with two on a CU, 58
 // with three).
@@ -483,6 +484,9 @@ template <class W, int MODE, int MT, int DEPTH>
 constexpr int kMinWaves =
     MODE == kDown && MT == 1 && DEPTH == 1 && sizeof(typename W::Row) == 2 && W::KS == 32 ? 6 : 1;
 
+// SLOT: a unit is an assignment and a tile (one row), else an expert and a tile. MT:
+// 16-row tiles in one pass over the weights; NS: matrices of an expert (gate and
+// up); DEPTH: steps of a wave in flight.
 template <class W, int MODE, int MT, int NS, bool SLOT, int DEPTH, bool EARLY>
 __global__ __launch_bounds__(kThreads, (kMinWaves<W, MODE, MT, DEPTH>)) void few_kernel(FewArgs p) {
   constexpr int PL = (MODE == kDown && sizeof(typename W::Row) == 2) ? 2 : 1;
@@ -1048,8 +1052,8 @@ int launch_format(FewArgs p, int format, int group, int64_t max_k, hipStream_t s
 }
 
 template <class W, int DEPTH, bool BY_ID>
-int launch_token(const SumArgs& p, const Stack& w, const MatEntry* entry, const void* h, int64_t ldh,
-                 int64_t lo, hipStream_t stream) {
+int launch_token(const SumArgs& p, const Stack& w, const MatEntry* entry, const void* h,
+                 int64_t ldh, int64_t lo, hipStream_t stream) {
   const int tiles = div_up(p.d, W::NC);
   const int64_t units = (int64_t)p.T * tiles;
   if (units > (1 << 30)) return VMOE_ERR_UNSUPPORTED;
@@ -1261,7 +1265,8 @@ extern "C" int vmoe_few_experts(const vmoe_few_weights* w, const void* x, int64_
   st = check_sizes(num_tokens, w->num_experts, top_k);
   if (st != VMOE_OK) return st;
   if (num_tokens == 0) return VMOE_OK;
-  st = check_rows(num_tokens, x, ldx, w->hidden, out, ldo, w->hidden, w->format == VMOE_FEW_F32 ? 4 : 8);
+  st = check_rows(num_tokens, x, ldx, w->hidden, out, ldo, w->hidden,
+                  w->format == VMOE_FEW_F32 ? 4 : 8);
   if (st != VMOE_OK) return st;
   if (!ids || !weights || !workspace) return VMOE_ERR_INVALID_ARG;
   if (!aligned16(workspace)) return VMOE_ERR_UNSUPPORTED;

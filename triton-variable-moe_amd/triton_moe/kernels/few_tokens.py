@@ -133,14 +133,14 @@ class _Experts:
         self._bytes: dict = {}  # (tokens, top_k) -> workspace bytes
 
     def __getstate__(self):
-        return {**self.__dict__, "_desc": None, "_desc_ptr": None}
+        return {**self.__dict__, "_desc": None}
 
-    def _new_desc(self) -> _FewWeights:
-        self._desc = _FewWeights(self._format, self._group, _ACT[self.activation],
-                                 self.num_experts, self.hidden, self._max_width)
-        self._desc.tiles1, self._desc.num_tiles1 = self._tiles.data_ptr(), self._tiles.numel()
-        self._desc_ptr = ctypes.addressof(self._desc)
-        return self._desc
+    def _new_desc(self, w1, scales1, ld1, table1, w2, scales2, ld2, table2) -> _FewWeights:
+        q = _FewWeights(self._format, self._group, _ACT[self.activation], self.num_experts,
+                        self.hidden, self._max_width, w1, scales1, ld1, table1, w2, scales2, ld2,
+                        table2, self._tiles.data_ptr(), self._tiles.numel())
+        q.at = ctypes.addressof(q)
+        return q
 
     def _workspace_bytes(self, T: int, k: int, what: str) -> int:
         """Of a call of this size (refused if it is too large); kept in _bytes."""
@@ -185,26 +185,25 @@ class FewTokenExperts(_Experts):
         each = [w for w in widths for _ in range(glu)]
         self._t1, _ = _entries(tuple(each), d, False, glu, w1.device)
         self._t2, _ = _entries(tuple(widths), d, True, 1, w1.device)
-        self._at = None
 
-    def _weights(self) -> int:
-        """Address of the description; where the weights' storage has moved
-        since the last call (module.to, .data assigned), it is read anew."""
+    def _weights(self) -> _FewWeights:
+        """The description of the weights (the caller holds it during its call);
+        where their storage has moved since the last one (module.to, .data
+        assigned), it is made anew."""
         a, b = self.w1, self.w2
-        at = (a.data_ptr(), b.data_ptr())
-        if self._desc is None or at != self._at:
+        q = self._desc
+        if q is None or q.w1 != a.data_ptr() or q.w2 != b.data_ptr():
             mult = 4 if self._format == _lib.FEW_F32 else 8
             for w, n in ((a, "w1"), (b, "w2")):
                 _weight(w, n, (self.dtype,), mult)
                 if w.device != self.device:
                     raise ValueError(f"{n} has moved to {w.device}: make a new handle")
-            if a.shape[0] != self.hidden or b.shape[1] != self.hidden:
-                raise ValueError("w1 or w2 has another shape now: make a new handle")
-            q = self._new_desc()
-            q.w1, q.w2, q.ldw1, q.ldw2 = at[0], at[1], a.stride(0), b.stride(0)
-            q.table1, q.table2 = self._t1.data_ptr(), self._t2.data_ptr()
-            self._at = at
-        return self._desc_ptr
+            if _check_layer(a, b, self.expert_widths, self.activation)[1] != self.hidden:
+                raise ValueError("w1 and w2 have another hidden size now: make a new handle")
+            q = self._desc = self._new_desc(
+                a.data_ptr(), None, a.stride(0), self._t1.data_ptr(), b.data_ptr(), None,
+                b.stride(0), self._t2.data_ptr())
+        return q
 
 
 def few_token_experts(w1, w2, expert_widths, activation="relu_squared") -> FewTokenExperts:
@@ -291,13 +290,14 @@ class QuantizedExperts(_Experts):
         self._init_common(_lib.FEW_Q4, group_size, activation, widths, d, torch.bfloat16,
                           w1.device)
 
-    def _weights(self) -> int:
-        if self._desc is None:
-            q = self._new_desc()
-            q.w1, q.scales1 = self.w1.codes.data_ptr(), self.w1.scales.data_ptr()
-            q.w2, q.scales2 = self.w2.codes.data_ptr(), self.w2.scales.data_ptr()
-            q.table1, q.table2 = self.w1._table.data_ptr(), self.w2._table.data_ptr()
-        return self._desc_ptr
+    def _weights(self) -> _FewWeights:
+        q = self._desc
+        if q is None:
+            a, b = self.w1, self.w2
+            q = self._desc = self._new_desc(
+                a.codes.data_ptr(), a.scales.data_ptr(), 0, a._table.data_ptr(),
+                b.codes.data_ptr(), b.scales.data_ptr(), 0, b._table.data_ptr())
+        return q
 
     def dequantize(self, dtype=torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """(w1, w2) that the 4-bit values stand for, as quantize_experts took them."""
@@ -368,6 +368,7 @@ def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True
     rows, at, ldx, T = _rows(x, d, dtype, dev, "x")
     wr, wr_at, ldwr, _ = _rows(router_weight, d, dtype, dev, "router_weight")
     n = experts._bytes.get((T, k)) or experts._workspace_bytes(T, k, "moe_few_tokens")
+    q = experts._weights()
     with _on(dev):
         out = torch.empty(x.shape, dtype=dtype, device=dev)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -375,7 +376,7 @@ def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True
         if return_routing:
             sel = torch.empty((T, k), dtype=torch.int32, device=dev)
             wts = torch.empty((T, k), dtype=torch.float32, device=dev)
-        _lib.call("vmoe_few_layer", experts._weights(), at, ldx, T, wr_at, ldwr, k,
+        _lib.call("vmoe_few_layer", q.at, at, ldx, T, wr_at, ldwr, k,
                   1 if normalize else 0, out.data_ptr(), d, _lib.ptr(sel), _lib.ptr(wts),
                   ws.data_ptr(), n, _lib.stream(dev))
     return (out, sel, wts) if return_routing else out
@@ -400,11 +401,12 @@ def experts_few_tokens(x, selected, weights, experts):
     if weights.device != dev:
         raise ValueError(f"weights are on {weights.device}, the experts on {dev}")
     n = experts._bytes.get((T, k)) or experts._workspace_bytes(T, k, "experts_few_tokens")
+    q = experts._weights()
     wts = weights if weights.is_contiguous() else weights.contiguous()
     with _on(dev):
         out = torch.empty(x.shape, dtype=dtype, device=dev)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.call("vmoe_few_experts", experts._weights(), at, ldx, T, ids.data_ptr(),
+        _lib.call("vmoe_few_experts", q.at, at, ldx, T, ids.data_ptr(),
                   int(ids.dtype == torch.int64), wts.data_ptr(),
                   int(wts.dtype == torch.bfloat16), k, out.data_ptr(), d, ws.data_ptr(), n,
                   _lib.stream(dev))

@@ -378,6 +378,7 @@ class TritonMoEMLP(nn.Module):
     # a generation step (not in the reference)
     # ------------------------------------------------------------------
 
+    @torch.compiler.disable
     @torch.no_grad()
     def few_tokens(self, x: torch.Tensor, experts=None, return_routing: bool = False):
         """The layer's output for a few tokens, for inference: x [..., n_embd],
