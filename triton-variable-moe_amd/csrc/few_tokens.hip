@@ -967,10 +967,15 @@ int launch_tiles(const FewArgs& p, hipStream_t stream) {
 
 template <class W, int MODE, int NS, int DEPTH = 1>
 int launch(const FewArgs& p, hipStream_t stream) {
-  // row tiles in one pass over the weights: the mean number of rows, doubled
-  const int64_t rows = p.ids.p || p.logits ? 2 * (int64_t)p.T * p.k / p.E : p.T;
-  return rows <= 16 ? launch_tiles<W, MODE, 1, NS, false, DEPTH>(p, stream)
-                    : launch_tiles<W, MODE, 2, NS, false, 1>(p, stream);
+  // Row tiles in one pass over the weights: the mean number of rows, doubled (64 experts
+  // 1024 x 256, 16 rows each: 15.6 us with one, 13.1 with two). Not for experts in 4
+  // bits, where two leave one workgroup to a CU (128 experts 2048 x 576, 16 rows each:
+  // 126 us both products with one, 171 with two).
+  if constexpr (W::KS != kQ4Rows || MODE == kPlain) {
+    const int64_t rows = p.ids.p || p.logits ? 2 * (int64_t)p.T * p.k / p.E : p.T;
+    if (rows > 16) return launch_tiles<W, MODE, 2, NS, false, 1>(p, stream);
+  }
+  return launch_tiles<W, MODE, 1, NS, false, DEPTH>(p, stream);
 }
 
 // Waves that split K, `steps` steps long for the longest matrix.
@@ -981,12 +986,15 @@ int split_waves(int64_t steps) {
 }
 
 // Whether a token's down projections run in one workgroup: while the call's pairs
-// read at most 2^24 weights of one matrix (2^23 in fp32). Measured over 1 to 48
-// tokens of seven layers: up to 20 % faster than the experts' products and their sum
-// at half of that, even at it, 5-8 % slower half above it (4 bits: 20 %).
+// read at most 2^24 weights of one matrix (2^23 in fp32; measured over 1 to 48 tokens
+// of seven layers: up to 20 % faster than the experts' products and their sum at half
+// of that, even at it, 5-8 % slower half above it, in 4 bits 20 %), or are a quarter of
+// the experts and hardly share one (2 tokens of 8 through 128 experts 2048 x 576: 32 us
+// so and 41 by experts, 4 bits 25 and 36; at a third of the experts either is faster).
 bool small_call(const vmoe_few_weights& w, int64_t pairs) {
   const double width = (double)w.num_tiles1 * kTileCols / w.num_experts;  // in the mean
-  return pairs * width * w.hidden <= (w.format == VMOE_FEW_F32 ? 1 << 23 : 1 << 24);
+  return pairs * 4 <= w.num_experts ||
+         pairs * width * w.hidden <= (w.format == VMOE_FEW_F32 ? 1 << 23 : 1 << 24);
 }
 
 // Whether, in such a call, the pairs share few experts: an up projection's workgroup
