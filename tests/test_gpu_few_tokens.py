@@ -649,3 +649,69 @@ def test_threads_share_a_handle(device):
         for t in threads:
             t.join()
         assert all(torch.equal(o, ref) for n in range(2) for o in got[n])
+
+
+@pytest.mark.parametrize("T", [4, 40])
+@pytest.mark.parametrize("dt", ["bf16", "f32", "q4"])
+def test_padding_holds_anything(device, dt, T):
+    """Rows without an expert may hold NaN, in x and in their weights: zeros come
+    out, and the other rows keep their bits."""
+    d, widths, k = 512, [1024] * 6, 2
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    x, _, w1, w2 = (t.to(device) for t in layer_inputs(97, d, widths, T, dtype=dtype))
+    e = K.quantize_experts(w1, w2, widths) if dt == "q4" else K.few_token_experts(w1, w2, widths)
+    ids = ids_of("padded", T, k, 6, 5).to(device)
+    ids[0, 1] = -1
+    wts = torch.rand(T, k, device=device)
+    clean = K.experts_few_tokens(x, ids, wts, e)
+    none = ids < 0
+    x[none.all(dim=1)] = float("nan")
+    wts[none] = float("nan")
+    out = K.experts_few_tokens(x, ids, wts, e)
+    assert torch.equal(out, clean) and (out[none.all(dim=1)] == 0).all()
+    if dt == "q4":
+        y = K.matvec_q4(x, e.w1, ids)
+        assert torch.isfinite(y).all() and (y[none] == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "q4"])
+def test_far_offsets(device, dt):
+    """Weights of more than 2^32 values: the last of 2048 experts, 8.6 GB into w1 and
+    w2 (in 4 bits, past 2^31 bytes)."""
+    d, w, E = 512, 4104, 2048
+    widths = [w] * E
+    used = [0, 1023, E - 2, E - 1]
+    w1 = torch.zeros(d, E * w, dtype=torch.bfloat16, device=device)
+    w2 = torch.zeros(E * w, d, dtype=torch.bfloat16, device=device)
+    assert w1.numel() > 2 ** 32
+    parts = {}
+    for i, e in enumerate(used):
+        a, b = normal(101 + i, d, w, std=0.03), normal(111 + i, w, d, std=0.03)
+        w1[:, e * w:e * w + w] = a.to(device)
+        w2[e * w:e * w + w] = b.to(device)
+        if dt == "q4":
+            a, b = plain_quantized(a, [w], False, 64)[0], plain_quantized(b, [w], True, 64)[0]
+        parts[e] = (a.to(D), b.to(D))
+    h = K.quantize_experts(w1, w2, widths, group_size=64) if dt == "q4" else \
+        K.few_token_experts(w1, w2, widths)
+    small1 = torch.cat([parts[e][0] for e in used], 1)
+    small2 = torch.cat([parts[e][1] for e in used], 0)
+    k = 3
+    x = normal(121, 8, d)
+    ids = torch.tensor([[t % 4, (t + 1) % 4, (t + 2) % 4] for t in range(8)])
+    wts = normal(122, 8, k, dtype=torch.float32)
+    far = torch.tensor(used)[ids]
+    ref, err = plain_experts(x.to(D), ids, wts.to(D), small1, small2, [w] * 4, "relu_squared",
+                             True)
+    # one-token down projections, and (past a quarter of the experts) by experts
+    for times in (1, 25):
+        out = K.experts_few_tokens(x.repeat(times, 1).to(device), far.repeat(times, 1).to(device),
+                                   wts.repeat(times, 1).to(device), h)
+        hold(out, ref.repeat(times, 1), err.repeat(times, 1), (dt, times))
+    if dt == "q4":
+        x = normal(123, 3, d)
+        y = K.matvec_q4(x.to(device), h.w1, torch.full((3, 1), E - 1, device=device))
+        ref, mag = x.to(D) @ parts[E - 1][0], x.to(D).abs() @ parts[E - 1][0].abs()
+        hold(y, ref[:, None], U16 * ref.abs()[:, None] + (d + 8) * U32 * mag[:, None])
+        v = h.w2.dequantize(torch.float32)[-w:].cpu().to(D)
+        assert torch.equal(v, parts[E - 1][1])
