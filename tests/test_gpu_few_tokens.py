@@ -158,11 +158,17 @@ LAYERS = [
     (256, "64x256", 4, 20, "f32", 0, True),
     (1024, "64x256", 8, 33, "q4", 32, True),
     (640, "130x256", 4, 33, "q4", 128, True),        # 4-bit weights not early
+    # few pairs, wide tiles
+    (328, "64x264,64x72", 8, 8, "bf16", 0, True),
+    (328, "64x264,64x72", 8, 8, "f32", 0, False),
+    (328, "64x264,64x72", 8, 8, "q4", 32, True),
+    (520, "100x200,28x328", 4, 7, "q4", 64, True),
+    (264, "256x136", 16, 8, "q4", 128, True),
 ]
 
 
 # the first seeds whose choice is clear (plain_choice), where 100 i is not
-SEEDS = {4: 930, 14: 1420, 22: 19370}
+SEEDS = {4: 930, 14: 1420, 22: 19370, 28: 2810}
 
 
 def layer_case(i):
@@ -216,6 +222,16 @@ EXPERTS = [
     (640, "64x256", 2, 20, "q4", 32, "swiglu", "wild"),
     (1024, "16x520", 3, 60, "f32", 0, "relu_squared", "wild"),
     (1024, "16x520", 3, 60, "bf16", 0, "relu_squared", "wild"),
+    # few pairs, wide tiles
+    (328, "64x264,64x72", 8, 8, "bf16", 0, "swiglu", "wild"),
+    (328, "64x264,64x72", 8, 8, "f32", 0, "swiglu", "padded"),
+    (328, "64x264,64x72", 8, 8, "q4", 32, "swiglu", "wild"),
+    (520, "100x200,28x328", 4, 7, "q4", 64, "swiglu", "one"),
+    (264, "256x136", 16, 8, "q4", 128, "swiglu", "wild"),
+    # few pairs, narrow tiles
+    (264, "32x136", 4, 4, "bf16", 0, "swiglu", "wild"),
+    (264, "32x136", 4, 4, "f32", 0, "swiglu", "wild"),
+    (264, "32x136", 4, 4, "q4", 64, "swiglu", "wild"),
 ]
 
 

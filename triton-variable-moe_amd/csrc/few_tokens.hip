@@ -1026,13 +1026,27 @@ int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
 
 template <int NS>
 int launch_slots(const FewArgs& p, int format, int group, hipStream_t stream) {
-  if (format == VMOE_FEW_BF16) return launch_tiles<WBf16<2>, kUp, 1, NS, true, 4>(p, stream);
-  if (format == VMOE_FEW_F32) return launch_tiles<WF32<2>, kUp, 1, NS, true, 2>(p, stream);
+  // Columns a workgroup: 64 (16 in 4 bits) where the call has enough tiles of 64, else
+  // less. Up projections of 8 experts a token: 4 tokens, experts 2048 x 576 in bf16
+  // 26 us with 32 columns and 24 with 64 (4 experts of 1024 x 512, 8 tokens: 13 and 12);
+  // 4 bits, experts of 2048 x 1024 / 512 / 256, 1, 2 and 4 tokens: 9.4, 16 and 24 us with
+  // 16 columns, 7.7, 8.8 and 12 with 64, but at 64 tiles 6.6 and 7.0. Gated 4-bit
+  // experts take 32, in two operands (2048 x 576, 4 tokens: 22 us with 16, 15 with
+  // 32, 16 with 64); fp32 always 32 (4 tokens: 39 us, 45 with 64).
+  const int64_t units = (int64_t)p.T * p.k * div_up(p.cols, 64);  // tiles of 64 columns
+  if (format == VMOE_FEW_BF16)
+    return units >= 256 ? launch_tiles<WBf16<4>, kUp, 1, NS, true, 4 / NS>(p, stream)
+                        : launch_tiles<WBf16<2>, kUp, 1, NS, true, 4>(p, stream);
+  if (format == VMOE_FEW_F32) return launch_tiles<WF32<2>, kUp, 1, NS, true, 4>(p, stream);
+#define SLOTS_Q4(GJ)                                                                      \
+  return units >= 128 ? launch_tiles<WQ4<4 / NS, GJ>, kUp, 1, NS, true, 1>(p, stream) \
+                      : launch_tiles<WQ4<1, GJ>, kUp, 1, NS, true, 2>(p, stream)
   switch (group) {
-    case 32: return launch_tiles<WQ4<1, 1>, kUp, 1, NS, true, 2>(p, stream);
-    case 64: return launch_tiles<WQ4<1, 2>, kUp, 1, NS, true, 2>(p, stream);
-    default: return launch_tiles<WQ4<1, 4>, kUp, 1, NS, true, 2>(p, stream);
+    case 32: SLOTS_Q4(1);
+    case 64: SLOTS_Q4(2);
+    default: SLOTS_Q4(4);
   }
+#undef SLOTS_Q4
 }
 
 // max_k: rows of the longest matrix.
