@@ -164,11 +164,17 @@ LAYERS = [
     (328, "64x264,64x72", 8, 8, "q4", 32, True),
     (520, "100x200,28x328", 4, 7, "q4", 64, True),
     (264, "256x136", 16, 8, "q4", 128, True),
+    # the smallest and the most experts
+    (64, "1x64", 1, 3, "bf16", 0, True),
+    (8, "3x8", 2, 1, "bf16", 0, True),
+    (4, "2x4", 1, 2, "f32", 0, False),
+    (8, "2x8", 2, 2, "q4", 32, True),
+    (64, "2048x8", 64, 4, "bf16", 0, True),
 ]
 
 
 # the first seeds whose choice is clear (plain_choice), where 100 i is not
-SEEDS = {4: 930, 14: 1420, 22: 19370, 28: 2810}
+SEEDS = {4: 930, 14: 1420, 22: 19370, 28: 2810, 33: 3350}
 
 
 def layer_case(i):
@@ -731,3 +737,29 @@ def test_far_offsets(device, dt):
         hold(y, ref[:, None], U16 * ref.abs()[:, None] + (d + 8) * U32 * mag[:, None])
         v = h.w2.dequantize(torch.float32)[-w:].cpu().to(D)
         assert torch.equal(v, parts[E - 1][1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_handle_follows_the_layout(device, dt):
+    """Weights whose layout changes while their address stays."""
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    widths = [64, 32]
+    x, wr, a, b = (v.to(device) for v in layer_inputs(31, 64, widths, 3, dtype=dtype))
+    room = torch.zeros(64 * 96 * 4, dtype=dtype, device=device)
+    w1 = torch.nn.Parameter(room[:64 * 96].view(64, 96))
+    w1.data.copy_(a)
+    e = K.few_token_experts(w1, b, widths)
+    first = K.moe_few_tokens(x, wr, e, 2)
+    w1.data = room.view(64, 4 * 96)[:, :96]  # rows further apart
+    w1.data.copy_(a)
+    assert torch.equal(K.moe_few_tokens(x, wr, e, 2), first)
+    w1.data = room[:64 * 96].view(96, 64)
+    with pytest.raises(ValueError):
+        K.moe_few_tokens(x, wr, e, 2)
+    other = torch.bfloat16 if dt == "f32" else torch.float32
+    w1.data = room.view(other)[:64 * 96].view(64, 96)
+    with pytest.raises(NotImplementedError):
+        K.moe_few_tokens(x, wr, e, 2)
+    w1.data = room[:64 * 96].view(64, 96)
+    w1.data.copy_(a)
+    assert torch.equal(K.moe_few_tokens(x, wr, e, 2), first)

@@ -30,7 +30,7 @@
 // share a CU (fewer of them fit: 10 to 30 % slower on large layers).
 //
 // Sums, logits, routing weights and the activation are fp32. The activations h
-// enter the second product as two bf16 halves, h = hi + lo to 2^-17: the matrix
+// enter the second product as two bf16 halves, h = hi + lo to 2^-16: the matrix
 // instructions are far from their limit, and one bf16 rounding of h would add as
 // much error as the output's own.
 #include <algorithm>
@@ -1026,19 +1026,19 @@ int launch_q4(const FewArgs& p, int group, hipStream_t stream) {
 
 template <int NS>
 int launch_slots(const FewArgs& p, int format, int group, hipStream_t stream) {
-  // Columns a workgroup: 64 (16 in 4 bits) where the call has enough tiles of 64, else
-  // less. Up projections of 8 experts a token: 4 tokens, experts 2048 x 576 in bf16
-  // 26 us with 32 columns and 24 with 64 (4 experts of 1024 x 512, 8 tokens: 13 and 12);
+  // Columns a workgroup: 64 where the call has enough tiles of 64, else 32, in 4 bits 16.
+  // Up projections of 8 experts a token: experts 2048 x 576 in bf16, 4 tokens: 26 us
+  // with 32 columns and 24 with 64 (4 experts of 1024 x 512, 8 tokens: 13 and 12).
   // 4 bits, experts of 2048 x 1024 / 512 / 256, 1, 2 and 4 tokens: 9.4, 16 and 24 us with
-  // 16 columns, 7.7, 8.8 and 12 with 64, but at 64 tiles 6.6 and 7.0. Gated 4-bit
-  // experts take 32, in two operands (2048 x 576, 4 tokens: 22 us with 16, 15 with
-  // 32, 16 with 64); fp32 always 32 (4 tokens: 39 us, 45 with 64).
+  // 16, 7.7, 8.8 and 12 with 64, but at 64 tiles 6.6 and 7.0. Gated 4-bit experts take
+  // 32 of each matrix (2048 x 576, 4 tokens: 22 us with 16, 15 with 32, 16 with 64),
+  // fp32 always 32 (the same call: 39 us, 45 with 64).
   const int64_t units = (int64_t)p.T * p.k * div_up(p.cols, 64);  // tiles of 64 columns
   if (format == VMOE_FEW_BF16)
     return units >= 256 ? launch_tiles<WBf16<4>, kUp, 1, NS, true, 4 / NS>(p, stream)
                         : launch_tiles<WBf16<2>, kUp, 1, NS, true, 4>(p, stream);
   if (format == VMOE_FEW_F32) return launch_tiles<WF32<2>, kUp, 1, NS, true, 4>(p, stream);
-#define SLOTS_Q4(GJ)                                                                      \
+#define SLOTS_Q4(GJ)                                                                  \
   return units >= 128 ? launch_tiles<WQ4<4 / NS, GJ>, kUp, 1, NS, true, 1>(p, stream) \
                       : launch_tiles<WQ4<1, GJ>, kUp, 1, NS, true, 2>(p, stream)
   switch (group) {

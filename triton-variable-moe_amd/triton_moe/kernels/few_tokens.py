@@ -188,11 +188,14 @@ class FewTokenExperts(_Experts):
 
     def _weights(self) -> _FewWeights:
         """The description of the weights (the caller holds it during its call);
-        where their storage has moved since the last one (module.to, .data
-        assigned), it is made anew."""
+        where their storage or layout has changed since the last one (module.to,
+        .data assigned), it is made anew."""
         a, b = self.w1, self.w2
         q = self._desc
-        if q is None or q.w1 != a.data_ptr() or q.w2 != b.data_ptr():
+        if (q is None or q.w1 != a.data_ptr() or q.w2 != b.data_ptr() or
+                a.dtype is not self.dtype or b.dtype is not self.dtype or
+                a.stride() != q.strides[0] or b.stride() != q.strides[1] or
+                a.shape != q.shapes[0] or b.shape != q.shapes[1]):
             mult = 4 if self._format == _lib.FEW_F32 else 8
             for w, n in ((a, "w1"), (b, "w2")):
                 _weight(w, n, (self.dtype,), mult)
@@ -200,9 +203,11 @@ class FewTokenExperts(_Experts):
                     raise ValueError(f"{n} has moved to {w.device}: make a new handle")
             if _check_layer(a, b, self.expert_widths, self.activation)[1] != self.hidden:
                 raise ValueError("w1 and w2 have another hidden size now: make a new handle")
-            q = self._desc = self._new_desc(
+            q = self._new_desc(
                 a.data_ptr(), None, a.stride(0), self._t1.data_ptr(), b.data_ptr(), None,
                 b.stride(0), self._t2.data_ptr())
+            q.strides, q.shapes = (a.stride(), b.stride()), (a.shape, b.shape)
+            self._desc = q  # (whole: other threads may use it from here on)
         return q
 
 
