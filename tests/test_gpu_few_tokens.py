@@ -763,3 +763,27 @@ def test_handle_follows_the_layout(device, dt):
     w1.data = room[:64 * 96].view(64, 96)
     w1.data.copy_(a)
     assert torch.equal(K.moe_few_tokens(x, wr, e, 2), first)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "q4"])
+def test_compiled(device, dt):
+    """Compiled programs call the operators as they are: strided operands, whose
+    aligned copies and workspace live until the launch, give the eager bits."""
+    d, widths, k = 136, [64, 72, 8], 2
+    x, wr, w1, w2 = (t.to(device) for t in layer_inputs(51, d, widths, 12))
+    e = K.quantize_experts(w1, w2, widths) if dt == "q4" else K.few_token_experts(w1, w2, widths)
+    q = K.quantize_matrices(w1, widths)
+    wt = wr.t().contiguous().t()
+
+    def program(v):
+        v = v.t().contiguous().t()
+        out, sel, wts = K.moe_few_tokens(v, wt, e, k, return_routing=True)
+        again = K.experts_few_tokens(v, sel.t().contiguous().t(), wts, e)
+        return out, sel, wts, again, K.matvec_q4(v, q, sel), q.dequantize()
+
+    ref = program(x)
+    torch.compiler.reset()
+    compiled = torch.compile(program, backend="eager")
+    for i in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(compiled(x), ref)), i
+    torch.compiler.reset()

@@ -94,12 +94,29 @@ def _tiles(widths: tuple, device) -> torch.Tensor:
                         dtype=torch.int32, device=device)
 
 
+def _untraced(fn):
+    """fn, run as it is also where its caller is compiled: it hands addresses to the
+    library, and a traced copy of it may let go of a tensor of which only the address
+    is used later (an aligned copy, the workspace) before the launch. (The test is
+    0.3 us of a call; torch.compiler.disable alone 0.5.)"""
+    plain = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        if torch.compiler.is_compiling():
+            return plain(*args, **kwargs)
+        return fn(*args, **kwargs)
+
+    return call
+
+
 _HERE = contextlib.nullcontext()
 
 
 def _on(device):
-    """The device as the current one (kernels and allocations go to it)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """The device as the current one (kernels and allocations go to it). (What
+    torch.cuda.current_device() reads; a device that holds tensors is initialised.)"""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 class _FewWeights(ctypes.Structure):
@@ -170,6 +187,7 @@ def _check_layer(w1, w2, widths, activation):
 class FewTokenExperts(_Experts):
     """Handle of bf16 or fp32 expert weights: few_token_experts."""
 
+    @torch.compiler.disable
     def __init__(self, w1, w2, expert_widths, activation="relu_squared"):
         f32 = w1.dtype == torch.float32
         mult = 4 if f32 else 8
@@ -225,6 +243,7 @@ def few_token_experts(w1, w2, expert_widths, activation="relu_squared") -> FewTo
 class QuantizedMatrices:
     """A stack of 4-bit matrices in the kernels' order: quantize_matrices."""
 
+    @torch.compiler.disable
     def __init__(self, w, lengths, stacked: str, group_size: int, each: int = 1):
         if stacked not in ("columns", "rows"):
             raise ValueError(f"stacked must be 'columns' or 'rows' (got {stacked!r})")
@@ -255,6 +274,7 @@ class QuantizedMatrices:
                       self.max_len, group_size, self.codes.data_ptr(), self.scales.data_ptr(),
                       _lib.stream(w.device))
 
+    @torch.compiler.disable
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         """The values, row-major: float32 exactly, bfloat16 rounded once."""
         if dtype not in (torch.bfloat16, torch.float32):
@@ -283,6 +303,7 @@ def quantize_matrices(w, lengths=None, stacked="columns", group_size=32) -> Quan
 class QuantizedExperts(_Experts):
     """Handle of 4-bit expert weights: quantize_experts."""
 
+    @torch.compiler.disable
     def __init__(self, w1, w2, expert_widths, activation="relu_squared", group_size=32):
         widths = _widths_of(expert_widths)
         for w, n in ((w1, "w1"), (w2, "w2")):
@@ -304,6 +325,7 @@ class QuantizedExperts(_Experts):
                 b.codes.data_ptr(), b.scales.data_ptr(), 0, b._table.data_ptr())
         return q
 
+    @torch.compiler.disable
     def dequantize(self, dtype=torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """(w1, w2) that the 4-bit values stand for, as quantize_experts took them."""
         return self.w1.dequantize(dtype), self.w2.dequantize(dtype)
@@ -352,6 +374,7 @@ def _check_count(T: int, k: int, what: str) -> None:
             f"(got {T} x {k}); larger batches are the layer's own forward's")
 
 
+@_untraced
 def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True,
                    return_routing: bool = False):
     """The whole layer for a few tokens: router, top_k experts of each token,
@@ -387,6 +410,7 @@ def moe_few_tokens(x, router_weight, experts, top_k: int, normalize: bool = True
     return (out, sel, wts) if return_routing else out
 
 
+@_untraced
 def experts_few_tokens(x, selected, weights, experts):
     """The experts' part of the layer for given choices: out[t] = sum_s
     weights[t, s] expert_{selected[t, s]}(x[t]).
@@ -432,6 +456,7 @@ def _ids(ids, T: int, device, what: str):
     return (ids if ids.is_contiguous() else ids.contiguous()), ids.shape[-1]
 
 
+@_untraced
 def matvec_q4(x, q: QuantizedMatrices, ids=None):
     """Products of a few rows with 4-bit matrices.
 

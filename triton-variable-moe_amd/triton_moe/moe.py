@@ -399,6 +399,7 @@ class TritonMoEMLP(nn.Module):
         return ft.moe_few_tokens(x, self.router.weight, experts, self.num_active_experts,
                                  self.norm_topk_prob, return_routing)
 
+    @torch.compiler.disable
     @torch.no_grad()
     def quantize_experts(self, group_size: int = 32):
         """A 4-bit copy of the expert weights, for few_tokens(x, experts=...):
