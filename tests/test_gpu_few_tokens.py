@@ -787,3 +787,72 @@ def test_compiled(device, dt):
     for i in range(3):
         assert all(torch.equal(a, b) for a, b in zip(compiled(x), ref)), i
     torch.compiler.reset()
+
+
+def other_router(m, kind):
+    """Makes m's router choose by more than its weight: expert i is pushed by
+    push[i]. Returns what undoes it, where something global was changed."""
+    push = torch.linspace(-3, 3, 8, device=m.w1.device)
+    r = m.router
+    if kind == "bias":
+        r.bias = torch.nn.Parameter(push.to(r.weight.dtype))
+    elif kind == "hook":
+        r.register_forward_hook(lambda mod, args, out: out + push.to(out.dtype))
+    elif kind == "pre_hook":
+        r.register_forward_pre_hook(lambda mod, args: (args[0].flip(-1),))
+    elif kind == "forward":
+        r.forward = lambda v: torch.nn.functional.linear(v, r.weight) + push.to(v.dtype)
+    elif kind == "class":
+        m.router = torch.nn.Sequential(r, torch.nn.Linear(8, 8))
+        m.router[1].to(r.weight.device, r.weight.dtype).bias.data.copy_(push)
+    else:
+        return torch.nn.modules.module.register_module_forward_hook(
+            lambda mod, args, out: out + push.to(out.dtype) if mod is r else None).remove
+    return lambda: None
+
+
+@pytest.mark.parametrize("kind", ["bias", "hook", "pre_hook", "forward", "class", "global_hook"])
+@pytest.mark.parametrize("dt", ["bf16", "f32", "q4"])
+def test_module_router(device, kind, dt):
+    """A router that is more than its weight chooses for few_tokens as it does for
+    forward: the same experts, the same weights."""
+    dtype = torch.float32 if dt == "f32" else torch.bfloat16
+    cfg = TritonMoEConfig(n_embd=256, expert_sizes=[(4, 128), (4, 64)], num_active_experts=2)
+    torch.manual_seed(5)
+    m = TritonMoEMLP(cfg).to(device).to(dtype)
+    with torch.no_grad():
+        m.router.weight.normal_(0, 0.1)
+    x = normal(131, 2, 9, 256, dtype=dtype).to(device)
+    e = m.quantize_experts() if dt == "q4" else K.few_token_experts(m.w1, m.w2, m.expert_widths)
+    plain = K.moe_few_tokens(x, m.router.weight, e, 2, return_routing=True)
+    given = e if dt == "q4" else None
+    assert torch.equal(m.few_tokens(x, experts=given), plain[0])
+    undo = other_router(m, kind)
+    try:
+        out, sel, wts = m.few_tokens(x, experts=given, return_routing=True)
+        full = m.forward_with_intermediates(x)
+        alone = m.few_tokens(x[0, 0], experts=given)
+        none = m.few_tokens(x[:0], experts=given, return_routing=True)
+    finally:
+        undo()
+    assert (full["selected_experts"].view(18, 2) != plain[1]).any()
+    assert sel.dtype == torch.int32 and wts.dtype == torch.float32
+    assert torch.equal(sel.long(), full["selected_experts"].view(18, 2))
+    assert torch.equal(wts, full["top_k_weights"].float().view(18, 2))
+    assert out.shape == x.shape and not out.requires_grad and alone.shape == (256,)
+    assert torch.equal(out.view(18, 256), K.experts_few_tokens(x.view(18, 256), sel, wts, e))
+    assert none[0].shape == (0, 9, 256) and none[1].shape == (0, 2) and none[2].shape == (0, 2)
+
+
+def test_module_router_refusals(device):
+    """Logits of another shape than the layer's experts are refused."""
+    cfg = TritonMoEConfig(n_embd=64, expert_sizes=[(4, 64)], num_active_experts=2)
+    m = TritonMoEMLP(cfg).to(device).to(torch.bfloat16)
+    m.router = torch.nn.Linear(64, 6).to(device).to(torch.bfloat16)
+    x = normal(132, 3, 64).to(device)
+    with pytest.raises(ValueError, match="logits"):
+        m.few_tokens(x)
+    m.router = torch.nn.Linear(64, 4).to(device).to(torch.bfloat16)
+    assert m.few_tokens(x).shape == (3, 64)
+    with pytest.raises(NotImplementedError, match="tokens"):
+        m.few_tokens(x[:1].expand(257, 64))

@@ -384,10 +384,13 @@ class TritonMoEMLP(nn.Module):
         """The layer's output for a few tokens, for inference: x [..., n_embd],
         at most few_tokens_max() tokens, without auxiliary losses or gradients
         (kernels.moe_few_tokens on this module's weights). experts: a handle
-        from quantize_experts() for 4-bit expert weights. The router's logits
-        are not rounded to bf16 as forward()'s are, so near ties between experts
-        may fall differently; the router's weight is used as it is, without the
-        router module's hooks."""
+        from quantize_experts() for 4-bit expert weights.
+
+        A plain router's logits are formed from its weight and are not rounded to
+        bf16 as forward()'s are, so near ties between experts may fall
+        differently. Any other router (one with a bias, forward hooks, a forward of
+        its own, or of another class) is called, and chooses as it does in
+        forward(); backward hooks do not matter here."""
         if experts is None:
             experts = _FEW_HANDLES.get(self)
             if experts is None or experts.w1 is not self.w1 or experts.w2 is not self.w2 or \
@@ -396,8 +399,33 @@ class TritonMoEMLP(nn.Module):
                 _FEW_HANDLES[self] = experts
         elif experts.expert_widths != self.expert_widths:
             raise ValueError("experts is a handle of other expert widths than this layer's")
+        if not self._router_is_weight():
+            return self._few_tokens_routed(x, experts, return_routing)
         return ft.moe_few_tokens(x, self.router.weight, experts, self.num_active_experts,
                                  self.norm_topk_prob, return_routing)
+
+    def _router_is_weight(self) -> bool:
+        """Whether the router's call is F.linear with its weight and nothing else."""
+        r = self.router
+        return (type(r) is RouterLinear and r.bias is None and "forward" not in r.__dict__ and
+                not (r._forward_hooks or r._forward_pre_hooks) and not _has_global_hook())
+
+    def _few_tokens_routed(self, x, experts, return_routing):
+        """few_tokens with the choice from self.router(x), taken as forward() takes it."""
+        x_flat = x.reshape(-1, x.shape[-1])
+        T, k = x_flat.shape[0], self.num_active_experts
+        if T == 0:
+            sel = torch.empty((0, k), dtype=torch.int32, device=x.device)
+            wts = torch.empty((0, k), dtype=torch.float32, device=x.device)
+        else:
+            logits = self.router(x_flat)
+            if logits.shape != (T, self.num_experts):
+                raise ValueError(f"the router's logits must be [{T}, {self.num_experts}] "
+                                 f"(got {tuple(logits.shape)})")
+            state = router_topk(logits, k, self.norm_topk_prob)
+            sel, wts = state.selected, state.weights.float()
+        out = ft.experts_few_tokens(x, sel, wts, experts)
+        return (out, sel, wts) if return_routing else out
 
     @torch.compiler.disable
     @torch.no_grad()
