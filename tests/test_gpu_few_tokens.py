@@ -856,3 +856,18 @@ def test_module_router_refusals(device):
     assert m.few_tokens(x).shape == (3, 64)
     with pytest.raises(NotImplementedError, match="tokens"):
         m.few_tokens(x[:1].expand(257, 64))
+
+
+def test_module_takes_its_own_kind_of_handle(device):
+    """A handle of another activation or hidden size than the layer's."""
+    cfg = TritonMoEConfig(n_embd=64, expert_sizes=[(2, 64)], num_active_experts=1)
+    m = TritonMoEMLP(cfg).to(device).to(torch.bfloat16)
+    x, _, w1, w2 = (t.to(device) for t in layer_inputs(141, 64, [64, 64], 3, "swiglu"))
+    for make in (K.quantize_experts, K.few_token_experts):
+        with pytest.raises(ValueError, match="activation"):
+            m.few_tokens(x, experts=make(w1, w2, [64, 64], "swiglu"))
+    wide = [t.to(device) for t in layer_inputs(142, 128, [64, 64], 3)]
+    with pytest.raises(ValueError, match="hidden"):
+        m.few_tokens(wide[0], experts=K.quantize_experts(wide[2], wide[3], [64, 64]))
+    same = K.few_token_experts(m.w1, m.w2, [64, 64])
+    assert torch.equal(m.few_tokens(x, experts=same), m.few_tokens(x))

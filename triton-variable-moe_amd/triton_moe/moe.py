@@ -399,6 +399,9 @@ class TritonMoEMLP(nn.Module):
                 _FEW_HANDLES[self] = experts
         elif experts.expert_widths != self.expert_widths:
             raise ValueError("experts is a handle of other expert widths than this layer's")
+        elif experts.activation != "relu_squared" or experts.hidden != self.config.n_embd:
+            raise ValueError(f"experts must be a handle of relu_squared activation and hidden size "
+                             f"{self.config.n_embd} (got {experts.activation}, {experts.hidden})")
         if not self._router_is_weight():
             return self._few_tokens_routed(x, experts, return_routing)
         return ft.moe_few_tokens(x, self.router.weight, experts, self.num_active_experts,
