@@ -871,3 +871,21 @@ def test_module_takes_its_own_kind_of_handle(device):
         m.few_tokens(wide[0], experts=K.quantize_experts(wide[2], wide[3], [64, 64]))
     same = K.few_token_experts(m.w1, m.w2, [64, 64])
     assert torch.equal(m.few_tokens(x, experts=same), m.few_tokens(x))
+
+
+def test_float32_module_with_4_bit_experts(device):
+    """4-bit experts take bf16 rows, so that a float32 layer cannot use them in
+    few_tokens; the error says what can be done, and that works."""
+    cfg = TritonMoEConfig(n_embd=64, expert_sizes=[(4, 64)], num_active_experts=2)
+    torch.manual_seed(6)
+    m = TritonMoEMLP(cfg).to(device)
+    q = m.quantize_experts()
+    x = normal(151, 3, 64).to(device)
+    for rows in (x, x.float()):
+        with pytest.raises(NotImplementedError, match="moe_few_tokens"):
+            m.few_tokens(rows, experts=q)
+    wr = m.router.weight.to(torch.bfloat16)
+    out = K.moe_few_tokens(x, wr, q, 2)
+    half = copy.deepcopy(m).to(torch.bfloat16)
+    assert torch.equal(half.few_tokens(x, experts=q), out)
+    assert m.few_tokens(x.float()).dtype == torch.float32

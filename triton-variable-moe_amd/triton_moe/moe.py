@@ -404,8 +404,14 @@ class TritonMoEMLP(nn.Module):
                              f"{self.config.n_embd} (got {experts.activation}, {experts.hidden})")
         if not self._router_is_weight():
             return self._few_tokens_routed(x, experts, return_routing)
-        return ft.moe_few_tokens(x, self.router.weight, experts, self.num_active_experts,
-                                 self.norm_topk_prob, return_routing)
+        wr = self.router.weight
+        if wr.dtype != experts.dtype:
+            raise NotImplementedError(
+                f"these experts take {experts.dtype} rows and router weights, this layer's router "
+                f"is {wr.dtype}: convert the layer, or call kernels.moe_few_tokens with a "
+                f"{experts.dtype} copy of the router's weight")
+        return ft.moe_few_tokens(x, wr, experts, self.num_active_experts, self.norm_topk_prob,
+                                 return_routing)
 
     def _router_is_weight(self) -> bool:
         """Whether the router's call is F.linear with its weight and nothing else."""
@@ -433,8 +439,10 @@ class TritonMoEMLP(nn.Module):
     @torch.compiler.disable
     @torch.no_grad()
     def quantize_experts(self, group_size: int = 32):
-        """A 4-bit copy of the expert weights, for few_tokens(x, experts=...):
-        kernels.quantize_experts. It does not follow later updates."""
+        """A 4-bit copy of the expert weights, for few_tokens(x, experts=...) of a
+        bfloat16 layer: kernels.quantize_experts. It does not follow later updates.
+        (A float32 layer's copy is for kernels.moe_few_tokens and
+        experts_few_tokens on bfloat16 rows.)"""
         return ft.quantize_experts(self.w1, self.w2, self.expert_widths, group_size=group_size)
 
     def forward_with_intermediates(self, x: torch.Tensor) -> dict[str, Any]:
