@@ -889,3 +889,27 @@ def test_float32_module_with_4_bit_experts(device):
     half = copy.deepcopy(m).to(torch.bfloat16)
     assert torch.equal(half.few_tokens(x, experts=q), out)
     assert m.few_tokens(x.float()).dtype == torch.float32
+
+
+def test_module_lets_go_of_replaced_weights(device):
+    """A layer that has run few_tokens keeps no parameter that was taken from it:
+    generation with a 4-bit copy, the layer's own weights freed."""
+    import gc
+    import weakref
+
+    cfg = TritonMoEConfig(n_embd=64, expert_sizes=[(4, 64)], num_active_experts=2)
+    torch.manual_seed(7)
+    m = TritonMoEMLP(cfg).to(device).to(torch.bfloat16)
+    x = normal(161, 3, 64).to(device)
+    first = m.few_tokens(x)
+    q = m.quantize_experts()
+    four = m.few_tokens(x, experts=q)
+    w1, w2 = m.w1.detach().clone(), m.w2.detach().clone()
+    old = [weakref.ref(m.w1), weakref.ref(m.w2)]
+    m.w1, m.w2 = (torch.nn.Parameter(torch.empty(0, device=device, dtype=torch.bfloat16))
+                  for _ in range(2))
+    gc.collect()
+    assert all(r() is None for r in old)
+    assert torch.equal(m.few_tokens(x, experts=q), four)
+    m.w1, m.w2 = torch.nn.Parameter(w1), torch.nn.Parameter(w2)
+    assert torch.equal(m.few_tokens(x), first)

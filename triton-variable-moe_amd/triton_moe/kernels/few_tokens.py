@@ -29,6 +29,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import weakref
 
 import torch
 
@@ -227,6 +228,14 @@ class FewTokenExperts(_Experts):
             q.strides, q.shapes = (a.stride(), b.stride()), (a.shape, b.shape)
             self._desc = q  # (whole: other threads may use it from here on)
         return q
+
+
+class ModuleExperts(FewTokenExperts):
+    """A layer's handle of its own parameters, which the layer keeps alive and may
+    replace: it holds them weakly. Its caller holds them during a call."""
+
+    w1 = property(lambda self: self._w1(), lambda self, w: setattr(self, "_w1", weakref.ref(w)))
+    w2 = property(lambda self: self._w2(), lambda self, w: setattr(self, "_w2", weakref.ref(w)))
 
 
 def few_token_experts(w1, w2, expert_widths, activation="relu_squared") -> FewTokenExperts:

@@ -393,9 +393,10 @@ class TritonMoEMLP(nn.Module):
         forward(); backward hooks do not matter here."""
         if experts is None:
             experts = _FEW_HANDLES.get(self)
-            if experts is None or experts.w1 is not self.w1 or experts.w2 is not self.w2 or \
-                    experts.device != self.w1.device or experts.dtype != self.w1.dtype:
-                experts = ft.few_token_experts(self.w1, self.w2, self.expert_widths)
+            w1, w2 = self.w1, self.w2  # (held here: the handle does not)
+            if experts is None or experts.w1 is not w1 or experts.w2 is not w2 or \
+                    experts.device != w1.device or experts.dtype != w1.dtype:
+                experts = ft.ModuleExperts(w1, w2, self.expert_widths)
                 _FEW_HANDLES[self] = experts
         elif experts.expert_widths != self.expert_widths:
             raise ValueError("experts is a handle of other expert widths than this layer's")
