@@ -148,3 +148,49 @@ def test_host_tensors_are_refused():
         K.quantize_matrices(w1, group_size=48)
     with pytest.raises(ValueError, match="stacked"):
         K.quantize_matrices(w1, stacked="diagonal")
+
+
+@pytest.fixture
+def host_handles(monkeypatch):
+    """Handles made of host tensors with nothing launched; the library calls
+    that operators make of them afterwards."""
+    from triton_moe.kernels import few_tokens as ft
+
+    made = []
+    with monkeypatch.context() as m:
+        m.setattr(ft._lib, "require_gpu", lambda *a: None)
+        m.setattr(ft._lib, "call", lambda *a: None)
+        m.setattr(ft._lib, "stream", lambda d: 0)
+        m.setattr(ft, "_on", lambda d: __import__("contextlib").nullcontext())
+        w1 = torch.randn(64, 128).to(torch.bfloat16)
+        w2 = torch.randn(128, 64).to(torch.bfloat16)
+        few, four = K.few_token_experts(w1, w2, [64, 64]), K.quantize_experts(w1, w2, [64, 64])
+    monkeypatch.setattr(ft._lib, "call", lambda *a: made.append(a))
+    monkeypatch.setattr(ft._lib, "stream", lambda d: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    return few, four, made
+
+
+@pytest.mark.parametrize("saved_from", ["cuda:0", "cuda:1"])
+def test_a_loaded_handle_is_where_its_tensors_are(host_handles, saved_from):
+    """A handle saved on a GPU and loaded elsewhere (torch.load with a
+    map_location) must not hand over addresses of another device: it is used where
+    its tensors are, and on the host not at all."""
+    import pickle
+
+    few, four, made = host_handles
+    for h in (few, four, four.w1, four.w2):
+        h.device = torch.device(saved_from)
+    few, four = pickle.loads(pickle.dumps((few, four)))
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    wr = torch.zeros(2, 64, dtype=torch.bfloat16)
+    ids = torch.zeros(2, 1, dtype=torch.int64)
+    for h in (few, four, four.w1, four.w2):
+        assert h.device == torch.device("cpu")
+    for call in (lambda: K.moe_few_tokens(x, wr, few, 1), lambda: K.moe_few_tokens(x, wr, four, 1),
+                 lambda: K.experts_few_tokens(x, ids, torch.ones(2, 1), few),
+                 lambda: K.experts_few_tokens(x, ids, torch.ones(2, 1), four),
+                 lambda: K.matvec_q4(x, four.w1, ids), lambda: four.dequantize()):
+        with pytest.raises(AssertionError, match="CUDA"):
+            call()
+    assert not made

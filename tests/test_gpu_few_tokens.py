@@ -913,3 +913,27 @@ def test_module_lets_go_of_replaced_weights(device):
     assert torch.equal(m.few_tokens(x, experts=q), four)
     m.w1, m.w2 = torch.nn.Parameter(w1), torch.nn.Parameter(w2)
     assert torch.equal(m.few_tokens(x), first)
+
+
+def test_saved_handles(device):
+    """Handles through torch.save: loaded onto the GPU they give the same bits, on
+    the host they are refused and can be saved again."""
+    import io
+
+    d, widths = 128, [64] * 4
+    x, wr, w1, w2 = (t.to(device) for t in layer_inputs(171, d, widths, 5))
+    for h in (K.few_token_experts(w1, w2, widths), K.quantize_experts(w1, w2, widths)):
+        ref = K.moe_few_tokens(x, wr, h, 2)
+        held = h
+        for where in ("cpu", "cuda:0"):
+            buf = io.BytesIO()
+            torch.save(held, buf)
+            buf.seek(0)
+            held = torch.load(buf, map_location=where, weights_only=False)
+            if where == "cpu":
+                assert held.device == torch.device("cpu")
+                with pytest.raises(AssertionError, match="CUDA"):
+                    K.moe_few_tokens(x.cpu(), wr.cpu(), held, 2)
+                with pytest.raises(ValueError, match="weights on cpu"):
+                    K.moe_few_tokens(x, wr, held, 2)
+        assert torch.equal(K.moe_few_tokens(x, wr, held, 2), ref)

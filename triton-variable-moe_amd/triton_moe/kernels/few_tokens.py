@@ -117,7 +117,11 @@ _HERE = contextlib.nullcontext()
 def _on(device):
     """The device as the current one (kernels and allocations go to it). (What
     torch.cuda.current_device() reads; a device that holds tensors is initialised.)"""
-    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+    if torch._C._cuda_getDevice() == device.index:
+        return _HERE
+    if device.type != "cuda":
+        raise AssertionError(f"weights must be on CUDA (these are on {device})")
+    return torch.cuda.device(device)
 
 
 class _FewWeights(ctypes.Structure):
@@ -152,6 +156,11 @@ class _Experts:
 
     def __getstate__(self):
         return {**self.__dict__, "_desc": None}
+
+    def __setstate__(self, state):
+        # (loaded, perhaps onto another device than it was saved from)
+        self.__dict__.update(state)
+        self.device = self._tiles.device
 
     def _new_desc(self, w1, scales1, ld1, table1, w2, scales2, ld2, table2) -> _FewWeights:
         q = _FewWeights(self._format, self._group, _ACT[self.activation], self.num_experts,
@@ -282,6 +291,11 @@ class QuantizedMatrices:
                       w.stride(0), self._table.data_ptr(), len(lengths), int(by_rows), fixed,
                       self.max_len, group_size, self.codes.data_ptr(), self.scales.data_ptr(),
                       _lib.stream(w.device))
+
+    def __setstate__(self, state):
+        # (loaded, perhaps onto another device than it was saved from)
+        self.__dict__.update(state)
+        self.device = self.codes.device
 
     @torch.compiler.disable
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
