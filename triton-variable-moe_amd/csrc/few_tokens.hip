@@ -970,13 +970,19 @@ int launch_tiles(const FewArgs& p, hipStream_t stream) {
   // Early weights where most experts have rows. They cost registers, in 4 bits so many
   // that fewer workgroups share a CU; where those come in several rounds, they cover
   // for one another without (128 experts 2048 x 512, 128 rows: 24 us with, 16 without).
-  if constexpr (!SLOT) {
-    const int64_t units = MODE == kUp ? (int64_t)p.num_tiles * kTileCols / (kWaves / p.wk * W::NC)
-                                      : (int64_t)p.E * div_up(p.cols, kWaves / p.wk * W::NC);
-    if ((int64_t)p.T * p.k >= p.E && (W::KS != kQ4Rows || units <= 512))
-      return launch_early<W, MODE, MT, NS, SLOT, DEPTH, true>(p, stream);
+  if constexpr (MT == 2 && W::KS != kQ4Rows) {
+    // (taken only from 8.5 pairs an expert on)
+    return launch_early<W, MODE, MT, NS, SLOT, DEPTH, true>(p, stream);
+  } else {
+    if constexpr (!SLOT) {
+      const int64_t units = MODE == kUp
+                                ? (int64_t)p.num_tiles * kTileCols / (kWaves / p.wk * W::NC)
+                                : (int64_t)p.E * div_up(p.cols, kWaves / p.wk * W::NC);
+      if ((int64_t)p.T * p.k >= p.E && (W::KS != kQ4Rows || units <= 512))
+        return launch_early<W, MODE, MT, NS, SLOT, DEPTH, true>(p, stream);
+    }
+    return launch_early<W, MODE, MT, NS, SLOT, DEPTH, false>(p, stream);
   }
-  return launch_early<W, MODE, MT, NS, SLOT, DEPTH, false>(p, stream);
 }
 
 template <class W, int MODE, int NS, int DEPTH = 1>
