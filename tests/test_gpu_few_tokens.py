@@ -937,3 +937,31 @@ def test_saved_handles(device):
                 with pytest.raises(ValueError, match="weights on cpu"):
                     K.moe_few_tokens(x, wr, held, 2)
         assert torch.equal(K.moe_few_tokens(x, wr, held, 2), ref)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_module_choices_differ_only_at_near_ties(device, dtype):
+    """Every expert that few_tokens and forward() do not both choose has a logit no
+    further from the other's than the roundings of forward()'s logits (one bf16
+    rounding of each; fp32 sums) can move them; every other choice is the same."""
+    cfg = TritonMoEConfig(n_embd=256, expert_sizes=[(24, 64), (8, 128)], num_active_experts=4)
+    torch.manual_seed(8)
+    m = TritonMoEMLP(cfg).to(device).to(dtype)
+    with torch.no_grad():
+        m.router.weight.normal_(0, 0.1)
+    x = normal(181, 256, 256, dtype=dtype).to(device)
+    _, sel, _ = m.few_tokens(x, return_routing=True)
+    there = m.forward_with_intermediates(x.view(1, 256, 256))["selected_experts"].view(256, 4)
+    sel, there = sel.cpu().long(), there.cpu()
+    xc, wr = x.cpu().to(D), m.router.weight.detach().cpu().to(D)
+    logits = xc @ wr.t()
+    off = (256 + 8) * U32 * (xc.abs() @ wr.abs().t()).max()
+    step = U16 if dtype == torch.bfloat16 else 0.0
+    for t in range(256):
+        one, two = set(sel[t].tolist()), set(there[t].tolist())
+        assert len(one) == len(two) == 4
+        for a in one - two:
+            for b in two - one:
+                la, lb = logits[t, a], logits[t, b]
+                assert la > lb - 2 * off  # (few_tokens takes the larger one)
+                assert la - lb <= step * (la.abs() + lb.abs()) + 2 * off
