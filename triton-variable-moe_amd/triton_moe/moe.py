@@ -51,6 +51,13 @@ from .kernels.router import (RouterAuxOp, RouterLinear, RouterWeightOp, router_b
 # it the router keeps its own call).
 _has_global_hook = getattr(nn.modules.module, "_has_any_global_hook", lambda: True)
 
+
+def _router_is_weight(r) -> bool:
+    """Whether a router's call is F.linear with its weight and nothing else."""
+    return (type(r) is RouterLinear and r.bias is None and "forward" not in r.__dict__ and
+            not (r._forward_hooks or r._forward_pre_hooks) and not _has_global_hook())
+
+
 # Each module's handle for few_tokens(), apart from the module: copying or
 # pickling a module does not meet it.
 _FEW_HANDLES = weakref.WeakKeyDictionary()
@@ -403,9 +410,10 @@ class TritonMoEMLP(nn.Module):
         elif experts.activation != "relu_squared" or experts.hidden != self.config.n_embd:
             raise ValueError(f"experts must be a handle of relu_squared activation and hidden size "
                              f"{self.config.n_embd} (got {experts.activation}, {experts.hidden})")
-        if not self._router_is_weight():
-            return self._few_tokens_routed(x, experts, return_routing)
-        wr = self.router.weight
+        router = self.router
+        if not _router_is_weight(router):
+            return self._few_tokens_routed(router, x, experts, return_routing)
+        wr = router.weight
         if wr.dtype != experts.dtype:
             raise NotImplementedError(
                 f"these experts take {experts.dtype} rows and router weights, this layer's router "
@@ -414,21 +422,15 @@ class TritonMoEMLP(nn.Module):
         return ft.moe_few_tokens(x, wr, experts, self.num_active_experts, self.norm_topk_prob,
                                  return_routing)
 
-    def _router_is_weight(self) -> bool:
-        """Whether the router's call is F.linear with its weight and nothing else."""
-        r = self.router
-        return (type(r) is RouterLinear and r.bias is None and "forward" not in r.__dict__ and
-                not (r._forward_hooks or r._forward_pre_hooks) and not _has_global_hook())
-
-    def _few_tokens_routed(self, x, experts, return_routing):
-        """few_tokens with the choice from self.router(x), taken as forward() takes it."""
+    def _few_tokens_routed(self, router, x, experts, return_routing):
+        """few_tokens with the choice from router(x), taken as forward() takes it."""
         x_flat = x.reshape(-1, x.shape[-1])
         T, k = x_flat.shape[0], self.num_active_experts
         if T == 0:
             sel = torch.empty((0, k), dtype=torch.int32, device=x.device)
             wts = torch.empty((0, k), dtype=torch.float32, device=x.device)
         else:
-            logits = self.router(x_flat)
+            logits = router(x_flat)
             if logits.shape != (T, self.num_experts):
                 raise ValueError(f"the router's logits must be [{T}, {self.num_experts}] "
                                  f"(got {tuple(logits.shape)})")
