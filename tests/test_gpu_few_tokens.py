@@ -965,3 +965,28 @@ def test_module_choices_differ_only_at_near_ties(device, dtype):
                 la, lb = logits[t, a], logits[t, b]
                 assert la > lb - 2 * off  # (few_tokens takes the larger one)
                 assert la - lb <= step * (la.abs() + lb.abs()) + 2 * off
+
+
+def test_module_router_in_a_graph(device):
+    """few_tokens with a hooked router, captured and replayed between eager calls."""
+    cfg = TritonMoEConfig(n_embd=256, expert_sizes=[(4, 128), (4, 64)], num_active_experts=2)
+    torch.manual_seed(9)
+    m = TritonMoEMLP(cfg).to(device).to(torch.bfloat16)
+    other_router(m, "hook")
+    inputs = [normal(191 + i, 1, 9, 256).to(device) for i in range(4)]
+    ref = [m.few_tokens(i, return_routing=True) for i in inputs]
+    x = inputs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m.few_tokens(x)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = m.few_tokens(x, return_routing=True)
+    for i, r in list(zip(inputs, ref)) * 2:
+        x.copy_(i)
+        g.replay()
+        eager = m.few_tokens(i)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, r)) and torch.equal(eager, r[0])
