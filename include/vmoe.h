@@ -812,10 +812,11 @@ int vmoe_moe_f32_backward(const void* saved, const float* logits, int64_t num_to
  * (a column of w1, a row of w2), its length along that axis, its first 4-bit
  * block, and (table1) its expert's first tile. table1 has an entry for each expert
  * (SwiGLU: two, gate and up), table2 one. tiles1 names the expert of each 64
- * columns: every expert has ceil(width / 64) tiles, in order. Activations and outputs are bf16 (fp32 for fp32 weights). hidden,
- * widths, starts and strides are multiples of 8 (fp32: 4), buffers 16-byte
- * aligned; lengths are at most max_width, hidden, max_width and strides of the
- * weights at most 2^24, x and the activations span less than 4 GiB.
+ * columns: every expert has ceil(width / 64) tiles, in order. Activations and
+ * outputs are bf16 (fp32 for fp32 weights). hidden, widths, starts and strides are
+ * multiples of 8 (fp32: 4), buffers 16-byte aligned; lengths are above 0 and at
+ * most max_width, hidden, max_width and strides of the weights at most 2^24, x and
+ * the activations span less than 4 GiB.
  *
  * vmoe_few_layer: logits = x router_weight^T in fp32; the top_k largest (ties:
  * the lowest index; NaN above all), weights sigmoid(logit), over their sum +

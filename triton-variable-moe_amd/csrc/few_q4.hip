@@ -8,8 +8,8 @@
 // maximum of a group is the maximum of four lanes. Bytes that are read or written
 // once go past the caches, and the codes through LDS, so that a store is a whole
 // kilobyte and not 64 pieces of it: 128 matrices 2048 x 576 in groups of 128, 302
-// MB, are laid out in 93 us (4.1 TB/s; 128 us before these two) and read back in 88
-// (102); a copy moves 5.2 TB/s.
+// MB, are laid out in 91 us (4.2 TB/s; 128 us before these two) and read back in 98
+// to 106 (3.6 to 3.9 TB/s); a copy moves 5.2 TB/s.
 //
 // The nearest value: |w| against the middles between values times the scale. Those
 // products are exact in fp32 (a scale of 8 bits, a middle of 3), so no choice

@@ -11,12 +11,14 @@
 // - No token is moved and no row is padded: a workgroup takes one expert and a
 //   tile of its columns, finds the rows that chose the expert, and gathers them
 //   as the 16-row operand of the matrix instructions.
-// - Weights go from memory to registers, each exactly once, straight into
-//   operand form. A lane's operand is 8 values of one column that are 8 rows
-//   apart in memory; the lane loads 8 rows of CPL adjacent columns and forms
-//   CPL operands by byte permutes, no LDS between. The sum over k may run in any
-//   order as long as both operands agree, so lane group g takes rows 8 g..8 g + 7
-//   of each 32. 4-bit matrices are stored in operand order (few_q4.h).
+// - Weights go from memory to registers straight into operand form. A lane's
+//   operand is 8 consecutive rows of one column; the lane loads 8 rows of CPL
+//   adjacent columns and forms CPL operands by byte permutes, no LDS between. The
+//   sum over k may run in any order as long as both operands agree, so lane group
+//   g takes rows 8 g..8 g + 7 of each 32. 4-bit matrices are stored in operand
+//   order (few_q4.h). An expert's weights are read once while its rows fit a pass
+//   (32 rows with two row tiles, else 16), and again for each further pass; where a
+//   workgroup takes a pair or a token, once for each of them that chose the expert.
 // - The waves of a workgroup split K; their partial sums meet in LDS in a fixed
 //   order, so results do not change from run to run.
 // - The router's choice needs no sort: expert e is chosen by a token if fewer
@@ -492,8 +494,9 @@ constexpr int kMinWaves =
 
 // Bound by reading weights: 32 tokens through 128 experts of 2048 x 576 (262 MB a
 // product) 58 us up and 57 down, 4.5 TB/s where a copy moves 5.2; 64 tokens through 64
-// of 1024 x 256 (33 MB) 10.7 and 10.3, of which 2.2 are the launch, 1 the tables, 2 the
-// joining of the waves; in 4 bits (8.9 MB) 7.3 and 7.9.
+// of 1024 x 256 (33 MB) 12.1 and 11.6 (10.7 and 10.3 where they lie in the last-level
+// cache), of which 2.2 are the launch, 1 the tables, 2 the joining of the waves; in 4 bits
+// (8.9 MB) 7.3 and 7.9.
 // SLOT: a unit is an assignment and a tile (one row), else an expert and a tile. MT:
 // 16-row tiles in one pass over the weights; NS: matrices of an expert (gate and
 // up); DEPTH: steps of a wave in flight.
@@ -1039,6 +1042,12 @@ int launch_slots(const FewArgs& p, int format, int group, hipStream_t stream) {
   // 16, 7.7, 8.8 and 12 with 64, but at 64 tiles 6.6 and 7.0. Gated 4-bit experts take
   // 32 of each matrix (2048 x 576, 4 tokens: 22 us with 16, 15 with 32, 16 with 64),
   // fp32 always 32 (the same call: 39 us, 45 with 64).
+  // Around the lines, the up launch alone, 128 experts, 8 a token, narrow / wide:
+  // 4 bits 2048 x 256 at 64, 96 and 128 tiles 4.8 / 5.6, 5.6 / 5.7 and 5.8 / 5.8,
+  // 2048 x 512 at 192 and 256 7.0 / 6.3 and 9.4 / 6.8 (gated 5.7 / 6.3, 7.7 / 6.7,
+  // 8.1 / 7.2; 10.7 / 9.8, 12.4 / 11.1): level between 96 and 128. bf16 2048 x 256 at
+  // 96 and 128 11.9 / 13.5 and 12.6 / 13.6, 2048 x 512 at 192 and 256 18.1 / 14.2 and
+  // 18.8 / 15.0: from about 160 tiles on wide ones win already.
   const int64_t units = (int64_t)p.T * p.k * div_up(p.cols, 64);  // tiles of 64 columns
   if (format == VMOE_FEW_BF16)
     return units >= 256 ? launch_tiles<WBf16<4>, kUp, 1, NS, true, 4 / NS>(p, stream)
