@@ -990,3 +990,15 @@ def test_module_router_in_a_graph(device):
         eager = m.few_tokens(i)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, r)) and torch.equal(eager, r[0])
+
+
+def test_module_router_on_another_device(device):
+    """Rows or logits on the host are refused."""
+    cfg = TritonMoEConfig(n_embd=64, expert_sizes=[(4, 64)], num_active_experts=2)
+    m = TritonMoEMLP(cfg).to(device).to(torch.bfloat16)
+    x = normal(201, 3, 64).to(device)
+    m.router.register_forward_hook(lambda mod, args, out: out.cpu())
+    with pytest.raises(ValueError, match="logits"):
+        m.few_tokens(x)
+    with pytest.raises(AssertionError, match="CUDA"):
+        m.few_tokens(x.cpu())

@@ -424,6 +424,7 @@ class TritonMoEMLP(nn.Module):
 
     def _few_tokens_routed(self, router, x, experts, return_routing):
         """few_tokens with the choice from router(x), taken as forward() takes it."""
+        _lib.require_gpu(x, "x")
         x_flat = x.reshape(-1, x.shape[-1])
         T, k = x_flat.shape[0], self.num_active_experts
         if T == 0:
@@ -431,10 +432,11 @@ class TritonMoEMLP(nn.Module):
             wts = torch.empty((0, k), dtype=torch.float32, device=x.device)
         else:
             logits = router(x_flat)
-            if logits.shape != (T, self.num_experts):
-                raise ValueError(f"the router's logits must be [{T}, {self.num_experts}] "
-                                 f"(got {tuple(logits.shape)})")
-            state = router_topk(logits, k, self.norm_topk_prob)
+            if logits.shape != (T, self.num_experts) or logits.device != x.device:
+                raise ValueError(f"the router's logits must be [{T}, {self.num_experts}] on "
+                                 f"{x.device} (got {tuple(logits.shape)} on {logits.device})")
+            with torch.cuda.device(x.device):  # (router_topk launches on the current one)
+                state = router_topk(logits, k, self.norm_topk_prob)
             sel, wts = state.selected, state.weights.float()
         out = ft.experts_few_tokens(x, sel, wts, experts)
         return (out, sel, wts) if return_routing else out
