@@ -885,6 +885,78 @@ int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids
                    int64_t k_rows, int64_t max_cols, int32_t group, void* y, int64_t ldy,
                    vmoe_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Dense operators beside the expert layer (no counterpart in the reference):
+ * layer norm, a linear layer with a fused epilogue, a gated feed-forward block.
+ * type: of rows, weights and outputs. Products are exact in fp32 sums, an output
+ * is rounded once; biases and the norm's weights are bf16 or fp32 on their own
+ * (*_f32). A weight is [in, out], or with *_transposed stored [out, in]; leading
+ * dimensions are of the stored matrix, multiples of 8 (fp32: 4), at most 2^20,
+ * as are in, out, hidden and width; buffers are 16-byte aligned, biases by their
+ * type. At most 2^22 rows. Workspaces need no initial value.
+ * ---------------------------------------------------------------------- */
+enum vmoe_dense_type { VMOE_DENSE_BF16 = 0, VMOE_DENSE_F32 = 1 };
+enum vmoe_dense_act {
+  VMOE_DENSE_NONE = 0,
+  VMOE_DENSE_RELU = 1,
+  VMOE_DENSE_RELU_SQUARED = 2,
+  VMOE_DENSE_SILU = 3,
+  VMOE_DENSE_GELU = 4,     /* z (1 + erf(z / sqrt 2)) / 2 */
+  VMOE_DENSE_GELU_TANH = 5 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+};
+
+/* y = act(x w + bias) + residual. bias, residual and z may be NULL; z [rows, out]
+ * fp32 takes x w + bias, which the backward pass of an activation reads. */
+size_t vmoe_linear_workspace_bytes(int32_t type, int64_t rows, int64_t in, int64_t out,
+                                   int32_t act, int32_t backward);
+int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t in,
+                        int64_t out, const void* w, int64_t ldw, int32_t w_transposed,
+                        const void* bias, int32_t bias_f32, int32_t act, const void* residual,
+                        int64_t ldr, void* y, int64_t ldy, float* z, void* workspace,
+                        size_t workspace_bytes, vmoe_stream_t stream);
+/* Gradients of x, w (in w's order) and bias; each may be NULL. */
+int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void* x, int64_t ldx,
+                         int64_t rows, int64_t in, int64_t out, const void* w, int64_t ldw,
+                         int32_t w_transposed, int32_t act, const float* z, void* gx,
+                         int64_t ldgx, void* gw, int64_t ldgw, void* gb, int32_t gb_f32,
+                         void* workspace, size_t workspace_bytes, vmoe_stream_t stream);
+
+/* [g | u] = x w1 + bias1, h = act(g) * u, y = h w2 + bias2 + residual; w1 is
+ * [hidden, 2 width], w2 [width, hidden]. h [rows, width] is written (rounded to the
+ * rows' type); z [rows, 2 width] fp32 takes [g | u] for the backward pass, or is
+ * NULL. */
+size_t vmoe_gated_workspace_bytes(int32_t type, int64_t rows, int64_t hidden, int64_t width,
+                                  int32_t backward);
+int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t hidden,
+                       int64_t width, const void* w1, int64_t ldw1, int32_t w1_transposed,
+                       const void* bias1, int32_t bias1_f32, int32_t act, const void* w2,
+                       int64_t ldw2, int32_t w2_transposed, const void* bias2,
+                       int32_t bias2_f32, const void* residual, int64_t ldr, void* h, float* z,
+                       void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                       vmoe_stream_t stream);
+int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, const void* x, int64_t ldx,
+                        int64_t rows, int64_t hidden, int64_t width, const void* w1, int64_t ldw1,
+                        int32_t w1_transposed, const void* w2, int64_t ldw2,
+                        int32_t w2_transposed, int32_t act, const void* h, const float* z,
+                        void* gx, int64_t ldgx, void* gw1, int64_t ldgw1, void* gb1,
+                        int32_t gb1_f32, void* gw2, int64_t ldgw2, void* gb2, int32_t gb2_f32,
+                        void* workspace, size_t workspace_bytes, vmoe_stream_t stream);
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over rows of d values, 1 to
+ * vmoe_layer_norm_max(); w, b and stats may be NULL. stats [rows, 2] fp32 takes
+ * mean and 1 / sqrt(var + eps). Any leading dimension (x, gy: 0, one row for all)
+ * and alignment; rows of whole 16 bytes are read faster. */
+int64_t vmoe_layer_norm_max(void);
+int vmoe_layer_norm(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t d,
+                    const void* w, int32_t w_f32, const void* b, int32_t b_f32, float eps,
+                    void* y, int64_t ldy, float* stats, vmoe_stream_t stream);
+size_t vmoe_layer_norm_workspace_bytes(int64_t rows, int64_t d);
+int vmoe_layer_norm_backward(int32_t type, const void* gy, int64_t ldgy, const void* x,
+                             int64_t ldx, int64_t rows, int64_t d, const void* w, int32_t w_f32,
+                             const float* stats, void* gx, int64_t ldgx, void* gw, int32_t gw_f32,
+                             void* gb, int32_t gb_f32, void* workspace, size_t workspace_bytes,
+                             vmoe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,272 @@
+// Matrix products of the dense operators on 128 x 128 and 64 x 64 tiles (bf16 and
+// fp32), and what goes with them: the joining of sums split along k, gradients
+// through the activation, column sums.
+//
+// Tiles: four waves, each a quarter of the tile in 32 x 32 blocks, both operands
+// by DMA into a ring of LDS stages of 128 bytes of k.
+
+#include "dense_launch.h"
+
+namespace vmoe {
+namespace dense {
+namespace {
+
+template <typename E, bool AT, bool BT, int EPI, int BM, int BN, int ST>
+__global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs p) {
+  constexpr int FM = BM / 64, FN = BN / 64;
+  constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
+  constexpr int OUT = EPI == EPI_GATED ? BN / 2 : BN;  // output columns of the tile
+  __shared__ __align__(1024) char lds_[ST * STAGE];
+  lds_char* lds = (lds_char*)lds_;
+  static_assert(4 * 32 * 32 * FN * 4 <= ST * STAGE, "epilogue scratch");
+  const Tile t = tile_of(p, blockIdx.x, 16);
+  const int64_t m0 = (int64_t)t.m * BM, n0 = (int64_t)t.n * OUT;
+  const int64_t k0 = t.slice * p.kper, k1 = min(p.K, k0 + p.kper);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  Stager<E, AT, BM, 4> sa;
+  Stager<E, BT, BN, 4> sb;
+  const char* a = static_cast<const char*>(p.a) +
+                  (AT ? k0 * p.lda + m0 : m0 * p.lda + k0) * E::kSize;
+  const char* b = static_cast<const char*>(p.b) +
+                  (BT ? k0 * p.ldb + n0 : n0 * p.ldb + k0) * E::kSize;
+  sa.init(a, p.lda, wave, [&](int r) -> int64_t { return m0 + r < p.M ? r : -1; });
+  sb.init(b, p.ldb, wave, [&](int r) -> int64_t {
+    if (EPI != EPI_GATED) return n0 + r < p.N ? r : -1;
+    // staged: for each wave column 32 gates, then the ups of the same outputs
+    const int o = (r >> 6) * 32 + (r & 31);
+    return n0 + o >= p.N ? -1 : ((r >> 5) & 1) ? p.N + o : o;
+  });
+
+  const int nk = (int)((k1 - k0 + kStageK<E> - 1) / kStageK<E>);
+  constexpr int PER = Stager<E, AT, BM, 4>::kInsts + Stager<E, BT, BN, 4>::kInsts;
+  const uint32_t la = lds_addr(lds) + wave * (Stager<E, AT, BM, 4>::kInsts * 1024);
+  const uint32_t lb = lds_addr(lds) + A_BYTES + wave * (Stager<E, BT, BN, 4>::kInsts * 1024);
+  auto issue = [&](int kt) {
+    const int64_t left = k1 - k0 - (int64_t)kt * kStageK<E>;
+    sa.issue(la + (kt % ST) * STAGE, left);
+    sb.issue(lb + (kt % ST) * STAGE, left);
+  };
+  f32x16_t acc[FM][FN] = {};
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s)
+    if (s < nk) issue(s);
+  for (int kt = 0; kt < nk; ++kt) {
+    if (kt + ST - 2 < nk) wait_vmcnt<(ST - 2) * PER>();
+    else wait_vmcnt<0>();
+    block_barrier();
+    if (kt + ST - 1 < nk) issue(kt + ST - 1);
+    const lds_char* st = lds + (kt % ST) * STAGE;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      typename E::Frag af[FM], bf[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) af[i] = frag<E, AT, BM>(st, (wm * FM + i) * 32, s);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) bf[j] = frag<E, BT, BN>(st + A_BYTES, (wn * FN + j) * 32, s);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mma(af[i], bf[j], acc[i][j]);
+    }
+  }
+  block_barrier();  // every wave has read the last stages
+  write_tile<E, EPI, FM, FN>(p, acc, lds + wave * (32 * 32 * FN * 4), m0 + wm * 32 * FM,
+                             n0 + wn * (EPI == EPI_GATED ? 32 : 32 * FN), t.slice,
+                             (int64_t)t.m * 2 + wm);
+}
+
+template <typename E, bool AT, bool BT, int EPI, int BM, int BN, int ST>
+int launch_tile(GemmArgs p, hipStream_t s) {
+  constexpr int OUT = EPI == EPI_GATED ? BN / 2 : BN;
+  p.tiles_m = (int)((p.M + BM - 1) / BM);
+  p.tiles_n = (int)((p.N + OUT - 1) / OUT);
+  const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  VMOE_LAUNCH((gemm_kernel<E, AT, BT, EPI, BM, BN, ST>), dim3((uint32_t)grid), dim3(256), 0, s, p);
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+
+template <typename E, bool AT, bool BT, int EPI>
+int launch_form(const GemmArgs& p, Tiles tiles, hipStream_t s) {
+  if constexpr (EPI != EPI_GATED) {
+    if (tiles == TILES_64) return launch_tile<E, AT, BT, EPI, 64, 64, 3>(p, s);
+  } else {
+    if (tiles == TILES_64) return launch_tile<E, AT, BT, EPI, 64, 128, 2>(p, s);
+  }
+  return launch_tile<E, AT, BT, EPI, 128, 128, 2>(p, s);
+}
+
+// ---------------------------------------------------------------------------
+// Sums split along k: part [splits, M, ldp] through the epilogue (EPI_GATED: the
+// gates' sums, then the ups').
+template <typename E, int EPI>
+__global__ __launch_bounds__(256) void join_kernel(GemmArgs p) {
+  const int64_t groups = (p.N + 7) / 8;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= p.M * groups) return;
+  const int64_t m = id / groups, n = (id - m * groups) * 8;
+  const bool two = n + 4 < p.N;
+  EpiCols<EPI> cols;
+  epi_cols<EPI>(p, n, cols);
+  float v[8] = {}, u[8] = {}, sg[8], su[8];
+  for (int s = 0; s < p.splits; ++s) {
+    const float* row = p.part + ((int64_t)s * p.M + m) * p.ldp;
+    float x[8];
+    load8<F32>(row, n, two, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += x[i];
+    if (EPI == EPI_GATED) {
+      load8<F32>(row, p.N + n, two, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] += x[i];
+    }
+  }
+  epi8<E, EPI>(p, cols, m, n, v, u, sg, su);
+}
+
+// dz = gy * act'(z), rounded, and the column sums of what it stores before
+// rounding: a workgroup takes kSumRows rows of 512 columns, part its row of them.
+constexpr int kSumRows = 64;
+template <typename E, bool ACT>
+__global__ __launch_bounds__(256) void act_grad_kernel(const void* gy, int64_t ldgy,
+                                                       const float* z, int64_t ldz, int act,
+                                                       void* dz, int64_t lddz, float* part,
+                                                       int64_t M, int64_t N) {
+  __shared__ float red[4][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = (int64_t)blockIdx.x * 512 + lane * 8;
+  const int64_t m0 = (int64_t)blockIdx.y * kSumRows;
+  const bool two = n + 4 < N;
+  float sum[8] = {};
+  if (n < N) {
+    const int64_t m1 = min(M, m0 + kSumRows);
+    for (int64_t m = m0 + wave; m < m1; m += 4) {
+      float g[8];
+      load8<E>(static_cast<const typename E::Store*>(gy) + m * ldgy, n, two, g);
+      if constexpr (ACT) {
+        float x[8];
+        load8<F32>(z + m * ldz, n, two, x);
+        act_switch(act, [&](auto A) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float slope;
+            act1<decltype(A)::value, true>(x[i], slope);
+            g[i] *= slope;
+          }
+        });
+        store8<E>(static_cast<typename E::Store*>(dz) + m * lddz, n, two, g);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += g[i];
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[wave][lane * 8 + i] = sum[i];
+  __syncthreads();
+#pragma unroll
+  for (int c = threadIdx.x; c < 512; c += 256) {
+    const int64_t col = (int64_t)blockIdx.x * 512 + c;
+    if (col < N)
+      part[(int64_t)blockIdx.y * N + col] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  }
+}
+
+// Column sums of part [rows, N] into out (bf16 or fp32): 16 columns a workgroup,
+// 16 threads a column.
+__global__ __launch_bounds__(256) void col_sum_kernel(const float* part, int64_t rows, int64_t N,
+                                                      void* out, int out_f32) {
+  __shared__ float red[16][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int64_t n = (int64_t)blockIdx.x * 16 + c;
+  float s = 0.0f;
+  if (n < N)
+    for (int64_t m = r; m < rows; m += 16) s += part[m * N + n];
+  red[r][c] = s;
+  __syncthreads();
+  if (r == 0 && n < N) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += red[i][c];
+    if (out_f32) static_cast<float*>(out)[n] = t;
+    else static_cast<uint16_t*>(out)[n] = (uint16_t)f32_to_bf16(t);
+  }
+}
+
+}  // namespace
+
+int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s) {
+  auto go = [&](auto e, auto f) -> int {
+    typedef decltype(e) E;
+    constexpr int F = decltype(f)::value;
+    constexpr bool AT = F == FORM_TT, BT = F != FORM_KK;
+    switch (epi) {
+      case EPI_LINEAR: return launch_form<E, AT, BT, EPI_LINEAR>(p, tiles, s);
+      case EPI_PARTIAL: return launch_form<E, AT, BT, EPI_PARTIAL>(p, tiles, s);
+      case EPI_GATED:
+        if constexpr (!AT) return launch_form<E, AT, BT, EPI_GATED>(p, tiles, s);
+        break;
+      case EPI_GATED_BWD:
+        if constexpr (!AT) return launch_form<E, AT, BT, EPI_GATED_BWD>(p, tiles, s);
+        break;
+    }
+    return VMOE_ERR_INVALID_ARG;
+  };
+  auto by_form = [&](auto e) -> int {
+    switch (form) {
+      case FORM_KK: return go(e, std::integral_constant<int, FORM_KK>());
+      case FORM_KT: return go(e, std::integral_constant<int, FORM_KT>());
+      default: return go(e, std::integral_constant<int, FORM_TT>());
+    }
+  };
+  return type == VMOE_DENSE_F32 ? by_form(F32()) : by_form(Bf16());
+}
+
+int join_splits(int type, Epi epi, const GemmArgs& p, hipStream_t s) {
+  const int64_t blocks = (p.M * ((p.N + 7) / 8) + 255) / 256;
+  auto go = [&](auto e) {
+    typedef decltype(e) E;
+    if (epi == EPI_LINEAR)
+      VMOE_LAUNCH((join_kernel<E, EPI_LINEAR>), dim3((uint32_t)blocks), dim3(256), 0, s, p);
+    else if (epi == EPI_GATED)
+      VMOE_LAUNCH((join_kernel<E, EPI_GATED>), dim3((uint32_t)blocks), dim3(256), 0, s, p);
+    else
+      VMOE_LAUNCH((join_kernel<E, EPI_GATED_BWD>), dim3((uint32_t)blocks), dim3(256), 0, s, p);
+  };
+  if (type == VMOE_DENSE_F32) go(F32());
+  else go(Bf16());
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+
+int64_t sum_rows(int64_t M) { return (M + kSumRows - 1) / kSumRows; }
+
+int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
+             void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s) {
+  const dim3 grid((uint32_t)((N + 511) / 512), (uint32_t)sum_rows(M));
+  auto go = [&](auto e) {
+    typedef decltype(e) E;
+    if (z)
+      VMOE_LAUNCH((act_grad_kernel<E, true>), grid, dim3(256), 0, s, gy, ldgy, z, ldz, act, dz,
+                  lddz, part, M, N);
+    else
+      VMOE_LAUNCH((act_grad_kernel<E, false>), grid, dim3(256), 0, s, gy, ldgy, z, ldz, act, dz,
+                  lddz, part, M, N);
+  };
+  if (type == VMOE_DENSE_F32) go(F32());
+  else go(Bf16());
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+
+int col_sum(const float* part, int64_t rows, int64_t N, void* out, int out_f32, hipStream_t s) {
+  VMOE_LAUNCH(col_sum_kernel, dim3((uint32_t)((N + 15) / 16)), dim3(256), 0, s, part, rows, N, out,
+              out_f32);
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+
+}  // namespace dense
+}  // namespace vmoe

@@ -1,0 +1,21 @@
+// What the dense operators' entry points (dense.hip) call.
+#pragma once
+
+#include "dense.h"
+
+namespace vmoe {
+namespace dense {
+
+enum Form { FORM_KK, FORM_KT, FORM_TT };  // A's, B's
+enum Tiles { TILES_64, TILES_128, TILES_256 };
+
+// dense_gemm.hip
+int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
+int join_splits(int type, Epi epi, const GemmArgs& p, hipStream_t s);
+int64_t sum_rows(int64_t M);  // rows of the sums that act_grad leaves
+int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
+             void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s);
+int col_sum(const float* part, int64_t rows, int64_t N, void* out, int out_f32, hipStream_t s);
+
+}  // namespace dense
+}  // namespace vmoe

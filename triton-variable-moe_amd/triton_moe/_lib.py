@@ -142,6 +142,24 @@ _SIGNATURES = {
     "vmoe_q4_dequantize": [_vp, _vp, _vp, _i32, _i32, _i64, _i64, _i32, _vp, _i32, _i64, _vp],
     "vmoe_q4_matvec": [_vp, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _i64, _i32,
                        _vp, _i64, _vp],
+    "vmoe_linear_workspace_bytes": [_i32, _i64, _i64, _i64, _i32, _i32],
+    "vmoe_linear_forward": [_i32, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32,
+                            _vp, _i64, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp],
+    "vmoe_linear_backward": [_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _i32,
+                             _vp, _vp, _i64, _vp, _i64, _vp, _i32, _vp, ctypes.c_size_t, _vp],
+    "vmoe_gated_workspace_bytes": [_i32, _i64, _i64, _i64, _i32],
+    "vmoe_gated_forward": [_i32, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32,
+                           _vp, _i64, _i32, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _vp,
+                           ctypes.c_size_t, _vp],
+    "vmoe_gated_backward": [_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp,
+                            _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i32, _vp,
+                            _i64, _vp, _i32, _vp, ctypes.c_size_t, _vp],
+    "vmoe_layer_norm_max": [],
+    "vmoe_layer_norm": [_i32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _i32, ctypes.c_float, _vp,
+                        _i64, _vp, _vp],
+    "vmoe_layer_norm_workspace_bytes": [_i64, _i64],
+    "vmoe_layer_norm_backward": [_i32, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp,
+                                 _i64, _vp, _i32, _vp, _i32, _vp, ctypes.c_size_t, _vp],
 }
 _RESTYPES = {
     "vmoe_status_string": ctypes.c_char_p,
@@ -152,6 +170,10 @@ _RESTYPES = {
     "vmoe_router_partial_floats": ctypes.c_size_t,
     "vmoe_router_linear_bwd_workspace_bytes": ctypes.c_size_t,
     "vmoe_few_workspace_bytes": ctypes.c_size_t,
+    "vmoe_linear_workspace_bytes": ctypes.c_size_t,
+    "vmoe_gated_workspace_bytes": ctypes.c_size_t,
+    "vmoe_layer_norm_workspace_bytes": ctypes.c_size_t,
+    "vmoe_layer_norm_max": _i64,
 }
 
 # Status codes (include/vmoe.h).
@@ -159,6 +181,9 @@ OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_WORKSPACE = 0, 1, 2, 3, 4
 ROUNDING = {"up": 0, "down": 1, "nearest": 2}
 ACT_NONE, ACT_RELU_SQUARED, ACT_SWIGLU = 0, 1, 2
 FEW_BF16, FEW_F32, FEW_Q4 = 0, 1, 2  # enum vmoe_few_format
+DENSE_BF16, DENSE_F32 = 0, 1  # enum vmoe_dense_type
+DENSE_ACT = {None: 0, "relu": 1, "relu_squared": 2, "silu": 3, "gelu": 4,
+             "gelu_tanh": 5}  # enum vmoe_dense_act
 INFO_ROWS, INFO_KEPT, INFO_ERRORS, INFO_LEN = 0, 1, 2, 4
 # Slots of vmoe_expert_layout's saved buffer (enum vmoe_expert_slot).
 (X_BIN_IDS, X_INDICES, X_TPE, X_BINS, X_PADDED_BINS, X_ROW_SRC, X_GATHER_MAP, X_ASSIGNMENT_ROW,

@@ -1,6 +1,6 @@
 """gfx950 HIP kernel implementations of the MoE operations (the
 export surface of triton_moe/kernels/__init__.py:18-40 of the reference, and the
-operators for a few tokens, which it lacks)."""
+operators for a few tokens and the dense operators, which it lacks)."""
 
 from .gather import padded_gather, padded_gather_autograd
 from .scatter import padded_scatter, padded_scatter_autograd
@@ -16,6 +16,7 @@ from .grouped_gemm import (
     GroupedGemmDown,
 )
 from .fused_cumsum import fused_route
+from .dense import fused_linear, gated_mlp, layer_norm, layer_norm_max
 from .few_tokens import (
     FewTokenExperts,
     QuantizedExperts,
@@ -62,4 +63,9 @@ __all__ = [
     "FewTokenExperts",
     "QuantizedExperts",
     "QuantizedMatrices",
+    # Dense operators beside the expert layer
+    "layer_norm",
+    "layer_norm_max",
+    "fused_linear",
+    "gated_mlp",
 ]
