@@ -116,138 +116,143 @@ __device__ __forceinline__ void act_switch(int act, F&& f) {
   }
 }
 
-// 8 consecutive values of a row. Rows are 16-byte aligned and n a multiple of 8;
-// float32 rows may end after the first 4 (`two` false).
-template <typename E>
-__device__ __forceinline__ void load8(const void* row, int64_t n, bool two, float (&v)[8]) {
-  if constexpr (E::kSize == 2) {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(row) + n);
+// C consecutive values of a row, 4 or 8 (8: bf16 alone). n is a multiple of C, rows
+// are 16-byte aligned.
+template <typename E, int C>
+__device__ __forceinline__ void load_c(const void* row, int64_t n, float (&v)[C]) {
+  if constexpr (E::kSize == 4) {
+    static_assert(C == 4, "16 bytes");
+    const f32x4_t w = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(row) + n);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) v[i] = w[i];
+  } else {
+    typedef uint32_t words __attribute__((ext_vector_type(C / 2)));
+    const words w = *reinterpret_cast<const words*>(static_cast<const uint16_t*>(row) + n);
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) {
       v[2 * i] = lo_f32(w[i]);
       v[2 * i + 1] = hi_f32(w[i]);
     }
-  } else {
-    const float* p = static_cast<const float*>(row) + n;
-    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p);
-    f32x4_t b = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (two) b = *reinterpret_cast<const f32x4_t*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = a[i];
-      v[4 + i] = b[i];
-    }
   }
 }
 
-template <typename E>
-__device__ __forceinline__ void store8(void* row, int64_t n, bool two, const float (&v)[8]) {
-  if constexpr (E::kSize == 2) {
-    u32x4_t w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(row) + n) = w;
+template <typename E, int C>
+__device__ __forceinline__ void store_c(void* row, int64_t n, const float (&v)[C]) {
+  if constexpr (E::kSize == 4) {
+    static_assert(C == 4, "16 bytes");
+    const f32x4_t w = {v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4_t*>(static_cast<float*>(row) + n) = w;
   } else {
-    float* p = static_cast<float*>(row) + n;
-    const f32x4_t a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    *reinterpret_cast<f32x4_t*>(p) = a;
-    if (two) *reinterpret_cast<f32x4_t*>(p + 4) = b;
+    typedef uint32_t words __attribute__((ext_vector_type(C / 2)));
+    words w;
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<words*>(static_cast<uint16_t*>(row) + n) = w;
   }
 }
 
-// 8 values of the bias from column n on (its address may be any multiple of its
+// C values of the bias from column n on (its address may be any multiple of its
 // type's size: a slice of a longer vector).
-__device__ __forceinline__ void bias8(const void* bias, int f32, int64_t n, bool two,
-                                      float (&v)[8]) {
-  const int m = two ? 8 : 4;
-  if (f32) {
+template <int C>
+__device__ __forceinline__ void bias_c(const void* bias, int f32, int64_t n, float (&v)[C]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < m ? static_cast<const float*>(bias)[n + i] : 0.0f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = i < m ? bf16_to_f32(static_cast<const uint16_t*>(bias)[n + i]) : 0.0f;
-  }
+  for (int i = 0; i < C; ++i)
+    v[i] = f32 ? static_cast<const float*>(bias)[n + i]
+               : bf16_to_f32(static_cast<const uint16_t*>(bias)[n + i]);
 }
 
-// The epilogue's operands that are the same for every row: the bias of 8 columns.
-template <int EPI>
+// Columns of a row that a thread takes in an epilogue: 16 bytes of its widest
+// buffer (the fp32 sums, pre-activations or outputs where there are any).
+template <typename E, int EPI>
+constexpr int kEpiCols = E::kSize == 2 && EPI == EPI_LINEAR ? 8 : 4;
+
+// What is the same for every row of C columns: their bias.
+template <int EPI, int C>
 struct EpiCols {
-  float b[8], b2[8];
+  float b[C], b2[C];
 };
-template <int EPI>
-__device__ __forceinline__ void epi_cols(const GemmArgs& p, int64_t n, EpiCols<EPI>& q) {
+template <int EPI, int C>
+__device__ __forceinline__ void epi_cols(const GemmArgs& p, int64_t n, EpiCols<EPI, C>& q) {
   if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q.b[i] = q.b2[i] = 0.0f;
+    for (int i = 0; i < C; ++i) q.b[i] = q.b2[i] = 0.0f;
     if (p.bias && n < p.N) {
-      const bool two = n + 4 < p.N;
-      bias8(p.bias, p.bias_f32, n, two, q.b);
-      if (EPI == EPI_GATED) bias8(p.bias, p.bias_f32, p.N + n, two, q.b2);
+      bias_c<C>(p.bias, p.bias_f32, n, q.b);
+      if (EPI == EPI_GATED) bias_c<C>(p.bias, p.bias_f32, p.N + n, q.b2);
     }
   }
 }
 
-// Row m, columns n .. n + 7 (the caller has checked m < M and n < N): v are the
-// sums, u the up half's for EPI_GATED. EPI_GATED_BWD adds what it stores, before
-// rounding, to sg and su (this thread's columns of the bias gradient).
-template <typename E, int EPI>
-__device__ __forceinline__ void epi8(const GemmArgs& p, const EpiCols<EPI>& q, int64_t m,
-                                     int64_t n, float (&v)[8], float (&u)[8], float (&sg)[8],
-                                     float (&su)[8]) {
-  const bool two = n + 4 < p.N;
+// EPI_GATED_BWD: the gates and ups of row m, columns n .. n + 3.
+struct GateUp {
+  f32x4_t g, u;
+};
+__device__ __forceinline__ GateUp load_z(const GemmArgs& p, int64_t m, int64_t n) {
+  GateUp q;
+  q.g = *reinterpret_cast<const f32x4_t*>(p.z + m * p.ldz + n);
+  q.u = *reinterpret_cast<const f32x4_t*>(p.z + m * p.ldz + p.N + n);
+  return q;
+}
+
+// Row m, columns n .. n + C - 1 (the caller has checked m < M and n < N): v are the
+// sums, u the up half's for EPI_GATED. KEEP: pre-activations are stored too, if
+// wanted. EPI_GATED_BWD adds what it stores, before rounding, to sg and su (this
+// thread's columns of the bias gradient).
+template <typename E, int EPI, int C, bool KEEP = true>
+__device__ __forceinline__ void epi_row(const GemmArgs& p, const EpiCols<EPI, C>& q, int64_t m,
+                                        int64_t n, float (&v)[C], float (&u)[C],
+                                        const GateUp& z, float (&sg)[C], float (&su)[C]) {
   typename E::Store* c = static_cast<typename E::Store*>(p.c) + m * p.ldc;
   float unused;
   if constexpr (EPI == EPI_LINEAR) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += q.b[i];
-    if (p.z) store8<F32>(p.z + m * p.ldz, n, two, v);
+    for (int i = 0; i < C; ++i) v[i] += q.b[i];
+    if constexpr (KEEP && C == 4)
+      if (p.z) store_c<F32, C>(p.z + m * p.ldz, n, v);
     act_switch(p.act, [&](auto A) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act1<decltype(A)::value, false>(v[i], unused);
+      for (int i = 0; i < C; ++i) v[i] = act1<decltype(A)::value, false>(v[i], unused);
     });
     if (p.res) {
-      float r[8];
-      load8<E>(static_cast<const typename E::Store*>(p.res) + m * p.ldr, n, two, r);
+      float r[C];
+      load_c<E, C>(static_cast<const typename E::Store*>(p.res) + m * p.ldr, n, r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += r[i];
+      for (int i = 0; i < C; ++i) v[i] += r[i];
     }
-    store8<E>(c, n, two, v);
+    store_c<E, C>(c, n, v);
   } else if constexpr (EPI == EPI_GATED) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < C; ++i) {
       v[i] += q.b[i];
       u[i] += q.b2[i];
     }
     if (p.z) {
-      store8<F32>(p.z + m * p.ldz, n, two, v);
-      store8<F32>(p.z + m * p.ldz + p.N, n, two, u);
+      store_c<F32, C>(p.z + m * p.ldz, n, v);
+      store_c<F32, C>(p.z + m * p.ldz + p.N, n, u);
     }
     act_switch(p.act, [&](auto A) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act1<decltype(A)::value, false>(v[i], unused) * u[i];
+      for (int i = 0; i < C; ++i) v[i] = act1<decltype(A)::value, false>(v[i], unused) * u[i];
     });
-    store8<E>(c, n, two, v);
+    store_c<E, C>(c, n, v);
   } else if constexpr (EPI == EPI_GATED_BWD) {
-    float g[8], up[8];
-    load8<F32>(p.z + m * p.ldz, n, two, g);
-    load8<F32>(p.z + m * p.ldz + p.N, n, two, up);
+    float g[C], up[C];
     act_switch(p.act, [&](auto A) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < C; ++i) {
         float slope;
-        const float a = act1<decltype(A)::value, true>(g[i], slope);
-        g[i] = v[i] * up[i] * slope;
+        const float a = act1<decltype(A)::value, true>(z.g[i], slope);
+        g[i] = v[i] * z.u[i] * slope;
         up[i] = v[i] * a;
       }
     });
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < C; ++i) {
       sg[i] += g[i];
       su[i] += up[i];
     }
-    store8<E>(c, n, two, g);
-    store8<E>(c + p.N, n, two, up);
+    store_c<E, C>(c, n, g);
+    store_c<E, C>(c + p.N, n, up);
   }
 }
 
@@ -400,28 +405,43 @@ __device__ __forceinline__ f32x16_t mma(f32x4_t a, f32x4_t b, f32x16_t acc) {
 
 // Writes the results of a wave: FM x FN blocks of 32 x 32 from (m0, n0) on, 32
 // rows at a time through the wave's own 32 x 32 FN x 4 bytes of LDS, so that
-// memory sees whole rows of 8 columns a lane. EPI_GATED: block 0 holds gates,
-// block 1 the ups of the same 32 columns. part_row: the row of p.part that takes
-// the wave's column sums.
+// memory sees whole rows, 16 bytes a lane. EPI_GATED: block 0 holds gates, block 1
+// the ups of the same 32 columns. part_row: the row of p.part that takes the wave's
+// column sums.
 template <typename E, int EPI, int FM, int FN>
 __device__ __forceinline__ void write_tile(const GemmArgs& p, const f32x16_t (&acc)[FM][FN],
                                            lds_char* scr, int64_t m0, int64_t n0, int slice,
                                            int64_t part_row) {
   constexpr int WN = 32 * FN, CH = WN / 4;        // staged columns, 16-byte chunks of a row
-  constexpr bool GATED = EPI == EPI_GATED;
+  constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
   static_assert(!GATED || FN == 2, "gate and up");
+  constexpr int C = kEpiCols<E, EPI>;
   constexpr int OUT = GATED ? 32 : WN;            // output columns
-  constexpr int LR = OUT / 8, RP = 64 / LR;       // lanes of a row, rows of a pass
+  constexpr int LR = OUT / C, RP = 64 / LR;       // lanes of a row, rows of a pass
+  constexpr int PASSES = 32 / RP;
   const int lane = threadIdx.x & 63;
-  const int64_t n = n0 + (lane % LR) * 8;
-  EpiCols<EPI> cols;
-  epi_cols<EPI>(p, n, cols);
-  float sg[8], su[8];
+  const int64_t n = n0 + (lane % LR) * C;
+  const bool n_ok = n < p.N;
+  EpiCols<EPI, C> cols;
+  epi_cols<EPI, C>(p, n, cols);
+  float sg[C], su[C];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sg[i] = su[i] = 0.0f;
+  for (int i = 0; i < C; ++i) sg[i] = su[i] = 0.0f;
   auto at = [&](int r, int c) {
     return scr + r * (WN * 4) + ((c ^ (CH == 16 ? r & 15 : (r >> 1) & 7)) << 4);
   };
+  // EPI_GATED_BWD: the gates and ups of a half of 32 rows are fetched while the half
+  // before is written, the first while the last rows' sums are staged
+  constexpr int HALF = BWD ? PASSES / 2 : 1;
+  GateUp z[2][HALF] = {};
+  auto fetch = [&](int i, int h) {
+#pragma unroll
+    for (int t = 0; t < HALF; ++t) {
+      const int64_t m = m0 + 32 * i + (h * HALF + t) * RP + lane / LR;
+      if (m < p.M && n_ok) z[h][t] = load_z(p, m, n);
+    }
+  };
+  if constexpr (BWD) fetch(0, 0);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     if (m0 + 32 * i >= p.M) break;
@@ -435,46 +455,62 @@ __device__ __forceinline__ void write_tile(const GemmArgs& p, const f32x16_t (&a
         *reinterpret_cast<lds_f32x4*>(at(lane & 31, 8 * j + 2 * g + (lane >> 5))) = v;
       }
     asm volatile("" ::: "memory");
+    if constexpr (EPI == EPI_LINEAR && C == 8) {
+      if (p.z) {  // the pre-activations first: 4 columns a lane
+        const int64_t nz = n0 + (lane % CH) * 4;
+        EpiCols<EPI, 4> qz;
+        epi_cols<EPI, 4>(p, nz, qz);
 #pragma unroll
-    for (int t = 0; t < 32 / RP; ++t) {
-      const int r = t * RP + lane / LR, c = 2 * (lane % LR);
-      const f32x4_t a = *reinterpret_cast<lds_f32x4*>(at(r, c));
-      const f32x4_t b = *reinterpret_cast<lds_f32x4*>(at(r, c + 1));
-      f32x4_t a2 = a, b2 = b;
-      if (GATED) {
-        a2 = *reinterpret_cast<lds_f32x4*>(at(r, c + 8));
-        b2 = *reinterpret_cast<lds_f32x4*>(at(r, c + 9));
+        for (int t = 0; t < CH / 2; ++t) {
+          const int r = t * (64 / CH) + lane / CH;
+          const f32x4_t a = *reinterpret_cast<lds_f32x4*>(at(r, lane % CH));
+          const float v[4] = {a[0] + qz.b[0], a[1] + qz.b[1], a[2] + qz.b[2], a[3] + qz.b[3]};
+          const int64_t m = m0 + 32 * i + r;
+          if (m < p.M && nz < p.N) store_c<F32, 4>(p.z + m * p.ldz, nz, v);
+        }
       }
-      const int64_t m = m0 + 32 * i + r;
-      if (m < p.M && n < p.N) {
-        float v[8], u[8];
+    }
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      if constexpr (BWD) {
+        if (t == 0) fetch(i, 1);
+        if (t == HALF && i + 1 < FM) fetch(i + 1, 0);
+      }
+      const int r = t * RP + lane / LR, c = (lane % LR) * (C / 4);
+      float v[C], u[C];
+#pragma unroll
+      for (int q = 0; q < C / 4; ++q) {
+        const f32x4_t a = *reinterpret_cast<lds_f32x4*>(at(r, c + q));
+        f32x4_t b = a;
+        if (GATED) b = *reinterpret_cast<lds_f32x4*>(at(r, c + q + 8));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = a[e];
-          v[4 + e] = b[e];
-          u[e] = a2[e];
-          u[4 + e] = b2[e];
+          v[4 * q + e] = a[e];
+          u[4 * q + e] = b[e];
         }
+      }
+      const int64_t m = m0 + 32 * i + r;
+      if (m < p.M && n_ok) {
         if constexpr (EPI == EPI_PARTIAL)
-          store8<F32>(p.part + ((int64_t)slice * p.M + m) * p.ldp, n, n + 4 < p.N, v);
+          store_c<F32, C>(p.part + ((int64_t)slice * p.M + m) * p.ldp, n, v);
         else
-          epi8<E, EPI>(p, cols, m, n, v, u, sg, su);
+          epi_row<E, EPI, C>(p, cols, m, n, v, u, z[t / HALF & 1][t % HALF], sg, su);
       }
     }
   }
-  if constexpr (EPI == EPI_GATED_BWD) {
+  if constexpr (BWD) {
     if (p.part && n0 < p.N && m0 < p.M) {
       // lanes of the same columns, in a fixed order
 #pragma unroll
       for (int o = LR; o < 64; o *= 2)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < C; ++i) {
           sg[i] += __shfl_xor(sg[i], o, 64);
           su[i] += __shfl_xor(su[i], o, 64);
         }
-      if (lane < LR && n < p.N) {
-        store8<F32>(p.part + part_row * p.ldp, n, n + 4 < p.N, sg);
-        store8<F32>(p.part + part_row * p.ldp + p.N, n, n + 4 < p.N, su);
+      if (lane < LR && n_ok) {
+        store_c<F32, C>(p.part + part_row * p.ldp, n, sg);
+        store_c<F32, C>(p.part + part_row * p.ldp + p.N, n, su);
       }
     }
   }

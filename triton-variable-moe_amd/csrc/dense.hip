@@ -54,12 +54,17 @@ Plan plan_of(int type, Epi epi, int64_t M, int64_t N, int64_t K) {
   const int64_t n = epi == EPI_GATED ? 2 * N : N;  // columns staged
   const int64_t stage = 128 / esize(type);
   auto count = [&](int64_t t, int64_t tn) { return cdiv(M, t) * cdiv(n, tn); };
-  q.tiles = count(128, 128) >= 256 ? TILES_128 : TILES_64;
-  const int64_t tiles = std::max<int64_t>(1, q.tiles == TILES_128 ? count(128, 128)
-                                             : epi == EPI_GATED ? count(64, 128) : count(64, 64));
+  q.tiles = type == VMOE_DENSE_BF16 && count(256, 256) >= 224 ? TILES_256
+            : count(128, 128) >= 256                          ? TILES_128
+                                                              : TILES_64;
+  const int64_t tiles = std::max<int64_t>(1, q.tiles == TILES_256   ? count(256, 256)
+                                             : q.tiles == TILES_128 ? count(128, 128)
+                                             : epi == EPI_GATED     ? count(64, 128)
+                                                                    : count(64, 64));
   q.splits = 1;
   const int64_t stages = cdiv(K, stage);
-  if (tiles < 256) q.splits = (int)std::max<int64_t>(1, std::min(512 / tiles, stages / 8));
+  if (tiles < 256 && q.tiles != TILES_256)
+    q.splits = (int)std::max<int64_t>(1, std::min(512 / tiles, stages / 8));
   q.kper = cdiv(stages, q.splits) * stage;
   q.splits = (int)cdiv(K, q.kper);
   q.part_bytes = q.splits > 1 ? align256((size_t)q.splits * M * n * 4) : 0;
@@ -82,7 +87,7 @@ int product(int type, Form form, Epi epi, GemmArgs p, float* part, int64_t* sums
     p.ldp = g.ldp;
     return join_splits(type, epi, p, s);
   }
-  if (sums) *sums = cdiv(p.M, q.tiles == TILES_64 ? 32 : 64);
+  if (sums) *sums = cdiv(p.M, q.tiles == TILES_64 ? 32 : q.tiles == TILES_128 ? 64 : 128);
   return gemm_tiles(type, form, epi, p, q.tiles, s);
 }
 
@@ -231,7 +236,7 @@ extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, 
   if (has_act || gb) {
     VMOE_TRY(act_grad(type, gy, ldgy, has_act ? z : nullptr, out, act, dz, out,
                       gb ? sums : nullptr, rows, out, s));
-    if (gb) VMOE_TRY(col_sum(sums, sum_rows(rows), out, gb, gb_f32, s));
+    if (gb) VMOE_TRY(col_sum(sums, sum_rows(rows), out, out, gb, gb_f32, nullptr, 0, s));
   }
   const void* g = has_act ? dz : gy;
   const int64_t ldg = has_act ? out : ldgy;
@@ -343,12 +348,13 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
       VMOE_TRY(act_grad(type, dz, w2x, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows, w2x, s));
       n = sum_rows(rows);
     }
-    if (gb1) VMOE_TRY(col_sum(sums, n, w2x, gb1, gb1_f32, s));
+    if (gb1) VMOE_TRY(col_sum(sums, n, w2x, w2x, gb1, gb1_f32, nullptr, 0, s));
   }
   if (gb2) {
     VMOE_TRY(act_grad(type, gy, ldgy, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows, hidden,
                       s));
-    VMOE_TRY(col_sum(sums, sum_rows(rows), hidden, gb2, gb2_f32, s));
+    VMOE_TRY(col_sum(sums, sum_rows(rows), hidden, hidden, gb2, gb2_f32, nullptr,
+                     0, s));
   }
   if (gw2)
     VMOE_TRY(product(type, FORM_TT, EPI_LINEAR,

@@ -11,22 +11,23 @@ namespace vmoe {
 namespace dense {
 namespace {
 
-template <typename E, bool AT, bool BT, int EPI, int BM, int BN, int ST>
-__global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs p) {
-  constexpr int FM = BM / 64, FN = BN / 64;
+template <typename E, bool AT, bool BT, int EPI, int BM, int BN, int ST, int WM = 2, int WN = 2>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
+  constexpr int NW = WM * WN;
+  constexpr int FM = BM / 32 / WM, FN = BN / 32 / WN;
   constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
   constexpr int OUT = EPI == EPI_GATED ? BN / 2 : BN;  // output columns of the tile
   __shared__ __align__(1024) char lds_[ST * STAGE];
   lds_char* lds = (lds_char*)lds_;
-  static_assert(4 * 32 * 32 * FN * 4 <= ST * STAGE, "epilogue scratch");
+  static_assert(NW * 32 * 32 * FN * 4 <= ST * STAGE, "epilogue scratch");
   const Tile t = tile_of(p, blockIdx.x, 16);
   const int64_t m0 = (int64_t)t.m * BM, n0 = (int64_t)t.n * OUT;
   const int64_t k0 = t.slice * p.kper, k1 = min(p.K, k0 + p.kper);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
 
-  Stager<E, AT, BM, 4> sa;
-  Stager<E, BT, BN, 4> sb;
+  Stager<E, AT, BM, NW> sa;
+  Stager<E, BT, BN, NW> sb;
   const char* a = static_cast<const char*>(p.a) +
                   (AT ? k0 * p.lda + m0 : m0 * p.lda + k0) * E::kSize;
   const char* b = static_cast<const char*>(p.b) +
@@ -40,9 +41,9 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs p) {
   });
 
   const int nk = (int)((k1 - k0 + kStageK<E> - 1) / kStageK<E>);
-  constexpr int PER = Stager<E, AT, BM, 4>::kInsts + Stager<E, BT, BN, 4>::kInsts;
-  const uint32_t la = lds_addr(lds) + wave * (Stager<E, AT, BM, 4>::kInsts * 1024);
-  const uint32_t lb = lds_addr(lds) + A_BYTES + wave * (Stager<E, BT, BN, 4>::kInsts * 1024);
+  constexpr int PER = Stager<E, AT, BM, NW>::kInsts + Stager<E, BT, BN, NW>::kInsts;
+  const uint32_t la = lds_addr(lds) + wave * (Stager<E, AT, BM, NW>::kInsts * 1024);
+  const uint32_t lb = lds_addr(lds) + A_BYTES + wave * (Stager<E, BT, BN, NW>::kInsts * 1024);
   auto issue = [&](int kt) {
     const int64_t left = k1 - k0 - (int64_t)kt * kStageK<E>;
     sa.issue(la + (kt % ST) * STAGE, left);
@@ -74,7 +75,7 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs p) {
   block_barrier();  // every wave has read the last stages
   write_tile<E, EPI, FM, FN>(p, acc, lds + wave * (32 * 32 * FN * 4), m0 + wm * 32 * FM,
                              n0 + wn * (EPI == EPI_GATED ? 32 : 32 * FN), t.slice,
-                             (int64_t)t.m * 2 + wm);
+                             (int64_t)t.m * WM + wm);
 }
 
 template <typename E, bool AT, bool BT, int EPI, int BM, int BN, int ST>
@@ -103,101 +104,114 @@ int launch_form(const GemmArgs& p, Tiles tiles, hipStream_t s) {
 // gates' sums, then the ups').
 template <typename E, int EPI>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs p) {
-  const int64_t groups = (p.N + 7) / 8;
+  const int64_t groups = p.N / 4;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= p.M * groups) return;
-  const int64_t m = id / groups, n = (id - m * groups) * 8;
-  const bool two = n + 4 < p.N;
-  EpiCols<EPI> cols;
-  epi_cols<EPI>(p, n, cols);
-  float v[8] = {}, u[8] = {}, sg[8], su[8];
+  const int64_t m = id / groups, n = (id - m * groups) * 4;
+  EpiCols<EPI, 4> cols;
+  epi_cols<EPI, 4>(p, n, cols);
+  float v[4] = {}, u[4] = {}, sg[4] = {}, su[4] = {};
+  GateUp z = {};
+  if constexpr (EPI == EPI_GATED_BWD) z = load_z(p, m, n);
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float* row = p.part + ((int64_t)s * p.M + m) * p.ldp;
-    float x[8];
-    load8<F32>(row, n, two, x);
+    float x[4];
+    load_c<F32, 4>(row, n, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += x[i];
+    for (int i = 0; i < 4; ++i) v[i] += x[i];
     if (EPI == EPI_GATED) {
-      load8<F32>(row, p.N + n, two, x);
+      load_c<F32, 4>(row, p.N + n, x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] += x[i];
+      for (int i = 0; i < 4; ++i) u[i] += x[i];
     }
   }
-  epi8<E, EPI>(p, cols, m, n, v, u, sg, su);
+  epi_row<E, EPI, 4>(p, cols, m, n, v, u, z, sg, su);
 }
 
 // dz = gy * act'(z), rounded, and the column sums of what it stores before
-// rounding: a workgroup takes kSumRows rows of 512 columns, part its row of them.
+// rounding: a workgroup takes kSumRows rows of 256 columns, part its row of them.
 constexpr int kSumRows = 64;
 template <typename E, bool ACT>
 __global__ __launch_bounds__(256) void act_grad_kernel(const void* gy, int64_t ldgy,
                                                        const float* z, int64_t ldz, int act,
                                                        void* dz, int64_t lddz, float* part,
                                                        int64_t M, int64_t N) {
-  __shared__ float red[4][512];
+  __shared__ float red[4][256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n = (int64_t)blockIdx.x * 512 + lane * 8;
+  const int64_t n = (int64_t)blockIdx.x * 256 + lane * 4;
   const int64_t m0 = (int64_t)blockIdx.y * kSumRows;
-  const bool two = n + 4 < N;
-  float sum[8] = {};
+  float sum[4] = {};
   if (n < N) {
     const int64_t m1 = min(M, m0 + kSumRows);
+#pragma unroll 4
     for (int64_t m = m0 + wave; m < m1; m += 4) {
-      float g[8];
-      load8<E>(static_cast<const typename E::Store*>(gy) + m * ldgy, n, two, g);
+      float g[4];
+      load_c<E, 4>(static_cast<const typename E::Store*>(gy) + m * ldgy, n, g);
       if constexpr (ACT) {
-        float x[8];
-        load8<F32>(z + m * ldz, n, two, x);
+        float x[4];
+        load_c<F32, 4>(z + m * ldz, n, x);
         act_switch(act, [&](auto A) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             float slope;
             act1<decltype(A)::value, true>(x[i], slope);
             g[i] *= slope;
           }
         });
-        store8<E>(static_cast<typename E::Store*>(dz) + m * lddz, n, two, g);
+        store_c<E, 4>(static_cast<typename E::Store*>(dz) + m * lddz, n, g);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += g[i];
+      for (int i = 0; i < 4; ++i) sum[i] += g[i];
     }
   }
   if (!part) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) red[wave][lane * 8 + i] = sum[i];
+  for (int i = 0; i < 4; ++i) red[wave][lane * 4 + i] = sum[i];
   __syncthreads();
-#pragma unroll
-  for (int c = threadIdx.x; c < 512; c += 256) {
-    const int64_t col = (int64_t)blockIdx.x * 512 + c;
-    if (col < N)
-      part[(int64_t)blockIdx.y * N + col] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-  }
+  const int c = threadIdx.x;
+  const int64_t col = (int64_t)blockIdx.x * 256 + c;
+  if (col < N)
+    part[(int64_t)blockIdx.y * N + col] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
 }
 
-// Column sums of part [rows, N] into out (bf16 or fp32): 16 columns a workgroup,
-// 16 threads a column.
+// Column sums of part [rows, N], the first `split` columns into out0, the others
+// into out1 (bf16 or fp32; null: not wanted): 16 columns a workgroup, 16 threads a
+// column, 8 loads of each under way.
 __global__ __launch_bounds__(256) void col_sum_kernel(const float* part, int64_t rows, int64_t N,
-                                                      void* out, int out_f32) {
+                                                      int64_t split, void* out0, int out0_f32,
+                                                      void* out1, int out1_f32) {
   __shared__ float red[16][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
   const int64_t n = (int64_t)blockIdx.x * 16 + c;
-  float s = 0.0f;
-  if (n < N)
-    for (int64_t m = r; m < rows; m += 16) s += part[m * N + n];
-  red[r][c] = s;
+  float s[8] = {};
+  if (n < N) {
+    int64_t m = r;
+    for (; m + 112 < rows; m += 128)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += part[(m + 16 * i) * N + n];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (m + 16 * i < rows) s[i] += part[(m + 16 * i) * N + n];
+  }
+  red[r][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
   if (r == 0 && n < N) {
     float t = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) t += red[i][c];
-    if (out_f32) static_cast<float*>(out)[n] = t;
-    else static_cast<uint16_t*>(out)[n] = (uint16_t)f32_to_bf16(t);
+    void* out = n < split ? out0 : out1;
+    const int f32 = n < split ? out0_f32 : out1_f32;
+    const int64_t at = n < split ? n : n - split;
+    if (out && f32) static_cast<float*>(out)[at] = t;
+    else if (out) static_cast<uint16_t*>(out)[at] = (uint16_t)f32_to_bf16(t);
   }
 }
 
 }  // namespace
 
 int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s) {
+  if (tiles == TILES_256) return gemm_big(form, epi, p, s);
   auto go = [&](auto e, auto f) -> int {
     typedef decltype(e) E;
     constexpr int F = decltype(f)::value;
@@ -225,7 +239,7 @@ int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hip
 }
 
 int join_splits(int type, Epi epi, const GemmArgs& p, hipStream_t s) {
-  const int64_t blocks = (p.M * ((p.N + 7) / 8) + 255) / 256;
+  const int64_t blocks = (p.M * (p.N / 4) + 255) / 256;
   auto go = [&](auto e) {
     typedef decltype(e) E;
     if (epi == EPI_LINEAR)
@@ -245,7 +259,7 @@ int64_t sum_rows(int64_t M) { return (M + kSumRows - 1) / kSumRows; }
 
 int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
              void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s) {
-  const dim3 grid((uint32_t)((N + 511) / 512), (uint32_t)sum_rows(M));
+  const dim3 grid((uint32_t)((N + 255) / 256), (uint32_t)sum_rows(M));
   auto go = [&](auto e) {
     typedef decltype(e) E;
     if (z)
@@ -261,9 +275,10 @@ int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz
   return VMOE_OK;
 }
 
-int col_sum(const float* part, int64_t rows, int64_t N, void* out, int out_f32, hipStream_t s) {
-  VMOE_LAUNCH(col_sum_kernel, dim3((uint32_t)((N + 15) / 16)), dim3(256), 0, s, part, rows, N, out,
-              out_f32);
+int col_sum(const float* part, int64_t rows, int64_t N, int64_t split, void* out0, int out0_f32,
+            void* out1, int out1_f32, hipStream_t s) {
+  VMOE_LAUNCH(col_sum_kernel, dim3((uint32_t)((N + 15) / 16)), dim3(256), 0, s, part, rows, N,
+              split, out0, out0_f32, out1, out1_f32);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
 }

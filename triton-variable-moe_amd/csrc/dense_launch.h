@@ -9,13 +9,17 @@ namespace dense {
 enum Form { FORM_KK, FORM_KT, FORM_TT };  // A's, B's
 enum Tiles { TILES_64, TILES_128, TILES_256 };
 
+// dense_big.hip: TILES_256, bf16
+int gemm_big(Form form, Epi epi, const GemmArgs& p, hipStream_t s);
 // dense_gemm.hip
 int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
 int join_splits(int type, Epi epi, const GemmArgs& p, hipStream_t s);
 int64_t sum_rows(int64_t M);  // rows of the sums that act_grad leaves
 int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
              void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s);
-int col_sum(const float* part, int64_t rows, int64_t N, void* out, int out_f32, hipStream_t s);
+// column sums of part [rows, N]: columns below `split` into out0, the others into out1
+int col_sum(const float* part, int64_t rows, int64_t N, int64_t split, void* out0, int out0_f32,
+            void* out1, int out1_f32, hipStream_t s);
 
 }  // namespace dense
 }  // namespace vmoe

@@ -8,9 +8,9 @@
 // A row belongs to 64 threads (one wave, no barrier) or, where it is long, to 256
 // or 1024; workgroups go on to further rows with the weights, and in the backward
 // pass their gradients' sums, in registers. Those sums are joined in a fixed
-// order: within a workgroup, then by norm_sum_kernel.
+// order: within a workgroup, then by a launch of their own.
 
-#include "dense.h"
+#include "dense_launch.h"
 
 namespace vmoe {
 namespace {
@@ -296,31 +296,6 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
   }
 }
 
-// gw and gb: sums of part [n, 2, d]. A workgroup takes 32 columns of one of them,
-// 8 threads a column.
-__global__ __launch_bounds__(256) void norm_sum_kernel(const float* part, int64_t n, int64_t d,
-                                                       void* gw, int gw_f32, void* gb,
-                                                       int gb_f32) {
-  __shared__ float red[8][32];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int64_t col = (int64_t)blockIdx.x * 32 + c;
-  void* out = blockIdx.y ? gb : gw;
-  if (!out) return;
-  const int f32 = blockIdx.y ? gb_f32 : gw_f32;
-  float s = 0.0f;
-  if (col < d)
-    for (int64_t k = r; k < n; k += 8) s += part[(2 * k + blockIdx.y) * d + col];
-  red[r][c] = s;
-  __syncthreads();
-  if (r == 0 && col < d) {
-    float v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v += red[k][c];
-    if (f32) static_cast<float*>(out)[col] = v;
-    else static_cast<uint16_t*>(out)[col] = (uint16_t)f32_to_bf16(v);
-  }
-}
-
 constexpr int64_t kMaxNorm = 16384;  // 1024 threads of 16 values
 constexpr int64_t kNormGroups = 1024;  // workgroups of a backward pass: rows of its sums
 
@@ -462,10 +437,6 @@ extern "C" int vmoe_layer_norm_backward(int32_t type, const void* gy, int64_t ld
     });
   };
   if (int st = type == VMOE_DENSE_F32 ? go(F32()) : go(Bf16())) return st;
-  if (wg) {
-    VMOE_LAUNCH(norm_sum_kernel, dim3((uint32_t)((d + 31) / 32), 2), dim3(256), 0, s, p.part,
-                groups, d, gw, gw_f32, gb, gb_f32);
-    VMOE_CHECK_LAUNCH();
-  }
+  if (wg) return dense::col_sum(p.part, groups, 2 * d, d, gw, gw_f32, gb, gb_f32, s);
   return VMOE_OK;
 }
