@@ -23,7 +23,8 @@ OUT = HERE / "triton_moe" / "libvmoe.so"
 OBJ = HERE / "_build"
 SOURCES = ["route.hip", "permute.hip", "permute_f32.hip", "gemm.hip", "gemm_few_rows.hip",
            "gemm_f32.hip", "router.hip", "router_bwd.hip", "expert.hip", "expert_f32.hip",
-           "few_tokens.hip", "few_q4.hip", "dense.hip", "dense_gemm.hip", "dense_big.hip", "norm.hip", "capi.hip"]
+           "few_tokens.hip", "few_q4.hip", "dense.hip", "dense_gemm.hip", "dense_big.hip",
+           "dense_few.hip", "norm.hip", "capi.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -40,13 +40,15 @@ struct F32 {
   typedef f32x4_t Frag;  // 16 bytes of a lane: 4 k
 };
 
-// What a product's results go through (see epi8).
+// What a product's results go through (see epi_row).
 enum Epi {
   EPI_LINEAR,    // act(acc + bias) + residual; acc + bias kept in z
   EPI_GATED,     // act(gate + bias) * (up + bias); gate and up kept in z
   EPI_GATED_BWD, // acc is dh: [dgate | dup] from z, with their column sums
-  EPI_PARTIAL,   // the fp32 sum of one slice of k
+  EPI_PARTIAL,   // the fp32 sums of one slice of k (dense_few.hip)
 };
+
+constexpr int kGroup256 = 8, kGroup = 16;  // row tiles of a group (see tile_of)
 
 struct GemmArgs {
   const void* a;
@@ -61,12 +63,16 @@ struct GemmArgs {
   int64_t ldc;
   float* z;           // fp32 pre-activations [M, ldz] (written; EPI_GATED_BWD: read), or null
   int64_t ldz;
-  float* part;        // EPI_PARTIAL: [splits, M, ldp]; EPI_GATED_BWD: column sums, or null
-  int64_t ldp;
+  float* sums;        // EPI_GATED_BWD: column sums [row blocks, 2 N], or null
   int32_t act;
-  int32_t splits;     // slices of k
-  int64_t kper;       // k of a slice (a multiple of the kernel's stage)
   int32_t tiles_m, tiles_n;
+  // The first `whole` tiles are one workgroup's; each of the others is `splits`
+  // workgroups', which take kper of k (a multiple of the kernel's stage) and leave
+  // their sums in part.
+  int32_t whole, splits;
+  int64_t kper;
+  float* part;        // dense_few.hip: [splits, M, ldp]; tiles: see write_part
+  int64_t ldp;
 };
 
 __device__ __forceinline__ float sigmoid(float x) {
@@ -406,12 +412,12 @@ __device__ __forceinline__ f32x16_t mma(f32x4_t a, f32x4_t b, f32x16_t acc) {
 // Writes the results of a wave: FM x FN blocks of 32 x 32 from (m0, n0) on, 32
 // rows at a time through the wave's own 32 x 32 FN x 4 bytes of LDS, so that
 // memory sees whole rows, 16 bytes a lane. EPI_GATED: block 0 holds gates, block 1
-// the ups of the same 32 columns. part_row: the row of p.part that takes the wave's
+// the ups of the same 32 columns. sum_row: the row of p.sums that takes the wave's
 // column sums.
 template <typename E, int EPI, int FM, int FN>
 __device__ __forceinline__ void write_tile(const GemmArgs& p, const f32x16_t (&acc)[FM][FN],
-                                           lds_char* scr, int64_t m0, int64_t n0, int slice,
-                                           int64_t part_row) {
+                                           lds_char* scr, int64_t m0, int64_t n0,
+                                           int64_t sum_row) {
   constexpr int WN = 32 * FN, CH = WN / 4;        // staged columns, 16-byte chunks of a row
   constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
   static_assert(!GATED || FN == 2, "gate and up");
@@ -490,16 +496,12 @@ __device__ __forceinline__ void write_tile(const GemmArgs& p, const f32x16_t (&a
         }
       }
       const int64_t m = m0 + 32 * i + r;
-      if (m < p.M && n_ok) {
-        if constexpr (EPI == EPI_PARTIAL)
-          store_c<F32, C>(p.part + ((int64_t)slice * p.M + m) * p.ldp, n, v);
-        else
-          epi_row<E, EPI, C>(p, cols, m, n, v, u, z[t / HALF & 1][t % HALF], sg, su);
-      }
+      if (m < p.M && n_ok)
+        epi_row<E, EPI, C>(p, cols, m, n, v, u, z[t / HALF & 1][t % HALF], sg, su);
     }
   }
   if constexpr (BWD) {
-    if (p.part && n0 < p.N && m0 < p.M) {
+    if (p.sums && n0 < p.N && m0 < p.M) {
       // lanes of the same columns, in a fixed order
 #pragma unroll
       for (int o = LR; o < 64; o *= 2)
@@ -509,27 +511,48 @@ __device__ __forceinline__ void write_tile(const GemmArgs& p, const f32x16_t (&a
           su[i] += __shfl_xor(su[i], o, 64);
         }
       if (lane < LR && n_ok) {
-        store_c<F32, C>(p.part + part_row * p.ldp, n, sg);
-        store_c<F32, C>(p.part + part_row * p.ldp + p.N, n, su);
+        store_c<F32, C>(p.sums + sum_row * 2 * p.N, n, sg);
+        store_c<F32, C>(p.sums + sum_row * 2 * p.N + p.N, n, su);
       }
     }
   }
 }
 
-// The tile of workgroup b: each XCD (b % 8) takes a contiguous run of tiles,
-// which go through groups of GM row tiles column by column, so that the tiles an
-// XCD works on at a time share operand rows and columns in its L2.
+// A wave's sums of a slice, in the order its registers hold them, so that every
+// store is a kilobyte in one piece: 4 values of each lane for block (i, j) and
+// register group g at ((i FN + j) 4 + g) 64 + lane (see mma for their rows and
+// columns). dst: the wave's part.
+template <int FM, int FN>
+__device__ __forceinline__ void write_part(const f32x16_t (&acc)[FM][FN], float* dst) {
+  f32x4_t* out = reinterpret_cast<f32x4_t*>(dst) + (threadIdx.x & 63);
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
+                           acc[i][j][4 * g + 3]};
+        out[((i * FN + j) * 4 + g) * 64] = v;
+      }
+}
+
+// Place t of n in which XCD b % 8 takes a contiguous run (workgroup b is the b / 8 th
+// of its XCD).
+__device__ __forceinline__ int xcd_run(int b, int n) {
+  const int x = b & 7;
+  return x * (n >> 3) + min(x, n & 7) + (b >> 3);
+}
+
+// The tile of workgroup b, and its slice of k (-1: all of it). Tiles go through
+// groups of GM row tiles column by column, so that the tiles an XCD works on at a
+// time share operand rows and columns in its L2.
 struct Tile {
   int m, n, slice;
+  int split;  // index among the split tiles
 };
-__device__ __forceinline__ Tile tile_of(const GemmArgs& p, int b, int GM) {
-  const int total = p.tiles_m * p.tiles_n * p.splits;
-  const int x = b & 7, q = total >> 3, r = total & 7;
-  int t = x * q + min(x, r) + (b >> 3);  // (workgroup b is the b / 8 th of XCD b % 8)
-  const int per = p.tiles_m * p.tiles_n;
-  Tile o;
-  o.slice = t / per;
-  t -= o.slice * per;
+__device__ __forceinline__ Tile tile_at(const GemmArgs& p, int t, int GM) {
+  Tile o = {};
   const int gsize = GM * p.tiles_n;
   const int g = t / gsize, first = g * GM;
   const int rows = min(GM, p.tiles_m - first);
@@ -537,6 +560,31 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& p, int b, int GM) {
   o.m = first + t % rows;
   o.n = t / rows;
   return o;
+}
+__device__ __forceinline__ Tile tile_of(const GemmArgs& p, int b, int GM) {
+  if (b < p.whole) {
+    Tile o = tile_at(p, xcd_run(b, p.whole), GM);
+    o.slice = -1;
+    return o;
+  }
+  const int rest = p.tiles_m * p.tiles_n - p.whole;
+  const int t = xcd_run(b - p.whole, rest * p.splits);
+  const int slice = t / rest, split = t - slice * rest;
+  Tile o = tile_at(p, p.whole + split, GM);
+  o.slice = slice;
+  o.split = split;
+  return o;
+}
+// k of the tile's workgroup: [first, last)
+__device__ __forceinline__ void tile_k(const GemmArgs& p, const Tile& t, int64_t& k0, int64_t& k1) {
+  k0 = t.slice < 0 ? 0 : t.slice * p.kper;
+  k1 = t.slice < 0 ? p.K : min(p.K, k0 + p.kper);
+}
+// Where the sums of its slice go (VALUES: of a tile).
+template <int VALUES>
+__device__ __forceinline__ float* tile_part(const GemmArgs& p, const Tile& t) {
+  const int rest = p.tiles_m * p.tiles_n - p.whole;
+  return p.part + ((int64_t)t.slice * rest + t.split) * VALUES;
 }
 
 }  // namespace dense

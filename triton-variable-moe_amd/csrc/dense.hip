@@ -41,54 +41,133 @@ int check_sizes(int type, int act, int64_t rows, int64_t a, int64_t b) {
     if (st_ != VMOE_OK) return st_;       \
   } while (0)
 
-// How a product runs: its tiles and the slices its k is cut into.
+// How a product runs.
 struct Plan {
   Tiles tiles;
-  int splits;
+  int tiles_m, tiles_n, whole, splits;  // see GemmArgs
   int64_t kper;
   size_t part_bytes;  // of the slices' sums
 };
 
-Plan plan_of(int type, Epi epi, int64_t M, int64_t N, int64_t K) {
-  Plan q;
-  const int64_t n = epi == EPI_GATED ? 2 * N : N;  // columns staged
+// A kernel of tiles: its size, the workgroups a CU holds, the microseconds a stage of k
+// takes each of them where a CU holds 1, 2, ..., and those that a round of workgroups
+// takes besides (first loads, epilogue). Measured at 16 and 80 stages: with a full
+// card bf16 tiles of 256 run 1360 TFLOP/s, of 128 1150, of 64 650; fp32 tiles of 128
+// 142, of 64 125.
+struct Kernel {
+  Tiles tiles;
+  int bm, bn, per_cu;
+  float stage[3], round;
+};
+constexpr Kernel kBf16[] = {{TILES_256, 256, 256, 1, {1.6f}, 14.0f},
+                            {TILES_128, 128, 128, 2, {0.66f, 0.95f}, 4.0f},
+                            {TILES_64, 64, 64, 3, {0.39f, 0.49f, 0.62f}, 2.0f}};
+constexpr Kernel kF32[] = {{TILES_128, 128, 128, 2, {2.03f, 3.8f}, 5.0f},
+                           {TILES_64, 64, 64, 3, {0.68f, 1.14f, 1.62f}, 2.0f}};
+constexpr int kCus = 256;
+
+// Few rows: whether the kernel that streams the weight takes a product, and how.
+bool plan_rows(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K, Plan& q) {
+  if (form == FORM_TT || epi == EPI_GATED_BWD || M > kFewRows) return false;
+  const int64_t n = epi == EPI_GATED ? 2 * N : N;
+  const int64_t bytes = n * K * esize(type);
+  if (M > 16 && bytes > (int64_t)32 << 20) return false;
+  const int cols = type == VMOE_DENSE_BF16 && form == FORM_KT && bytes > (int64_t)12 << 20 ? 64 : 32;
+  q.tiles = cols == 64 ? ROWS_64 : ROWS_32;
+  q.tiles_m = 1;
+  q.tiles_n = (int)cdiv(n, cols);
   const int64_t stage = 128 / esize(type);
-  auto count = [&](int64_t t, int64_t tn) { return cdiv(M, t) * cdiv(n, tn); };
-  q.tiles = type == VMOE_DENSE_BF16 && count(256, 256) >= 224 ? TILES_256
-            : count(128, 128) >= 256                          ? TILES_128
-                                                              : TILES_64;
-  const int64_t tiles = std::max<int64_t>(1, q.tiles == TILES_256   ? count(256, 256)
-                                             : q.tiles == TILES_128 ? count(128, 128)
-                                             : epi == EPI_GATED     ? count(64, 128)
-                                                                    : count(64, 64));
-  q.splits = 1;
-  const int64_t stages = cdiv(K, stage);
-  if (tiles < 256 && q.tiles != TILES_256)
-    q.splits = (int)std::max<int64_t>(1, std::min(512 / tiles, stages / 8));
-  q.kper = cdiv(stages, q.splits) * stage;
+  const int64_t most = K <= 1024 && cols == 32 ? 1 : K / 512;
+  const int64_t s = std::max<int64_t>(1, std::min<int64_t>(cdiv(kCus, q.tiles_n), most));
+  q.kper = cdiv(cdiv(K, stage), s) * stage;
   q.splits = (int)cdiv(K, q.kper);
+  q.whole = 0;
   q.part_bytes = q.splits > 1 ? align256((size_t)q.splits * M * n * 4) : 0;
-  return q;
+  return true;
 }
 
-// One product with its epilogue. part: Plan::part_bytes. sums (EPI_GATED_BWD):
-// the rows of column sums written to p.part, 0 where the slices were joined.
-int product(int type, Form form, Epi epi, GemmArgs p, float* part, int64_t* sums, hipStream_t s) {
-  const Plan q = plan_of(type, epi, p.M, p.N, p.K);
+// Every kernel's time is estimated and the least taken. Tiles that do not fill the
+// card a whole number of times leave it partly idle at the end: the remaining ones are
+// split along k, where that is estimated to take less time with the joining (3 us and
+// 0.22 us for each MB of sums, measured at 4 to 67 MB).
+Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
+  Plan best = {};
+  if (plan_rows(type, form, epi, M, N, K, best)) return best;
+  const int64_t n = epi == EPI_GATED ? 2 * N : N;  // columns staged
+  const int64_t stage = 128 / esize(type), stages = cdiv(K, stage);
+  float least = 0.0f;
+  const bool bf16 = type == VMOE_DENSE_BF16;
+  for (int i = 0; i < (bf16 ? 3 : 2); ++i) {
+    const Kernel& k = bf16 ? kBf16[i] : kF32[i];
+    const int bn = k.tiles == TILES_64 && epi == EPI_GATED ? 128 : k.bn;
+    const float scale = bn == k.bn ? 1.0f : 1.6f;
+    Plan q = {};
+    q.tiles = k.tiles;
+    q.tiles_m = (int)cdiv(M, k.bm);
+    q.tiles_n = (int)cdiv(n, bn);
+    const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
+    const int slots = kCus * k.per_cu;
+    const int rest = (int)(tiles % slots);
+    float time = (float)(tiles / slots) * ((float)stages * k.stage[k.per_cu - 1] + k.round);
+    q.whole = (int)tiles;
+    q.splits = 1;
+    q.kper = stages * stage;
+    if (rest) {
+      float tail = (float)stages * k.stage[cdiv(rest, kCus) - 1];
+      for (int r = 1; r <= k.per_cu; ++r) {
+        const int64_t s = std::min<int64_t>(r * kCus / rest, stages / 4);
+        if (s < 2) continue;
+        const int64_t per = cdiv(stages, s), units = rest * cdiv(stages, per);
+        const float mb = (float)units * (float)(k.bm * bn * 4) * 1e-6f;
+        const float t = (float)per * k.stage[cdiv(units, kCus) - 1] + 3.0f + mb * 0.22f;
+        if (t < tail) {
+          tail = t;
+          q.whole = (int)(tiles - rest);
+          q.splits = (int)cdiv(stages, per);
+          q.kper = per * stage;
+        }
+      }
+      time += tail + k.round;
+    }
+    time *= scale;
+    const int64_t split = tiles - q.whole;
+    q.part_bytes = align256((size_t)split * q.splits * k.bm * bn * 4);
+    if (!best.splits || time < least) {
+      best = q;
+      least = time;
+    }
+  }
+  return best;
+}
+
+// Rows of column sums an EPI_GATED_BWD product leaves: one for each wave row (half a
+// tile) that holds rows.
+int64_t gated_sum_rows(const Plan& q, int64_t M) {
+  return cdiv(M, q.tiles == TILES_256 ? 128 : q.tiles == TILES_128 ? 64 : 32);
+}
+
+// One product with its epilogue. part: Plan::part_bytes.
+int product(int type, Form form, Epi epi, GemmArgs p, const Plan& q, float* part, hipStream_t s) {
+  p.tiles_m = q.tiles_m;
+  p.tiles_n = q.tiles_n;
+  p.whole = q.whole;
   p.splits = q.splits;
   p.kper = q.kper;
-  if (sums) *sums = 0;
-  if (q.splits > 1) {
+  p.part = part;
+  if (q.tiles == ROWS_32 || q.tiles == ROWS_64) {
+    p.ldp = epi == EPI_GATED ? 2 * p.N : p.N;
+    const int cols = q.tiles == ROWS_64 ? 64 : 32;
+    if (q.splits == 1) return gemm_few(type, form, epi, p, cols, s);
     GemmArgs g = p;
-    g.N = g.ldp = epi == EPI_GATED ? 2 * p.N : p.N;
-    g.part = part;
-    VMOE_TRY(gemm_tiles(type, form, EPI_PARTIAL, g, q.tiles, s));
-    p.part = part;
-    p.ldp = g.ldp;
-    return join_splits(type, epi, p, s);
+    g.N = p.ldp;
+    VMOE_TRY(gemm_few(type, form, EPI_PARTIAL, g, cols, s));
+    return join_rows(type, epi, p, s);
   }
-  if (sums) *sums = cdiv(p.M, q.tiles == TILES_64 ? 32 : q.tiles == TILES_128 ? 64 : 128);
-  return gemm_tiles(type, form, epi, p, q.tiles, s);
+  VMOE_TRY(gemm_tiles(type, form, epi, p, q.tiles, s));
+  return q.splits > 1 ? join_tiles(type, epi, p, q.tiles, s) : VMOE_OK;
+}
+int product(int type, Form form, Epi epi, const GemmArgs& p, float* part, hipStream_t s) {
+  return product(type, form, epi, p, plan_of(type, form, epi, p.M, p.N, p.K), part, s);
 }
 
 GemmArgs args(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N,
@@ -117,20 +196,25 @@ GemmArgs weight_grad_args(int transposed, const void* x, int64_t ldx, int64_t in
                     : args(x, ldx, g, ldg, in, out, rows, gw, ldgw);
 }
 size_t weight_grad_bytes(int type, int64_t in, int64_t out, int64_t rows, int transposed) {
-  return transposed ? plan_of(type, EPI_LINEAR, out, in, rows).part_bytes
-                    : plan_of(type, EPI_LINEAR, in, out, rows).part_bytes;
+  return transposed ? plan_of(type, FORM_TT, EPI_LINEAR, out, in, rows).part_bytes
+                    : plan_of(type, FORM_TT, EPI_LINEAR, in, out, rows).part_bytes;
 }
 
-// Workspace: the slices' sums of one product at a time, then each buffer.
+// Workspace: the slices' sums of one product at a time, then each buffer. It does not
+// depend on the weights' order: the larger of both.
 struct Bytes {
   size_t part, grads, sums, total;
 };
+size_t either_order(int type, Epi epi, int64_t M, int64_t N, int64_t K) {
+  return std::max(plan_of(type, FORM_KK, epi, M, N, K).part_bytes,
+                  plan_of(type, FORM_KT, epi, M, N, K).part_bytes);
+}
 Bytes linear_bytes(int type, int64_t rows, int64_t in, int64_t out, int act, int backward) {
   Bytes b = {};
   if (!backward) {
-    b.part = plan_of(type, EPI_LINEAR, rows, out, in).part_bytes;
+    b.part = either_order(type, EPI_LINEAR, rows, out, in);
   } else {
-    b.part = std::max({plan_of(type, EPI_LINEAR, rows, in, out).part_bytes,
+    b.part = std::max({either_order(type, EPI_LINEAR, rows, in, out),
                        weight_grad_bytes(type, in, out, rows, 0),
                        weight_grad_bytes(type, in, out, rows, 1)});
     if (act != VMOE_DENSE_NONE) b.grads = align256((size_t)rows * out * esize(type));
@@ -142,18 +226,17 @@ Bytes linear_bytes(int type, int64_t rows, int64_t in, int64_t out, int act, int
 Bytes gated_bytes(int type, int64_t rows, int64_t d, int64_t width, int backward) {
   Bytes b = {};
   if (!backward) {
-    b.part = std::max(plan_of(type, EPI_GATED, rows, width, d).part_bytes,
-                      plan_of(type, EPI_LINEAR, rows, d, width).part_bytes);
+    b.part = std::max(either_order(type, EPI_GATED, rows, width, d),
+                      either_order(type, EPI_LINEAR, rows, d, width));
   } else {
-    b.part = std::max({plan_of(type, EPI_GATED_BWD, rows, width, d).part_bytes,
-                       plan_of(type, EPI_LINEAR, rows, d, 2 * width).part_bytes,
+    const Plan q = plan_of(type, FORM_KK, EPI_GATED_BWD, rows, width, d);
+    b.part = std::max({q.part_bytes, either_order(type, EPI_LINEAR, rows, d, 2 * width),
                        weight_grad_bytes(type, d, 2 * width, rows, 0),
                        weight_grad_bytes(type, d, 2 * width, rows, 1),
                        weight_grad_bytes(type, width, d, rows, 0),
                        weight_grad_bytes(type, width, d, rows, 1)});
     b.grads = align256((size_t)rows * 2 * width * esize(type));
-    b.sums = align256((size_t)std::max(std::max(sum_rows(rows), cdiv(rows, 32)) * 2 * width,
-                                       sum_rows(rows) * d) * 4);
+    b.sums = align256((size_t)std::max(gated_sum_rows(q, rows) * 2 * width, sum_rows(rows) * d) * 4);
   }
   b.total = b.part + b.grads + b.sums;
   return b;
@@ -207,7 +290,7 @@ extern "C" int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int
   p.z = z;
   p.ldz = out;
   return product(type, forward_form(w_transposed), EPI_LINEAR, p, static_cast<float*>(workspace),
-                 nullptr, reinterpret_cast<hipStream_t>(stream));
+                 reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void* x,
@@ -242,11 +325,11 @@ extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, 
   const int64_t ldg = has_act ? out : ldgy;
   if (gx)
     VMOE_TRY(product(type, input_grad_form(w_transposed), EPI_LINEAR,
-                     args(g, ldg, w, ldw, rows, in, out, gx, ldgx), part, nullptr, s));
+                     args(g, ldg, w, ldw, rows, in, out, gx, ldgx), part, s));
   if (gw)
     VMOE_TRY(product(type, FORM_TT, EPI_LINEAR,
                      weight_grad_args(w_transposed, x, ldx, in, g, ldg, out, rows, gw, ldgw), part,
-                     nullptr, s));
+                     s));
   return VMOE_OK;
 }
 
@@ -295,14 +378,14 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
   p.act = act;
   p.z = z;
   p.ldz = 2 * width;
-  VMOE_TRY(product(type, forward_form(w1_transposed), EPI_GATED, p, part, nullptr, s));
+  VMOE_TRY(product(type, forward_form(w1_transposed), EPI_GATED, p, part, s));
   GemmArgs q = args(h, width, w2, ldw2, rows, hidden, width, y, ldy);
   q.bias = bias2;
   q.bias_f32 = bias2_f32;
   q.act = VMOE_DENSE_NONE;
   q.res = residual;
   q.ldr = ldr;
-  return product(type, forward_form(w2_transposed), EPI_LINEAR, q, part, nullptr, s);
+  return product(type, forward_form(w2_transposed), EPI_LINEAR, q, part, s);
 }
 
 extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, const void* x,
@@ -340,15 +423,12 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
     p.act = act;
     p.z = const_cast<float*>(z);
     p.ldz = w2x;
-    p.part = gb1 ? sums : nullptr;
-    p.ldp = w2x;
-    int64_t n = 0;
-    VMOE_TRY(product(type, input_grad_form(w2_transposed), EPI_GATED_BWD, p, part, &n, s));
-    if (gb1 && n == 0) {  // joined slices: sums of the rounded gradients
-      VMOE_TRY(act_grad(type, dz, w2x, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows, w2x, s));
-      n = sum_rows(rows);
-    }
-    if (gb1) VMOE_TRY(col_sum(sums, n, w2x, w2x, gb1, gb1_f32, nullptr, 0, s));
+    p.sums = gb1 ? sums : nullptr;
+    const Form form = input_grad_form(w2_transposed);
+    const Plan q = plan_of(type, form, EPI_GATED_BWD, rows, width, hidden);
+    VMOE_TRY(product(type, form, EPI_GATED_BWD, p, q, part, s));
+    if (gb1)
+      VMOE_TRY(col_sum(sums, gated_sum_rows(q, rows), w2x, w2x, gb1, gb1_f32, nullptr, 0, s));
   }
   if (gb2) {
     VMOE_TRY(act_grad(type, gy, ldgy, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows, hidden,
@@ -359,13 +439,13 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
   if (gw2)
     VMOE_TRY(product(type, FORM_TT, EPI_LINEAR,
                      weight_grad_args(w2_transposed, h, width, width, gy, ldgy, hidden, rows, gw2,
-                                      ldgw2), part, nullptr, s));
+                                      ldgw2), part, s));
   if (gx)
     VMOE_TRY(product(type, input_grad_form(w1_transposed), EPI_LINEAR,
-                     args(dz, w2x, w1, ldw1, rows, hidden, w2x, gx, ldgx), part, nullptr, s));
+                     args(dz, w2x, w1, ldw1, rows, hidden, w2x, gx, ldgx), part, s));
   if (gw1)
     VMOE_TRY(product(type, FORM_TT, EPI_LINEAR,
                      weight_grad_args(w1_transposed, x, ldx, hidden, dz, w2x, w2x, rows, gw1,
-                                      ldgw1), part, nullptr, s));
+                                      ldgw1), part, s));
   return VMOE_OK;
 }

@@ -31,9 +31,10 @@ __global__ __launch_bounds__(512, 2) void big_kernel(GemmArgs p) {
   constexpr int OUT = EPI == EPI_GATED ? 128 : 256;  // output columns of the tile
   __shared__ __align__(1024) char lds_[8 * kHalf];
   lds_char* lds = (lds_char*)lds_;
-  const Tile t = tile_of(p, blockIdx.x, 8);
+  const Tile t = tile_of(p, blockIdx.x, kGroup256);
   const int64_t m0 = (int64_t)t.m * 256, n0 = (int64_t)t.n * OUT;
-  const int64_t k0 = t.slice * p.kper, k1 = min(p.K, k0 + p.kper);
+  int64_t k0, k1;
+  tile_k(p, t, k0, k1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3;
 
@@ -135,18 +136,16 @@ __global__ __launch_bounds__(512, 2) void big_kernel(GemmArgs p) {
   wait_vmcnt<0>();
   if (wm == 0) block_barrier();
   block_barrier();  // every wave has read the last stage, no DMA is in flight
-  write_tile<E, EPI, 4, 2>(p, acc, lds + wave * 8192, m0 + wm * 128,
-                           n0 + wn * (EPI == EPI_GATED ? 32 : 64), t.slice,
-                           (int64_t)t.m * 2 + wm);
+  if (t.slice >= 0)
+    write_part<4, 2>(acc, tile_part<65536>(p, t) + wave * 8192);
+  else
+    write_tile<E, EPI, 4, 2>(p, acc, lds + wave * 8192, m0 + wm * 128,
+                             n0 + wn * (EPI == EPI_GATED ? 32 : 64), (int64_t)t.m * 2 + wm);
 }
 
 template <bool AT, bool BT, int EPI>
-int launch(GemmArgs p, hipStream_t s) {
-  constexpr int OUT = EPI == EPI_GATED ? 128 : 256;
-  p.tiles_m = (int)((p.M + 255) / 256);
-  p.tiles_n = (int)((p.N + OUT - 1) / OUT);
-  const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  VMOE_LAUNCH((big_kernel<AT, BT, EPI>), dim3((uint32_t)grid), dim3(512), 0, s, p);
+int launch(const GemmArgs& p, hipStream_t s) {
+  VMOE_LAUNCH((big_kernel<AT, BT, EPI>), dim3(workgroups(p)), dim3(512), 0, s, p);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
 }
@@ -154,7 +153,6 @@ int launch(GemmArgs p, hipStream_t s) {
 template <bool AT, bool BT>
 int by_epi(Epi epi, const GemmArgs& p, hipStream_t s) {
   if (epi == EPI_LINEAR) return launch<AT, BT, EPI_LINEAR>(p, s);
-  if (epi == EPI_PARTIAL) return launch<AT, BT, EPI_PARTIAL>(p, s);
   if constexpr (!AT) {
     if (epi == EPI_GATED) return launch<AT, BT, EPI_GATED>(p, s);
     return launch<AT, BT, EPI_GATED_BWD>(p, s);

@@ -1,5 +1,5 @@
 // Matrix products of the dense operators on 128 x 128 and 64 x 64 tiles (bf16 and
-// fp32), and what goes with them: the joining of sums split along k, gradients
+// fp32), and what goes with them: the joining of tiles split along k, gradients
 // through the activation, column sums.
 //
 // Tiles: four waves, each a quarter of the tile in 32 x 32 blocks, both operands
@@ -20,9 +20,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
   __shared__ __align__(1024) char lds_[ST * STAGE];
   lds_char* lds = (lds_char*)lds_;
   static_assert(NW * 32 * 32 * FN * 4 <= ST * STAGE, "epilogue scratch");
-  const Tile t = tile_of(p, blockIdx.x, 16);
+  const Tile t = tile_of(p, blockIdx.x, kGroup);
   const int64_t m0 = (int64_t)t.m * BM, n0 = (int64_t)t.n * OUT;
-  const int64_t k0 = t.slice * p.kper, k1 = min(p.K, k0 + p.kper);
+  int64_t k0, k1;
+  tile_k(p, t, k0, k1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
@@ -72,19 +73,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
         for (int j = 0; j < FN; ++j) acc[i][j] = mma(af[i], bf[j], acc[i][j]);
     }
   }
+  if (t.slice >= 0) {
+    write_part<FM, FN>(acc, tile_part<BM * BN>(p, t) + wave * (BM * BN / NW));
+    return;
+  }
   block_barrier();  // every wave has read the last stages
   write_tile<E, EPI, FM, FN>(p, acc, lds + wave * (32 * 32 * FN * 4), m0 + wm * 32 * FM,
-                             n0 + wn * (EPI == EPI_GATED ? 32 : 32 * FN), t.slice,
-                             (int64_t)t.m * WM + wm);
+                             n0 + wn * (EPI == EPI_GATED ? 32 : 32 * FN), (int64_t)t.m * WM + wm);
 }
 
 template <typename E, bool AT, bool BT, int EPI, int BM, int BN, int ST>
-int launch_tile(GemmArgs p, hipStream_t s) {
-  constexpr int OUT = EPI == EPI_GATED ? BN / 2 : BN;
-  p.tiles_m = (int)((p.M + BM - 1) / BM);
-  p.tiles_n = (int)((p.N + OUT - 1) / OUT);
-  const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  VMOE_LAUNCH((gemm_kernel<E, AT, BT, EPI, BM, BN, ST>), dim3((uint32_t)grid), dim3(256), 0, s, p);
+int launch_tile(const GemmArgs& p, hipStream_t s) {
+  VMOE_LAUNCH((gemm_kernel<E, AT, BT, EPI, BM, BN, ST>), dim3(workgroups(p)), dim3(256), 0, s, p);
   VMOE_CHECK_LAUNCH();
   return VMOE_OK;
 }
@@ -100,19 +100,80 @@ int launch_form(const GemmArgs& p, Tiles tiles, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Sums split along k: part [splits, M, ldp] through the epilogue (EPI_GATED: the
-// gates' sums, then the ups').
+// Split tiles: the sums of their slices, in order, through the epilogue. Waves of the
+// product in WM x WN, FM x FN blocks each; a workgroup takes the FM blocks of one wave
+// and block column (EPI_GATED: of both), a wave of it one register group (see
+// write_part).
+template <typename E, int EPI, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(256) void join_kernel(GemmArgs p, int gm) {
+  constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
+  constexpr int NW = WM * WN, J = GATED ? 1 : FN, VALUES = NW * FM * FN * 1024;
+  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+  int id = blockIdx.x;
+  const int j = id % J;
+  id /= J;
+  const int wave = id % NW, split = id / NW;
+  const Tile t = tile_at(p, p.whole + split, gm);
+  const int wm = wave / WN, wn = wave % WN;
+  const int64_t m0 = ((int64_t)t.m * WM + wm) * 32 * FM + (lane & 31);
+  const int64_t n = ((int64_t)t.n * WN + wn) * 32 * J + 32 * j + 8 * g + 4 * (lane >> 5);
+  const int64_t step = (int64_t)(p.tiles_m * p.tiles_n - p.whole) * VALUES;
+  const float* part =
+      p.part + (int64_t)split * VALUES + (wave * FM * FN * 4 + j * 4 + g) * 256 + lane * 4;
+  const bool n_ok = n < p.N;
+  EpiCols<EPI, 4> cols;
+  epi_cols<EPI, 4>(p, n, cols);
+  float sg[4] = {}, su[4] = {};
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t m = m0 + 32 * i;
+    if (m >= p.M || !n_ok) continue;
+    GateUp z = {};
+    if constexpr (BWD) z = load_z(p, m, n);
+    float v[4] = {}, u[4] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      float x[4];
+      load_c<F32, 4>(part + s * step, i * FN * 1024, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += x[e];
+      if constexpr (GATED) {
+        load_c<F32, 4>(part + s * step, (i * FN + 1) * 1024, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] += x[e];
+      }
+    }
+    epi_row<E, EPI, 4>(p, cols, m, n, v, u, z, sg, su);
+  }
+  if constexpr (BWD) {
+    if (p.sums && m0 - (lane & 31) < p.M) {
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sg[e] += __shfl_xor(sg[e], o, 64);
+          su[e] += __shfl_xor(su[e], o, 64);
+        }
+      if ((lane & 31) == 0 && n_ok) {
+        float* row = p.sums + ((int64_t)t.m * WM + wm) * 2 * p.N;
+        store_c<F32, 4>(row, n, sg);
+        store_c<F32, 4>(row + p.N, n, su);
+      }
+    }
+  }
+}
+
+// The same for the sums of dense_few.hip, [splits, M, ldp] (EPI_GATED: gates, then
+// ups).
 template <typename E, int EPI>
-__global__ __launch_bounds__(256) void join_kernel(GemmArgs p) {
+__global__ __launch_bounds__(128) void join_rows_kernel(GemmArgs p) {
   const int64_t groups = p.N / 4;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
   if (id >= p.M * groups) return;
   const int64_t m = id / groups, n = (id - m * groups) * 4;
   EpiCols<EPI, 4> cols;
   epi_cols<EPI, 4>(p, n, cols);
-  float v[4] = {}, u[4] = {}, sg[4] = {}, su[4] = {};
-  GateUp z = {};
-  if constexpr (EPI == EPI_GATED_BWD) z = load_z(p, m, n);
+  float v[4] = {}, u[4] = {}, none[4] = {};
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float* row = p.part + ((int64_t)s * p.M + m) * p.ldp;
@@ -120,13 +181,13 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs p) {
     load_c<F32, 4>(row, n, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += x[i];
-    if (EPI == EPI_GATED) {
+    if constexpr (EPI == EPI_GATED) {
       load_c<F32, 4>(row, p.N + n, x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] += x[i];
     }
   }
-  epi_row<E, EPI, 4>(p, cols, m, n, v, u, z, sg, su);
+  epi_row<E, EPI, 4>(p, cols, m, n, v, u, GateUp(), none, none);
 }
 
 // dz = gy * act'(z), rounded, and the column sums of what it stores before
@@ -216,15 +277,10 @@ int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hip
     typedef decltype(e) E;
     constexpr int F = decltype(f)::value;
     constexpr bool AT = F == FORM_TT, BT = F != FORM_KK;
-    switch (epi) {
-      case EPI_LINEAR: return launch_form<E, AT, BT, EPI_LINEAR>(p, tiles, s);
-      case EPI_PARTIAL: return launch_form<E, AT, BT, EPI_PARTIAL>(p, tiles, s);
-      case EPI_GATED:
-        if constexpr (!AT) return launch_form<E, AT, BT, EPI_GATED>(p, tiles, s);
-        break;
-      case EPI_GATED_BWD:
-        if constexpr (!AT) return launch_form<E, AT, BT, EPI_GATED_BWD>(p, tiles, s);
-        break;
+    if (epi == EPI_LINEAR) return launch_form<E, AT, BT, EPI_LINEAR>(p, tiles, s);
+    if constexpr (!AT) {
+      if (epi == EPI_GATED) return launch_form<E, AT, BT, EPI_GATED>(p, tiles, s);
+      if (epi == EPI_GATED_BWD) return launch_form<E, AT, BT, EPI_GATED_BWD>(p, tiles, s);
     }
     return VMOE_ERR_INVALID_ARG;
   };
@@ -238,16 +294,43 @@ int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hip
   return type == VMOE_DENSE_F32 ? by_form(F32()) : by_form(Bf16());
 }
 
-int join_splits(int type, Epi epi, const GemmArgs& p, hipStream_t s) {
-  const int64_t blocks = (p.M * (p.N / 4) + 255) / 256;
+namespace {
+template <typename E, int EPI, int WM, int WN, int FM, int FN>
+int launch_join(const GemmArgs& p, int gm, hipStream_t s) {
+  const int rest = p.tiles_m * p.tiles_n - p.whole;
+  const int blocks = rest * WM * WN * (EPI == EPI_GATED ? 1 : FN);
+  VMOE_LAUNCH((join_kernel<E, EPI, WM, WN, FM, FN>), dim3((uint32_t)blocks), dim3(256), 0, s, p,
+              gm);
+  VMOE_CHECK_LAUNCH();
+  return VMOE_OK;
+}
+template <typename E, int EPI>
+int join_epi(const GemmArgs& p, Tiles tiles, hipStream_t s) {
+  if constexpr (E::kSize == 2)
+    if (tiles == TILES_256) return launch_join<E, EPI, 2, 4, 4, 2>(p, kGroup256, s);
+  if (tiles == TILES_128) return launch_join<E, EPI, 2, 2, 2, 2>(p, kGroup, s);
+  return launch_join<E, EPI, 2, 2, 1, EPI == EPI_GATED ? 2 : 1>(p, kGroup, s);
+}
+}  // namespace
+
+int join_tiles(int type, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s) {
+  auto go = [&](auto e) -> int {
+    typedef decltype(e) E;
+    if (epi == EPI_LINEAR) return join_epi<E, EPI_LINEAR>(p, tiles, s);
+    if (epi == EPI_GATED) return join_epi<E, EPI_GATED>(p, tiles, s);
+    return join_epi<E, EPI_GATED_BWD>(p, tiles, s);
+  };
+  return type == VMOE_DENSE_F32 ? go(F32()) : go(Bf16());
+}
+
+int join_rows(int type, Epi epi, const GemmArgs& p, hipStream_t s) {
+  const dim3 grid((uint32_t)((p.M * (p.N / 4) + 127) / 128));
   auto go = [&](auto e) {
     typedef decltype(e) E;
     if (epi == EPI_LINEAR)
-      VMOE_LAUNCH((join_kernel<E, EPI_LINEAR>), dim3((uint32_t)blocks), dim3(256), 0, s, p);
-    else if (epi == EPI_GATED)
-      VMOE_LAUNCH((join_kernel<E, EPI_GATED>), dim3((uint32_t)blocks), dim3(256), 0, s, p);
+      VMOE_LAUNCH((join_rows_kernel<E, EPI_LINEAR>), grid, dim3(128), 0, s, p);
     else
-      VMOE_LAUNCH((join_kernel<E, EPI_GATED_BWD>), dim3((uint32_t)blocks), dim3(256), 0, s, p);
+      VMOE_LAUNCH((join_rows_kernel<E, EPI_GATED>), grid, dim3(128), 0, s, p);
   };
   if (type == VMOE_DENSE_F32) go(F32());
   else go(Bf16());

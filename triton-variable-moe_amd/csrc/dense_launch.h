@@ -7,13 +7,22 @@ namespace vmoe {
 namespace dense {
 
 enum Form { FORM_KK, FORM_KT, FORM_TT };  // A's, B's
-enum Tiles { TILES_64, TILES_128, TILES_256 };
+enum Tiles { ROWS_32, ROWS_64, TILES_64, TILES_128, TILES_256 };  // ROWS: dense_few.hip
+
+inline uint32_t workgroups(const GemmArgs& p) {
+  return (uint32_t)(p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.splits);
+}
 
 // dense_big.hip: TILES_256, bf16
 int gemm_big(Form form, Epi epi, const GemmArgs& p, hipStream_t s);
-// dense_gemm.hip
+// dense_few.hip: at most kFewRows rows, workgroups of `cols` (32 or 64) columns
+constexpr int64_t kFewRows = 64;
+int gemm_few(int type, Form form, Epi epi, const GemmArgs& p, int cols, hipStream_t s);
+// dense_gemm.hip: the product on tiles; the epilogue of its split tiles; the epilogue
+// of gemm_few's slices
 int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
-int join_splits(int type, Epi epi, const GemmArgs& p, hipStream_t s);
+int join_tiles(int type, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
+int join_rows(int type, Epi epi, const GemmArgs& p, hipStream_t s);
 int64_t sum_rows(int64_t M);  // rows of the sums that act_grad leaves
 int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
              void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s);
