@@ -1,25 +1,29 @@
-"""Builds libvmoe.so (the gfx950 HIP kernels behind include/vmoe.h).
+"""Builds libvmoe.so (the gfx950 HIP kernels behind include/vmoe.h) and _dense.so (the
+extension module that calls the dense operators of it from torch).
 
 Usage: python triton-variable-moe_amd/build.py [--jobs N]
 
-The library is written next to the Python package
-(triton_moe/libvmoe.so) so the package finds it without an install step.
+Both are written into the Python package (triton_moe/) so that it finds them without
+an install step.
 """
 
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 REPO = HERE.parent
 CSRC = HERE / "csrc"
 OUT = HERE / "triton_moe" / "libvmoe.so"
+DENSE = HERE / "triton_moe" / "_dense.so"
 OBJ = HERE / "_build"
 SOURCES = ["route.hip", "permute.hip", "permute_f32.hip", "gemm.hip", "gemm_few_rows.hip",
            "gemm_f32.hip", "router.hip", "router_bwd.hip", "expert.hip", "expert_f32.hip",
@@ -57,9 +61,46 @@ def _compile(src: str) -> Path:
     return obj
 
 
+def _torch_dir() -> Path:
+    spec = importlib.util.find_spec("torch")  # (found, not imported)
+    if spec is None:
+        raise RuntimeError("torch not found")
+    return Path(spec.origin).parent
+
+
+def _compile_dense() -> Path:
+    """The extension module that calls the dense operators: host code alone, with
+    torch's headers."""
+    torch = _torch_dir()
+    obj = OBJ / "dense_torch.o"
+    rocm = Path(hipcc()).resolve().parents[1]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-Wall",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{REPO / 'include'}",
+           "-isystem", str(torch / "include"),
+           "-isystem", str(torch / "include/torch/csrc/api/include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(rocm / "include"),
+           "-c", str(CSRC / "dense_torch.cpp"), "-o", str(obj)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for dense_torch.cpp:\n{res.stdout}\n{res.stderr}")
+    return obj
+
+
+def _link_dense(obj: Path) -> None:
+    tmp = DENSE.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-shared", str(obj), "-o", str(tmp),
+           f"-L{OUT.parent}", f"-l:{OUT.name}", f"-L{_torch_dir() / 'lib'}", "-lc10", "-lc10_hip",
+           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, DENSE)
+
+
 def build(jobs: int = 4, verbose: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
+        dense = ex.submit(_compile_dense)
         objs = list(ex.map(_compile, SOURCES))
     tmp = OUT.with_suffix(".so.tmp")
     cmd = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
@@ -67,8 +108,9 @@ def build(jobs: int = 4, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, OUT)
+    _link_dense(dense.result())
     if verbose:
-        print(f"built {OUT}")
+        print(f"built {OUT}, {DENSE}")
     return OUT
 
 

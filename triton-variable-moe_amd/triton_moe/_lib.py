@@ -219,6 +219,26 @@ def lib() -> ctypes.CDLL:
         raise RuntimeError(f"libvmoe.so unavailable: {exc}") from exc
 
 
+_dense = None
+
+
+def dense():
+    """The dense operators' extension module (csrc/dense_torch.cpp); raises RuntimeError
+    if it cannot be loaded."""
+    global _dense
+    if _dense is not None:
+        return _dense
+    lib()
+    try:
+        from . import _dense as module
+    except ImportError as exc:
+        raise RuntimeError(f"triton_moe._dense unavailable ({exc}); build it with "
+                           "`python triton-variable-moe_amd/build.py`") from exc
+    module.set_timer(_launch_timer)
+    _dense = module
+    return module
+
+
 def check(status: int, what: str) -> None:
     if status != OK:
         msg = lib().vmoe_status_string(status).decode()
@@ -238,6 +258,8 @@ _launch_timer = None
 def set_launch_timer(timer) -> None:
     global _launch_timer
     _launch_timer = timer
+    if _dense is not None:
+        _dense.set_timer(timer)
 
 
 _FNS: dict = {}
