@@ -51,17 +51,18 @@ struct Plan {
 
 // A kernel of tiles: its size, the workgroups a CU holds, the microseconds a stage of k
 // takes each of them where a CU holds 1, 2, ..., and those that a round of workgroups
-// takes besides (first loads, epilogue). Measured at 16 and 80 stages: with a full
-// card bf16 tiles of 256 run 1360 TFLOP/s, of 128 1150, of 64 650; fp32 tiles of 128
-// 142, of 64 125.
+// takes besides (first loads, epilogue). Measured at 16 and 80 stages, where operands
+// stay in the last-level cache bf16 tiles of 256 run 1360 TFLOP/s, of 128 1150, of 64
+// 650, fp32 tiles of 128 142, of 64 125; bf16 stages of products that read from memory
+// take 1.15 to 1.3 times as long, which is what stands here.
 struct Kernel {
   Tiles tiles;
   int bm, bn, per_cu;
   float stage[3], round;
 };
-constexpr Kernel kBf16[] = {{TILES_256, 256, 256, 1, {1.6f}, 14.0f},
-                            {TILES_128, 128, 128, 2, {0.66f, 0.95f}, 4.0f},
-                            {TILES_64, 64, 64, 3, {0.39f, 0.49f, 0.62f}, 2.0f}};
+constexpr Kernel kBf16[] = {{TILES_256, 256, 256, 1, {1.85f}, 14.0f},
+                            {TILES_128, 128, 128, 2, {0.87f, 1.15f}, 4.0f},
+                            {TILES_64, 64, 64, 3, {0.45f, 0.55f, 0.70f}, 2.0f}};
 constexpr Kernel kF32[] = {{TILES_128, 128, 128, 2, {2.03f, 3.8f}, 5.0f},
                            {TILES_64, 64, 64, 3, {0.68f, 1.14f, 1.62f}, 2.0f}};
 constexpr int kCus = 256;
@@ -106,28 +107,39 @@ Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
     q.tiles_m = (int)cdiv(M, k.bm);
     q.tiles_n = (int)cdiv(n, bn);
     const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
-    const int slots = kCus * k.per_cu;
-    const int rest = (int)(tiles % slots);
-    float time = (float)(tiles / slots) * ((float)stages * k.stage[k.per_cu - 1] + k.round);
-    q.whole = (int)tiles;
     q.splits = 1;
     q.kper = stages * stage;
-    if (rest) {
-      float tail = (float)stages * k.stage[cdiv(rest, kCus) - 1];
-      for (int r = 1; r <= k.per_cu; ++r) {
-        const int64_t s = std::min<int64_t>(r * kCus / rest, stages / 4);
-        if (s < 2) continue;
-        const int64_t per = cdiv(stages, s), units = rest * cdiv(stages, per);
-        const float mb = (float)units * (float)(k.bm * bn * 4) * 1e-6f;
-        const float t = (float)per * k.stage[cdiv(units, kCus) - 1] + 3.0f + mb * 0.22f;
-        if (t < tail) {
-          tail = t;
-          q.whole = (int)(tiles - rest);
-          q.splits = (int)cdiv(stages, per);
-          q.kper = per * stage;
+    // rounds of k.per_cu tiles a CU, then one of `last` and the rest
+    const int each = (int)(tiles / kCus), last = each % k.per_cu;
+    float time = (float)(each / k.per_cu) * ((float)stages * k.stage[k.per_cu - 1] + k.round);
+    if (tiles % (kCus * k.per_cu)) {
+      float tail = (float)stages * k.stage[tiles % kCus ? last : last - 1];
+      q.whole = (int)tiles;
+      // `beside` of the last round's tiles stay whole, the others' slices fill r places
+      // of each CU
+      for (int beside = 0; beside <= last; beside += std::max(last, 1)) {
+        const int rest = (int)(tiles - (int64_t)(each - last + beside) * kCus);
+        if (!rest) continue;
+        const float base = beside ? (float)stages * k.stage[beside - 1] : 0.0f;
+        for (int r = 1; beside + r <= k.per_cu; ++r) {
+          const int64_t slices = std::min<int64_t>(r * kCus / rest, stages / 4);
+          if (slices < 2) continue;
+          const int64_t per = cdiv(stages, slices);
+          const int units = rest * (int)cdiv(stages, per), u = (int)cdiv(units, kCus);
+          const float mb = (float)units * (float)(k.bm * bn * 4) * 1e-6f;
+          const float more = k.stage[beside + u - 1] - (beside ? k.stage[beside - 1] : 0.0f);
+          const float t = base + (float)per * more + 3.0f + mb * 0.22f;
+          if (t < tail) {
+            tail = t;
+            q.whole = (int)(tiles - rest);
+            q.splits = (int)cdiv(stages, per);
+            q.kper = per * stage;
+          }
         }
       }
       time += tail + k.round;
+    } else {
+      q.whole = (int)tiles;
     }
     time *= scale;
     const int64_t split = tiles - q.whole;
@@ -218,7 +230,7 @@ Bytes linear_bytes(int type, int64_t rows, int64_t in, int64_t out, int act, int
                        weight_grad_bytes(type, in, out, rows, 0),
                        weight_grad_bytes(type, in, out, rows, 1)});
     if (act != VMOE_DENSE_NONE) b.grads = align256((size_t)rows * out * esize(type));
-    b.sums = align256((size_t)sum_rows(rows) * out * 4);
+    b.sums = align256((size_t)sum_rows(rows, out) * out * 4);
   }
   b.total = b.part + b.grads + b.sums;
   return b;
@@ -236,7 +248,7 @@ Bytes gated_bytes(int type, int64_t rows, int64_t d, int64_t width, int backward
                        weight_grad_bytes(type, width, d, rows, 0),
                        weight_grad_bytes(type, width, d, rows, 1)});
     b.grads = align256((size_t)rows * 2 * width * esize(type));
-    b.sums = align256((size_t)std::max(gated_sum_rows(q, rows) * 2 * width, sum_rows(rows) * d) * 4);
+    b.sums = align256((size_t)std::max(gated_sum_rows(q, rows) * 2 * width, sum_rows(rows, d) * d) * 4);
   }
   b.total = b.part + b.grads + b.sums;
   return b;
@@ -319,7 +331,7 @@ extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, 
   if (has_act || gb) {
     VMOE_TRY(act_grad(type, gy, ldgy, has_act ? z : nullptr, out, act, dz, out,
                       gb ? sums : nullptr, rows, out, s));
-    if (gb) VMOE_TRY(col_sum(sums, sum_rows(rows), out, out, gb, gb_f32, nullptr, 0, s));
+    if (gb) VMOE_TRY(col_sum(sums, sum_rows(rows, out), out, out, gb, gb_f32, nullptr, 0, s));
   }
   const void* g = has_act ? dz : gy;
   const int64_t ldg = has_act ? out : ldgy;
@@ -433,7 +445,7 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
   if (gb2) {
     VMOE_TRY(act_grad(type, gy, ldgy, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows, hidden,
                       s));
-    VMOE_TRY(col_sum(sums, sum_rows(rows), hidden, hidden, gb2, gb2_f32, nullptr,
+    VMOE_TRY(col_sum(sums, sum_rows(rows, hidden), hidden, hidden, gb2, gb2_f32, nullptr,
                      0, s));
   }
   if (gw2)

@@ -191,20 +191,19 @@ __global__ __launch_bounds__(128) void join_rows_kernel(GemmArgs p) {
 }
 
 // dz = gy * act'(z), rounded, and the column sums of what it stores before
-// rounding: a workgroup takes kSumRows rows of 256 columns, part its row of them.
-constexpr int kSumRows = 64;
+// rounding: a workgroup takes `per` rows of 256 columns, part its row of them.
 template <typename E, bool ACT>
 __global__ __launch_bounds__(256) void act_grad_kernel(const void* gy, int64_t ldgy,
                                                        const float* z, int64_t ldz, int act,
                                                        void* dz, int64_t lddz, float* part,
-                                                       int64_t M, int64_t N) {
+                                                       int64_t M, int64_t N, int per) {
   __shared__ float red[4][256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n = (int64_t)blockIdx.x * 256 + lane * 4;
-  const int64_t m0 = (int64_t)blockIdx.y * kSumRows;
+  const int64_t m0 = (int64_t)blockIdx.y * per;
   float sum[4] = {};
   if (n < N) {
-    const int64_t m1 = min(M, m0 + kSumRows);
+    const int64_t m1 = min(M, m0 + per);
 #pragma unroll 4
     for (int64_t m = m0 + wave; m < m1; m += 4) {
       float g[4];
@@ -338,19 +337,31 @@ int join_rows(int type, Epi epi, const GemmArgs& p, hipStream_t s) {
   return VMOE_OK;
 }
 
-int64_t sum_rows(int64_t M) { return (M + kSumRows - 1) / kSumRows; }
+// Rows of a workgroup of act_grad: 64, fewer where that leaves the card short of
+// workgroups.
+static int act_grad_rows(int64_t M, int64_t N) {
+  const int64_t cols = (N + 255) / 256;
+  int per = 64;
+  while (per > 16 && (M + per - 1) / per * cols < 2048) per /= 2;
+  return per;
+}
+int64_t sum_rows(int64_t M, int64_t N) {
+  const int per = act_grad_rows(M, N);
+  return (M + per - 1) / per;
+}
 
 int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
              void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s) {
-  const dim3 grid((uint32_t)((N + 255) / 256), (uint32_t)sum_rows(M));
+  const dim3 grid((uint32_t)((N + 255) / 256), (uint32_t)sum_rows(M, N));
+  const int per = act_grad_rows(M, N);
   auto go = [&](auto e) {
     typedef decltype(e) E;
     if (z)
       VMOE_LAUNCH((act_grad_kernel<E, true>), grid, dim3(256), 0, s, gy, ldgy, z, ldz, act, dz,
-                  lddz, part, M, N);
+                  lddz, part, M, N, per);
     else
       VMOE_LAUNCH((act_grad_kernel<E, false>), grid, dim3(256), 0, s, gy, ldgy, z, ldz, act, dz,
-                  lddz, part, M, N);
+                  lddz, part, M, N, per);
   };
   if (type == VMOE_DENSE_F32) go(F32());
   else go(Bf16());

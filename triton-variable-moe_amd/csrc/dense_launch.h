@@ -23,7 +23,7 @@ int gemm_few(int type, Form form, Epi epi, const GemmArgs& p, int cols, hipStrea
 int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
 int join_tiles(int type, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
 int join_rows(int type, Epi epi, const GemmArgs& p, hipStream_t s);
-int64_t sum_rows(int64_t M);  // rows of the sums that act_grad leaves
+int64_t sum_rows(int64_t M, int64_t N);  // rows of the sums that act_grad leaves
 int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, int act,
              void* dz, int64_t lddz, float* part, int64_t M, int64_t N, hipStream_t s);
 // column sums of part [rows, N]: columns below `split` into out0, the others into out1

@@ -7,7 +7,10 @@
 // centred sum of squares and the result; statistics, gradients and sums are fp32.
 // A row belongs to 64 threads (one wave, no barrier) or, where it is long, to 256
 // or 1024; workgroups go on to further rows with the weights, and in the backward
-// pass their gradients' sums, in registers. Those sums are joined in a fixed
+// pass their gradients' sums, in registers. The forward pass fetches a row while the
+// one before is worked on (32768 x 2048 in bf16: 64 -> 48 us with 256 threads a row
+// instead of 64, 5.6 TB/s); the backward pass, with two streams of rows, gained
+// nothing by that (77 to 81 us, 5.0 to 5.2 TB/s). Those sums are joined in a fixed
 // order: within a workgroup, then by a launch of their own.
 
 #include "dense_launch.h"
@@ -21,32 +24,48 @@ using dense::F32;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// VEC values at p[i]: 16 bytes of the rows' type at once (VEC = 1: one value).
+// VEC values of a row as they lie in memory: 16 bytes, or one value (VEC = 1).
+template <typename E, int VEC>
+struct Raw {
+  static constexpr bool kWide = VEC > 1;
+  static_assert(!kWide || VEC * E::kSize == 16, "16 bytes");
+  std::conditional_t<kWide, u32x4, typename E::Store> q;
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    q = *reinterpret_cast<const decltype(q)*>(static_cast<const typename E::Store*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    if constexpr (!kWide) {
+      if constexpr (E::kSize == 4) v[0] = q;
+      else v[0] = bf16_to_f32(q);
+    } else if constexpr (E::kSize == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(q[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = lo_f32(q[e]);
+        v[2 * e + 1] = hi_f32(q[e]);
+      }
+    }
+  }
+};
+
+// VEC values at p[i] (rows' values come as Raw): a weight, of either type.
 template <typename E, int VEC>
 __device__ __forceinline__ void load_vec(const void* p, int64_t i, float* v) {
-  if constexpr (VEC == 1) {
-    if constexpr (E::kSize == 4) v[0] = static_cast<const float*>(p)[i];
-    else v[0] = bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
-  } else if constexpr (E::kSize == 4) {
-#pragma unroll
-    for (int j = 0; j < VEC / 4; ++j) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i + 4 * j);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * j + e] = w[e];
-    }
-  } else if constexpr (VEC == 8) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[2 * e] = lo_f32(w[e]);
-      v[2 * e + 1] = hi_f32(w[e]);
-    }
-  } else {
+  if constexpr (VEC * E::kSize == 32) {
+    load_vec<E, VEC / 2>(p, i, v);
+    load_vec<E, VEC / 2>(p, i + VEC / 2, v + VEC / 2);
+  } else if constexpr (VEC * E::kSize == 8) {
     const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
     v[0] = lo_f32(w.x);
     v[1] = hi_f32(w.x);
     v[2] = lo_f32(w.y);
     v[3] = hi_f32(w.y);
+  } else {
+    Raw<E, VEC> q;
+    q.load(p, i);
+    q.get(v);
   }
 }
 
@@ -146,9 +165,19 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_fwd_kernel(NormArgs p)
     }
   }
   const float inv = 1.0f / (float)p.d;
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; r < p.rows;
-       r += (int64_t)gridDim.x * ROWS) {
-    const typename E::Store* row = static_cast<const typename E::Store*>(p.x) + r * p.ldx;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  Raw<E, VEC> next[NCH];
+  auto fetch = [&](int64_t row) {
+    const typename E::Store* at = static_cast<const typename E::Store*>(p.x) + row * p.ldx;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int64_t i = ((int64_t)c * TPR + t) * VEC;
+      if (i < p.d) next[c].load(at, i);
+    }
+  };
+  if (r < p.rows) fetch(r);
+  for (; r < p.rows; r += step) {
     float x[NCH][VEC];
     float s[1] = {0.0f};
 #pragma unroll
@@ -156,8 +185,9 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_fwd_kernel(NormArgs p)
       const int64_t i = ((int64_t)c * TPR + t) * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) x[c][e] = 0.0f;
-      if (i < p.d) load_vec<E, VEC>(row, i, x[c]);
+      if (i < p.d) next[c].get(x[c]);
     }
+    if (r + step < p.rows) fetch(r + step);
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -209,8 +239,9 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
     if (i < p.d && p.w) load_weight<VEC>(p.w, p.w_f32, i, w[c]);
   }
   const float inv = 1.0f / (float)p.d;
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; r < p.rows;
-       r += (int64_t)gridDim.x * ROWS) {
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  for (; r < p.rows; r += step) {
     const typename E::Store* row = static_cast<const typename E::Store*>(p.x) + r * p.ldx;
     const typename E::Store* grow = static_cast<const typename E::Store*>(p.gy) + r * p.ldgy;
     const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * r);
@@ -299,9 +330,8 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
 constexpr int64_t kMaxNorm = 16384;  // 1024 threads of 16 values
 constexpr int64_t kNormGroups = 1024;  // workgroups of a backward pass: rows of its sums
 
-// Threads of a row by its length; forward: up to 32 values a thread, backward
-// (which holds five rows' worth): 16.
-inline int norm_threads(int64_t d, int per) { return d <= 64 * per ? 64 : d <= 256 * per ? 256 : 1024; }
+// Threads of a row by its length: up to 16 values a thread.
+inline int norm_threads(int64_t d) { return d <= 1024 ? 64 : d <= 4096 ? 256 : 1024; }
 
 inline int64_t norm_groups(int64_t rows, int tpr) {
   const int64_t per = tpr < 256 ? 256 / tpr : 1;
@@ -312,10 +342,10 @@ inline int64_t norm_groups(int64_t rows, int tpr) {
 
 // f(TPR, VEC, NCH) for rows of d values; vec: the widest load that rows and
 // weights allow, in values (1, or 16 bytes).
-template <typename E, int MAXV, typename F>
+template <typename E, typename F>
 int norm_pick(int64_t d, bool vec, F&& f) {
   constexpr int V = 16 / E::kSize;
-  const int tpr = norm_threads(d, MAXV);
+  const int tpr = norm_threads(d);
   auto width = [&](auto T) -> int {
     constexpr int TPR = decltype(T)::value;
     auto chunks = [&](auto VEC_) -> int {
@@ -323,9 +353,6 @@ int norm_pick(int64_t d, bool vec, F&& f) {
       typedef std::integral_constant<int, TPR> I;
       if (d <= TPR * 8) return f(I(), VEC_, std::integral_constant<int, 8 / VEC>());
       if (d <= TPR * 16) return f(I(), VEC_, std::integral_constant<int, 16 / VEC>());
-      // (1024 threads: kMaxNorm values are 16 each)
-      if constexpr (MAXV > 16 && TPR < 1024)
-        return f(I(), VEC_, std::integral_constant<int, 32 / VEC>());
       return VMOE_ERR_UNSUPPORTED;
     };
     if (vec) return chunks(std::integral_constant<int, V>());
@@ -372,7 +399,7 @@ extern "C" int vmoe_layer_norm(int32_t type, const void* x, int64_t ldx, int64_t
     constexpr int V = 16 / E::kSize;
     const bool vec = d % V == 0 && ldx % V == 0 && ldy % V == 0 && al16(x) && al16(y) &&
                      al16(w) && al16(b);
-    return norm_pick<E, 32>(d, vec, [&](auto T, auto VEC, auto N) -> int {
+    return norm_pick<E>(d, vec, [&](auto T, auto VEC, auto N) -> int {
       constexpr int TPR = decltype(T)::value;
       const int64_t per = TPR < 256 ? 256 / TPR : 1;
       const int64_t need = (rows + per - 1) / per;
@@ -388,7 +415,7 @@ extern "C" int vmoe_layer_norm(int32_t type, const void* x, int64_t ldx, int64_t
 
 extern "C" size_t vmoe_layer_norm_workspace_bytes(int64_t rows, int64_t d) {
   if (rows <= 0 || d <= 0 || d > kMaxNorm) return 0;
-  return (size_t)norm_groups(rows, norm_threads(d, 16)) * 2 * d * 4;
+  return (size_t)norm_groups(rows, norm_threads(d)) * 2 * d * 4;
 }
 
 extern "C" int vmoe_layer_norm_backward(int32_t type, const void* gy, int64_t ldgy, const void* x,
@@ -418,13 +445,13 @@ extern "C" int vmoe_layer_norm_backward(int32_t type, const void* gy, int64_t ld
   p.gy = gy; p.ldgy = ldgy;
   p.part = static_cast<float*>(workspace);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t groups = norm_groups(rows, norm_threads(d, 16));
+  const int64_t groups = norm_groups(rows, norm_threads(d));
   auto go = [&](auto e) -> int {
     typedef decltype(e) E;
     constexpr int V = 16 / E::kSize;
     const bool vec = d % V == 0 && ldx % V == 0 && ldgy % V == 0 && (!gx || ldgx % V == 0) &&
                      al16(x) && al16(gy) && al16(gx) && al16(w);
-    return norm_pick<E, 16>(d, vec, [&](auto T, auto VEC, auto N) -> int {
+    return norm_pick<E>(d, vec, [&](auto T, auto VEC, auto N) -> int {
       constexpr int TPR = decltype(T)::value, VE = decltype(VEC)::value, NC = decltype(N)::value;
       if (wg)
         VMOE_LAUNCH((norm_bwd_kernel<E, TPR, VE, NC, true>), dim3((uint32_t)groups),
