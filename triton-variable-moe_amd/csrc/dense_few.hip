@@ -222,13 +222,14 @@ int launch(GemmArgs p, hipStream_t s) {
 
 template <typename E, bool T, int EPI>
 int by_rows(const GemmArgs& p, int cols, hipStream_t s) {
-  if (cols == 32)
-    return p.M <= 16   ? launch<E, T, EPI, 1, 32>(p, s)
-           : p.M <= 32 ? launch<E, T, EPI, 2, 32>(p, s)
-                       : launch<E, T, EPI, 4, 32>(p, s);
-  return p.M <= 16   ? launch<E, T, EPI, 1, 64>(p, s)
-         : p.M <= 32 ? launch<E, T, EPI, 2, 64>(p, s)
-                     : launch<E, T, EPI, 4, 64>(p, s);
+  if constexpr (T && E::kSize == 2)
+    if (cols == 64)
+      return p.M <= 16   ? launch<E, T, EPI, 1, 64>(p, s)
+             : p.M <= 32 ? launch<E, T, EPI, 2, 64>(p, s)
+                         : launch<E, T, EPI, 4, 64>(p, s);
+  return p.M <= 16   ? launch<E, T, EPI, 1, 32>(p, s)
+         : p.M <= 32 ? launch<E, T, EPI, 2, 32>(p, s)
+                     : launch<E, T, EPI, 4, 32>(p, s);
 }
 
 template <typename E, bool T>

@@ -343,6 +343,7 @@ static int act_grad_rows(int64_t M, int64_t N) {
   const int64_t cols = (N + 255) / 256;
   int per = 64;
   while (per > 16 && (M + per - 1) / per * cols < 2048) per /= 2;
+  while ((M + per - 1) / per > 32768) per *= 2;  // (a grid's second dimension)
   return per;
 }
 int64_t sum_rows(int64_t M, int64_t N) {

@@ -15,7 +15,8 @@ inline uint32_t workgroups(const GemmArgs& p) {
 
 // dense_big.hip: TILES_256, bf16
 int gemm_big(Form form, Epi epi, const GemmArgs& p, hipStream_t s);
-// dense_few.hip: at most kFewRows rows, workgroups of `cols` (32 or 64) columns
+// dense_few.hip: at most kFewRows rows, workgroups of `cols` columns (32, or for T-form
+// weights in bf16 64)
 constexpr int64_t kFewRows = 64;
 int gemm_few(int type, Form form, Epi epi, const GemmArgs& p, int cols, hipStream_t s);
 // dense_gemm.hip: the product on tiles; the epilogue of its split tiles; the epilogue
