@@ -906,7 +906,8 @@ enum vmoe_dense_act {
 };
 
 /* y = act(x w + bias) + residual. bias, residual and z may be NULL; z [rows, out]
- * fp32 takes x w + bias, which the backward pass of an activation reads. */
+ * fp32 takes x w + bias, which the backward pass of an activation reads. That of relu
+ * and relu squared reads y instead where z is NULL and there was no residual. */
 size_t vmoe_linear_workspace_bytes(int32_t type, int64_t rows, int64_t in, int64_t out,
                                    int32_t act, int32_t backward);
 int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t in,
@@ -917,9 +918,10 @@ int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, 
 /* Gradients of x, w (in w's order) and bias; each may be NULL. */
 int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void* x, int64_t ldx,
                          int64_t rows, int64_t in, int64_t out, const void* w, int64_t ldw,
-                         int32_t w_transposed, int32_t act, const float* z, void* gx,
-                         int64_t ldgx, void* gw, int64_t ldgw, void* gb, int32_t gb_f32,
-                         void* workspace, size_t workspace_bytes, vmoe_stream_t stream);
+                         int32_t w_transposed, int32_t act, const float* z, const void* y,
+                         int64_t ldy, void* gx, int64_t ldgx, void* gw, int64_t ldgw, void* gb,
+                         int32_t gb_f32, void* workspace, size_t workspace_bytes,
+                         vmoe_stream_t stream);
 
 /* [g | u] = x w1 + bias1, h = act(g) * u, y = h w2 + bias2 + residual; w1 is
  * [hidden, 2 width], w2 [width, hidden]. h [rows, width] is written (rounded to the

@@ -133,17 +133,18 @@ def test_linear_entry(change, status):
 
 
 def linear_bwd(type=0, gy=P, ldgy=64, x=P, ldx=64, rows=2, i=64, o=64, w=P, ldw=64, tr=0, act=0,
-               z=None, gx=P, ldgx=64, gw=P, ldgw=64, gb=P, ws=P, n=HUGE):
+               z=None, y=None, ldy=64, gx=P, ldgx=64, gw=P, ldgw=64, gb=P, ws=P, n=HUGE):
     if n == "short":
         n = _lib.lib().vmoe_linear_workspace_bytes(type, rows, i, o, act, 1) - 1
-    return _lib.lib().vmoe_linear_backward(type, gy, ldgy, x, ldx, rows, i, o, w, ldw, tr, act, z, gx,
-                                           ldgx, gw, ldgw, gb, 0, ws, n, None)
+    return _lib.lib().vmoe_linear_backward(type, gy, ldgy, x, ldx, rows, i, o, w, ldw, tr, act, z, y,
+                                           ldy, gx, ldgx, gw, ldgw, gb, 0, ws, n, None)
 
 
 @pytest.mark.parametrize("change,status", SIZES + [
     (dict(rows=0), OK), (dict(gy=None), BAD), (dict(ldgy=56), BAD), (dict(x=None), BAD),
     (dict(w=None), BAD), (dict(ldgx=56), BAD), (dict(gx=P + 8), NOT), (dict(gw=P + 8), NOT),
-    (dict(ldgw=56), BAD), (dict(act=1), BAD), (dict(act=1, z=P + 4), NOT), (dict(n=0), WS),
+    (dict(ldgw=56), BAD), (dict(act=1), BAD), (dict(act=1, z=P + 4), NOT),
+    (dict(act=3, y=P), BAD), (dict(act=2, y=P, ldy=56), BAD), (dict(act=2, y=P + 8), NOT), (dict(n=0), WS),
     (dict(ws=None), BAD), (dict(ws=P + 8), NOT),
     (dict(n="short"), WS),
 ])

@@ -308,9 +308,10 @@ extern "C" int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int
 extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void* x,
                                     int64_t ldx, int64_t rows, int64_t in, int64_t out,
                                     const void* w, int64_t ldw, int32_t w_transposed,
-                                    int32_t act, const float* z, void* gx, int64_t ldgx, void* gw,
-                                    int64_t ldgw, void* gb, int32_t gb_f32, void* workspace,
-                                    size_t workspace_bytes, vmoe_stream_t stream) {
+                                    int32_t act, const float* z, const void* y, int64_t ldy,
+                                    void* gx, int64_t ldgx, void* gw, int64_t ldgw, void* gb,
+                                    int32_t gb_f32, void* workspace, size_t workspace_bytes,
+                                    vmoe_stream_t stream) {
   VMOE_TRY(check_sizes(type, act, rows, in, out));
   if (rows == 0) return VMOE_OK;
   VMOE_TRY(check_rows(type, gy, out, ldgy));
@@ -318,7 +319,11 @@ extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, 
   if (gx) VMOE_TRY(check_weight(type, w, ldw, w_transposed, in, out));
   if (gx) VMOE_TRY(check_rows(type, gx, in, ldgx));
   if (gw) VMOE_TRY(check_weight(type, gw, ldgw, w_transposed, in, out));
-  if (act != VMOE_DENSE_NONE && !z) return VMOE_ERR_INVALID_ARG;
+  const bool has_act = act != VMOE_DENSE_NONE;
+  const bool from_y = has_act && !z;
+  if (from_y && act != VMOE_DENSE_RELU && act != VMOE_DENSE_RELU_SQUARED)
+    return VMOE_ERR_INVALID_ARG;
+  if (from_y) VMOE_TRY(check_rows(type, y, out, ldy));
   if (z && !aligned(z)) return VMOE_ERR_UNSUPPORTED;
   const Bytes b = linear_bytes(type, rows, in, out, act, 1);
   VMOE_TRY(check_workspace(workspace, workspace_bytes, b.total));
@@ -327,10 +332,9 @@ extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, 
   float* part = reinterpret_cast<float*>(ws);
   void* dz = ws + b.part;
   float* sums = reinterpret_cast<float*>(ws + b.part + b.grads);
-  const bool has_act = act != VMOE_DENSE_NONE;
   if (has_act || gb) {
-    VMOE_TRY(act_grad(type, gy, ldgy, has_act ? z : nullptr, out, act, dz, out,
-                      gb ? sums : nullptr, rows, out, s));
+    VMOE_TRY(act_grad(type, gy, ldgy, has_act ? z : nullptr, out, from_y ? y : nullptr, ldy, act,
+                      dz, out, gb ? sums : nullptr, rows, out, s));
     if (gb) VMOE_TRY(col_sum(sums, sum_rows(rows, out), out, out, gb, gb_f32, nullptr, 0, s));
   }
   const void* g = has_act ? dz : gy;
@@ -443,8 +447,8 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
       VMOE_TRY(col_sum(sums, gated_sum_rows(q, rows), w2x, w2x, gb1, gb1_f32, nullptr, 0, s));
   }
   if (gb2) {
-    VMOE_TRY(act_grad(type, gy, ldgy, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows, hidden,
-                      s));
+    VMOE_TRY(act_grad(type, gy, ldgy, nullptr, 0, nullptr, 0, VMOE_DENSE_NONE, nullptr, 0, sums, rows,
+                      hidden, s));
     VMOE_TRY(col_sum(sums, sum_rows(rows, hidden), hidden, hidden, gb2, gb2_f32, nullptr,
                      0, s));
   }

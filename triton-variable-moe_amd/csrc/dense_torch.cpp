@@ -340,9 +340,11 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& b_, const M
 struct FusedLinear : torch::autograd::Function<FusedLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b,
                         const Maybe& r, int64_t act) {
+    // relu's and relu squared's slopes follow from the output, unless a residual is in it
+    const bool from_y = !r && (act == VMOE_DENSE_RELU || act == VMOE_DENSE_RELU_SQUARED);
     Tensor z;
-    Tensor y = linear_forward(x, w, b, r, (int)act, act ? &z : nullptr);
-    ctx->save_for_backward({x, w, b ? *b : Tensor(), z});
+    Tensor y = linear_forward(x, w, b, r, (int)act, act && !from_y ? &z : nullptr);
+    ctx->save_for_backward({x, w, b ? *b : Tensor(), z, from_y ? y : Tensor()});
     ctx->saved_data["act"] = act;
     ctx->saved_data["residual"] = r.has_value();
     return y;
@@ -352,7 +354,7 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
     {
       const at::AutoGradMode off(false);
       const variable_list s = ctx->get_saved_variables();
-      const Tensor &x = s[0], &w = s[1], &b = s[2], &z = s[3], &gy = gys[0];
+      const Tensor &x = s[0], &w = s[1], &b = s[2], &z = s[3], &y = s[4], &gy = gys[0];
       const int act = (int)ctx->saved_data["act"].toInt();
       const auto need =
           needs<4>(ctx, {true, true, b.defined(), ctx->saved_data["residual"].toBool()});
@@ -375,9 +377,9 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
           call("vmoe_linear_backward", [&] {
             return vmoe_linear_backward(
                 type, g.p(), g.ld, m.p(), m.ld, rows, in, n_out, wm.p(), wm.ld, wm.tr, act,
-                z.defined() ? static_cast<const float*>(z.const_data_ptr()) : nullptr, out_ptr(gx),
-                in, out_ptr(gw), ld_of(gw, wm.tr), out_ptr(gb), f32(gb), out_ptr(ws), n,
-                stream_of(x));
+                z.defined() ? static_cast<const float*>(z.const_data_ptr()) : nullptr,
+                y.defined() ? y.const_data_ptr() : nullptr, n_out, out_ptr(gx), in, out_ptr(gw),
+                ld_of(gw, wm.tr), out_ptr(gb), f32(gb), out_ptr(ws), n, stream_of(x));
           });
         }
         out[0] = gx;
