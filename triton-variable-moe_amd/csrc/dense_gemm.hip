@@ -101,63 +101,93 @@ int launch_form(const GemmArgs& p, Tiles tiles, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // Split tiles: the sums of their slices, in order, through the epilogue. Waves of the
-// product in WM x WN, FM x FN blocks each; a workgroup takes the FM blocks of one wave
-// and block column (EPI_GATED: of both), a wave of it one register group (see
-// write_part).
+// product in WM x WN, FM x FN blocks of 32 x 32 each. A workgroup takes one wave's
+// row of FN blocks (EPI_GATED_BWD, for its column sums: all FM of them): they are read as they lie (see write_part; a wave of
+// the workgroup one register group, the next row while this one is worked on), turned
+// in LDS, and written as rows: 64 columns in one piece (EPI_GATED: 32), where lanes
+// that kept their values would write 32 pieces of 4 columns.
 template <typename E, int EPI, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs p, int gm) {
   constexpr bool GATED = EPI == EPI_GATED, BWD = EPI == EPI_GATED_BWD;
-  constexpr int NW = WM * WN, J = GATED ? 1 : FN, VALUES = NW * FM * FN * 1024;
+  constexpr int NW = WM * WN, VALUES = NW * FM * FN * 1024;
+  constexpr int COLS = 32 * FN, OUT = GATED ? 32 : COLS;  // staged and output columns
+  constexpr int PITCH = COLS + 4;                         // (banks: 16 bytes off a row)
+  constexpr int LR = OUT / 4, RP = 256 / LR;              // threads of a row, rows at a time
+  __shared__ __align__(16) float turn[2][32 * PITCH];
   const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-  int id = blockIdx.x;
-  const int j = id % J;
-  id /= J;
-  const int wave = id % NW, split = id / NW;
+  constexpr int PER = BWD ? FM : 1;  // rows of blocks of a workgroup
+  const int first = blockIdx.x % (FM / PER) * PER, unit = blockIdx.x / (FM / PER);
+  const int wave = unit % NW, split = unit / NW;
   const Tile t = tile_at(p, p.whole + split, gm);
   const int wm = wave / WN, wn = wave % WN;
-  const int64_t m0 = ((int64_t)t.m * WM + wm) * 32 * FM + (lane & 31);
-  const int64_t n = ((int64_t)t.n * WN + wn) * 32 * J + 32 * j + 8 * g + 4 * (lane >> 5);
-  const int64_t step = (int64_t)(p.tiles_m * p.tiles_n - p.whole) * VALUES;
-  const float* part =
-      p.part + (int64_t)split * VALUES + (wave * FM * FN * 4 + j * 4 + g) * 256 + lane * 4;
+  const int64_t m0 = ((int64_t)t.m * WM + wm) * 32 * FM;
+  const int64_t n0 = ((int64_t)t.n * WN + wn) * OUT;
+  if (m0 + 32 * first >= p.M || n0 >= p.N) return;
+  const int c = (threadIdx.x % LR) * 4;
+  const int64_t n = n0 + c;
   const bool n_ok = n < p.N;
+  const int64_t step = (int64_t)(p.tiles_m * p.tiles_n - p.whole) * VALUES;
+  const float* part = p.part + (int64_t)split * VALUES + (wave * FM * FN * 4 + g) * 256 + lane * 4;
   EpiCols<EPI, 4> cols;
   epi_cols<EPI, 4>(p, n, cols);
   float sg[4] = {}, su[4] = {};
+  f32x4_t sum[FN];
+  auto read = [&](int i) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t m = m0 + 32 * i;
-    if (m >= p.M || !n_ok) continue;
-    GateUp z = {};
-    if constexpr (BWD) z = load_z(p, m, n);
-    float v[4] = {}, u[4] = {};
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      float x[4];
-      load_c<F32, 4>(part + s * step, i * FN * 1024, x);
+    for (int j = 0; j < FN; ++j)
+      sum[j] = *reinterpret_cast<const f32x4_t*>(part + (i * FN + j) * 1024);
+#pragma unroll 8
+    for (int s = 1; s < p.splits; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += x[e];
-      if constexpr (GATED) {
-        load_c<F32, 4>(part + s * step, (i * FN + 1) * 1024, x);
+      for (int j = 0; j < FN; ++j)
+        sum[j] += *reinterpret_cast<const f32x4_t*>(part + s * step + (i * FN + j) * 1024);
+  };
+  read(first);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] += x[e];
+  for (int k = 0; k < PER; ++k) {
+    const int i = first + k;
+    float* buf = turn[k & 1];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      *reinterpret_cast<f32x4_t*>(buf + (lane & 31) * PITCH + 32 * j + 8 * g + 4 * (lane >> 5)) =
+          sum[j];
+    if (k + 1 < PER) read(i + 1);
+    __syncthreads();
+#pragma unroll
+    for (int r = threadIdx.x / LR; r < 32; r += RP) {
+      const int64_t m = m0 + 32 * i + r;
+      if (m >= p.M || !n_ok) continue;
+      float v[4], u[4] = {};
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(buf + r * PITCH + c);
+      const f32x4_t b = *reinterpret_cast<const f32x4_t*>(buf + r * PITCH + (GATED ? 32 : 0) + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        u[e] = b[e];
       }
+      GateUp z = {};
+      if constexpr (BWD) z = load_z(p, m, n);
+      epi_row<E, EPI, 4>(p, cols, m, n, v, u, z, sg, su);
     }
-    epi_row<E, EPI, 4>(p, cols, m, n, v, u, z, sg, su);
   }
   if constexpr (BWD) {
-    if (p.sums && m0 - (lane & 31) < p.M) {
+    if (p.sums) {
+      // threads of the same columns, in order
+      __shared__ __align__(16) float part_sums[2][RP][OUT];
+      const int r = threadIdx.x / LR;
 #pragma unroll
-      for (int o = 1; o < 32; o *= 2)
+      for (int e = 0; e < 4; ++e) {
+        part_sums[0][r][c + e] = sg[e];
+        part_sums[1][r][c + e] = su[e];
+      }
+      __syncthreads();
+      for (int id = threadIdx.x; id < 2 * OUT; id += 256) {
+        const int q = id / OUT, col = id % OUT;
+        float total = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sg[e] += __shfl_xor(sg[e], o, 64);
-          su[e] += __shfl_xor(su[e], o, 64);
-        }
-      if ((lane & 31) == 0 && n_ok) {
-        float* row = p.sums + ((int64_t)t.m * WM + wm) * 2 * p.N;
-        store_c<F32, 4>(row, n, sg);
-        store_c<F32, 4>(row + p.N, n, su);
+        for (int i = 0; i < RP; ++i) total += part_sums[q][i][col];
+        if (n0 + col < p.N)
+          p.sums[((int64_t)t.m * WM + wm) * 2 * p.N + q * p.N + n0 + col] = total;
       }
     }
   }
@@ -308,7 +338,7 @@ namespace {
 template <typename E, int EPI, int WM, int WN, int FM, int FN>
 int launch_join(const GemmArgs& p, int gm, hipStream_t s) {
   const int rest = p.tiles_m * p.tiles_n - p.whole;
-  const int blocks = rest * WM * WN * (EPI == EPI_GATED ? 1 : FN);
+  const int blocks = rest * WM * WN * (EPI == EPI_GATED_BWD ? 1 : FM);
   VMOE_LAUNCH((join_kernel<E, EPI, WM, WN, FM, FN>), dim3((uint32_t)blocks), dim3(256), 0, s, p,
               gm);
   VMOE_CHECK_LAUNCH();
