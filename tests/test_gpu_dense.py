@@ -474,6 +474,44 @@ def test_weight_at_an_address_that_is_not_aligned(device):
                                                                .t().contiguous().t()))
 
 
+def test_negative_views(device):
+    g = gen(18)
+    x, w, b = rnd(g, 9, 64), rnd(g, 64, 64), rnd(g, 64)
+    nx, nw, nb = (torch.complex(torch.zeros_like(t), -t).conj().imag for t in (x, w, b))
+    assert nx.is_neg() and torch.equal(nx, x)
+    assert torch.equal(K.layer_norm(nx, nb, nb), K.layer_norm(x, b, b))
+    assert torch.equal(K.fused_linear(nx, nw, nb, "gelu", nx), K.fused_linear(x, w, b, "gelu", x))
+    assert torch.equal(K.gated_mlp(nx, nw, nw[:32], "reglu", nb, nb, nx),
+                       K.gated_mlp(x, w, w[:32], "reglu", b, b, x))
+
+
+def test_offsets_past_32_bits(device):
+    """Rows behind the first 4 GiB, and 2^31 values, of inputs and outputs."""
+    rows, d = 300_000, 8192
+    x = torch.zeros(rows, d, device="cuda", dtype=BF16)
+    g = gen(19)
+    at = [0, 1, 131_071, 131_072, 262_143, 262_144, 262_145, rows - 1]
+    values = rnd(g, len(at), d, dtype=BF16)
+    x[at] = values
+    y = K.layer_norm(x)
+    (want, *_), (t, *_) = norm_reference(values, None, None, values, 1e-5)
+    close(y[at], want, t + half(x) * want.abs(), "layer_norm")
+    assert not y[5].any() and not y[rows - 2].any()
+    del y
+    for n in (8, 264):
+        w = matrix(g, d, n, BF16, n == 8)
+        y = K.fused_linear(x, w)
+        (want, *_), (t, *_) = linear_reference(values, w, None, None, rnd(g, len(at), n, dtype=BF16),
+                                               None)
+        close(y[at], want, t + half(x) * (want.abs() + t), f"fused_linear {n}")
+        assert not y[rows - 2].any()
+    w = matrix(g, 8, d, BF16, False)  # a long output
+    y = K.fused_linear(x[:, :8], w, residual=x)
+    (want, *_), (t, *_) = linear_reference(values[:, :8], w, None, values, values, None)
+    close(y[at], want, t + half(x) * (want.abs() + t), "long output")
+    assert not y[rows - 2].any()
+
+
 def test_no_rows(device):
     w1 = torch.ones(16, 64, device="cuda", requires_grad=True)
     w2 = torch.ones(32, 16, device="cuda", requires_grad=True)

@@ -124,9 +124,12 @@ struct Mat {
 };
 
 Tensor fresh(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+// (a view that stands for its negative, as of a conjugate's imaginary part)
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 
 // t as rows of `cols` values, contiguous and 16-byte aligned: in place, or a copy.
-Mat rows_of(const Tensor& t, int64_t cols) {
+Mat rows_of(const Tensor& given, int64_t cols) {
+  const Tensor t = plain(given);
   Mat m;
   m.t = t.dim() == 2 ? t : t.reshape({-1, cols});
   const int64_t mult = 16 / (int64_t)t.element_size();
@@ -140,7 +143,8 @@ Mat rows_of(const Tensor& t, int64_t cols) {
 }
 
 // A weight [in, out]: in place in either order, or a copy in the nearer one.
-Mat weight_of(const Tensor& w) {
+Mat weight_of(const Tensor& given) {
+  const Tensor w = plain(given);
   Mat m;
   const int64_t mult = 16 / (int64_t)w.element_size();
   const int64_t a = w.stride(0), b = w.stride(1);
@@ -164,7 +168,8 @@ Mat weight_of(const Tensor& w) {
 }
 
 // Rows of a norm: contiguous, at any distance (0: one row for all).
-Mat norm_rows(const Tensor& t, int64_t d) {
+Mat norm_rows(const Tensor& given, int64_t d) {
+  const Tensor t = plain(given);
   Mat m;
   m.t = t.dim() == 2 ? t : t.reshape({-1, d});
   const int64_t rows = m.t.size(0), s = m.t.stride(0);
@@ -173,9 +178,10 @@ Mat norm_rows(const Tensor& t, int64_t d) {
   return m;
 }
 
-Maybe contiguous(const Maybe& v) {
-  if (!v || v->numel() < 2 || v->stride(0) == 1) return v;
-  return v->contiguous();
+Maybe contiguous(const Maybe& given) {
+  if (!given) return given;
+  const Tensor v = plain(*given);
+  return v.numel() < 2 || v.stride(0) == 1 ? v : v.contiguous();
 }
 
 Tensor empty(at::IntArrayRef shape, const Tensor& x) { return at::empty(shape, x.options()); }
