@@ -10,6 +10,15 @@
 // byte permutes turn 8 rows into the operands of those columns. K-form: a lane's 16
 // bytes are an operand of one column. Rows of x come as operands too, 16 bytes a lane
 // and tile of 16 rows; they are in cache after the first workgroup.
+//
+// Measured at one row, weights from memory, joining included, us (floor at 5.2 TB/s):
+// 1024 x 4096 stored [out, in] 5.0 (1.6), [in, out] 6.1; 2048 x 2048 6.6 and 6.9 (1.6);
+// 5632 x 2048 10.0 and 9.4 (4.4); gated 2048 x 5632 14.4 and 15.4 (8.9); 8192 x 8192
+// 27.5 and 28.1 (25.8). A CU draws 20 to 60 GB/s, so that weights below some 40 MB are
+// bound by starting, one or two chains of loads and the joining. 64 columns for T-form
+// weights over 12 MB: whole 128-byte lines of a k-row (gated 2048 x 5632 16.7 -> 15.4,
+// 8192 x 8192 36 -> 28); below, and for K-form, 32 give more workgroups. 16 waves a
+// workgroup, or one step a batch, changed nothing above the noise.
 
 #include "dense_launch.h"
 

@@ -10,7 +10,7 @@
 // pass their gradients' sums, in registers. The forward pass fetches a row while the
 // one before is worked on (32768 x 2048 in bf16: 64 -> 48 us with 256 threads a row
 // instead of 64, 5.6 TB/s); the backward pass, with two streams of rows, gained
-// nothing by that (77 to 81 us, 5.0 to 5.2 TB/s). Those sums are joined in a fixed
+// nothing by that (77 to 83 us, 4.9 to 5.2 TB/s). Those sums are joined in a fixed
 // order: within a workgroup, then by a launch of their own.
 
 #include "dense_launch.h"
