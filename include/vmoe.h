@@ -905,6 +905,12 @@ enum vmoe_dense_act {
   VMOE_DENSE_GELU_TANH = 5 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
 };
 
+/* Products of few rows that are split along k are joined within their launch where a
+ * call gets arrival words: vmoe_dense_arrival_words() uint32 that are zero when it
+ * starts and are left zero; calls that may run at the same time need words of their
+ * own. NULL: a second launch joins them, with the same bits. */
+int32_t vmoe_dense_arrival_words(void);
+
 /* y = act(x w + bias) + residual. bias, residual and z may be NULL; z [rows, out]
  * fp32 takes x w + bias, which the backward pass of an activation reads. That of relu
  * and relu squared reads y instead where z is NULL and there was no residual. */
@@ -914,7 +920,7 @@ int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, 
                         int64_t out, const void* w, int64_t ldw, int32_t w_transposed,
                         const void* bias, int32_t bias_f32, int32_t act, const void* residual,
                         int64_t ldr, void* y, int64_t ldy, float* z, void* workspace,
-                        size_t workspace_bytes, vmoe_stream_t stream);
+                        size_t workspace_bytes, uint32_t* words, vmoe_stream_t stream);
 /* Gradients of x, w (in w's order) and bias; each may be NULL. */
 int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void* x, int64_t ldx,
                          int64_t rows, int64_t in, int64_t out, const void* w, int64_t ldw,
@@ -935,7 +941,7 @@ int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, i
                        int64_t ldw2, int32_t w2_transposed, const void* bias2,
                        int32_t bias2_f32, const void* residual, int64_t ldr, void* h, float* z,
                        void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
-                       vmoe_stream_t stream);
+                       uint32_t* words, vmoe_stream_t stream);
 int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, const void* x, int64_t ldx,
                         int64_t rows, int64_t hidden, int64_t width, const void* w1, int64_t ldw1,
                         int32_t w1_transposed, const void* w2, int64_t ldw2,

@@ -110,9 +110,9 @@ def test_layer_norm_backward_entry(change, status):
 
 
 def linear(type=0, x=P, ldx=64, rows=2, i=64, o=64, w=P, ldw=64, tr=0, act=0, r=None, ldr=64, y=P,
-           ldy=64, z=None, ws=P, n=HUGE):
+           ldy=64, z=None, ws=P, n=HUGE, words=None):
     return _lib.lib().vmoe_linear_forward(type, x, ldx, rows, i, o, w, ldw, tr, None, 0, act, r, ldr, y,
-                                          ldy, z, ws, n, None)
+                                          ldy, z, ws, n, words, None)
 
 
 SIZES = [(dict(type=2), BAD), (dict(act=6), BAD), (dict(act=-1), BAD), (dict(rows=-1), BAD),
@@ -126,7 +126,7 @@ SIZES = [(dict(type=2), BAD), (dict(act=6), BAD), (dict(act=-1), BAD), (dict(row
     (dict(ldw=56), BAD), (dict(ldw=60), BAD), (dict(o=128, ldw=64, ldy=128), BAD),
     (dict(i=128, ldx=128, tr=1, ldw=64), BAD), (dict(ldw=(1 << 20) + 8), NOT), (dict(y=None), BAD),
     (dict(ldy=56), BAD), (dict(y=P + 4), NOT), (dict(r=P, ldr=56), BAD), (dict(r=P + 2), NOT),
-    (dict(z=P + 8), NOT),
+    (dict(z=P + 8), NOT), (dict(words=P + 2), NOT),
 ])
 def test_linear_entry(change, status):
     assert linear(**change) == status
@@ -153,9 +153,9 @@ def test_linear_backward_entry(change, status):
 
 
 def gated(type=0, x=P, ldx=64, rows=2, d=64, width=32, w1=P, ldw1=64, t1=0, act=3, w2=P, ldw2=64, t2=0,
-          r=None, ldr=64, h=P, z=None, y=P, ldy=64, ws=P, n=HUGE):
+          r=None, ldr=64, h=P, z=None, y=P, ldy=64, ws=P, n=HUGE, words=None):
     return _lib.lib().vmoe_gated_forward(type, x, ldx, rows, d, width, w1, ldw1, t1, None, 0, act, w2,
-                                         ldw2, t2, None, 0, r, ldr, h, z, y, ldy, ws, n, None)
+                                         ldw2, t2, None, 0, r, ldr, h, z, y, ldy, ws, n, words, None)
 
 
 @pytest.mark.parametrize("change,status", SIZES + [
@@ -163,6 +163,7 @@ def gated(type=0, x=P, ldx=64, rows=2, d=64, width=32, w1=P, ldw1=64, t1=0, act=
     (dict(x=None), BAD), (dict(w1=None), BAD), (dict(ldw1=56), BAD), (dict(w2=None), BAD),
     (dict(ldw2=56), BAD), (dict(t2=1, ldw2=24), BAD), (dict(h=None), BAD), (dict(h=P + 8), NOT),
     (dict(y=None), BAD), (dict(z=P + 8), NOT), (dict(r=P + 8), NOT), (dict(ldr=56, r=P), BAD),
+    (dict(words=P + 1), NOT),
     # the ups of a weight stored [2 width, hidden] lie 2 GiB behind the gates
     (dict(t1=1, ldw1=1 << 20, width=1024), NOT),
 ])

@@ -737,6 +737,48 @@ def test_captured_step(rows, device):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_few_rows_joined_in_their_launch(dtype, device):
+    """Products of few rows that are split along k: joined by the last workgroup of the
+    launch in eager calls, by a launch of their own in a graph, with the same bits, again
+    and again, and on two streams at once."""
+    g = gen(20)
+    calls = []
+    for rows, k, n in ((1, 2048, 2048), (5, 4104, 72), (23, 4096, 264), (61, 2056, 136), (64, 5632, 8),
+                       (17, 1544, 2504)):
+        for transposed in (False, True):
+            x, w = rnd(g, rows, k, dtype=dtype), matrix(g, k, n, dtype, transposed)
+            b, r = rnd(g, n, dtype=dtype), rnd(g, rows, n, dtype=dtype)
+            (want, *_), (t, *_) = linear_reference(x, w, b, r, r, "silu")
+            y = K.fused_linear(x, w, b, "silu", r)
+            close(y, want, t + half(y) * (want.abs() + t), f"{rows} {k} {n} {transposed}")
+            calls.append(lambda x=x, w=w, b=b, r=r: K.fused_linear(x, w, b, "silu", r))
+    for rows, d, width in ((1, 2056, 2600), (30, 1544, 2056)):
+        for transposed in (False, True):
+            x, w1 = rnd(g, rows, d, dtype=dtype), matrix(g, d, 2 * width, dtype, transposed)
+            w2 = matrix(g, width, d, dtype, not transposed)
+            (want, *_), (t, *_) = gated_reference(x, w1, w2, None, None, x, x, "geglu")
+            y = K.gated_mlp(x, w1, w2, "geglu", None, None, x)
+            close(y, want, t + half(y) * (want.abs() + t), f"gated {rows} {transposed}", 2)
+            calls.append(lambda x=x, w1=w1, w2=w2: K.gated_mlp(x, w1, w2, "geglu", None, None, x))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([c() for c in calls])
+        graph.replay()
+        torch.cuda.synchronize()
+        for ys in (*got, captured):
+            assert all(torch.equal(a, b) for a, b in zip(ys, want))
+
+
 def test_two_streams_at_once(device):
     """Calls on two streams share nothing."""
     p = block_params(BF16)

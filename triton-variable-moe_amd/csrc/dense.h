@@ -71,8 +71,9 @@ struct GemmArgs {
   // their sums in part.
   int32_t whole, splits;
   int64_t kper;
-  float* part;        // dense_few.hip: [splits, M, ldp]; tiles: see write_part
+  float* part;        // dense_few.hip: [splits, M, ldp] (words: its own); tiles: see write_part
   int64_t ldp;
+  uint32_t* words;    // dense_few.hip: arrival words, or null
 };
 
 __device__ __forceinline__ float sigmoid(float x) {

@@ -66,6 +66,7 @@ constexpr Kernel kBf16[] = {{TILES_256, 256, 256, 1, {1.85f}, 14.0f},
 constexpr Kernel kF32[] = {{TILES_128, 128, 128, 2, {2.03f, 3.8f}, 5.0f},
                            {TILES_64, 64, 64, 3, {0.68f, 1.14f, 1.62f}, 2.0f}};
 constexpr int kCus = 256;
+static_assert(kCus <= kFewWords, "a split product of few rows has fewer column blocks than CUs");
 
 // Few rows: whether the kernel that streams the weight takes a product, and how. Up to
 // 16 rows always (one row of 1024 x 4096: 5.0 us, on tiles 8.4); up to 64 for weights
@@ -85,9 +86,9 @@ bool plan_rows(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K, Pl
   const int64_t most = K <= 1024 && cols == 32 ? 1 : K / 512;
   const int64_t s = std::max<int64_t>(1, std::min<int64_t>(cdiv(kCus, q.tiles_n), most));
   q.kper = cdiv(cdiv(K, stage), s) * stage;
-  q.splits = (int)cdiv(K, q.kper);
+  q.splits = (int)cdiv(K, q.kper);  // (more than one: fewer than kFewWords column blocks)
   q.whole = 0;
-  q.part_bytes = q.splits > 1 ? align256((size_t)q.splits * M * n * 4) : 0;
+  q.part_bytes = q.splits > 1 ? align256((size_t)q.splits * M * q.tiles_n * cols * 4) : 0;
   return true;
 }
 
@@ -175,7 +176,7 @@ int product(int type, Form form, Epi epi, GemmArgs p, const Plan& q, float* part
   if (q.tiles == ROWS_32 || q.tiles == ROWS_64) {
     p.ldp = epi == EPI_GATED ? 2 * p.N : p.N;
     const int cols = q.tiles == ROWS_64 ? 64 : 32;
-    if (q.splits == 1) return gemm_few(type, form, epi, p, cols, s);
+    if (q.splits == 1 || p.words) return gemm_few(type, form, epi, p, cols, s);
     GemmArgs g = p;
     g.N = p.ldp;
     VMOE_TRY(gemm_few(type, form, EPI_PARTIAL, g, cols, s));
@@ -278,6 +279,8 @@ int check_weight(int type, const void* w, int64_t ldw, int transposed, int64_t i
 using namespace vmoe;
 using namespace vmoe::dense;
 
+extern "C" int32_t vmoe_dense_arrival_words(void) { return kFewWords; }
+
 extern "C" size_t vmoe_linear_workspace_bytes(int32_t type, int64_t rows, int64_t in, int64_t out,
                                               int32_t act, int32_t backward) {
   if (check_sizes(type, act, rows, in, out) != VMOE_OK) return 0;
@@ -289,7 +292,7 @@ extern "C" int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int
                                    int32_t w_transposed, const void* bias, int32_t bias_f32,
                                    int32_t act, const void* residual, int64_t ldr, void* y,
                                    int64_t ldy, float* z, void* workspace, size_t workspace_bytes,
-                                   vmoe_stream_t stream) {
+                                   uint32_t* words, vmoe_stream_t stream) {
   VMOE_TRY(check_sizes(type, act, rows, in, out));
   if (rows == 0) return VMOE_OK;
   VMOE_TRY(check_rows(type, x, in, ldx));
@@ -297,6 +300,7 @@ extern "C" int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int
   VMOE_TRY(check_rows(type, y, out, ldy));
   if (residual) VMOE_TRY(check_rows(type, residual, out, ldr));
   if (z && !aligned(z)) return VMOE_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(words) & 3) return VMOE_ERR_UNSUPPORTED;
   VMOE_TRY(check_workspace(workspace, workspace_bytes,
                            linear_bytes(type, rows, in, out, act, 0).total));
   GemmArgs p = args(x, ldx, w, ldw, rows, out, in, y, ldy);
@@ -307,6 +311,7 @@ extern "C" int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int
   p.ldr = ldr;
   p.z = z;
   p.ldz = out;
+  p.words = words;
   return product(type, forward_form(w_transposed), EPI_LINEAR, p, static_cast<float*>(workspace),
                  reinterpret_cast<hipStream_t>(stream));
 }
@@ -380,7 +385,7 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
                                   int32_t w2_transposed, const void* bias2, int32_t bias2_f32,
                                   const void* residual, int64_t ldr, void* h, float* z, void* y,
                                   int64_t ldy, void* workspace, size_t workspace_bytes,
-                                  vmoe_stream_t stream) {
+                                  uint32_t* words, vmoe_stream_t stream) {
   VMOE_TRY(check_sizes(type, act, rows, hidden, width));
   if (rows == 0) return VMOE_OK;
   VMOE_TRY(check_rows(type, x, hidden, ldx));
@@ -390,6 +395,7 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
   VMOE_TRY(check_rows(type, y, hidden, ldy));
   if (residual) VMOE_TRY(check_rows(type, residual, hidden, ldr));
   if (z && !aligned(z)) return VMOE_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(words) & 3) return VMOE_ERR_UNSUPPORTED;
   VMOE_TRY(check_workspace(workspace, workspace_bytes,
                            gated_bytes(type, rows, hidden, width, 0).total));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -400,6 +406,7 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
   p.act = act;
   p.z = z;
   p.ldz = 2 * width;
+  p.words = words;
   VMOE_TRY(product(type, forward_form(w1_transposed), EPI_GATED, p, part, s));
   GemmArgs q = args(h, width, w2, ldw2, rows, hidden, width, y, ldy);
   q.bias = bias2;
@@ -407,6 +414,7 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
   q.act = VMOE_DENSE_NONE;
   q.res = residual;
   q.ldr = ldr;
+  q.words = words;
   return product(type, forward_form(w2_transposed), EPI_LINEAR, q, part, s);
 }
 

@@ -112,7 +112,14 @@ struct Step {
   }
 };
 
-// D: steps of a wave's batch; the next batch's loads are under way during one.
+// Sums of slices travel between XCDs, whose L2s are not coherent with one another:
+// they are written and read with device-scope cache policy (sc1).
+constexpr int kDevice = 16;
+
+// D: steps of a wave's batch; the next batch's loads are under way during one. A slice
+// of k (EPI_PARTIAL aside) leaves its sums in part [column block][slice][M][CB] and
+// counts itself in the block's arrival word, by an increment that wraps to zero at the
+// last one, which adds the slices in order. No workgroup waits for another.
 template <typename E, bool T, int EPI, int RT, int CB, int NW, int D>
 __global__ __launch_bounds__(NW * 64) void few_rows_kernel(GemmArgs p) {
   typedef Step<E, T, RT, CB> S;
@@ -191,6 +198,53 @@ __global__ __launch_bounds__(NW * 64) void few_rows_kernel(GemmArgs p) {
       for (int j = 0; j < kCols; ++j) row[T ? c * kCols + j : 16 * j + c] = acc[t][j][r];
     }
   __syncthreads();
+  if constexpr (EPI != EPI_PARTIAL)
+    if (p.splits > 1) {
+      __shared__ uint32_t arrived;
+      const int64_t block = n0 / OUT, slice_bytes = p.M * CB * 4;
+      const auto part = make_rsrc(reinterpret_cast<uint64_t>(p.part) +
+                                  (uint64_t)(block * p.splits * slice_bytes));
+      for (int id = threadIdx.x; id < (int)p.M * (CB / 4); id += NW * 64) {
+        const int m = id / (CB / 4), col = (id % (CB / 4)) * 4;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int w = 0; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(&sums[w][m][col]);
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4_t, v), part,
+            (uint32_t)(slice * slice_bytes) + (m * CB + col) * 4, 0, kDevice);
+      }
+      wait_vmcnt<0>();  // this wave's sums are at the device-coherent level
+      __syncthreads();
+      if (threadIdx.x == 0)
+        arrived = __builtin_amdgcn_atomic_inc32(p.words + block, (uint32_t)(p.splits - 1),
+                                                __ATOMIC_RELAXED, "agent");
+      __syncthreads();
+      if (arrived != (uint32_t)(p.splits - 1)) return;
+      for (int id = threadIdx.x; id < (int)p.M * (OUT / 4); id += NW * 64) {
+        const int m = id / (OUT / 4), col = (id % (OUT / 4)) * 4;
+        const int64_t n = n0 + col;
+        if (n >= p.N) continue;
+        float v[4] = {}, u[4] = {}, none[4] = {};
+#pragma unroll 4
+        for (int q = 0; q < p.splits; ++q) {
+          const uint32_t at = (uint32_t)(q * slice_bytes) + (m * CB + col) * 4;
+          const f32x4 a = __builtin_bit_cast(
+              f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, at, 0, kDevice));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] += a[i];
+          if constexpr (GATED) {
+            const f32x4 b = __builtin_bit_cast(
+                f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, at + OUT * 4, 0, kDevice));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] += b[i];
+          }
+        }
+        EpiCols<EPI, 4> cols;
+        epi_cols<EPI, 4>(p, n, cols);
+        epi_row<E, EPI, 4>(p, cols, m, n, v, u, GateUp(), none, none);
+      }
+      return;
+    }
   constexpr int kGroups = OUT / 4;
   for (int id = threadIdx.x; id < RT * 16 * kGroups; id += NW * 64) {
     const int m = id / kGroups, col = (id % kGroups) * 4;

@@ -18,6 +18,7 @@ int gemm_big(Form form, Epi epi, const GemmArgs& p, hipStream_t s);
 // dense_few.hip: at most kFewRows rows, workgroups of `cols` columns (32, or for T-form
 // weights in bf16 64)
 constexpr int64_t kFewRows = 64;
+constexpr int kFewWords = 256;  // arrival words: column blocks of a product that is split
 int gemm_few(int type, Form form, Epi epi, const GemmArgs& p, int cols, hipStream_t s);
 // dense_gemm.hip: the product on tiles; the epilogue of its split tiles; the epilogue
 // of gemm_few's slices

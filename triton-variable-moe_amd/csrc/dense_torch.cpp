@@ -9,11 +9,16 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/InferenceMode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <map>
+#include <mutex>
 
 #include "vmoe.h"
 
@@ -59,6 +64,27 @@ void call(const char* name, F&& f) {
 
 vmoe_stream_t stream_of(const Tensor& x) {
   return reinterpret_cast<vmoe_stream_t>(c10::hip::getCurrentHIPStream(x.get_device()).stream());
+}
+
+// The current stream's arrival words, for products of few rows (which alone use them):
+// zero-filled once, and every call leaves them zero. Calls on one stream run in order,
+// so they share them. A captured call gets none: its graph may be replayed on any
+// stream, beside calls or graphs of the one it was captured on.
+uint32_t* words_of(const Tensor& x, int64_t rows, size_t workspace_bytes) {
+  if (rows > 64 || !workspace_bytes) return nullptr;
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    return nullptr;
+  static std::mutex& lock = *new std::mutex;  // (never destroyed: nor is the memory freed
+  static auto& all = *new std::map<std::pair<int64_t, int64_t>, Tensor>;  // at exit)
+  const std::pair<int64_t, int64_t> key(x.get_device(),
+                                        c10::hip::getCurrentHIPStream(x.get_device()).id());
+  const std::lock_guard<std::mutex> held(lock);
+  Tensor& t = all[key];
+  if (!t.defined()) {
+    const c10::InferenceMode normal(false);
+    t = at::zeros({vmoe_dense_arrival_words()}, x.options().dtype(at::kInt));
+  }
+  return static_cast<uint32_t*>(t.mutable_data_ptr());
 }
 
 // ---------------------------------------------------------------------------
@@ -338,7 +364,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& b_, const M
     return vmoe_linear_forward(type, m.p(), m.ld, rows, in, out, wm.p(), wm.ld, wm.tr, ptr(b),
                                f32(b), act, rm.p(), rm.ld, y.mutable_data_ptr(), out,
                                z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
-                               out_ptr(ws), n, stream_of(x));
+                               out_ptr(ws), n, words_of(x, rows, n), stream_of(x));
   });
   return y;
 }
@@ -438,7 +464,8 @@ Tensor gated_forward(const Tensor& x, const Tensor& w1, const Tensor& w2, const 
                               f32(b1), act, m2.p(), m2.ld, m2.tr, ptr(b2), f32(b2), rm.p(), rm.ld,
                               h.mutable_data_ptr(),
                               z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
-                              y.mutable_data_ptr(), d, out_ptr(ws), n, stream_of(x));
+                              y.mutable_data_ptr(), d, out_ptr(ws), n, words_of(x, rows, n),
+                              stream_of(x));
   });
   return y;
 }

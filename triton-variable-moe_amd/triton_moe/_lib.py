@@ -144,17 +144,18 @@ _SIGNATURES = {
                        _vp, _i64, _vp],
     "vmoe_linear_workspace_bytes": [_i32, _i64, _i64, _i64, _i32, _i32],
     "vmoe_linear_forward": [_i32, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32,
-                            _vp, _i64, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp],
+                            _vp, _i64, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp, _vp],
     "vmoe_linear_backward": [_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _i32,
                              _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp,
                              ctypes.c_size_t, _vp],
     "vmoe_gated_workspace_bytes": [_i32, _i64, _i64, _i64, _i32],
     "vmoe_gated_forward": [_i32, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32,
                            _vp, _i64, _i32, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _vp,
-                           ctypes.c_size_t, _vp],
+                           ctypes.c_size_t, _vp, _vp],
     "vmoe_gated_backward": [_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp,
                             _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i32, _vp,
                             _i64, _vp, _i32, _vp, ctypes.c_size_t, _vp],
+    "vmoe_dense_arrival_words": [],
     "vmoe_layer_norm_max": [],
     "vmoe_layer_norm": [_i32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _i32, ctypes.c_float, _vp,
                         _i64, _vp, _vp],
