@@ -779,6 +779,20 @@ def test_few_rows_joined_in_their_launch(dtype, device):
             assert all(torch.equal(a, b) for a, b in zip(ys, want))
 
 
+def test_inference_mode_first(device):
+    """What a stream keeps is made in inference mode and used outside of it."""
+    g = gen(22)
+    x, w = rnd(g, 2, 4096, dtype=BF16), matrix(g, 4096, 64, BF16, False).requires_grad_()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        with torch.inference_mode():
+            a = K.fused_linear(x, w)
+        b = K.fused_linear(x, w)
+        b.sum().backward()
+    torch.cuda.synchronize()
+    assert a.is_inference() and torch.equal(a, b) and w.grad is not None
+
+
 def test_two_streams_at_once(device):
     """Calls on two streams share nothing."""
     p = block_params(BF16)

@@ -11,7 +11,8 @@
 // bytes are an operand of one column. Rows of x come as operands too, 16 bytes a lane
 // and tile of 16 rows; they are in cache after the first workgroup.
 //
-// Measured at one row, weights from memory, joining included, us (floor at 5.2 TB/s):
+// Measured at one row, weights from memory, joined by a second launch, us (floor at
+// 5.2 TB/s):
 // 1024 x 4096 stored [out, in] 5.0 (1.6), [in, out] 6.1; 2048 x 2048 6.6 and 6.9 (1.6);
 // 5632 x 2048 10.0 and 9.4 (4.4); gated 2048 x 5632 14.4 and 15.4 (8.9); 8192 x 8192
 // 27.5 and 28.1 (25.8). A CU draws 20 to 60 GB/s, so that weights below some 40 MB are
@@ -119,7 +120,10 @@ constexpr int kDevice = 16;
 // D: steps of a wave's batch; the next batch's loads are under way during one. A slice
 // of k (EPI_PARTIAL aside) leaves its sums in part [column block][slice][M][CB] and
 // counts itself in the block's arrival word, by an increment that wraps to zero at the
-// last one, which adds the slices in order. No workgroup waits for another.
+// last one, which adds the slices in order. No workgroup waits for another. That takes
+// 2 to 2.8 us at the end of the launch (stores to the device-coherent level, the word,
+// loads from there), about what a second launch takes the device (2.8 and the gap before
+// it), and saves the host one: 2048 x 2048, one row, 8.2 -> 6.0 us a call.
 template <typename E, bool T, int EPI, int RT, int CB, int NW, int D>
 __global__ __launch_bounds__(NW * 64) void few_rows_kernel(GemmArgs p) {
   typedef Step<E, T, RT, CB> S;
