@@ -71,8 +71,8 @@ static_assert(kCus <= kFewWords, "a split product of few rows has fewer column b
 // Few rows: whether the kernel that streams the weight takes a product, and how. Up to
 // 16 rows always (one row of 1024 x 4096: 5.0 us, on tiles 8.4); up to 64 for weights
 // of at most 32 MB (61 rows of 1024 x 4096: 9.2 and 9.7; of 8192 x 8192: 41 and 36). k
-// is split for a workgroup a CU, 512 of k or more each: 4096 x 1024 14.5 -> 7.0; not at
-// k <= 1024, where the joining costs more (1024 x 4096: 6.1 whole, 6.7 in two).
+// is split for a workgroup a CU, about 512 of k or more each (a round of the waves'
+// loads): 4096 x 1024 14.5 -> 7.0; not at k <= 1024, where the joining costs more (1024 x 4096: 6.1 whole, 6.7 in two).
 bool plan_rows(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K, Plan& q) {
   if (form == FORM_TT || epi == EPI_GATED_BWD || M > kFewRows) return false;
   const int64_t n = epi == EPI_GATED ? 2 * N : N;
@@ -83,7 +83,7 @@ bool plan_rows(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K, Pl
   q.tiles_m = 1;
   q.tiles_n = (int)cdiv(n, cols);
   const int64_t stage = 128 / esize(type);
-  const int64_t most = K <= 1024 && cols == 32 ? 1 : K / 512;
+  const int64_t most = K <= 1024 && cols == 32 ? 1 : cdiv(K, 512);
   const int64_t s = std::max<int64_t>(1, std::min<int64_t>(cdiv(kCus, q.tiles_n), most));
   q.kper = cdiv(cdiv(K, stage), s) * stage;
   q.splits = (int)cdiv(K, q.kper);  // (more than one: fewer than kFewWords column blocks)
@@ -96,9 +96,9 @@ bool plan_rows(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K, Pl
 // a whole number of times leave it partly idle at the end: the remaining ones are split
 // along k, where that is estimated to take less time with the joining (3 us and 0.22 us
 // for each MB of sums, measured at 4 to 67 MB). Of 52 products drawn over the whole
-// range those on tiles take 6 % longer than with the best of a sweep over tiles and
-// splits, those of few rows 16 % less than on tiles.
-Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
+// range those on tiles take 4 % longer than with the best of a sweep over tiles and
+// splits, those of few rows 15 % less than on tiles.
+Plan estimate(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
   Plan best = {};
   if (plan_rows(type, form, epi, M, N, K, best)) return best;
   const int64_t n = epi == EPI_GATED ? 2 * N : N;  // columns staged
@@ -108,7 +108,8 @@ Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
   for (int i = 0; i < (bf16 ? 3 : 2); ++i) {
     const Kernel& k = bf16 ? kBf16[i] : kF32[i];
     const int bn = k.tiles == TILES_64 && epi == EPI_GATED ? 128 : k.bn;
-    const float scale = bn == k.bn ? 1.0f : 1.6f;
+    const float scale = bn == k.bn ? 1.0f : 1.8f;
+    auto stage_us = [&](int residents) { return scale * k.stage[residents - 1]; };
     Plan q = {};
     q.tiles = k.tiles;
     q.tiles_m = (int)cdiv(M, k.bm);
@@ -118,24 +119,31 @@ Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
     q.kper = stages * stage;
     // rounds of k.per_cu tiles a CU, then one of `last` and the rest
     const int each = (int)(tiles / kCus), last = each % k.per_cu;
-    float time = (float)(each / k.per_cu) * ((float)stages * k.stage[k.per_cu - 1] + k.round);
+    float time = (float)(each / k.per_cu) * ((float)stages * stage_us(k.per_cu) + k.round);
     if (tiles % (kCus * k.per_cu)) {
-      float tail = (float)stages * k.stage[tiles % kCus ? last : last - 1];
+      float tail = (float)stages * stage_us(tiles % kCus ? last + 1 : last);
       q.whole = (int)tiles;
-      // `beside` of the last round's tiles stay whole, the others' slices fill r places
-      // of each CU
+      // `beside` of the last round's tiles stay whole, the others' slices fill the free
+      // places of each CU r / free times
       for (int beside = 0; beside <= last; beside += std::max(last, 1)) {
         const int rest = (int)(tiles - (int64_t)(each - last + beside) * kCus);
         if (!rest) continue;
-        const float base = beside ? (float)stages * k.stage[beside - 1] : 0.0f;
-        for (int r = 1; beside + r <= k.per_cu; ++r) {
+        const int free = k.per_cu - beside;
+        const float base = beside ? (float)stages * stage_us(beside) : 0.0f;
+        int64_t before = 0;
+        for (int r = 1; r <= 4 * free; ++r) {
           const int64_t slices = std::min<int64_t>(r * kCus / rest, stages / 4);
-          if (slices < 2) continue;
+          if (slices < 2 || slices == before) continue;
+          before = slices;
           const int64_t per = cdiv(stages, slices);
           const int units = rest * (int)cdiv(stages, per), u = (int)cdiv(units, kCus);
           const float mb = (float)units * (float)(k.bm * bn * 4) * 1e-6f;
-          const float more = k.stage[beside + u - 1] - (beside ? k.stage[beside - 1] : 0.0f);
-          const float t = base + (float)per * more + 3.0f + mb * 0.22f;
+          float t = 3.0f + mb * 0.22f;
+          if (u <= free)
+            t += base + (float)per * (stage_us(beside + u) - (beside ? stage_us(beside) : 0.0f));
+          else  // every place taken to the end
+            t += (float)(beside * stages + cdiv(u, free) * free * per) *
+                 stage_us(k.per_cu) / (float)k.per_cu;
           if (t < tail) {
             tail = t;
             q.whole = (int)(tiles - rest);
@@ -148,7 +156,6 @@ Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
     } else {
       q.whole = (int)tiles;
     }
-    time *= scale;
     const int64_t split = tiles - q.whole;
     q.part_bytes = align256((size_t)split * q.splits * k.bm * bn * 4);
     if (!best.splits || time < least) {
@@ -157,6 +164,25 @@ Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
     }
   }
   return best;
+}
+
+// The plan of a product; the last few are kept (an estimate takes 0.2 us, a backward call asks
+// for up to twelve).
+Plan plan_of(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K) {
+  struct Kept {
+    int64_t key[4];
+    Plan plan;
+  };
+  constexpr int kKept = 64;
+  static thread_local Kept kept[kKept] = {};  // (no product's key is zeros: M > 0)
+  const int64_t key[4] = {M, N, K, type + 2 * form + 6 * epi};
+  const uint64_t mix = (uint64_t)(M * 31 + N) * 31 + (uint64_t)(K * 31 + key[3]);
+  Kept& e = kept[(mix * 0x9E3779B97F4A7C15ull) >> 58];
+  if (!std::equal(key, key + 4, e.key)) {
+    e.plan = estimate(type, form, epi, M, N, K);
+    std::copy(key, key + 4, e.key);
+  }
+  return e.plan;
 }
 
 // Rows of column sums an EPI_GATED_BWD product leaves: one for each wave row (half a
