@@ -111,7 +111,8 @@ def norm_reference(x, w, b, gy, eps):
     (70, 72, "same"), (9, 511, "same"), (33, 512, "f32"), (4, 1000, "other"), (1, 1024, "none"),
     (6, 1025, "same"), (130, 2048, "f32"), (3, 2056, "same"), (7, 4095, "same"), (5, 4096, "same"),
     (3, 5000, "none"), (2, 8193, "same"), (2, 16384, "f32"), (4101, 40, "same"),
-    (2500, 260, "none"),
+    (2500, 260, "none"), (9, 7, "f32"), (300, 47, "same"), (33, 63, "other"), (40, 65, "same"),
+    (90, 129, "none"), (21, 255, "same"), (5, 509, "f32"), (3, 2049, "same"), (2, 16383, "same"),
 ])
 def test_layer_norm(rows, d, wtype, dtype, device):
     g = gen(rows * 31 + d)

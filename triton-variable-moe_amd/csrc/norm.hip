@@ -5,13 +5,16 @@
 //
 // Memory bound: a row is read once and kept in registers (fp32) for the mean, the
 // centred sum of squares and the result; statistics, gradients and sums are fp32.
-// A row belongs to 64 threads (one wave, no barrier) or, where it is long, to 256
-// or 1024; workgroups go on to further rows with the weights, and in the backward
+// A row belongs to 8, 16 or 64 threads (within a wave, no barrier) or, where it is
+// long, to 256 or 1024; workgroups go on to further rows with the weights, and in the backward
 // pass their gradients' sums, in registers. The forward pass fetches a row while the
 // one before is worked on (32768 x 2048 in bf16: 64 -> 48 us with 256 threads a row
 // instead of 64, 5.6 TB/s); the backward pass, with two streams of rows, gained
 // nothing by that (77 to 83 us, 4.9 to 5.2 TB/s). Those sums are joined in a fixed
-// order: within a workgroup, then by a launch of their own.
+// order: within a workgroup, then by a launch of their own. Rows of any length are read
+// 16 bytes at a time (see Span): 16384 x 4095 in bf16, both passes, 489 us value by
+// value, 240 so, 157 for 4096. Short rows by 8 or 16 threads instead of 64: 300000 x 47
+// forward 62 -> 18 us, 300000 x 128 62 -> 29 (5.2 TB/s).
 
 #include "dense_launch.h"
 
@@ -24,77 +27,112 @@ using dense::F32;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// VEC values of a row as they lie in memory: 16 bytes, or one value (VEC = 1).
-template <typename E, int VEC>
-struct Raw {
-  static constexpr bool kWide = VEC > 1;
-  static_assert(!kWide || VEC * E::kSize == 16, "16 bytes");
-  std::conditional_t<kWide, u32x4, typename E::Store> q;
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
-    q = *reinterpret_cast<const decltype(q)*>(static_cast<const typename E::Store*>(p) + i);
-  }
-  __device__ __forceinline__ void get(float* v) const {
-    if constexpr (!kWide) {
-      if constexpr (E::kSize == 4) v[0] = q;
-      else v[0] = bf16_to_f32(q);
-    } else if constexpr (E::kSize == 4) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(q[e]);
+template <typename E>
+constexpr int kVec = 16 / E::kSize;  // values of a chunk
+
+// A chunk of a row: 16 bytes from value i of p on. AL: rows are of whole chunks and
+// aligned to them; else chunks have the alignment of a value (rows shorter than a chunk:
+// d values, one by one).
+template <typename E, bool AL>
+struct Chunk {
+  static constexpr int V = kVec<E>;
+  typedef typename E::Store Store;
+  u32x4 q;
+
+  __device__ __forceinline__ void load(const void* p, int64_t i, int64_t d) {
+    const Store* at = static_cast<const Store*>(p) + i;
+    if constexpr (AL) {
+      q = *reinterpret_cast<const u32x4*>(at);
+    } else if (d >= V) {
+      __builtin_memcpy(&q, at, 16);
     } else {
+      Store v[V] = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < V; ++e)
+        if (e < d) v[e] = at[e];
+      __builtin_memcpy(&q, v, 16);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (V == 4) {
+        v[e] = __uint_as_float(q[e]);
+      } else {
         v[2 * e] = lo_f32(q[e]);
         v[2 * e + 1] = hi_f32(q[e]);
       }
     }
   }
+  static __device__ __forceinline__ void store(void* p, int64_t i, int64_t d,
+                                               const float (&v)[V]) {
+    Store* at = static_cast<Store*>(p) + i;
+    u32x4 q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (V == 4) q[e] = __float_as_uint(v[e]);
+      else q[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+    }
+    if constexpr (AL) {
+      *reinterpret_cast<u32x4*>(at) = q;
+    } else if (d >= V) {
+      __builtin_memcpy(at, &q, 16);
+    } else {
+      Store w[V];
+      __builtin_memcpy(w, &q, 16);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < d) at[e] = w[e];
+    }
+  }
 };
 
-// VEC values at p[i] (rows' values come as Raw): a weight, of either type.
-template <typename E, int VEC>
-__device__ __forceinline__ void load_vec(const void* p, int64_t i, float* v) {
-  if constexpr (VEC * E::kSize == 32) {
-    load_vec<E, VEC / 2>(p, i, v);
-    load_vec<E, VEC / 2>(p, i + VEC / 2, v + VEC / 2);
-  } else if constexpr (VEC * E::kSize == 8) {
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    v[0] = lo_f32(w.x);
-    v[1] = hi_f32(w.x);
-    v[2] = lo_f32(w.y);
-    v[3] = hi_f32(w.y);
-  } else {
-    Raw<E, VEC> q;
-    q.load(p, i);
-    q.get(v);
-  }
+// What chunk c of thread t covers. A row's last chunk ends at its end: where the row is
+// not of whole chunks it begins among the values of the chunk before, which it reads and
+// writes too (the same bits), but which count there (lo) in sums.
+struct Span {
+  int64_t i;   // first value
+  int lo, hi;  // those of its values that count
+  bool on;     // any
+  __device__ __forceinline__ bool counts(int e) const { return e >= lo && e < hi; }
+};
+template <typename E, int TPR, bool AL>
+__device__ __forceinline__ Span span_of(int64_t d, int c, int t) {
+  constexpr int V = kVec<E>;
+  const int64_t first = ((int64_t)c * TPR + t) * V;
+  if (AL) return {first, 0, first < d ? V : 0, first < d};
+  const int64_t i = max((int64_t)0, min(first, d - V));
+  return {i, (int)min((int64_t)V, first - i), first < d ? (int)min((int64_t)V, d - i) : 0, first < d};
 }
 
-template <typename E, int VEC>
-__device__ __forceinline__ void store_vec(void* p, int64_t i, const float* v) {
-  if constexpr (VEC == 1) {
-    if constexpr (E::kSize == 4) static_cast<float*>(p)[i] = v[0];
-    else static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_bf16(v[0]);
-  } else if constexpr (E::kSize == 4) {
+// V values of a weight from value i on, of either type.
+template <int V, bool AL>
+__device__ __forceinline__ void load_weight(const void* p, int f32, int64_t i, int64_t d,
+                                            float (&v)[V]) {
+  if constexpr (AL) {
+    if (f32) {
 #pragma unroll
-    for (int j = 0; j < VEC / 4; ++j) {
-      const f32x4 w = {v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
-      *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i + 4 * j) = w;
+      for (int h = 0; h < V / 4; ++h) {
+        const f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = w[e];
+      }
+    } else {
+      typedef uint32_t words __attribute__((ext_vector_type(V / 2)));
+      const words w = *reinterpret_cast<const words*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) {
+        v[2 * e] = lo_f32(w[e]);
+        v[2 * e + 1] = hi_f32(w[e]);
+      }
     }
-  } else if constexpr (VEC == 8) {
-    u32x4 w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = w;
   } else {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
-        make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < d)
+        v[e] = f32 ? static_cast<const float*>(p)[i + e]
+                   : bf16_to_f32(static_cast<const uint16_t*>(p)[i + e]);
   }
-}
-
-template <int VEC>
-__device__ __forceinline__ void load_weight(const void* p, int f32, int64_t i, float* v) {
-  if (f32) load_vec<F32, VEC>(p, i, v);
-  else load_vec<Bf16, VEC>(p, i, v);
 }
 
 // Sums over the TPR threads of a row, the same value in each of them. red: one
@@ -105,7 +143,7 @@ __device__ __forceinline__ void row_sums(float (&v)[Q], float (*red)[Q][16], int
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v[q] += __shfl_xor(v[q], o, 64);
+    for (int o = TPR < 64 ? TPR / 2 : 32; o > 0; o >>= 1) v[q] += __shfl_xor(v[q], o, 64);
   }
   if constexpr (TPR > 64) {
     constexpr int NW = TPR / 64;
@@ -144,64 +182,61 @@ struct NormArgs {
 template <int TPR>
 constexpr int kNormThreads = TPR < 256 ? 256 : TPR;
 
-template <typename E, int TPR, int VEC, int NCH>
+template <typename E, int TPR, int NCH, bool AL>
 __global__ __launch_bounds__(kNormThreads<TPR>) void norm_fwd_kernel(NormArgs p) {
-  constexpr int ROWS = kNormThreads<TPR> / TPR;
+  constexpr int ROWS = kNormThreads<TPR> / TPR, V = kVec<E>;
   __shared__ float red[2][1][16];
   const int t = threadIdx.x % TPR;
   int flip = 0;
-  float w[NCH][VEC], b[NCH][VEC];
+  float w[NCH][V], b[NCH][V];
+  Span span[NCH];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
-    const int64_t i = ((int64_t)c * TPR + t) * VEC;
+    span[c] = span_of<E, TPR, AL>(p.d, c, t);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
+    for (int e = 0; e < V; ++e) {
       w[c][e] = 1.0f;
       b[c][e] = 0.0f;
     }
-    if (i < p.d) {
-      if (p.w) load_weight<VEC>(p.w, p.w_f32, i, w[c]);
-      if (p.b) load_weight<VEC>(p.b, p.b_f32, i, b[c]);
+    if (span[c].on) {
+      if (p.w) load_weight<V, AL>(p.w, p.w_f32, span[c].i, p.d, w[c]);
+      if (p.b) load_weight<V, AL>(p.b, p.b_f32, span[c].i, p.d, b[c]);
     }
   }
   const float inv = 1.0f / (float)p.d;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-  Raw<E, VEC> next[NCH];
+  Chunk<E, AL> next[NCH];
   auto fetch = [&](int64_t row) {
     const typename E::Store* at = static_cast<const typename E::Store*>(p.x) + row * p.ldx;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      const int64_t i = ((int64_t)c * TPR + t) * VEC;
-      if (i < p.d) next[c].load(at, i);
-    }
+    for (int c = 0; c < NCH; ++c)
+      if (span[c].on) next[c].load(at, span[c].i, p.d);
   };
   if (r < p.rows) fetch(r);
   for (; r < p.rows; r += step) {
-    float x[NCH][VEC];
+    float x[NCH][V];
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int64_t i = ((int64_t)c * TPR + t) * VEC;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[c][e] = 0.0f;
-      if (i < p.d) next[c].get(x[c]);
+      for (int e = 0; e < V; ++e) x[c][e] = 0.0f;
+      if (span[c].on) next[c].get(x[c]);
     }
     if (r + step < p.rows) fetch(r + step);
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[0] += x[c][e];
+      for (int e = 0; e < V; ++e) s[0] += AL || span[c].counts(e) ? x[c][e] : 0.0f;
     row_sums<TPR, 1>(s, red, flip);
     const float mean = s[0] * inv;
     s[0] = 0.0f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const bool in = ((int64_t)c * TPR + t) * VEC < p.d;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
+      for (int e = 0; e < V; ++e) {
         x[c][e] -= mean;
-        s[0] += in ? x[c][e] * x[c][e] : 0.0f;
+        s[0] += (AL ? span[c].on : span[c].counts(e)) ? x[c][e] * x[c][e] : 0.0f;
       }
     }
     row_sums<TPR, 1>(s, red, flip);
@@ -211,67 +246,69 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_fwd_kernel(NormArgs p)
     typename E::Store* out = static_cast<typename E::Store*>(p.y) + r * p.ldy;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int64_t i = ((int64_t)c * TPR + t) * VEC;
-      float y[VEC];
+      float y[V];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) y[e] = x[c][e] * rstd * w[c][e] + b[c][e];
-      if (i < p.d) store_vec<E, VEC>(out, i, y);
+      for (int e = 0; e < V; ++e) y[e] = x[c][e] * rstd * w[c][e] + b[c][e];
+      if (span[c].on) Chunk<E, AL>::store(out, span[c].i, p.d, y);
     }
   }
 }
 
 // WG: gw and gb are wanted (part).
-template <typename E, int TPR, int VEC, int NCH, bool WG>
+template <typename E, int TPR, int NCH, bool AL, bool WG>
 __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p) {
-  constexpr int ROWS = kNormThreads<TPR> / TPR;
+  constexpr int ROWS = kNormThreads<TPR> / TPR, V = kVec<E>;
   __shared__ float red[2][2][16];
   const int t = threadIdx.x % TPR;
   int flip = 0;
-  float w[NCH][VEC], gw[NCH][VEC], gb[NCH][VEC];
+  float w[NCH][V], gw[NCH][V], gb[NCH][V];
+  Span span[NCH];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
-    const int64_t i = ((int64_t)c * TPR + t) * VEC;
+    span[c] = span_of<E, TPR, AL>(p.d, c, t);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
+    for (int e = 0; e < V; ++e) {
       w[c][e] = 1.0f;
       gw[c][e] = gb[c][e] = 0.0f;
     }
-    if (i < p.d && p.w) load_weight<VEC>(p.w, p.w_f32, i, w[c]);
+    if (span[c].on && p.w) load_weight<V, AL>(p.w, p.w_f32, span[c].i, p.d, w[c]);
   }
   const float inv = 1.0f / (float)p.d;
   const int64_t step = (int64_t)gridDim.x * ROWS;
-  int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-  for (; r < p.rows; r += step) {
+  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; r < p.rows; r += step) {
     const typename E::Store* row = static_cast<const typename E::Store*>(p.x) + r * p.ldx;
     const typename E::Store* grow = static_cast<const typename E::Store*>(p.gy) + r * p.ldgy;
     const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * r);
-    float x[NCH][VEC], g[NCH][VEC];
+    float x[NCH][V], g[NCH][V];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int64_t i = ((int64_t)c * TPR + t) * VEC;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
+      for (int e = 0; e < V; ++e) {
         x[c][e] = st.x;
         g[c][e] = 0.0f;
       }
-      if (i < p.d) {
-        load_vec<E, VEC>(row, i, x[c]);
-        load_vec<E, VEC>(grow, i, g[c]);
+      if (span[c].on) {
+        Chunk<E, AL> qx, qg;
+        qx.load(row, span[c].i, p.d);
+        qg.load(grow, span[c].i, p.d);
+        qx.get(x[c]);
+        qg.get(g[c]);
       }
     }
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
+      for (int e = 0; e < V; ++e) {
         x[c][e] = (x[c][e] - st.x) * st.y;
         if (WG) {
           gw[c][e] += g[c][e] * x[c][e];
           gb[c][e] += g[c][e];
         }
         g[c][e] *= w[c][e];
-        s[0] += g[c][e];
-        s[1] += g[c][e] * x[c][e];
+        const float n = AL || span[c].counts(e) ? g[c][e] : 0.0f;
+        s[0] += n;
+        s[1] += n * x[c][e];
       }
     if (p.y) {
       row_sums<TPR, 2>(s, red, flip);
@@ -279,11 +316,10 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
       typename E::Store* out = static_cast<typename E::Store*>(p.y) + r * p.ldy;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const int64_t i = ((int64_t)c * TPR + t) * VEC;
-        float y[VEC];
+        float y[V];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) y[e] = st.y * (g[c][e] - m0 - x[c][e] * m1);
-        if (i < p.d) store_vec<E, VEC>(out, i, y);
+        for (int e = 0; e < V; ++e) y[e] = st.y * (g[c][e] - m0 - x[c][e] * m1);
+        if (span[c].on) Chunk<E, AL>::store(out, span[c].i, p.d, y);
       }
     }
   }
@@ -292,23 +328,36 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
     if constexpr (ROWS == 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const int64_t i = ((int64_t)c * TPR + t) * VEC;
-        if (i < p.d) {
-          store_vec<F32, VEC>(dst, i, gw[c]);
-          store_vec<F32, VEC>(dst + p.d, i, gb[c]);
+        const int64_t i = span[c].i;
+        if constexpr (AL) {
+          if (span[c].on)
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+              *reinterpret_cast<f32x4*>(dst + i + e) =
+                  f32x4{gw[c][e], gw[c][e + 1], gw[c][e + 2], gw[c][e + 3]};
+              *reinterpret_cast<f32x4*>(dst + p.d + i + e) =
+                  f32x4{gb[c][e], gb[c][e + 1], gb[c][e + 2], gb[c][e + 3]};
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (span[c].counts(e)) {
+              dst[i + e] = gw[c][e];
+              dst[p.d + i + e] = gb[c][e];
+            }
         }
       }
     } else {
-      // the waves of a workgroup, in order
-      constexpr int D = NCH * VEC * TPR;
+      // the rows of a workgroup, in order
+      constexpr int D = NCH * V * TPR;
       __shared__ float sum[2][D];
       for (int k = 0; k < ROWS; ++k) {
         if ((int)(threadIdx.x / TPR) == k) {
 #pragma unroll
           for (int c = 0; c < NCH; ++c)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const int i = (c * VEC + e) * TPR + t;
+            for (int e = 0; e < V; ++e) {
+              const int i = (c * V + e) * TPR + t;
               sum[0][i] = k ? sum[0][i] + gw[c][e] : gw[c][e];
               sum[1][i] = k ? sum[1][i] + gb[c][e] : gb[c][e];
             }
@@ -316,11 +365,11 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
         __syncthreads();
       }
       for (int i = threadIdx.x; i < D; i += kNormThreads<TPR>) {
-        const int ce = i / TPR, c = ce / VEC, e = ce % VEC;
-        const int64_t col = ((int64_t)c * TPR + i % TPR) * VEC + e;
-        if (col < p.d) {
-          dst[col] = sum[0][i];
-          dst[p.d + col] = sum[1][i];
+        const int ce = i / TPR, c = ce / V, e = ce % V;
+        const Span q = span_of<E, TPR, AL>(p.d, c, i % TPR);
+        if (q.counts(e)) {
+          dst[q.i + e] = sum[0][i];
+          dst[p.d + q.i + e] = sum[1][i];
         }
       }
     }
@@ -330,8 +379,10 @@ __global__ __launch_bounds__(kNormThreads<TPR>) void norm_bwd_kernel(NormArgs p)
 constexpr int64_t kMaxNorm = 16384;  // 1024 threads of 16 values
 constexpr int64_t kNormGroups = 1024;  // workgroups of a backward pass: rows of its sums
 
-// Threads of a row by its length: up to 16 values a thread.
-inline int norm_threads(int64_t d) { return d <= 1024 ? 64 : d <= 4096 ? 256 : 1024; }
+// Threads of a row by its length: up to 16 values a thread (8 threads: 8).
+inline int norm_threads(int64_t d) {
+  return d <= 64 ? 8 : d <= 256 ? 16 : d <= 1024 ? 64 : d <= 4096 ? 256 : 1024;
+}
 
 inline int64_t norm_groups(int64_t rows, int tpr) {
   const int64_t per = tpr < 256 ? 256 / tpr : 1;
@@ -340,27 +391,28 @@ inline int64_t norm_groups(int64_t rows, int tpr) {
   return g < most ? g : most;
 }
 
-// f(TPR, VEC, NCH) for rows of d values; vec: the widest load that rows and
-// weights allow, in values (1, or 16 bytes).
+// f(TPR, NCH, AL) for rows of d values; al: whether rows and weights are of whole
+// aligned chunks.
 template <typename E, typename F>
-int norm_pick(int64_t d, bool vec, F&& f) {
-  constexpr int V = 16 / E::kSize;
-  const int tpr = norm_threads(d);
+int norm_pick(int64_t d, bool al, F&& f) {
+  constexpr int V = kVec<E>;
   auto width = [&](auto T) -> int {
     constexpr int TPR = decltype(T)::value;
-    auto chunks = [&](auto VEC_) -> int {
-      constexpr int VEC = decltype(VEC_)::value;
-      typedef std::integral_constant<int, TPR> I;
-      if (d <= TPR * 8) return f(I(), VEC_, std::integral_constant<int, 8 / VEC>());
-      if (d <= TPR * 16) return f(I(), VEC_, std::integral_constant<int, 16 / VEC>());
-      return VMOE_ERR_UNSUPPORTED;
+    auto chunks = [&](auto N) -> int {
+      return al ? f(T, N, std::true_type()) : f(T, N, std::false_type());
     };
-    if (vec) return chunks(std::integral_constant<int, V>());
-    return chunks(std::integral_constant<int, 1>());
+    if (d <= TPR * 8) return chunks(std::integral_constant<int, 8 / V>());
+    if constexpr (TPR > 8)
+      if (d <= TPR * 16) return chunks(std::integral_constant<int, 16 / V>());
+    return VMOE_ERR_UNSUPPORTED;
   };
-  if (tpr == 64) return width(std::integral_constant<int, 64>());
-  if (tpr == 256) return width(std::integral_constant<int, 256>());
-  return width(std::integral_constant<int, 1024>());
+  switch (norm_threads(d)) {
+    case 8: return width(std::integral_constant<int, 8>());
+    case 16: return width(std::integral_constant<int, 16>());
+    case 64: return width(std::integral_constant<int, 64>());
+    case 256: return width(std::integral_constant<int, 256>());
+    default: return width(std::integral_constant<int, 1024>());
+  }
 }
 
 int check_norm(int type, int64_t rows, int64_t d) {
@@ -399,12 +451,12 @@ extern "C" int vmoe_layer_norm(int32_t type, const void* x, int64_t ldx, int64_t
     constexpr int V = 16 / E::kSize;
     const bool vec = d % V == 0 && ldx % V == 0 && ldy % V == 0 && al16(x) && al16(y) &&
                      al16(w) && al16(b);
-    return norm_pick<E>(d, vec, [&](auto T, auto VEC, auto N) -> int {
+    return norm_pick<E>(d, vec, [&](auto T, auto N, auto AL) -> int {
       constexpr int TPR = decltype(T)::value;
       const int64_t per = TPR < 256 ? 256 / TPR : 1;
       const int64_t need = (rows + per - 1) / per;
       const uint32_t grid = (uint32_t)(need < 2048 ? need : 2048);
-      VMOE_LAUNCH((norm_fwd_kernel<E, TPR, decltype(VEC)::value, decltype(N)::value>), dim3(grid),
+      VMOE_LAUNCH((norm_fwd_kernel<E, TPR, decltype(N)::value, decltype(AL)::value>), dim3(grid),
                   dim3(kNormThreads<TPR>), 0, s, p);
       VMOE_CHECK_LAUNCH();
       return VMOE_OK;
@@ -451,13 +503,14 @@ extern "C" int vmoe_layer_norm_backward(int32_t type, const void* gy, int64_t ld
     constexpr int V = 16 / E::kSize;
     const bool vec = d % V == 0 && ldx % V == 0 && ldgy % V == 0 && (!gx || ldgx % V == 0) &&
                      al16(x) && al16(gy) && al16(gx) && al16(w);
-    return norm_pick<E>(d, vec, [&](auto T, auto VEC, auto N) -> int {
-      constexpr int TPR = decltype(T)::value, VE = decltype(VEC)::value, NC = decltype(N)::value;
+    return norm_pick<E>(d, vec, [&](auto T, auto N, auto AL) -> int {
+      constexpr int TPR = decltype(T)::value, NC = decltype(N)::value;
+      constexpr bool A = decltype(AL)::value;
       if (wg)
-        VMOE_LAUNCH((norm_bwd_kernel<E, TPR, VE, NC, true>), dim3((uint32_t)groups),
+        VMOE_LAUNCH((norm_bwd_kernel<E, TPR, NC, A, true>), dim3((uint32_t)groups),
                     dim3(kNormThreads<TPR>), 0, s, p);
       else
-        VMOE_LAUNCH((norm_bwd_kernel<E, TPR, VE, NC, false>), dim3((uint32_t)groups),
+        VMOE_LAUNCH((norm_bwd_kernel<E, TPR, NC, A, false>), dim3((uint32_t)groups),
                     dim3(kNormThreads<TPR>), 0, s, p);
       VMOE_CHECK_LAUNCH();
       return VMOE_OK;
