@@ -888,8 +888,8 @@ int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids
 /* ------------------------------------------------------------------------
  * Dense operators beside the expert layer (no counterpart in the reference):
  * layer norm, a linear layer with a fused epilogue, a gated feed-forward block.
- * type: of rows, weights and outputs. Products are exact in fp32 sums, an output
- * is rounded once; biases and the norm's weights are bf16 or fp32 on their own
+ * type: of rows, weights and outputs. Sums are fp32, an output is rounded
+ * once; biases and the norm's weights are bf16 or fp32 on their own
  * (*_f32). A weight is [in, out], or with *_transposed stored [out, in]; leading
  * dimensions are of the stored matrix, multiples of 8 (fp32: 4), at most 2^20,
  * as are in, out, hidden and width; buffers are 16-byte aligned, biases by their
@@ -953,7 +953,7 @@ int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, const void* 
 /* y = (x - mean) / sqrt(var + eps) * w + b over rows of d values, 1 to
  * vmoe_layer_norm_max(); w, b and stats may be NULL. stats [rows, 2] fp32 takes
  * mean and 1 / sqrt(var + eps). Any leading dimension (x, gy: 0, one row for all)
- * and alignment; rows of whole 16 bytes are read faster. */
+ * and alignment; rows of whole aligned 16 bytes are read faster. */
 int64_t vmoe_layer_norm_max(void);
 int vmoe_layer_norm(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t d,
                     const void* w, int32_t w_f32, const void* b, int32_t b_f32, float eps,
