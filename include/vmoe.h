@@ -913,7 +913,7 @@ int32_t vmoe_dense_arrival_words(void);
 
 /* y = act(x w + bias) + residual. bias, residual and z may be NULL; z [rows, out]
  * fp32 takes x w + bias, which the backward pass of an activation reads. That of relu
- * and relu squared reads y instead where z is NULL and there was no residual. */
+ * reads y instead where z is NULL and there was no residual. */
 size_t vmoe_linear_workspace_bytes(int32_t type, int64_t rows, int64_t in, int64_t out,
                                    int32_t act, int32_t backward);
 int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t in,

@@ -144,7 +144,8 @@ def linear_bwd(type=0, gy=P, ldgy=64, x=P, ldx=64, rows=2, i=64, o=64, w=P, ldw=
     (dict(rows=0), OK), (dict(gy=None), BAD), (dict(ldgy=56), BAD), (dict(x=None), BAD),
     (dict(w=None), BAD), (dict(ldgx=56), BAD), (dict(gx=P + 8), NOT), (dict(gw=P + 8), NOT),
     (dict(ldgw=56), BAD), (dict(act=1), BAD), (dict(act=1, z=P + 4), NOT),
-    (dict(act=3, y=P), BAD), (dict(act=2, y=P, ldy=56), BAD), (dict(act=2, y=P + 8), NOT), (dict(n=0), WS),
+    (dict(act=3, y=P), BAD), (dict(act=2, y=P), BAD), (dict(act=1, y=P, ldy=56), BAD),
+    (dict(act=1, y=P + 8), NOT), (dict(n=0), WS),
     (dict(ws=None), BAD), (dict(ws=P + 8), NOT),
     (dict(n="short"), WS),
 ])

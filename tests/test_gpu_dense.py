@@ -211,9 +211,6 @@ def linear_reference(x, w, b, r, gy, act):
         y, ty = y + r64, ty + 2 * U * (y.abs() + r64.abs())
     s, ds = slope(act, z), slope_error(act, z, dz)
     gz, tgz = g64 * s, g64.abs() * (ds + 2 * U * s.abs())
-    if act == "relu_squared" and r is None:
-        # the slope is 2 sqrt(y) of the rounded y: half of y's relative error
-        tgz = tgz + half(x) / 2 * (gz.abs() + tgz)
     rounded = tgz + (hx if act else 0.0) * (gz.abs() + tgz)  # the products' operand
     gx, gw, gb = gz @ w64.t(), x64.t() @ gz, gz.sum(0)
     tgx = rounded @ w64.abs().t() + (n + 8) * U * (gz.abs() @ w64.abs().t())
@@ -677,7 +674,7 @@ def test_forward_mode_is_refused(device):
 def test_replaced_values_are_refused_in_the_backward_pass(device):
     p = block_params(F32)
     x = rnd(gen(7), 9, 264).requires_grad_()
-    for act, residual, kept in (("relu", None, True), ("relu_squared", None, True),
+    for act, residual, kept in (("relu", None, True), ("relu_squared", None, False),
                                 ("relu", x, False), ("silu", None, False)):
         y = K.fused_linear(x, p["w"], activation=act, residual=residual)
         y.mul_(2)

@@ -358,8 +358,7 @@ extern "C" int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, 
   if (gw) VMOE_TRY(check_weight(type, gw, ldgw, w_transposed, in, out));
   const bool has_act = act != VMOE_DENSE_NONE;
   const bool from_y = has_act && !z;
-  if (from_y && act != VMOE_DENSE_RELU && act != VMOE_DENSE_RELU_SQUARED)
-    return VMOE_ERR_INVALID_ARG;
+  if (from_y && act != VMOE_DENSE_RELU) return VMOE_ERR_INVALID_ARG;
   if (from_y) VMOE_TRY(check_rows(type, y, out, ldy));
   if (z && !aligned(z)) return VMOE_ERR_UNSUPPORTED;
   const Bytes b = linear_bytes(type, rows, in, out, act, 1);

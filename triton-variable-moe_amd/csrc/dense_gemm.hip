@@ -229,10 +229,10 @@ __global__ __launch_bounds__(128) void join_rows_kernel(GemmArgs p) {
 
 // dz = gy * act'(z), rounded, and the column sums of what it stores before
 // rounding: a workgroup takes `per` rows of 256 columns, part its row of them. Where
-// the output y says what the slope is (relu: y > 0; relu squared: 2 sqrt(y), whose
-// relative error is half that of y's rounding), z is not kept: 8192 x 4096 in bf16 the
-// forward pass writes, and this one reads, 134 MB less (58 -> 37 us, 5.4 TB/s; the
-// forward product 125 -> 98). Fewer rows a workgroup where rows are few: 2051 x 2048 in
+// the output y says what the slope is (relu: y > 0), z is not kept: 8192 x 4096 in bf16
+// the forward pass writes, and this one reads, 134 MB less (58 -> 37 us, 5.4 TB/s; the
+// forward product 125 -> 98). The same for relu squared, 2 sqrt(y) of the rounded y,
+// took the weight's gradient from 2.3e-3 to 2.5e-3 off float64: not done. Fewer rows a workgroup where rows are few: 2051 x 2048 in
 // fp32 19 -> 10 us.
 enum SlopeOf { SLOPE_NONE, SLOPE_Z, SLOPE_Y };
 template <typename E, SlopeOf FROM>
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const void* gy, int64_t l
         load_c<E, 4>(static_cast<const typename E::Store*>(z) + m * ldz, n, y);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          g[i] *= act == VMOE_DENSE_RELU ? (y[i] > 0.0f ? 1.0f : y[i]) : 2.0f * sqrtf(y[i]);
+          g[i] *= y[i] > 0.0f ? 1.0f : y[i];
       }
       if constexpr (FROM != SLOPE_NONE)
         store_c<E, 4>(static_cast<typename E::Store*>(dz) + m * lddz, n, g);

@@ -26,7 +26,7 @@ int gemm_tiles(int type, Form form, Epi epi, const GemmArgs& p, Tiles tiles, hip
 int join_tiles(int type, Epi epi, const GemmArgs& p, Tiles tiles, hipStream_t s);
 int join_rows(int type, Epi epi, const GemmArgs& p, hipStream_t s);
 int64_t sum_rows(int64_t M, int64_t N);  // rows of the sums that act_grad leaves
-// (z, or for relu and relu squared y; neither: dz is gy and not written)
+// (z, or for relu y; neither: dz is gy and not written)
 int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz, const void* y,
              int64_t ldy, int act, void* dz, int64_t lddz, float* part, int64_t M, int64_t N,
              hipStream_t s);

@@ -372,8 +372,8 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& b_, const M
 struct FusedLinear : torch::autograd::Function<FusedLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b,
                         const Maybe& r, int64_t act) {
-    // relu's and relu squared's slopes follow from the output, unless a residual is in it
-    const bool from_y = !r && (act == VMOE_DENSE_RELU || act == VMOE_DENSE_RELU_SQUARED);
+    // relu's slope follows from the output, unless a residual is in it
+    const bool from_y = !r && act == VMOE_DENSE_RELU;
     Tensor z;
     Tensor y = linear_forward(x, w, b, r, (int)act, act && !from_y ? &z : nullptr);
     ctx->save_for_backward({x, w, b ? *b : Tensor(), z, from_y ? y : Tensor()});

@@ -51,8 +51,8 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     "relu", "relu_squared", "silu", "gelu" or "gelu_tanh". x and weight are bf16 or fp32
     (the same), bias either; in and out multiples of 8 (fp32: 4). Sums, bias,
     activation and residual are fp32, the output is rounded once. With an activation
-    x weight + bias is kept in fp32 for the backward pass; with relu or relu_squared and
-    no residual the output is kept instead (it must not be changed in place)."""
+    x weight + bias is kept in fp32 for the backward pass; with relu and no residual the
+    output is kept instead (it must not be changed in place)."""
     act = _ACT.get(activation)
     if act is None:
         raise ValueError(f"Unknown activation: {activation} (expected one of "
