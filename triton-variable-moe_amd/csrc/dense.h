@@ -62,6 +62,7 @@ struct GemmArgs {
   int64_t ldc;
   float* z;           // fp32 pre-activations [M, ldz] (written; EPI_GATED_BWD: read), or null
   int64_t ldz;
+  int32_t z_past;     // z goes past the caches
   float* sums;        // EPI_GATED_BWD: column sums [row blocks, 2 N], or null
   int32_t act;
   int32_t tiles_m, tiles_n;
@@ -157,6 +158,29 @@ __device__ __forceinline__ void store_c(void* row, int64_t n, const float (&v)[C
   }
 }
 
+// 4 pre-activations kept for the backward pass; `past` (see kPastCache): past the caches.
+__device__ __forceinline__ f32x4_t load_z4(const float* p, int past) {
+  const f32x4_t* q = reinterpret_cast<const f32x4_t*>(p);
+  if (!past) return *q;
+  // (the two asm statements keep the compiler from merging the branches, which would
+  // lose the hint)
+  asm volatile("");
+  const f32x4_t v = __builtin_nontemporal_load(q);
+  asm volatile("");
+  return v;
+}
+__device__ __forceinline__ void store_z4(float* p, int past, const float (&v)[4]) {
+  const f32x4_t w = {v[0], v[1], v[2], v[3]};
+  f32x4_t* q = reinterpret_cast<f32x4_t*>(p);
+  if (past) {
+    asm volatile("");
+    __builtin_nontemporal_store(w, q);
+    asm volatile("");
+  } else {
+    *q = w;
+  }
+}
+
 // C values of the bias from column n on (its address may be any multiple of its
 // type's size: a slice of a longer vector).
 template <int C>
@@ -195,8 +219,8 @@ struct GateUp {
 };
 __device__ __forceinline__ GateUp load_z(const GemmArgs& p, int64_t m, int64_t n) {
   GateUp q;
-  q.g = *reinterpret_cast<const f32x4_t*>(p.z + m * p.ldz + n);
-  q.u = *reinterpret_cast<const f32x4_t*>(p.z + m * p.ldz + p.N + n);
+  q.g = load_z4(p.z + m * p.ldz + n, p.z_past);
+  q.u = load_z4(p.z + m * p.ldz + p.N + n, p.z_past);
   return q;
 }
 
@@ -214,7 +238,7 @@ __device__ __forceinline__ void epi_row(const GemmArgs& p, const EpiCols<EPI, C>
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] += q.b[i];
     if constexpr (KEEP && C == 4)
-      if (p.z) store_c<F32, C>(p.z + m * p.ldz, n, v);
+      if (p.z) store_z4(p.z + m * p.ldz + n, p.z_past, v);
     act_switch(p.act, [&](auto A) {
 #pragma unroll
       for (int i = 0; i < C; ++i) v[i] = act1<decltype(A)::value, false>(v[i], unused);
@@ -233,8 +257,8 @@ __device__ __forceinline__ void epi_row(const GemmArgs& p, const EpiCols<EPI, C>
       u[i] += q.b2[i];
     }
     if (p.z) {
-      store_c<F32, C>(p.z + m * p.ldz, n, v);
-      store_c<F32, C>(p.z + m * p.ldz + p.N, n, u);
+      store_z4(p.z + m * p.ldz + n, p.z_past, v);
+      store_z4(p.z + m * p.ldz + p.N + n, p.z_past, u);
     }
     act_switch(p.act, [&](auto A) {
 #pragma unroll
@@ -472,7 +496,7 @@ __device__ __forceinline__ void write_tile(const GemmArgs& p, const f32x16_t (&a
           const f32x4_t a = *reinterpret_cast<lds_f32x4*>(at(r, lane % CH));
           const float v[4] = {a[0] + qz.b[0], a[1] + qz.b[1], a[2] + qz.b[2], a[3] + qz.b[3]};
           const int64_t m = m0 + 32 * i + r;
-          if (m < p.M && nz < p.N) store_c<F32, 4>(p.z + m * p.ldz, nz, v);
+          if (m < p.M && nz < p.N) store_z4(p.z + m * p.ldz + nz, p.z_past, v);
         }
       }
     }

@@ -337,6 +337,7 @@ extern "C" int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int
   p.ldr = ldr;
   p.z = z;
   p.ldz = out;
+  p.z_past = z_past(rows, out);
   p.words = words;
   return product(type, forward_form(w_transposed), EPI_LINEAR, p, static_cast<float*>(workspace),
                  reinterpret_cast<hipStream_t>(stream));
@@ -431,6 +432,7 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
   p.act = act;
   p.z = z;
   p.ldz = 2 * width;
+  p.z_past = z_past(rows, 2 * width);
   p.words = words;
   VMOE_TRY(product(type, forward_form(w1_transposed), EPI_GATED, p, part, s));
   GemmArgs q = args(h, width, w2, ldw2, rows, hidden, width, y, ldy);
@@ -478,6 +480,7 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
     p.act = act;
     p.z = const_cast<float*>(z);
     p.ldz = w2x;
+    p.z_past = z_past(rows, w2x);
     p.sums = gb1 ? sums : nullptr;
     const Form form = input_grad_form(w2_transposed);
     const Plan q = plan_of(type, form, EPI_GATED_BWD, rows, width, hidden);

@@ -230,8 +230,8 @@ __global__ __launch_bounds__(128) void join_rows_kernel(GemmArgs p) {
 // dz = gy * act'(z), rounded, and the column sums of what it stores before
 // rounding: a workgroup takes `per` rows of 256 columns, part its row of them. Where
 // the output y says what the slope is (relu: y > 0), z is not kept: 8192 x 4096 in bf16
-// the forward pass writes, and this one reads, 134 MB less (58 -> 37 us, 5.4 TB/s; the
-// forward product 125 -> 98). The same for relu squared, 2 sqrt(y) of the rounded y,
+// the forward pass writes, and this one reads, 134 MB less (55 -> 37 us, 5.4 TB/s; the
+// forward product 118 -> 98). The same for relu squared, 2 sqrt(y) of the rounded y,
 // took the weight's gradient from 2.3e-3 to 2.5e-3 off float64: not done. Fewer rows a workgroup where rows are few: 2051 x 2048 in
 // fp32 19 -> 10 us.
 enum SlopeOf { SLOPE_NONE, SLOPE_Z, SLOPE_Y };
@@ -239,7 +239,7 @@ template <typename E, SlopeOf FROM>
 __global__ __launch_bounds__(256) void act_grad_kernel(const void* gy, int64_t ldgy,
                                                        const void* z, int64_t ldz, int act,
                                                        void* dz, int64_t lddz, float* part,
-                                                       int64_t M, int64_t N, int per) {
+                                                       int64_t M, int64_t N, int per, int past) {
   __shared__ float red[4][256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n = (int64_t)blockIdx.x * 256 + lane * 4;
@@ -252,8 +252,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const void* gy, int64_t l
       float g[4];
       load_c<E, 4>(static_cast<const typename E::Store*>(gy) + m * ldgy, n, g);
       if constexpr (FROM == SLOPE_Z) {
-        float x[4];
-        load_c<F32, 4>(static_cast<const float*>(z) + m * ldz, n, x);
+        const f32x4_t x = load_z4(static_cast<const float*>(z) + m * ldz + n, past);
         act_switch(act, [&](auto A) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -406,18 +405,18 @@ int act_grad(int type, const void* gy, int64_t ldgy, const float* z, int64_t ldz
              int64_t ldy, int act, void* dz, int64_t lddz, float* part, int64_t M, int64_t N,
              hipStream_t s) {
   const dim3 grid((uint32_t)((N + 255) / 256), (uint32_t)sum_rows(M, N));
-  const int per = act_grad_rows(M, N);
+  const int per = act_grad_rows(M, N), past = z_past(M, N);
   auto go = [&](auto e) {
     typedef decltype(e) E;
     if (z)
       VMOE_LAUNCH((act_grad_kernel<E, SLOPE_Z>), grid, dim3(256), 0, s, gy, ldgy, z, ldz, act, dz,
-                  lddz, part, M, N, per);
+                  lddz, part, M, N, per, past);
     else if (y)
       VMOE_LAUNCH((act_grad_kernel<E, SLOPE_Y>), grid, dim3(256), 0, s, gy, ldgy, y, ldy, act, dz,
-                  lddz, part, M, N, per);
+                  lddz, part, M, N, per, past);
     else
       VMOE_LAUNCH((act_grad_kernel<E, SLOPE_NONE>), grid, dim3(256), 0, s, gy, ldgy, z, ldz, act,
-                  dz, lddz, part, M, N, per);
+                  dz, lddz, part, M, N, per, past);
   };
   if (type == VMOE_DENSE_F32) go(F32());
   else go(Bf16());

@@ -9,6 +9,13 @@ namespace dense {
 enum Form { FORM_KK, FORM_KT, FORM_TT };  // A's, B's
 enum Tiles { ROWS_32, ROWS_64, TILES_64, TILES_128, TILES_256 };  // ROWS: dense_few.hip
 
+// Pre-activations of 64 MB or more are written and read past the caches: a pass reads
+// them once, and the last-level cache (256 MB) keeps what the next launches read
+// (8192 x 1024 x 4096, 134 MB: 337 -> 321 us a training pass; 16384 x 2048 x 8192 gated,
+// 1 GB: 4870 -> 4797; 2051 x 768 x 2048, 17 MB, lost by it: 214 -> 219).
+constexpr int64_t kPastCache = 64 << 20;
+inline int z_past(int64_t rows, int64_t cols) { return rows * cols * 4 >= kPastCache; }
+
 inline uint32_t workgroups(const GemmArgs& p) {
   return (uint32_t)(p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.splits);
 }
