@@ -313,9 +313,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(uint64_t a) {
 }
 
 // (inline asm, so that the compiler does not wait for the DMA before every LDS
-// read; no register output, M0 declared clobbered)
+// read; no register output, M0 declared clobbered. A load to LDS may read M0 one wait
+// state after its write at the earliest: s_nop, as the compiler puts it)
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                ::"v"(voff), "s"(r), "s"(lds) : "memory", "m0");
 }
 

@@ -386,9 +386,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base,
 // any LDS read it cannot prove disjoint, which empties the ring. The kernels
 // order DMA completion themselves with wait_vmcnt + block_barrier. The asm
 // has no register outputs (the data goes to LDS), so no register is written
-// behind the compiler's back; M0 is declared clobbered.
+// behind the compiler's back; M0 is declared clobbered. A load to LDS may read
+// M0 one wait state after its write at the earliest: s_nop, as the compiler
+// puts it between the two.
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                :: "v"(voff), "s"(r), "s"(lds) : "memory", "m0");
 }
 
@@ -396,7 +398,7 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, u
 // windows of the T-form gather), under the same rules as dma16.
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t voff, lds_char* dst) {
   const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(dst));
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
                :: "v"(voff), "s"(r), "s"(lds) : "memory", "m0");
 }
 

@@ -58,9 +58,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base) {
 }
 
 // 16 bytes per lane into LDS at lds + 16 * lane; the data never passes through
-// registers, so completion is ordered by the waits in the loop.
+// registers, so completion is ordered by the waits in the loop (s_nop: the wait
+// state between a write of M0 and a load to LDS).
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                :: "v"(voff), "s"(r), "s"(lds) : "memory", "m0");
 }
 
