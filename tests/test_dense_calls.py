@@ -1,0 +1,69 @@
+"""Calls of the dense operators that are settled on the host."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from triton_moe import kernels as K
+
+
+class Wrapper(torch.Tensor):
+    """A tensor whose values are in another one, as a distributed tensor's are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, strides=inner.stride(),
+                                                   dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        args = [a.inner if isinstance(a, Wrapper) else a for a in args]
+        return func(*args, **(kwargs or {}))
+
+
+def freed(t):
+    t = t.clone(memory_format=torch.contiguous_format)
+    t.untyped_storage().resize_(0)
+    return t
+
+
+def freed_slice(t):
+    """(its address is not 0)"""
+    flat = torch.zeros(t.numel() + 64, dtype=t.dtype, device=t.device)
+    out = flat[64:].view(t.shape)
+    flat.untyped_storage().resize_(0)
+    return out
+
+
+def cut(t):
+    t = t.clone(memory_format=torch.contiguous_format)
+    t.untyped_storage().resize_(t.numel() * t.element_size() - 1)
+    return t
+
+
+WITHOUT_MEMORY = [Wrapper, freed, freed_slice, cut]
+
+
+def calls(x, w, v, of):
+    """(operand, call) with one operand as `of` gives it; w [8, 8], v [8]."""
+    wide, w2, v2 = torch.cat([w, w], 1), w, torch.cat([v, v])
+    return [("weight", lambda: K.layer_norm(x, of(v), v)), ("bias", lambda: K.layer_norm(x, v, of(v))),
+            ("weight", lambda: K.fused_linear(x, of(w))), ("bias", lambda: K.fused_linear(x, w, of(v))),
+            ("residual", lambda: K.fused_linear(x, w, v, "relu", of(x))),
+            ("w1", lambda: K.gated_mlp(x, of(wide), w2)), ("w2", lambda: K.gated_mlp(x, wide, of(w2))),
+            ("bias1", lambda: K.gated_mlp(x, wide, w2, bias1=of(v2))),
+            ("bias2", lambda: K.gated_mlp(x, wide, w2, bias2=of(v))),
+            ("residual", lambda: K.gated_mlp(x, wide, w2, residual=of(x)))]
+
+
+@pytest.mark.parametrize("of", WITHOUT_MEMORY)
+def test_operands_without_memory(of):
+    """An operand whose values are elsewhere, or gone, is refused: it does not count as
+    not given."""
+    for what, call in calls(torch.zeros(3, 8), torch.zeros(8, 8), torch.zeros(8), of):
+        with pytest.raises(NotImplementedError, match=f"{what} has no memory"):
+            call()

@@ -95,9 +95,24 @@ void check_type(const Tensor& t, const char* what) {
                               " must be bfloat16 or float32 (got ", t.scalar_type(), ")");
   TORCH_CHECK_NOT_IMPLEMENTED(t.layout() == at::kStrided, what, " must be a strided tensor");
 }
+// A tensor's values may be elsewhere (a wrapper's, such as a distributed tensor's) or
+// gone (a freed storage): its address is then no address, and the C entry points read
+// NULL as "not given".
+bool in_memory(const Tensor& t) {
+  if (t.numel() == 0) return true;
+  if (!t.has_storage()) return false;
+  const at::Storage& s = t.storage();
+  return s.data() && at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.element_size(),
+                                                      t.storage_offset()) <= s.nbytes();
+}
+void check_memory(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(in_memory(t), what, " has no memory here (the values of a wrapper, or "
+                              "a storage that was freed)");
+}
 // x, after the checks that need no device
 void check_device(const Tensor& x) {
   if (!x.is_cuda()) throw NotOnGpu{"x must be on CUDA"};
+  check_memory(x, "x");
 }
 void check_like(const Tensor& t, const char* what, const Tensor& x) {
   TORCH_CHECK_VALUE(t.scalar_type() == x.scalar_type(), what, " must have x's type, ",
@@ -105,6 +120,7 @@ void check_like(const Tensor& t, const char* what, const Tensor& x) {
   TORCH_CHECK_VALUE(t.device() == x.device(), what, " must be on x's device, ", x.device(),
                     " (got ", t.device(), ")");
   TORCH_CHECK_NOT_IMPLEMENTED(t.layout() == at::kStrided, what, " must be a strided tensor");
+  check_memory(t, what);
 }
 void check_vector(const Maybe& v, const char* what, int64_t n, const Tensor& x) {
   if (!v) return;
@@ -113,6 +129,7 @@ void check_vector(const Maybe& v, const char* what, int64_t n, const Tensor& x) 
   check_type(*v, what);
   TORCH_CHECK_VALUE(v->device() == x.device(), what, " must be on x's device, ", x.device(),
                     " (got ", v->device(), ")");
+  check_memory(*v, what);
 }
 void check_residual(const Maybe& r, at::IntArrayRef shape, const Tensor& x) {
   if (!r) return;
@@ -138,6 +155,13 @@ int type_of(const Tensor& x) {
 int f32(const Maybe& v) { return v && v->scalar_type() == at::kFloat; }
 int f32(const Tensor& v) { return v.defined() && v.scalar_type() == at::kFloat; }
 const void* ptr(const Maybe& v) { return v ? v->const_data_ptr() : nullptr; }
+// What a forward pass has saved.
+const void* saved_ptr(const Tensor& v) {
+  if (!v.defined()) return nullptr;
+  check_memory(v, "a saved tensor");
+  return v.const_data_ptr();
+}
+const float* saved_floats(const Tensor& v) { return static_cast<const float*>(saved_ptr(v)); }
 void* out_ptr(const Tensor& v) { return v.defined() ? v.mutable_data_ptr() : nullptr; }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
 
@@ -150,8 +174,12 @@ struct Mat {
 };
 
 Tensor fresh(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
-// (a view that stands for its negative, as of a conjugate's imaginary part)
-Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+// A view that stands for its negative, as of a conjugate's imaginary part, gets memory
+// of its own. (The check again: backward passes read saved tensors and a given gradient.)
+Tensor plain(const Tensor& t) {
+  check_memory(t, "an operand");
+  return t.is_neg() ? t.resolve_neg() : t;
+}
 
 // t as rows of `cols` values, contiguous and 16-byte aligned: in place, or a copy.
 Mat rows_of(const Tensor& given, int64_t cols) {
@@ -314,9 +342,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const Tensor ws = workspace(n, x);
         call("vmoe_layer_norm_backward", [&] {
           return vmoe_layer_norm_backward(
-              type_of(x), g.p(), g.ld, m.p(), m.ld, rows, d, ptr(w), f32(w),
-              static_cast<const float*>(stats.const_data_ptr()), out_ptr(gx), d, out_ptr(gw),
-              f32(gw), out_ptr(gb), f32(gb), out_ptr(ws), n, stream_of(x));
+              type_of(x), g.p(), g.ld, m.p(), m.ld, rows, d, ptr(w), f32(w), saved_floats(stats),
+              out_ptr(gx), d, out_ptr(gw), f32(gw), out_ptr(gb), f32(gb), out_ptr(ws), n,
+              stream_of(x));
         });
       }
       out[0] = gx;
@@ -409,9 +437,8 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
           call("vmoe_linear_backward", [&] {
             return vmoe_linear_backward(
                 type, g.p(), g.ld, m.p(), m.ld, rows, in, n_out, wm.p(), wm.ld, wm.tr, act,
-                z.defined() ? static_cast<const float*>(z.const_data_ptr()) : nullptr,
-                y.defined() ? y.const_data_ptr() : nullptr, n_out, out_ptr(gx), in, out_ptr(gw),
-                ld_of(gw, wm.tr), out_ptr(gb), f32(gb), out_ptr(ws), n, stream_of(x));
+                saved_floats(z), saved_ptr(y), n_out, out_ptr(gx), in, out_ptr(gw), ld_of(gw, wm.tr),
+                out_ptr(gb), f32(gb), out_ptr(ws), n, stream_of(x));
           });
         }
         out[0] = gx;
@@ -510,10 +537,10 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
           call("vmoe_gated_backward", [&] {
             return vmoe_gated_backward(
                 type, g.p(), g.ld, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, m1.tr, m2.p(),
-                m2.ld, m2.tr, (int)ctx->saved_data["act"].toInt(), h.const_data_ptr(),
-                static_cast<const float*>(z.const_data_ptr()), out_ptr(gx), d, out_ptr(gw1),
-                ld_of(gw1, m1.tr), out_ptr(gb1), f32(gb1), out_ptr(gw2), ld_of(gw2, m2.tr),
-                out_ptr(gb2), f32(gb2), out_ptr(ws), n, stream_of(x));
+                m2.ld, m2.tr, (int)ctx->saved_data["act"].toInt(), saved_ptr(h), saved_floats(z),
+                out_ptr(gx), d, out_ptr(gw1), ld_of(gw1, m1.tr), out_ptr(gb1), f32(gb1),
+                out_ptr(gw2), ld_of(gw2, m2.tr), out_ptr(gb2), f32(gb2), out_ptr(ws), n,
+                stream_of(x));
           });
         }
         out[0] = gx;
