@@ -101,8 +101,11 @@ __device__ __forceinline__ float act1(float z, float& slope) {
   } else if constexpr (ACT == VMOE_DENSE_GELU_TANH) {
     // (1 + tanh v) / 2 = sigmoid(2 v), v = sqrt(2 / pi) (z + 0.044715 z^3)
     const float s = sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
-    if (SLOPE)
-      slope = s + z * (s * (1.0f - s)) * (1.5957691216057308f * (1.0f + 0.134145f * z * z));
+    if (SLOPE) {
+      // (z^2 must not overflow: beyond 64 s (1 - s) is 0)
+      const float c = fminf(fabsf(z), 64.0f);
+      slope = s + z * (s * (1.0f - s)) * (1.5957691216057308f * (1.0f + 0.134145f * c * c));
+    }
     return z * s;
   } else {
     if (SLOPE) slope = 1.0f;
