@@ -2,9 +2,15 @@
 
 from __future__ import annotations
 
+import os
+import shutil
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from triton_moe import _lib
 from triton_moe import kernels as K
 
 
@@ -67,3 +73,42 @@ def test_operands_without_memory(of):
     for what, call in calls(torch.zeros(3, 8), torch.zeros(8, 8), torch.zeros(8), of):
         with pytest.raises(NotImplementedError, match=f"{what} has no memory"):
             call()
+
+
+def run_python(code, **env):
+    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          env={**os.environ, **env})
+
+
+def test_library_of_another_place(tmp_path):
+    """VMOE_LIB names the one library of the process: the dense operators call it too, and
+    need none in the package's directory."""
+    package = tmp_path / "package" / "triton_moe"
+    here = _lib.LIB_PATH.parent
+    shutil.copytree(here, package, ignore=shutil.ignore_patterns("libvmoe.so", "__pycache__"))
+    library = tmp_path / "elsewhere.so"
+    shutil.copy(_lib.LIB_PATH, library)
+    for path in (package.parent, here.parent):
+        out = run_python("import sys; sys.path.insert(0, %r)\n"
+                         "from triton_moe import _lib, kernels\n"
+                         "import torch\n"
+                         "_lib.dense()\n"
+                         "try: kernels.layer_norm(torch.zeros(1, kernels.layer_norm_max() + 1))\n"
+                         "except NotImplementedError as e: print(e)\n"
+                         "names = {l.split()[-1] for l in open('/proc/self/maps') if '/' in l}\n"
+                         "print(sorted(n for n in names if 'vmoe' in n or 'elsewhere' in n))\n"
+                         % str(path), VMOE_LIB=str(library))
+        assert out.returncode == 0, out.stderr
+        assert "rows of at most 16384" in out.stdout
+        assert out.stdout.strip().endswith(f"['{library}']"), out.stdout
+
+
+def test_module_without_a_library():
+    """The extension module by itself calls nothing."""
+    out = run_python("import sys, torch; sys.path.insert(0, %r)\n"
+                     "from triton_moe import _dense\n"
+                     "try: _dense.layer_norm(torch.zeros(1, 8), None, None, 1e-5)\n"
+                     "except RuntimeError as e: print(e)\n"
+                     "try: _dense.use(0)\n"
+                     "except RuntimeError as e: print(e)\n" % str(_lib.LIB_PATH.parent.parent))
+    assert out.returncode == 0 and out.stdout.count("library") == 2, out.stdout + out.stderr

@@ -89,8 +89,7 @@ def _compile_dense() -> Path:
 def _link_dense(obj: Path) -> None:
     tmp = DENSE.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-shared", str(obj), "-o", str(tmp),
-           f"-L{OUT.parent}", f"-l:{OUT.name}", f"-L{_torch_dir() / 'lib'}", "-lc10", "-lc10_hip",
-           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           f"-L{_torch_dir() / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ldl"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")

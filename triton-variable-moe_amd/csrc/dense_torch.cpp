@@ -7,6 +7,7 @@
 // rows 117 us, with 4 and 24 us of kernels.
 
 #include <Python.h>
+#include <dlfcn.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/InferenceMode.h>
@@ -37,7 +38,29 @@ struct NotOnGpu {
 };
 
 // ---------------------------------------------------------------------------
-// Calls of the library.
+// Calls of the library: the one that the package has loaded (use(), below), which need
+// not be the one beside this module.
+
+#define VMOE_ENTRIES(ENTRY)                                                          \
+  ENTRY(vmoe_status_string)                                                          \
+  ENTRY(vmoe_layer_norm_max)                                                         \
+  ENTRY(vmoe_layer_norm)                                                             \
+  ENTRY(vmoe_layer_norm_workspace_bytes)                                             \
+  ENTRY(vmoe_layer_norm_backward)                                                    \
+  ENTRY(vmoe_dense_arrival_words)                                                    \
+  ENTRY(vmoe_linear_workspace_bytes)                                                 \
+  ENTRY(vmoe_linear_forward)                                                         \
+  ENTRY(vmoe_linear_backward)                                                        \
+  ENTRY(vmoe_gated_workspace_bytes)                                                  \
+  ENTRY(vmoe_gated_forward)                                                          \
+  ENTRY(vmoe_gated_backward)
+
+struct Library {
+  bool loaded = false;
+#define VMOE_ENTRY(name) decltype(&::name) name = nullptr;
+  VMOE_ENTRIES(VMOE_ENTRY)
+#undef VMOE_ENTRY
+} lib;
 
 PyObject* g_timer = nullptr;  // observer of launches (begin(name), end(name)), or null
 
@@ -56,7 +79,7 @@ void call(const char* name, F&& f) {
   const int status = f();
   if (seen) observe("end", name);
   if (status == VMOE_OK) return;
-  const char* what = vmoe_status_string(status);
+  const char* what = lib.vmoe_status_string(status);
   TORCH_CHECK_NOT_IMPLEMENTED(status != VMOE_ERR_UNSUPPORTED, name, ": ", what);
   TORCH_CHECK_VALUE(status != VMOE_ERR_INVALID_ARG, name, ": ", what);
   TORCH_CHECK(false, name, ": ", what, " (status ", status, ")");
@@ -82,7 +105,7 @@ uint32_t* words_of(const Tensor& x, int64_t rows, size_t workspace_bytes) {
   Tensor& t = all[key];
   if (!t.defined()) {
     const c10::InferenceMode normal(false);
-    t = at::zeros({vmoe_dense_arrival_words()}, x.options().dtype(at::kInt));
+    t = at::zeros({lib.vmoe_dense_arrival_words()}, x.options().dtype(at::kInt));
   }
   return static_cast<uint32_t*>(t.mutable_data_ptr());
 }
@@ -304,7 +327,7 @@ Tensor norm_forward(const Tensor& x, const Maybe& w_, const Maybe& b_, double ep
   Tensor y = empty(x.sizes(), x);
   if (stats) *stats = empty_f32({rows, 2}, x);
   call("vmoe_layer_norm", [&] {
-    return vmoe_layer_norm(type_of(x), m.p(), m.ld, rows, d, ptr(w), f32(w), ptr(b), f32(b),
+    return lib.vmoe_layer_norm(type_of(x), m.p(), m.ld, rows, d, ptr(w), f32(w), ptr(b), f32(b),
                            (float)eps, y.mutable_data_ptr(), d,
                            stats ? static_cast<float*>(stats->mutable_data_ptr()) : nullptr,
                            stream_of(x));
@@ -338,10 +361,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         zero({gw, gb});
       } else {
         const Mat m = norm_rows(x, d), g = norm_rows(gy, d);
-        const size_t n = need[1] || need[2] ? vmoe_layer_norm_workspace_bytes(rows, d) : 0;
+        const size_t n = need[1] || need[2] ? lib.vmoe_layer_norm_workspace_bytes(rows, d) : 0;
         const Tensor ws = workspace(n, x);
         call("vmoe_layer_norm_backward", [&] {
-          return vmoe_layer_norm_backward(
+          return lib.vmoe_layer_norm_backward(
               type_of(x), g.p(), g.ld, m.p(), m.ld, rows, d, ptr(w), f32(w), saved_floats(stats),
               out_ptr(gx), d, out_ptr(gw), f32(gw), out_ptr(gb), f32(gb), out_ptr(ws), n,
               stream_of(x));
@@ -360,7 +383,7 @@ Tensor layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
   TORCH_CHECK_VALUE(x.dim() > 0, "x must have at least one dimension");
   const int64_t d = x.size(-1);
   TORCH_CHECK_VALUE(d > 0, "the last dimension of x must not be empty");
-  TORCH_CHECK_NOT_IMPLEMENTED(d <= vmoe_layer_norm_max(), "rows of at most ", vmoe_layer_norm_max(),
+  TORCH_CHECK_NOT_IMPLEMENTED(d <= lib.vmoe_layer_norm_max(), "rows of at most ", lib.vmoe_layer_norm_max(),
                               " values (got ", d, ")");
   check_vector(w, "weight", d, x);
   check_vector(b, "bias", d, x);
@@ -386,10 +409,10 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& b_, const M
   Tensor y = empty(shape, x);
   if (z) *z = empty_f32({rows, out}, x);
   const int type = type_of(x);
-  const size_t n = vmoe_linear_workspace_bytes(type, rows, in, out, act, 0);
+  const size_t n = lib.vmoe_linear_workspace_bytes(type, rows, in, out, act, 0);
   const Tensor ws = workspace(n, x);
   call("vmoe_linear_forward", [&] {
-    return vmoe_linear_forward(type, m.p(), m.ld, rows, in, out, wm.p(), wm.ld, wm.tr, ptr(b),
+    return lib.vmoe_linear_forward(type, m.p(), m.ld, rows, in, out, wm.p(), wm.ld, wm.tr, ptr(b),
                                f32(b), act, rm.p(), rm.ld, y.mutable_data_ptr(), out,
                                z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
                                out_ptr(ws), n, words_of(x, rows, n), stream_of(x));
@@ -432,10 +455,10 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
           const Mat m = rows_of(x, in), g = rows_of(gy, n_out);
           const int64_t rows = m.t.size(0);
           const int type = type_of(x);
-          const size_t n = vmoe_linear_workspace_bytes(type, rows, in, n_out, act, 1);
+          const size_t n = lib.vmoe_linear_workspace_bytes(type, rows, in, n_out, act, 1);
           const Tensor ws = workspace(n, x);
           call("vmoe_linear_backward", [&] {
-            return vmoe_linear_backward(
+            return lib.vmoe_linear_backward(
                 type, g.p(), g.ld, m.p(), m.ld, rows, in, n_out, wm.p(), wm.ld, wm.tr, act,
                 saved_floats(z), saved_ptr(y), n_out, out_ptr(gx), in, out_ptr(gw), ld_of(gw, wm.tr),
                 out_ptr(gb), f32(gb), out_ptr(ws), n, stream_of(x));
@@ -484,10 +507,10 @@ Tensor gated_forward(const Tensor& x, const Tensor& w1, const Tensor& w2, const 
   h = empty({rows, width}, x);
   if (z) *z = empty_f32({rows, 2 * width}, x);
   const int type = type_of(x);
-  const size_t n = vmoe_gated_workspace_bytes(type, rows, d, width, 0);
+  const size_t n = lib.vmoe_gated_workspace_bytes(type, rows, d, width, 0);
   const Tensor ws = workspace(n, x);
   call("vmoe_gated_forward", [&] {
-    return vmoe_gated_forward(type, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, m1.tr, ptr(b1),
+    return lib.vmoe_gated_forward(type, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, m1.tr, ptr(b1),
                               f32(b1), act, m2.p(), m2.ld, m2.tr, ptr(b2), f32(b2), rm.p(), rm.ld,
                               h.mutable_data_ptr(),
                               z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
@@ -532,10 +555,10 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
           const Mat m = rows_of(x, d), g = rows_of(gy, d);
           const int64_t rows = m.t.size(0);
           const int type = type_of(x);
-          const size_t n = vmoe_gated_workspace_bytes(type, rows, d, width, 1);
+          const size_t n = lib.vmoe_gated_workspace_bytes(type, rows, d, width, 1);
           const Tensor ws = workspace(n, x);
           call("vmoe_gated_backward", [&] {
-            return vmoe_gated_backward(
+            return lib.vmoe_gated_backward(
                 type, g.p(), g.ld, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, m1.tr, m2.p(),
                 m2.ld, m2.tr, (int)ctx->saved_data["act"].toInt(), saved_ptr(h), saved_floats(z),
                 out_ptr(gx), d, out_ptr(gw1), ld_of(gw1, m1.tr), out_ptr(gb1), f32(gb1),
@@ -604,6 +627,7 @@ struct NoGil {
 template <typename F>
 PyObject* guarded(F&& f) {
   HANDLE_TH_ERRORS
+  TORCH_CHECK(lib.loaded, "no library in use");
   try {
     const auto run = f();
     Tensor y;
@@ -655,6 +679,23 @@ PyObject* py_gated_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {
             act] { return gated_mlp(x, w1, w2, b1, b2, r, (int)act); };
   });
 }
+// use(handle): calls go to the library that dlopen gave this handle for.
+PyObject* py_use(PyObject*, PyObject* handle) {
+  HANDLE_TH_ERRORS
+  void* h = PyLong_AsVoidPtr(handle);
+  if (PyErr_Occurred()) return nullptr;
+  TORCH_CHECK(h, "no handle of a library");
+  Library found;
+#define VMOE_ENTRY(name)                                               \
+  found.name = reinterpret_cast<decltype(&::name)>(dlsym(h, #name));   \
+  TORCH_CHECK(found.name, "the library has no " #name);
+  VMOE_ENTRIES(VMOE_ENTRY)
+#undef VMOE_ENTRY
+  found.loaded = true;
+  lib = found;
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
 PyObject* py_set_timer(PyObject*, PyObject* timer) {
   Py_XINCREF(timer == Py_None ? nullptr : timer);
   Py_XDECREF(g_timer);
@@ -666,6 +707,7 @@ PyMethodDef kMethods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))py_layer_norm, METH_FASTCALL, nullptr},
     {"fused_linear", (PyCFunction)(void (*)(void))py_fused_linear, METH_FASTCALL, nullptr},
     {"gated_mlp", (PyCFunction)(void (*)(void))py_gated_mlp, METH_FASTCALL, nullptr},
+    {"use", py_use, METH_O, nullptr},
     {"set_timer", py_set_timer, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dense", nullptr, -1, kMethods,

@@ -230,12 +230,13 @@ def dense():
     global _dense
     if _dense is not None:
         return _dense
-    lib()
+    library = lib()
     try:
         from . import _dense as module
     except ImportError as exc:
         raise RuntimeError(f"triton_moe._dense unavailable ({exc}); build it with "
                            "`python triton-variable-moe_amd/build.py`") from exc
+    module.use(library._handle)  # (VMOE_LIB may name another one than the package's)
     module.set_timer(_launch_timer)
     _dense = module
     return module
