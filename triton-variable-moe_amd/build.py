@@ -4,7 +4,8 @@ extension module that calls the dense operators of it from torch).
 Usage: python triton-variable-moe_amd/build.py [--jobs N]
 
 Both are written into the Python package (triton_moe/) so that it finds them without
-an install step.
+an install step. libvmoe.so needs hipcc alone; without torch's headers or a C++ compiler
+it is built without the extension module.
 """
 
 from __future__ import annotations
@@ -63,9 +64,24 @@ def _compile(src: str) -> Path:
 
 def _torch_dir() -> Path:
     spec = importlib.util.find_spec("torch")  # (found, not imported)
-    if spec is None:
+    if spec is None or spec.origin is None:
         raise RuntimeError("torch not found")
     return Path(spec.origin).parent
+
+
+def _dense_lacks() -> str | None:
+    """What the extension module would need and is not there."""
+    compiler = os.environ.get("CXX", "g++")
+    if shutil.which(compiler) is None:
+        return f"no C++ compiler ({compiler})"
+    try:
+        torch = _torch_dir()
+    except RuntimeError as exc:
+        return str(exc)
+    for header in (torch / "include/ATen/ATen.h", Path(sysconfig.get_paths()["include"]) / "Python.h"):
+        if not header.exists():
+            return f"no {header}"
+    return None
 
 
 def _compile_dense() -> Path:
@@ -98,8 +114,9 @@ def _link_dense(obj: Path) -> None:
 
 def build(jobs: int = 4, verbose: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
+    lacks = _dense_lacks()
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
-        dense = ex.submit(_compile_dense)
+        dense = None if lacks else ex.submit(_compile_dense)
         objs = list(ex.map(_compile, SOURCES))
     tmp = OUT.with_suffix(".so.tmp")
     cmd = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
@@ -107,9 +124,14 @@ def build(jobs: int = 4, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, OUT)
-    _link_dense(dense.result())
+    if dense:
+        _link_dense(dense.result())
+    else:
+        DENSE.unlink(missing_ok=True)  # (of an earlier build)
+        print(f"{DENSE.name} is not built: {lacks}; the dense operators need it",
+              file=sys.stderr)
     if verbose:
-        print(f"built {OUT}, {DENSE}")
+        print(f"built {OUT}" + (f", {DENSE}" if dense else ""))
     return OUT
 
 
