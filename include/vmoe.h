@@ -921,7 +921,8 @@ int vmoe_linear_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, 
                         const void* bias, int32_t bias_f32, int32_t act, const void* residual,
                         int64_t ldr, void* y, int64_t ldy, float* z, void* workspace,
                         size_t workspace_bytes, uint32_t* words, vmoe_stream_t stream);
-/* Gradients of x, w (in w's order) and bias; each may be NULL. */
+/* Gradients of x, w (in w's order) and bias; each may be NULL, and so may x without gw
+ * and w without gx. */
 int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void* x, int64_t ldx,
                          int64_t rows, int64_t in, int64_t out, const void* w, int64_t ldw,
                          int32_t w_transposed, int32_t act, const float* z, const void* y,
@@ -932,7 +933,8 @@ int vmoe_linear_backward(int32_t type, const void* gy, int64_t ldgy, const void*
 /* [g | u] = x w1 + bias1, h = act(g) * u, y = h w2 + bias2 + residual; w1 is
  * [hidden, 2 width], w2 [width, hidden]. h [rows, width] is written (rounded to the
  * rows' type); z [rows, 2 width] fp32 takes [g | u] for the backward pass, or is
- * NULL. */
+ * NULL. The backward pass reads x for gw1, w1 for gx, w2 and z for gx, gw1 and gb1, h for
+ * gw2; each may be NULL where nothing that reads it is asked for. */
 size_t vmoe_gated_workspace_bytes(int32_t type, int64_t rows, int64_t hidden, int64_t width,
                                   int32_t backward);
 int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int64_t rows, int64_t hidden,

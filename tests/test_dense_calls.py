@@ -112,3 +112,20 @@ def test_module_without_a_library():
                      "try: _dense.use(0)\n"
                      "except RuntimeError as e: print(e)\n" % str(_lib.LIB_PATH.parent.parent))
     assert out.returncode == 0 and out.stdout.count("library") == 2, out.stdout + out.stderr
+
+
+def test_what_a_backward_pass_does_not_read_is_not_asked_for():
+    """At the C entry points (no call here reaches a launch: the workspace is short)."""
+    lib, p, short = _lib.lib(), 0x1000, _lib.ERR_WORKSPACE
+
+    def gated(x=None, w1=None, w2=None, h=None, z=None, gx=None, gw1=None, gb1=None, gw2=None, gb2=None):
+        return lib.vmoe_gated_backward(0, p, 64, x, 64, 2, 64, 32, w1, 64, 0, w2, 64, 0, 3, h, z, gx, 64,
+                                       gw1, 64, gb1, 0, gw2, 64, gb2, 0, p, 0, None)
+    assert gated(gb2=p) == short
+    assert gated(h=p, gw2=p) == short
+    assert gated(w2=p, z=p, gb1=p) == short
+    assert gated(x=p, w2=p, z=p, gw1=p) == short
+    assert gated(w1=p, w2=p, z=p, gx=p) == short
+    for lacks in (dict(gw2=p), dict(z=p, gb1=p), dict(w2=p, gb1=p), dict(w2=p, z=p, gw1=p),
+                  dict(w2=p, z=p, gx=p), dict(w1=p, z=p, gx=p)):
+        assert gated(**lacks) == _lib.ERR_INVALID_ARG

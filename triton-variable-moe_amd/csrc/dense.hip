@@ -393,13 +393,13 @@ extern "C" size_t vmoe_gated_workspace_bytes(int32_t type, int64_t rows, int64_t
 }
 
 namespace {
-// (the up columns of a weight stored [2 width, hidden] are addressed from the
-// gate's by a 32-bit offset)
-int check_gated_weights(int type, const void* w1, int64_t ldw1, int t1, const void* w2,
-                        int64_t ldw2, int t2, int64_t d, int64_t width) {
-  VMOE_TRY(check_weight(type, w1, ldw1, t1, d, 2 * width));
-  VMOE_TRY(check_weight(type, w2, ldw2, t2, width, d));
-  if (t1 && (width + 256) * ldw1 * esize(type) >= (int64_t)1 << 31) return VMOE_ERR_UNSUPPORTED;
+// The weights that are read. (The up columns of a weight stored [2 width, hidden] are
+// addressed from the gate's by a 32-bit offset.)
+int check_gated_weights(int type, bool read1, const void* w1, int64_t ldw1, int t1, bool read2,
+                        const void* w2, int64_t ldw2, int t2, int64_t d, int64_t width) {
+  if (read1) VMOE_TRY(check_weight(type, w1, ldw1, t1, d, 2 * width));
+  if (read2) VMOE_TRY(check_weight(type, w2, ldw2, t2, width, d));
+  if (read1 && t1 && (width + 256) * ldw1 * esize(type) >= (int64_t)1 << 31) return VMOE_ERR_UNSUPPORTED;
   return VMOE_OK;
 }
 }  // namespace
@@ -415,8 +415,8 @@ extern "C" int vmoe_gated_forward(int32_t type, const void* x, int64_t ldx, int6
   VMOE_TRY(check_sizes(type, act, rows, hidden, width));
   if (rows == 0) return VMOE_OK;
   VMOE_TRY(check_rows(type, x, hidden, ldx));
-  VMOE_TRY(check_gated_weights(type, w1, ldw1, w1_transposed, w2, ldw2, w2_transposed, hidden,
-                               width));
+  VMOE_TRY(check_gated_weights(type, true, w1, ldw1, w1_transposed, true, w2, ldw2, w2_transposed,
+                               hidden, width));
   VMOE_TRY(check_rows(type, h, width, width));
   VMOE_TRY(check_rows(type, y, hidden, ldy));
   if (residual) VMOE_TRY(check_rows(type, residual, hidden, ldr));
@@ -457,9 +457,9 @@ extern "C" int vmoe_gated_backward(int32_t type, const void* gy, int64_t ldgy, c
   VMOE_TRY(check_sizes(type, act, rows, hidden, width));
   if (rows == 0) return VMOE_OK;
   VMOE_TRY(check_rows(type, gy, hidden, ldgy));
-  VMOE_TRY(check_gated_weights(type, w1, ldw1, w1_transposed, w2, ldw2, w2_transposed, hidden,
-                               width));
   const bool inner = gx || gw1 || gb1;  // what needs the gradient of [gate | up]
+  VMOE_TRY(check_gated_weights(type, gx, w1, ldw1, w1_transposed, inner, w2, ldw2, w2_transposed,
+                               hidden, width));
   if (inner && !z) return VMOE_ERR_INVALID_ARG;
   if (z && !aligned(z)) return VMOE_ERR_UNSUPPORTED;
   if (gw1) VMOE_TRY(check_rows(type, x, hidden, ldx));

@@ -176,7 +176,6 @@ int type_of(const Tensor& x) {
   return x.scalar_type() == at::kFloat ? VMOE_DENSE_F32 : VMOE_DENSE_BF16;
 }
 int f32(const Maybe& v) { return v && v->scalar_type() == at::kFloat; }
-int f32(const Tensor& v) { return v.defined() && v.scalar_type() == at::kFloat; }
 const void* ptr(const Maybe& v) { return v ? v->const_data_ptr() : nullptr; }
 // What a forward pass has saved.
 const void* saved_ptr(const Tensor& v) {
@@ -220,27 +219,25 @@ Mat rows_of(const Tensor& given, int64_t cols) {
 }
 
 // A weight [in, out]: in place in either order, or a copy in the nearer one.
-Mat weight_of(const Tensor& given) {
+bool in_order(const Tensor& w, int tr) {  // whether it is read in place
+  const int64_t ld = w.stride(tr), mult = 16 / (int64_t)w.element_size();
+  return w.stride(1 - tr) == 1 && ld >= w.size(1 - tr) && ld % mult == 0 && ld <= kMaxLd && aligned(w);
+}
+int weight_order(const Tensor& w) {
+  if (in_order(w, 0)) return 0;
+  return in_order(w, 1) || (w.stride(0) == 1 && w.stride(1) != 1);
+}
+Mat weight_of(const Tensor& given, int order = -1) {  // (0 or 1: in that order)
   const Tensor w = plain(given);
   Mat m;
-  const int64_t mult = 16 / (int64_t)w.element_size();
-  const int64_t a = w.stride(0), b = w.stride(1);
-  if (aligned(w)) {
-    if (b == 1 && a >= w.size(1) && a % mult == 0 && a <= kMaxLd) {
-      m.t = w;
-      m.ld = a;
-      return m;
-    }
-    if (a == 1 && b >= w.size(0) && b % mult == 0 && b <= kMaxLd) {
-      m.t = w;
-      m.ld = b;
-      m.tr = 1;
-      return m;
-    }
+  m.tr = order < 0 ? weight_order(w) : order;
+  if (in_order(w, m.tr)) {
+    m.t = w;
+    m.ld = w.stride(m.tr);
+  } else {
+    m.t = fresh(m.tr ? w.t() : w);
+    m.ld = m.t.size(1);
   }
-  m.tr = a == 1 && b != 1;
-  m.t = fresh(m.tr ? w.t() : w);
-  m.ld = m.t.size(1);
   return m;
 }
 
@@ -268,9 +265,13 @@ Tensor empty_f32(at::IntArrayRef shape, const Tensor& x) {
 Tensor workspace(size_t bytes, const Tensor& x) {
   return bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
 }
-// An uninitialised gradient of a weight [in, out] in the order the kernels read it.
-Tensor like_weight(const Tensor& w, int tr) {
-  return tr ? empty({w.size(1), w.size(0)}, w).t() : empty(w.sizes(), w);
+// Uninitialised gradients: of a vector, and of a weight [in, out] in the order the
+// kernels read it.
+Tensor vector_grad(int64_t n, bool f32, const Tensor& gy) {
+  return f32 ? empty_f32({n}, gy) : at::empty({n}, gy.options().dtype(at::kBFloat16));
+}
+Tensor weight_grad(int64_t in, int64_t out, int tr, const Tensor& gy) {
+  return tr ? empty({out, in}, gy).t() : empty({in, out}, gy);
 }
 int64_t ld_of(const Tensor& g, int tr) {
   return !g.defined() ? 0 : tr ? g.size(0) : g.size(1);
@@ -306,6 +307,32 @@ variable_list gradients(variable_list g) {
   return g;
 }
 
+// A forward pass saves what the gradients that can be asked for read, and no more: no
+// pre-activations for a residual's gradient, no rows where the weight has none, no bias.
+bool wants(const Tensor& t) { return t.requires_grad(); }
+bool wants(const Maybe& t) { return t && t->requires_grad(); }
+Tensor keep(bool read, const Tensor& t) { return read ? t : Tensor(); }
+Tensor keep(bool read, const Maybe& t) { return read && t ? *t : Tensor(); }
+
+// What else a backward pass has to know of its operands, in one value.
+struct How {
+  bool vector1 = false, vector1_f32 = false;  // a bias (a norm's weight): given, its type
+  bool vector2 = false, vector2_f32 = false;  // the second one (a norm's bias)
+  bool residual = false;
+  bool tr1 = false, tr2 = false;  // weights' orders
+  int act = 0;
+  int64_t size = 0;  // of a weight: linear's in, a gated block's width
+  void save(AutogradContext* ctx) const {
+    ctx->saved_data["how"] = size << 16 | act << 8 | vector1 | vector1_f32 << 1 | vector2 << 2 |
+                             vector2_f32 << 3 | residual << 4 | tr1 << 5 | tr2 << 6;
+  }
+  static How of(const AutogradContext* ctx) {
+    const int64_t v = ctx->saved_data.at("how").toInt();
+    return {bool(v & 1),  bool(v & 2),  bool(v & 4),          bool(v & 8), bool(v & 16),
+            bool(v & 32), bool(v & 64), int(v >> 8 & 0xFF), v >> 16};
+  }
+};
+
 // Which of an operator's tensors need gradients. (Autograd counts the given ones.)
 template <size_t N>
 std::array<bool, N> needs(const AutogradContext* ctx, const std::array<bool, N>& given) {
@@ -340,7 +367,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                         double eps) {
     Tensor stats;
     Tensor y = norm_forward(x, w, b, eps, &stats);
-    ctx->save_for_backward({x, w ? *w : Tensor(), b ? *b : Tensor(), stats});
+    ctx->save_for_backward({x, keep(wants(x), w), stats});
+    How{w.has_value(), bool(f32(w)), b.has_value(), bool(f32(b))}.save(ctx);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& gys) {
@@ -348,15 +376,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     {
       const at::AutoGradMode off(false);
       const variable_list s = ctx->get_saved_variables();
-      const Tensor &x = s[0], &b = s[2], &stats = s[3], &gy = gys[0];
+      const Tensor &x = s[0], &stats = s[2], &gy = gys[0];
+      const How how = How::of(ctx);
       const Maybe w = s[1].defined() ? contiguous(s[1]) : Maybe();
-      const auto need = needs<3>(ctx, {true, s[1].defined(), b.defined()});
+      const auto need = needs<3>(ctx, {true, how.vector1, how.vector2});
       const c10::DeviceGuard on(x.device());
       const int64_t d = x.size(-1), rows = stats.size(0);
       Tensor gx, gw, gb;
       if (need[0]) gx = empty(x.sizes(), x);
-      if (need[1]) gw = empty({d}, s[1]);
-      if (need[2]) gb = empty({d}, b);
+      if (need[1]) gw = vector_grad(d, how.vector1_f32, gy);
+      if (need[2]) gb = vector_grad(d, how.vector2_f32, gy);
       if (rows == 0) {
         zero({gw, gb});
       } else {
@@ -366,8 +395,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         call("vmoe_layer_norm_backward", [&] {
           return lib.vmoe_layer_norm_backward(
               type_of(x), g.p(), g.ld, m.p(), m.ld, rows, d, ptr(w), f32(w), saved_floats(stats),
-              out_ptr(gx), d, out_ptr(gw), f32(gw), out_ptr(gb), f32(gb), out_ptr(ws), n,
-              stream_of(x));
+              out_ptr(gx), d, out_ptr(gw), how.vector1_f32, out_ptr(gb), how.vector2_f32,
+              out_ptr(ws), n, stream_of(x));
         });
       }
       out[0] = gx;
@@ -423,45 +452,49 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& b_, const M
 struct FusedLinear : torch::autograd::Function<FusedLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b,
                         const Maybe& r, int64_t act) {
+    const bool slope = act && (wants(x) || wants(w) || wants(b));
     // relu's slope follows from the output, unless a residual is in it
     const bool from_y = !r && act == VMOE_DENSE_RELU;
     Tensor z;
-    Tensor y = linear_forward(x, w, b, r, (int)act, act && !from_y ? &z : nullptr);
-    ctx->save_for_backward({x, w, b ? *b : Tensor(), z, from_y ? y : Tensor()});
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["residual"] = r.has_value();
+    Tensor y = linear_forward(x, w, b, r, (int)act, slope && !from_y ? &z : nullptr);
+    ctx->save_for_backward({keep(wants(w), x), keep(wants(x), w), z, keep(slope && from_y, y)});
+    How{b.has_value(), bool(f32(b)), false, false, r.has_value(),
+        bool(weight_order(plain(w))), false, (int)act, w.size(0)}.save(ctx);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& gys) {
     variable_list out(5);
+    const How how = How::of(ctx);
     {
       const at::AutoGradMode off(false);
       const variable_list s = ctx->get_saved_variables();
-      const Tensor &x = s[0], &w = s[1], &b = s[2], &z = s[3], &y = s[4], &gy = gys[0];
-      const int act = (int)ctx->saved_data["act"].toInt();
-      const auto need =
-          needs<4>(ctx, {true, true, b.defined(), ctx->saved_data["residual"].toBool()});
+      const Tensor &x = s[0], &w = s[1], &z = s[2], &y = s[3], &gy = gys[0];
+      const auto need = needs<4>(ctx, {true, true, how.vector1, how.residual});
       if (need[0] || need[1] || need[2]) {
-        const c10::DeviceGuard on(x.device());
-        const int64_t in = w.size(0), n_out = w.size(1);
-        const Mat wm = weight_of(w);
+        const c10::DeviceGuard on(gy.device());
+        const int64_t in = how.size, n_out = gy.size(-1);
         Tensor gx, gw, gb;
-        if (need[0]) gx = empty(x.sizes(), x);
-        if (need[1]) gw = like_weight(w, wm.tr);
-        if (need[2]) gb = empty({n_out}, b);
-        if (x.numel() == 0) {
+        if (need[0]) {
+          at::DimVector shape(gy.sizes());
+          shape.back() = in;
+          gx = empty(shape, gy);
+        }
+        if (need[1]) gw = weight_grad(in, n_out, how.tr1, gy);
+        if (need[2]) gb = vector_grad(n_out, how.vector1_f32, gy);
+        if (gy.numel() == 0) {
           zero({gw, gb});
         } else {
-          const Mat m = rows_of(x, in), g = rows_of(gy, n_out);
-          const int64_t rows = m.t.size(0);
-          const int type = type_of(x);
-          const size_t n = lib.vmoe_linear_workspace_bytes(type, rows, in, n_out, act, 1);
-          const Tensor ws = workspace(n, x);
+          const Mat g = rows_of(gy, n_out);
+          const Mat m = need[1] ? rows_of(x, in) : Mat(), wm = need[0] ? weight_of(w, how.tr1) : Mat();
+          const int64_t rows = g.t.size(0);
+          const int type = type_of(gy);
+          const size_t n = lib.vmoe_linear_workspace_bytes(type, rows, in, n_out, how.act, 1);
+          const Tensor ws = workspace(n, gy);
           call("vmoe_linear_backward", [&] {
             return lib.vmoe_linear_backward(
-                type, g.p(), g.ld, m.p(), m.ld, rows, in, n_out, wm.p(), wm.ld, wm.tr, act,
-                saved_floats(z), saved_ptr(y), n_out, out_ptr(gx), in, out_ptr(gw), ld_of(gw, wm.tr),
-                out_ptr(gb), f32(gb), out_ptr(ws), n, stream_of(x));
+                type, g.p(), g.ld, m.p(), m.ld, rows, in, n_out, wm.p(), wm.ld, how.tr1, how.act,
+                saved_floats(z), saved_ptr(y), n_out, out_ptr(gx), in, out_ptr(gw),
+                ld_of(gw, how.tr1), out_ptr(gb), how.vector1_f32, out_ptr(ws), n, stream_of(gy));
           });
         }
         out[0] = gx;
@@ -470,7 +503,7 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
       }
     }
     out = gradients(std::move(out));
-    if (ctx->saved_data["residual"].toBool()) out[3] = gys[0];
+    if (how.residual) out[3] = gys[0];
     return out;
   }
 };
@@ -523,47 +556,51 @@ Tensor gated_forward(const Tensor& x, const Tensor& w1, const Tensor& w2, const 
 struct GatedMLP : torch::autograd::Function<GatedMLP> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w2,
                         const Maybe& b1, const Maybe& b2, const Maybe& r, int64_t act) {
+    const bool inner = wants(x) || wants(w1) || wants(b1);  // what needs the gradients of g and u
     Tensor h, z;
-    Tensor y = gated_forward(x, w1, w2, b1, b2, r, (int)act, h, &z);
-    ctx->save_for_backward({x, w1, w2, b1 ? *b1 : Tensor(), b2 ? *b2 : Tensor(), h, z});
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["residual"] = r.has_value();
+    Tensor y = gated_forward(x, w1, w2, b1, b2, r, (int)act, h, inner ? &z : nullptr);
+    ctx->save_for_backward({keep(wants(w1), x), keep(wants(x), w1), keep(inner, w2),
+                            keep(wants(w2), h), z});
+    How{b1.has_value(), bool(f32(b1)), b2.has_value(), bool(f32(b2)), r.has_value(),
+        bool(weight_order(plain(w1))), bool(weight_order(plain(w2))), (int)act,
+        w2.size(0)}.save(ctx);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& gys) {
     variable_list out(7);
+    const How how = How::of(ctx);
     {
       const at::AutoGradMode off(false);
       const variable_list s = ctx->get_saved_variables();
-      const Tensor &x = s[0], &w1 = s[1], &w2 = s[2], &b1 = s[3], &b2 = s[4], &h = s[5], &z = s[6];
-      const Tensor& gy = gys[0];
-      const auto need = needs<6>(ctx, {true, true, true, b1.defined(), b2.defined(),
-                                       ctx->saved_data["residual"].toBool()});
-      if (need[0] || need[1] || need[2] || need[3] || need[4]) {
-        const c10::DeviceGuard on(x.device());
-        const int64_t width = w2.size(0), d = w2.size(1);
-        const Mat m1 = weight_of(w1), m2 = weight_of(w2);
+      const Tensor &x = s[0], &w1 = s[1], &w2 = s[2], &h = s[3], &z = s[4], &gy = gys[0];
+      const auto need = needs<6>(ctx, {true, true, true, how.vector1, how.vector2, how.residual});
+      const bool inner = need[0] || need[1] || need[3];
+      if (inner || need[2] || need[4]) {
+        const c10::DeviceGuard on(gy.device());
+        const int64_t width = how.size, d = gy.size(-1);
         Tensor gx, gw1, gw2, gb1, gb2;
-        if (need[0]) gx = empty(x.sizes(), x);
-        if (need[1]) gw1 = like_weight(w1, m1.tr);
-        if (need[2]) gw2 = like_weight(w2, m2.tr);
-        if (need[3]) gb1 = empty({2 * width}, b1);
-        if (need[4]) gb2 = empty({d}, b2);
-        if (x.numel() == 0) {
+        if (need[0]) gx = empty(gy.sizes(), gy);
+        if (need[1]) gw1 = weight_grad(d, 2 * width, how.tr1, gy);
+        if (need[2]) gw2 = weight_grad(width, d, how.tr2, gy);
+        if (need[3]) gb1 = vector_grad(2 * width, how.vector1_f32, gy);
+        if (need[4]) gb2 = vector_grad(d, how.vector2_f32, gy);
+        if (gy.numel() == 0) {
           zero({gw1, gw2, gb1, gb2});
         } else {
-          const Mat m = rows_of(x, d), g = rows_of(gy, d);
-          const int64_t rows = m.t.size(0);
-          const int type = type_of(x);
+          const Mat g = rows_of(gy, d), m = need[1] ? rows_of(x, d) : Mat();
+          const Mat m1 = need[0] ? weight_of(w1, how.tr1) : Mat();
+          const Mat m2 = inner ? weight_of(w2, how.tr2) : Mat();
+          const int64_t rows = g.t.size(0);
+          const int type = type_of(gy);
           const size_t n = lib.vmoe_gated_workspace_bytes(type, rows, d, width, 1);
-          const Tensor ws = workspace(n, x);
+          const Tensor ws = workspace(n, gy);
           call("vmoe_gated_backward", [&] {
             return lib.vmoe_gated_backward(
-                type, g.p(), g.ld, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, m1.tr, m2.p(),
-                m2.ld, m2.tr, (int)ctx->saved_data["act"].toInt(), saved_ptr(h), saved_floats(z),
-                out_ptr(gx), d, out_ptr(gw1), ld_of(gw1, m1.tr), out_ptr(gb1), f32(gb1),
-                out_ptr(gw2), ld_of(gw2, m2.tr), out_ptr(gb2), f32(gb2), out_ptr(ws), n,
-                stream_of(x));
+                type, g.p(), g.ld, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, how.tr1, m2.p(),
+                m2.ld, how.tr2, how.act, saved_ptr(h), saved_floats(z), out_ptr(gx), d,
+                out_ptr(gw1), ld_of(gw1, how.tr1), out_ptr(gb1), how.vector1_f32, out_ptr(gw2),
+                ld_of(gw2, how.tr2), out_ptr(gb2), how.vector2_f32, out_ptr(ws), n,
+                stream_of(gy));
           });
         }
         out[0] = gx;
@@ -574,7 +611,7 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
       }
     }
     out = gradients(std::move(out));
-    if (ctx->saved_data["residual"].toBool()) out[5] = gys[0];
+    if (how.residual) out[5] = gys[0];
     return out;
   }
 };

@@ -12,7 +12,9 @@ order: rows contiguous, or the transposed view of a matrix stored [out, in]
 (linear.weight.t()); gradients come in the same order. Tensors that the kernels cannot
 read in place (rows not contiguous, or not aligned to 16 bytes) are copied. Calls run
 on the current stream of x's device without a host sync, allocate from torch's
-allocator, record gradients where autograd does, and can be captured into a graph.
+allocator, record gradients where autograd does, and can be captured into a graph. A
+recorded call saves what the gradients that can be asked for read (no pre-activations
+for a residual's or w2's, no x where the weight takes none; layer_norm always x).
 Gradients cannot be differentiated again, and there are no forward-mode derivatives.
 """
 
