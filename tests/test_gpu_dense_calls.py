@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from test_dense_calls import WITHOUT_MEMORY, Wrapper, calls, freed
+from triton_moe import _lib
 from triton_moe import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -178,3 +179,36 @@ def test_negative_transposed_weight(device):
     got = [torch.autograd.grad(K.fused_linear(x, v, None, "silu"), (x, v), gy)
            for v in (n.detach().requires_grad_(), w.t().detach().requires_grad_())]
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_an_observer_s_error_reaches_the_caller(device):
+    """As it does from the package's other operators, forward and backward."""
+    class Timer:
+        def __init__(self, bad):
+            self.bad, self.seen = bad, []
+
+        def begin(self, name):
+            self.note("begin", name)
+
+        def end(self, name):
+            self.note("end", name)
+
+        def note(self, *what):
+            self.seen.append(what)
+            if what == self.bad:
+                raise KeyError("observer")
+
+    x = randn(4, 64).requires_grad_()
+    for bad, direction in ((("begin", "vmoe_layer_norm"), 0), (("end", "vmoe_layer_norm"), 0),
+                           (("begin", "vmoe_layer_norm_backward"), 1),
+                           (("end", "vmoe_layer_norm_backward"), 1)):
+        y = K.layer_norm(x)
+        t = Timer(bad)
+        _lib.set_launch_timer(t)
+        try:
+            with pytest.raises(KeyError, match="observer"):
+                y.sum().backward() if direction else K.layer_norm(x)
+        finally:
+            _lib.set_launch_timer(None)
+        assert t.seen[-1] == bad
+    K.layer_norm(x).sum().backward()

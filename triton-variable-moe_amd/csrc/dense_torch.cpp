@@ -65,11 +65,18 @@ struct Library {
 PyObject* g_timer = nullptr;  // observer of launches (begin(name), end(name)), or null
 
 void observe(const char* method, const char* name) {
-  const PyGILState_STATE gil = PyGILState_Ensure();
-  PyObject* r = g_timer ? PyObject_CallMethod(g_timer, method, "s", name) : nullptr;
-  if (!r) PyErr_Clear();
-  Py_XDECREF(r);
-  PyGILState_Release(gil);
+  struct Gil {
+    PyGILState_STATE state = PyGILState_Ensure();
+    ~Gil() { PyGILState_Release(state); }
+  } gil;
+  if (!g_timer) return;
+  PyObject* r = PyObject_CallMethod(g_timer, method, "s", name);
+  if (!r) {  // the observer's own error, for the caller
+    python_error error;
+    error.persist();
+    throw error;
+  }
+  Py_DECREF(r);
 }
 
 template <typename F>
