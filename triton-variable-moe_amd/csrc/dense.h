@@ -228,10 +228,10 @@ __device__ __forceinline__ GateUp load_z(const GemmArgs& p, int64_t m, int64_t n
 }
 
 // Row m, columns n .. n + C - 1 (the caller has checked m < M and n < N): v are the
-// sums, u the up half's for EPI_GATED. KEEP: pre-activations are stored too, if
-// wanted. EPI_GATED_BWD adds what it stores, before rounding, to sg and su (this
-// thread's columns of the bias gradient).
-template <typename E, int EPI, int C, bool KEEP = true>
+// sums, u the up half's for EPI_GATED. Pre-activations are stored too, if wanted (of 8
+// columns by write_tile, 4 columns a lane). EPI_GATED_BWD adds what it stores, before
+// rounding, to sg and su (this thread's columns of the bias gradient).
+template <typename E, int EPI, int C>
 __device__ __forceinline__ void epi_row(const GemmArgs& p, const EpiCols<EPI, C>& q, int64_t m,
                                         int64_t n, float (&v)[C], float (&u)[C],
                                         const GateUp& z, float (&sg)[C], float (&su)[C]) {
@@ -240,7 +240,7 @@ __device__ __forceinline__ void epi_row(const GemmArgs& p, const EpiCols<EPI, C>
   if constexpr (EPI == EPI_LINEAR) {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] += q.b[i];
-    if constexpr (KEEP && C == 4)
+    if constexpr (C == 4)
       if (p.z) store_z4(p.z + m * p.ldz + n, p.z_past, v);
     act_switch(p.act, [&](auto A) {
 #pragma unroll
