@@ -300,12 +300,17 @@ __device__ __forceinline__ void wait_vmcnt() {
 }
 
 // Barrier without the fences of __syncthreads(), which would wait for every DMA
-// in flight. LDS reads are consumed by matrix instructions before it, DMAs are
-// waited for with wait_vmcnt.
-__device__ __forceinline__ void block_barrier() {
+// in flight: those are waited for with wait_vmcnt. The caller has no LDS read in flight.
+__device__ __forceinline__ void bare_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+// The same where there may be LDS reads: another wave's DMA may write after the barrier
+// what they read, and the matrix instructions that use them may come later.
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  bare_barrier();
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(uint64_t a) {

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(512, 2) void big_kernel(GemmArgs p) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if constexpr (decltype(N)::value >= 0) wait_vmcnt<decltype(N)::value>();
     __builtin_amdgcn_sched_barrier(0);
-    block_barrier();
+    bare_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](int h, int j) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(512, 2) void big_kernel(GemmArgs p) {
       for (int i = 0; i < 2; ++i) acc[2 * h + i][j] = mma(af[i][s], bf[j][s], acc[2 * h + i][j]);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
-    block_barrier();
+    bare_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
   std::integral_constant<int, -1> none;
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(512, 2) void big_kernel(GemmArgs p) {
   fetch(0, a0); fetch(0, b0); fetch(0, b1); fetch(0, a1);
   fetch(1, a0); fetch(1, b0); fetch(1, b1); fetch(1, a1);
   wait_vmcnt<12>();
-  block_barrier();
-  if (wm == 1) block_barrier();
+  bare_barrier();
+  if (wm == 1) bare_barrier();
   __builtin_amdgcn_sched_barrier(0);
   for (int kt = 0; kt < nk; ++kt) {
     const lds_char* st = lds + (kt & 1) * (4 * kHalf);
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(512, 2) void big_kernel(GemmArgs p) {
     multiply(1, 0);
   }
   wait_vmcnt<0>();
-  if (wm == 0) block_barrier();
-  block_barrier();  // every wave has read the last stage, no DMA is in flight
+  if (wm == 0) bare_barrier();
+  bare_barrier();  // every wave has read the last stage, no DMA is in flight
   if (t.slice >= 0)
     write_part<4, 2>(acc, tile_part<65536>(p, t) + wave * 8192);
   else
