@@ -212,3 +212,90 @@ def test_an_observer_s_error_reaches_the_caller(device):
             _lib.set_launch_timer(None)
         assert t.seen[-1] == bad
     K.layer_norm(x).sum().backward()
+
+
+def step(x, p):
+    h = K.fused_linear(K.layer_norm(x, p[0], p[1]), p[2], p[3], "gelu", x)
+    return K.gated_mlp(h, p[4], p[5], "swiglu", None, p[3], h)
+
+
+def parameters(dtype=torch.bfloat16, d=264, width=520):
+    p = [randn(d, seed=1), randn(d, seed=2), randn(d, d, seed=3, dtype=dtype) * 0.06,
+         randn(d, seed=4, dtype=dtype), randn(2 * width, d, seed=5, dtype=dtype).t() * 0.06,
+         randn(width, d, seed=6, dtype=dtype) * 0.04]
+    return [t.detach().requires_grad_() for t in p]
+
+
+@pytest.mark.parametrize("rows", [7, 300])
+def test_recomputed_and_moved_aside(rows, device):
+    """Under torch's checkpoints, and with what is saved kept on the host: the bits of the
+    plain step."""
+    from torch.utils.checkpoint import checkpoint
+
+    p, x = parameters(), randn(rows, 264, dtype=torch.bfloat16).requires_grad_()
+    gy = randn(rows, 264, seed=9, dtype=torch.bfloat16)
+    want = [step(x, p), *torch.autograd.grad(step(x, p), [x, *p], gy)]
+    for reentrant in (False, True):
+        for t in (x, *p):
+            t.grad = None
+        y = checkpoint(step, x, p, use_reentrant=reentrant)
+        y.backward(gy)
+        assert all(torch.equal(a, b) for a, b in zip(want, [y, *(t.grad for t in (x, *p))]))
+    with torch.autograd.graph.save_on_cpu():
+        y = step(x, p)
+    got = [y, *torch.autograd.grad(y, [x, *p], gy)]
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    y = step(x, p)  # twice through one graph
+    for _ in range(2):
+        got = torch.autograd.grad(y, [x, *p], gy, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(want[1:], got))
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_calls_of_several_threads(own_stream, device):
+    """On one stream and on streams of their own, products of few rows (which share a
+    stream's arrival words) among them."""
+    import threading
+
+    p = parameters()
+    wide = randn(4096, 520, seed=7, dtype=torch.bfloat16) * 0.02
+    xs = [randn(rows, 264, seed=rows, dtype=torch.bfloat16) for rows in (1, 5, 40, 300)]
+    fs = [randn(rows, 4096, seed=rows, dtype=torch.bfloat16) for rows in (1, 5, 40, 300)]
+
+    def work(i):
+        x = xs[i].detach().requires_grad_()
+        y = step(x, p)
+        return [y.detach(), *torch.autograd.grad(y.float().sum(), [x, *p]), K.fused_linear(fs[i], wide)]
+    want = [work(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in xs], []
+
+    def thread(i):
+        try:
+            s = torch.cuda.Stream() if own_stream else torch.cuda.default_stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i].append(work(i))
+        except BaseException as e:  # noqa: BLE001 - raised below
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for w, runs in zip(want, got):
+        assert len(runs) == 20
+        for r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
+
+
+def test_transforms_are_refused(device):
+    """A batched or traced tensor's values are not in its own memory."""
+    x, w = randn(3, 4, 8), randn(8, 8)
+    with pytest.raises(NotImplementedError, match="x has no memory"):
+        torch.vmap(lambda t: K.fused_linear(t, w))(x)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.grad(lambda t: K.layer_norm(t).sum())(x)
