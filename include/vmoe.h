@@ -889,7 +889,8 @@ int vmoe_q4_matvec(const void* x, int64_t ldx, int64_t num_rows, const void* ids
  * Dense operators beside the expert layer (no counterpart in the reference):
  * layer norm, a linear layer with a fused epilogue, a gated feed-forward block.
  * type: of rows, weights and outputs. Sums are fp32, an output is rounded
- * once; biases and the norm's weights are bf16 or fp32 on their own
+ * once (in bf16 the gated block's h and the gradients through an activation are
+ * rounded too, as operands of the next product); biases and the norm's weights are bf16 or fp32 on their own
  * (*_f32). A weight is [in, out], or with *_transposed stored [out, in]; leading
  * dimensions are of the stored matrix, multiples of 8 (fp32: 4), at most 2^20,
  * as are in, out, hidden and width; buffers are 16-byte aligned, biases by their

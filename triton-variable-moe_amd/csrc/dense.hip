@@ -72,7 +72,10 @@ static_assert(kCus <= kFewWords, "a split product of few rows has fewer column b
 // 16 rows always (one row of 1024 x 4096: 5.0 us, on tiles 8.4); up to 64 for weights
 // of at most 32 MB (61 rows of 1024 x 4096: 9.2 and 9.7; of 8192 x 8192: 41 and 36). k
 // is split for a workgroup a CU, about 512 of k or more each (a round of the waves'
-// loads): 4096 x 1024 14.5 -> 7.0; not at k <= 1024, where the joining costs more (1024 x 4096: 6.1 whole, 6.7 in two).
+// loads): 4096 x 1024 14.5 -> 7.0; not at k <= 1024, where the joining costs more: k 512
+// always (61 rows and 4096 columns 6.6 whole, 6.8 in two), k 1024 with 8192 columns (one
+// row 5.6 and 7.1, 61 rows 9.5 and 11.5) or one row of 4096 (5.2 and 5.9). From 33 rows
+// and up to 4096 columns two slices would be ahead there (61 rows 9.3 and 8.4).
 bool plan_rows(int type, Form form, Epi epi, int64_t M, int64_t N, int64_t K, Plan& q) {
   if (form == FORM_TT || epi == EPI_GATED_BWD || M > kFewRows) return false;
   const int64_t n = epi == EPI_GATED ? 2 * N : N;

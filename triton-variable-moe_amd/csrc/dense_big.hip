@@ -20,9 +20,10 @@
 // 1320 TFLOP/s; weight gradients 1240 to 1270; a plain tile loop of the same size 900).
 // k 2048: the epilogue, 7 to 50 us in which the CU multiplies nothing (gated, 16384 x
 // 8192, fp32 gates and ups kept: 1130 us, 970 TFLOP/s; its gradient, which reads them
-// again, 1 GB: 790 to 810 us, 690 TFLOP/s). First workgroups started 20 to 40 us apart, so
-// that the CUs' epilogues do not meet, took 8 % off the gradient and nothing off the
-// others: not kept.
+// again, 1 GB: 790 to 810 us, 690 TFLOP/s; its epilogue spills 7 of 256 registers, 32
+// bytes a lane). First workgroups started 20 to 40 us apart, so that the CUs' epilogues
+// do not meet, took 8 % off the gradient and nothing off the others: open, for that
+// epilogue alone.
 
 #include "dense_launch.h"
 

@@ -11,8 +11,9 @@ enum Tiles { ROWS_32, ROWS_64, TILES_64, TILES_128, TILES_256 };  // ROWS: dense
 
 // Pre-activations of 64 MB or more are written and read past the caches: a pass reads
 // them once, and the last-level cache (256 MB) keeps what the next launches read
-// (8192 x 1024 x 4096, 134 MB: 337 -> 321 us a training pass; 16384 x 2048 x 8192 gated,
-// 1 GB: 4870 -> 4797; 2051 x 768 x 2048, 17 MB, lost by it: 214 -> 219).
+// (a training pass of 8192 x 1024 x 4096, 128 MB: 353 -> 335 us; 6144 rows, 96 MB: 278 ->
+// 266; gated 4096 x 1024 x 2816, 88 MB: 360 -> 339; 8192 rows, 176 MB: 647 -> 576. At 64 MB
+// 187 and 188, below that it loses 0.5 to 3 %: 32 MB 111.8 -> 112.8, 16 MB 77 -> 80).
 constexpr int64_t kPastCache = 64 << 20;
 inline int z_past(int64_t rows, int64_t cols) { return rows * cols * 4 >= kPastCache; }
 

@@ -7,18 +7,19 @@
 // centred sum of squares and the result; statistics, gradients and sums are fp32. The
 // mean's own error (a share of |x|, not of the spread) is the mean of the centred values
 // and is taken out of them: a row of 65537.3 gives 0, where without that 768 values gave
-// 0.98 (32768 x 2048 in bf16 52.6 -> 53 us; 8192 x 8192, with 1024 threads a row, 55.5 ->
-// 59.7). The backward pass reads the mean as one float, off by half a unit of its last place.
+// 0.98 (32768 x 2048 in bf16 52.6 -> 53 us with its values out of the caches; 8192 x 8192,
+// with 1024 threads a row, 55.5 -> 60). The backward pass reads the mean as one float, off by half a unit of its last place.
 // A row belongs to 8, 16 or 64 threads (within a wave, no barrier) or, where it is
 // long, to 256 or 1024; workgroups go on to further rows with the weights, and in the backward
 // pass their gradients' sums, in registers. The forward pass fetches a row while the
 // one before is worked on (32768 x 2048 in bf16: 64 -> 48 us with 256 threads a row
-// instead of 64, 5.6 TB/s); the backward pass, with two streams of rows, gained
+// instead of 64; 49 now, 5.5 TB/s); the backward pass, with two streams of rows, gained
 // nothing by that (77 to 83 us, 4.9 to 5.2 TB/s). Those sums are joined in a fixed
 // order: within a workgroup, then by a launch of their own. Rows of any length are read
 // 16 bytes at a time (see Span): 16384 x 4095 in bf16, both passes, 489 us value by
 // value, 240 so, 157 for 4096. Short rows by 8 or 16 threads instead of 64: 300000 x 47
-// forward 62 -> 18 us, 300000 x 128 62 -> 29 (5.2 TB/s).
+// forward 62 -> 18 us, 300000 x 128 62 -> 29 (5.2 TB/s). Unaligned rows of more than 8192
+// values spill in the backward pass (bf16 20 bytes a lane, fp32 52).
 
 #include "dense_launch.h"
 

@@ -54,7 +54,8 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     (the same), bias either; in and out multiples of 8 (fp32: 4). Sums, bias,
     activation and residual are fp32, the output is rounded once. With an activation
     x weight + bias is kept in fp32 for the backward pass; with relu and no residual the
-    output is kept instead (it must not be changed in place)."""
+    output is kept instead (it must not be changed in place). The gradient through the
+    activation is rounded to x's type, as an operand of the gradients' products."""
     act = _ACT.get(activation)
     if act is None:
         raise ValueError(f"Unknown activation: {activation} (expected one of "
@@ -70,8 +71,8 @@ def gated_mlp(x, w1, w2, activation="swiglu", bias1=None, bias2=None, residual=N
     on the gate), "geglu", "geglu_tanh" or "reglu". Both projections, the activation and
     the product are one kernel, the second product with bias and residual another. x and
     the weights are bf16 or fp32 (the same), biases either; d and width multiples of 8
-    (fp32: 4). h is rounded to x's type, as an operand of the second product; the
-    backward pass keeps g and u in fp32."""
+    (fp32: 4). h is rounded to x's type, as an operand of the second product, and so are
+    the gradients of g and u; the backward pass keeps g and u in fp32."""
     act = _GATE_ACT.get(activation)
     if act is None:
         raise ValueError(f"Unknown activation: {activation} (expected one of {sorted(_GATES)})")
