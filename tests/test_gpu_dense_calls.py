@@ -299,3 +299,20 @@ def test_transforms_are_refused(device):
         torch.vmap(lambda t: K.fused_linear(t, w))(x)
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.grad(lambda t: K.layer_norm(t).sum())(x)
+
+
+def test_a_call_among_fake_tensors_leaves_nothing(device):
+    """Where torch makes tensors without memory a call fails; what a stream keeps is not
+    made of them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, w = randn(2, 4096), randn(4096, 64, seed=1)
+    want = K.fused_linear(x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(Exception):
+            K.fused_linear(x, w)
+        got = K.fused_linear(x, w)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -362,9 +362,9 @@ Tensor norm_forward(const Tensor& x, const Maybe& w_, const Maybe& b_, double ep
   if (stats) *stats = empty_f32({rows, 2}, x);
   call("vmoe_layer_norm", [&] {
     return lib.vmoe_layer_norm(type_of(x), m.p(), m.ld, rows, d, ptr(w), f32(w), ptr(b), f32(b),
-                           (float)eps, y.mutable_data_ptr(), d,
-                           stats ? static_cast<float*>(stats->mutable_data_ptr()) : nullptr,
-                           stream_of(x));
+                               (float)eps, y.mutable_data_ptr(), d,
+                               stats ? static_cast<float*>(stats->mutable_data_ptr()) : nullptr,
+                               stream_of(x));
   });
   return y;
 }
@@ -449,9 +449,9 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Maybe& b_, const M
   const Tensor ws = workspace(n, x);
   call("vmoe_linear_forward", [&] {
     return lib.vmoe_linear_forward(type, m.p(), m.ld, rows, in, out, wm.p(), wm.ld, wm.tr, ptr(b),
-                               f32(b), act, rm.p(), rm.ld, y.mutable_data_ptr(), out,
-                               z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
-                               out_ptr(ws), n, words_of(x, rows, n), stream_of(x));
+                                   f32(b), act, rm.p(), rm.ld, y.mutable_data_ptr(), out,
+                                   z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
+                                   out_ptr(ws), n, words_of(x, rows, n), stream_of(x));
   });
   return y;
 }
@@ -551,11 +551,11 @@ Tensor gated_forward(const Tensor& x, const Tensor& w1, const Tensor& w2, const 
   const Tensor ws = workspace(n, x);
   call("vmoe_gated_forward", [&] {
     return lib.vmoe_gated_forward(type, m.p(), m.ld, rows, d, width, m1.p(), m1.ld, m1.tr, ptr(b1),
-                              f32(b1), act, m2.p(), m2.ld, m2.tr, ptr(b2), f32(b2), rm.p(), rm.ld,
-                              h.mutable_data_ptr(),
-                              z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
-                              y.mutable_data_ptr(), d, out_ptr(ws), n, words_of(x, rows, n),
-                              stream_of(x));
+                                  f32(b1), act, m2.p(), m2.ld, m2.tr, ptr(b2), f32(b2), rm.p(), rm.ld,
+                                  h.mutable_data_ptr(),
+                                  z ? static_cast<float*>(z->mutable_data_ptr()) : nullptr,
+                                  y.mutable_data_ptr(), d, out_ptr(ws), n, words_of(x, rows, n),
+                                  stream_of(x));
   });
   return y;
 }
